@@ -328,6 +328,141 @@ int32_t sq_gdn_prefill(const sq_prefill_args *args, sq_stream_t stream);
 int32_t sq_kda_prefill(const sq_prefill_args *args, sq_stream_t stream);
 
 /*
+ * Operators around the recurrent state, no counterpart in the reference (its
+ * models run them in the host framework): the residual norm before a
+ * recurrent layer's projections, the short causal convolution between
+ * projection and state, and the selective state space scan, the state pass of
+ * layers whose decay and input depend on the token.  Statistics, sums and
+ * states are fp32.  Row strides are in elements, the last axis is contiguous;
+ * 16-byte aligned rows of a multiple of 8 values take wide accesses.
+ */
+
+/*
+ * Root-mean-square norm (normalize = 1), or the e4m3 quantization alone
+ * (normalize = 0: no weight, no residual, scale required).
+ *   x, residual  [rows, hidden] in dtype; residual may be NULL
+ *   weight       [hidden] in weight_dtype
+ *   residual_out [rows, hidden] in dtype, contiguous: x + residual rounded
+ *                once (may be residual's own contiguous buffer); NULL without residual
+ *   out          [rows, hidden] contiguous: h / sqrt(mean(h^2) + eps) * weight
+ *                with h = x + residual unrounded; in dtype, or e4m3 when scale is given
+ *   scale        [rows, ceil(hidden / 128)] fp32 or NULL: per 128 channels
+ *                max(max |y|, 1e-30) / 448; out = e4m3(y / scale)
+ * hidden <= 65536.
+ */
+typedef struct sq_norm_args {
+    const void *x;
+    const void *residual;
+    const void *weight;
+    void *residual_out;
+    void *out;
+    float *scale;
+    int64_t x_stride;
+    int64_t residual_stride;
+    int32_t rows;
+    int32_t hidden;
+    int32_t dtype;
+    int32_t weight_dtype;
+    int32_t normalize;
+    float eps;
+} sq_norm_args;
+
+int32_t sq_rms_norm(const sq_norm_args *args, sq_stream_t stream);
+
+/*
+ * Causal convolution of `taps` (2 to 4) inputs a channel over concatenated
+ * sequences: y_t = act(bias + sum_j weight[:, j] x_{t - taps + 1 + j}), act =
+ * SiLU or the identity.  Sequence n owns tokens [cu_seqlens[n],
+ * cu_seqlens[n + 1]), clamped to [0, tokens); tokens of no sequence are left
+ * unwritten.
+ *   x       [tokens, channels] in dtype; y the same, contiguous
+ *   weight  [channels, taps] fp32, bias [channels] fp32 or NULL
+ *   initial_state, final_state  [num_seqs or num_slots, channels, taps - 1] in
+ *           dtype, oldest input first: the inputs before the first token (NULL:
+ *           zeros) and the last taps - 1 ones (NULL: not kept); may be one buffer
+ *   slots   [num_seqs] rows of the states, or NULL for row n.  A slot <= 0 or
+ *           >= num_slots (flagged in status) gives zero outputs and no state.
+ * sq_causal_conv_step: one token of each of num_seqs = tokens requests;
+ * final_state is read and updated in place (cu_seqlens, initial_state unused).
+ */
+typedef struct sq_conv_args {
+    const void *x;
+    const float *weight;
+    const float *bias;
+    void *y;
+    const void *initial_state;
+    void *final_state;
+    const int64_t *slots;
+    const int32_t *cu_seqlens;
+    int32_t *status;
+    int64_t x_stride;
+    int64_t num_slots;
+    int32_t tokens;
+    int32_t num_seqs;
+    int32_t channels;
+    int32_t taps;
+    int32_t dtype;
+    int32_t silu;
+} sq_conv_args;
+
+int32_t sq_causal_conv(const sq_conv_args *args, sq_stream_t stream);
+int32_t sq_causal_conv_step(const sq_conv_args *args, sq_stream_t stream);
+
+/*
+ * Selective state space scan over concatenated sequences (as above), channel
+ * d reading group d / (channels / groups):
+ *   dt' = softplus(dt + dt_bias)  (or dt + dt_bias without softplus)
+ *   h[d, n] <- exp(dt' a[d, n]) h[d, n] + dt' u b[group, n]
+ *   y[d]     = (sum_n c[group, n] h[d, n] + d[d] u) silu(z)
+ *   u, dt, z  [tokens, channels] in dtype (z may be NULL); y the same, contiguous
+ *   b, c      [tokens, groups, states] in dtype, a token's groups contiguous
+ *   a         [channels, states] fp32, 16-byte aligned; d, dt_bias [channels] fp32 or NULL
+ *   initial_state, final_state  [num_seqs or num_slots, channels, states] fp32,
+ *             16-byte aligned, NULL as for the convolution; may be one buffer
+ *   slots     as for the convolution
+ *   workspace caller-owned, sq_selective_scan_workspace_bytes(...) bytes, 16-byte
+ *             aligned: where few channels and sequences would leave SMs idle, long
+ *             sequences are cut into chunks scanned side by side.  NULL / 0: not cut.
+ * states in {4, 8, 16, 32, 64}.  sq_selective_scan_step: one token of each of
+ * num_seqs = tokens requests, final_state read and updated in place.
+ */
+typedef struct sq_scan_args {
+    const void *u;
+    const void *dt;
+    const void *z;
+    const void *b;
+    const void *c;
+    const float *a;
+    const float *d;
+    const float *dt_bias;
+    void *y;
+    const float *initial_state;
+    float *final_state;
+    const int64_t *slots;
+    const int32_t *cu_seqlens;
+    int32_t *status;
+    void *workspace;
+    int64_t workspace_bytes;
+    int64_t u_stride;
+    int64_t dt_stride;
+    int64_t z_stride;
+    int64_t b_stride;
+    int64_t c_stride;
+    int64_t num_slots;
+    int32_t tokens;
+    int32_t num_seqs;
+    int32_t channels;
+    int32_t states;
+    int32_t groups;
+    int32_t dtype;
+    int32_t softplus;
+} sq_scan_args;
+
+int64_t sq_selective_scan_workspace_bytes(int32_t tokens, int32_t num_seqs, int32_t channels, int32_t states, int32_t groups);
+int32_t sq_selective_scan(const sq_scan_args *args, sq_stream_t stream);
+int32_t sq_selective_scan_step(const sq_scan_args *args, sq_stream_t stream);
+
+/*
  * Self-test of the division used by the register-resident decode kernels: for
  * i < n, out[i] = a[i] / b[i] computed with a correctly rounded reciprocal of
  * the fp16 value b[i] (given as its bits) and one Markstein correction.  It

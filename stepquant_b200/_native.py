@@ -45,6 +45,28 @@ class SqPrefillArgs(ctypes.Structure):
                 ("workspace", _p), ("workspace_bytes", _i64), ("status", _p)]
 
 
+class SqNormArgs(ctypes.Structure):
+    _fields_ = [("x", _p), ("residual", _p), ("weight", _p), ("residual_out", _p), ("out", _p), ("scale", _p),
+                ("x_stride", _i64), ("residual_stride", _i64), ("rows", _i32), ("hidden", _i32), ("dtype", _i32),
+                ("weight_dtype", _i32), ("normalize", _i32), ("eps", ctypes.c_float)]
+
+
+class SqConvArgs(ctypes.Structure):
+    _fields_ = [("x", _p), ("weight", _p), ("bias", _p), ("y", _p), ("initial_state", _p), ("final_state", _p),
+                ("slots", _p), ("cu_seqlens", _p), ("status", _p), ("x_stride", _i64), ("num_slots", _i64),
+                ("tokens", _i32), ("num_seqs", _i32), ("channels", _i32), ("taps", _i32), ("dtype", _i32),
+                ("silu", _i32)]
+
+
+class SqScanArgs(ctypes.Structure):
+    _fields_ = [("u", _p), ("dt", _p), ("z", _p), ("b", _p), ("c", _p), ("a", _p), ("d", _p), ("dt_bias", _p),
+                ("y", _p), ("initial_state", _p), ("final_state", _p), ("slots", _p), ("cu_seqlens", _p),
+                ("status", _p), ("workspace", _p), ("workspace_bytes", _i64), ("u_stride", _i64), ("dt_stride", _i64),
+                ("z_stride", _i64), ("b_stride", _i64), ("c_stride", _i64), ("num_slots", _i64), ("tokens", _i32),
+                ("num_seqs", _i32), ("channels", _i32), ("states", _i32), ("groups", _i32), ("dtype", _i32),
+                ("softplus", _i32)]
+
+
 _SIGNATURES = {
     "sq_version": (_i32, []),
     "sq_error_string": (ctypes.c_char_p, [_i32]),
@@ -67,6 +89,12 @@ _SIGNATURES = {
     "sq_gdn_prefill": (_i32, [_p, _p]),
     "sq_gdn_prefill_workspace_bytes": (_i64, [_i32, _i32, _i32]),
     "sq_kda_prefill": (_i32, [_p, _p]),
+    "sq_rms_norm": (_i32, [_p, _p]),
+    "sq_causal_conv": (_i32, [_p, _p]),
+    "sq_causal_conv_step": (_i32, [_p, _p]),
+    "sq_selective_scan": (_i32, [_p, _p]),
+    "sq_selective_scan_step": (_i32, [_p, _p]),
+    "sq_selective_scan_workspace_bytes": (_i64, [_i32] * 5),
 }
 
 EXPORTED = tuple(_SIGNATURES)
@@ -130,3 +158,47 @@ def require_cuda(*tensors):
     for t in tensors:
         if t is not None and t.device.type != "cuda":
             raise ValueError("stepquant_b200 operates on CUDA tensors only (no CPU fallback)")
+
+
+def launch(entry, args, device):
+    """Run a C entry point taking (args, stream) on ``device``'s current stream."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return check(entry(ctypes.byref(args), stream_handle()))
+    return check(entry(ctypes.byref(args), stream_handle()))
+
+
+def same_device(device, **tensors):
+    """The layer operators' operands lie on one CUDA device."""
+    require_cuda_device(device)
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name}: expected a tensor on {device}, got {t.device}")
+
+
+def require_cuda_device(device):
+    if device.type != "cuda":
+        raise ValueError("stepquant_b200 operates on CUDA tensors only (no CPU fallback)")
+
+
+def rows_of(x, name):
+    """[..., dim] -> [rows, dim] with a contiguous last axis and one row stride (copied when it has none)."""
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"{name}: unsupported dtype {x.dtype}; use float32, bfloat16 or float16")
+    if x.dim() != 2:
+        if x.dim() < 1:
+            raise ValueError(f"{name}: expected [..., dim]")
+        x = x.reshape(-1, x.shape[-1])
+    if x.stride(1) != 1 and x.shape[1] != 1:
+        x = x.contiguous()
+    return x
+
+
+def address(tensor):
+    return None if tensor is None else tensor.data_ptr()
+
+
+def aligned(x):
+    """x contiguous with a 16-byte aligned base (copied when it is not)."""
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()

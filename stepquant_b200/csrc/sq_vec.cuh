@@ -1,0 +1,63 @@
+// Typed access to eight consecutive values, shared by the layer operators
+// (norm, convolution, scan, block-scaled product).
+#pragma once
+
+#include "sq_common.cuh"
+
+namespace sq {
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+template <class T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+
+// Eight values starting at p: 16-byte accesses when `whole` (p 16-byte aligned
+// and all eight present), else the first n one by one and zeros after them.
+template <class T>
+__device__ __forceinline__ void load8(const T *p, bool whole, int n, float (&x)[8]) {
+    if (whole) {
+        constexpr int kPer = 16 / sizeof(T);
+        T v[8];
+#pragma unroll
+        for (int i = 0; i < 8 / kPer; ++i)
+            *reinterpret_cast<uint4 *>(v + i * kPer) = *reinterpret_cast<const uint4 *>(p + i * kPer);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_float(v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = i < n ? to_float(p[i]) : 0.f;
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void store8(T *p, bool whole, int n, const float (&x)[8]) {
+    if (whole) {
+        constexpr int kPer = 16 / sizeof(T);
+        T v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = from_float<T>(x[i]);
+#pragma unroll
+        for (int i = 0; i < 8 / kPer; ++i)
+            *reinterpret_cast<uint4 *>(p + i * kPer) = *reinterpret_cast<const uint4 *>(v + i * kPer);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = from_float<T>(x[i]);
+    }
+}
+
+// x sigmoid(x) with the exponential and the reciprocal of the special function
+// unit (a few units in the last place of fp32; -inf gives 0 as its limit does
+// in the quotient form x / (1 + e^-x), NaN stays NaN).
+__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
+
+inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace sq

@@ -1,0 +1,144 @@
+"""Short causal convolution of recurrent layers (csrc/sq_conv.cu).
+
+``causal_conv1d``       concatenated prompts, keyword names of
+                        ``prefill.chunk_gated_delta_rule``.
+``causal_conv1d_step``  one token of each request, the state updated in place.
+
+y[t, d] = act(bias[d] + sum_j weight[d, j] x[t - W + 1 + j, d]) with W = 2 to 4
+taps.  A state row [channels, W - 1] holds the inputs before the next token,
+oldest first, in x's dtype.  Asynchronous on the current stream.
+"""
+import torch
+
+from .. import _native as N
+
+
+def sequence_ends(cu_seqlens, tokens, device):
+    """int32 boundaries on ``device`` (default: one sequence of all tokens)."""
+    if cu_seqlens is None:
+        return torch.tensor([0, tokens], dtype=torch.int32).to(device, non_blocking=True)
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+        raise ValueError("cu_seqlens: expected [sequences + 1]")
+    return cu_seqlens.to(device=device, dtype=torch.int32).contiguous()
+
+
+def slot_rows(slots, count, device):
+    """int64 state rows of ``count`` requests, or None."""
+    if slots is None:
+        return None
+    if slots.dim() != 1 or slots.numel() != count:
+        raise ValueError(f"slots: expected [{count}]")
+    return slots.to(device=device, dtype=torch.int64).contiguous()
+
+
+def _filter(weight, bias, channels):
+    if weight.dim() == 3 and weight.shape[1] == 1:
+        weight = weight[:, 0]
+    if weight.dim() != 2 or weight.shape[0] != channels:
+        raise ValueError(f"weight: expected [{channels}, taps]")
+    if not 2 <= weight.shape[1] <= 4:
+        raise NotImplementedError("the convolution is built for 2 to 4 taps")
+    if bias is not None and tuple(bias.shape) != (channels,):
+        raise ValueError(f"bias: expected [{channels}]")
+    return weight.float().contiguous(), None if bias is None else bias.float().contiguous()
+
+
+def _activation(name):
+    if name not in (None, "silu"):
+        raise ValueError("activation: expected 'silu' or None")
+    return 1 if name == "silu" else 0
+
+
+def _state(state, rows, channels, taps, dtype, name):
+    if state.dim() != 3 or tuple(state.shape[1:]) != (channels, taps - 1) or (rows is not None and state.shape[0] != rows):
+        raise ValueError(f"{name}: expected [{'rows' if rows is None else rows}, {channels}, {taps - 1}]")
+    if state.dtype != dtype:
+        raise ValueError(f"{name}: expected dtype {dtype}, got {state.dtype}")
+    return state
+
+
+def _launch(entry, rows, y, weight, bias, initial, final, slots, cu, status, seqs, activation, device):
+    p = N.address
+    args = N.SqConvArgs(p(rows), p(weight), p(bias), p(y), p(initial), p(final), p(slots), p(cu), p(status),
+                        rows.stride(0), 0 if final is None else final.shape[0], rows.shape[0], seqs, rows.shape[1],
+                        weight.shape[1], N.dtype_code(rows.dtype), activation)
+    N.launch(entry, args, device)
+
+
+def causal_conv1d(x, weight, bias=None, *, initial_state=None, output_final_state=True, activation="silu",
+                  cu_seqlens=None):
+    """Convolution of concatenated sequences: (y, final_state).
+
+    x: [T, D] or [1, T, D] float32, bfloat16 or float16, rows any stride apart;
+    weight: [D, W] (or [D, 1, W]), bias: [D], both used in fp32; cu_seqlens:
+    [N + 1] boundaries (default: one sequence); initial_state: [N, D, W - 1] in
+    x's dtype, or None (zeros).  y has x's shape and dtype; final_state [N, D,
+    W - 1] or None when ``output_final_state`` is false.
+    """
+    shape = x.shape
+    if x.dim() == 3 and shape[0] != 1:
+        raise ValueError("x: expected a leading batch of 1 (concatenated sequences)")
+    if x.dim() not in (2, 3) or shape[-1] < 1:
+        raise ValueError("x: expected [tokens, channels]")
+    rows = N.rows_of(x, "x")
+    tokens, channels = rows.shape
+    weight, bias = _filter(weight, bias, channels)
+    activation = _activation(activation)
+    device = x.device
+    N.same_device(device, weight=weight, bias=bias, initial_state=initial_state)
+    cu = sequence_ends(cu_seqlens, tokens, device)
+    seqs, taps = cu.numel() - 1, weight.shape[1]
+    if initial_state is not None:
+        initial_state = _state(initial_state, seqs, channels, taps, x.dtype, "initial_state").contiguous()
+    final = torch.empty(seqs, channels, taps - 1, device=device, dtype=x.dtype) if output_final_state else None
+    y = torch.empty(shape, device=device, dtype=x.dtype)
+    _launch(N.lib().sq_causal_conv, rows, y, weight, bias, initial_state, final, None, cu, None, seqs, activation, device)
+    return y, final
+
+
+def causal_conv1d_extend(x, state, weight, bias=None, *, slots, cu_seqlens=None, activation="silu", status=None):
+    """``causal_conv1d`` on a pool of states [S, D, W - 1]: sequence n continues
+    from, and updates in place, row slots[n].  A slot <= 0 (padding) or outside
+    the pool (flagged in ``status``, an int32 word) gives zero outputs."""
+    rows = N.rows_of(x, "x")
+    tokens, channels = rows.shape
+    weight, bias = _filter(weight, bias, channels)
+    activation = _activation(activation)
+    device = x.device
+    N.same_device(device, weight=weight, bias=bias, state=state, status=status)
+    cu = sequence_ends(cu_seqlens, tokens, device)
+    seqs = cu.numel() - 1
+    state = _pool_state(state, channels, weight.shape[1], x.dtype)
+    y = torch.empty(x.shape, device=device, dtype=x.dtype)
+    _launch(N.lib().sq_causal_conv, rows, y, weight, bias, state, state, slot_rows(slots, seqs, device), cu, status, seqs,
+            activation, device)
+    return y
+
+
+def _pool_state(state, channels, taps, dtype):
+    _state(state, None, channels, taps, dtype, "state")
+    if not state.is_contiguous():
+        raise ValueError("state: updated in place, expected a contiguous tensor")
+    return state
+
+
+def causal_conv1d_step(x, state, weight, bias=None, *, slots=None, activation="silu", status=None):
+    """One token of each request: x [B, D] -> y [B, D]; ``state`` [S, D, W - 1]
+    (x's dtype, contiguous) is updated in place at rows ``slots`` [B] (None: row
+    i for request i, S = B).  Slots are distinct; padding and slots outside the
+    pool as in ``causal_conv1d_extend``."""
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError("x: expected [batch, channels]")
+    rows = N.rows_of(x, "x")
+    batch, channels = rows.shape
+    weight, bias = _filter(weight, bias, channels)
+    activation = _activation(activation)
+    device = x.device
+    N.same_device(device, weight=weight, bias=bias, state=state, status=status)
+    state = _pool_state(state, channels, weight.shape[1], x.dtype)
+    if slots is None and state.shape[0] != batch:
+        raise ValueError(f"state: expected {batch} rows without slots")
+    y = torch.empty(batch, channels, device=device, dtype=x.dtype)
+    _launch(N.lib().sq_causal_conv_step, rows, y, weight, bias, None, state, slot_rows(slots, batch, device), None, status,
+            batch, activation, device)
+    return y

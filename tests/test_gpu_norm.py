@@ -1,0 +1,152 @@
+"""rms_norm, rms_norm_fp8 and quantize_fp8 (csrc/sq_norm.cu) against 64-bit arithmetic.
+
+Tolerances: the mean of n squares is off by at most ~80 roundings (64 serial
+terms of a thread, then a tree), half of that after the root, plus the
+reciprocal root's two and the products': REL = 64 * 2^-24 of |y|.  Rounding is
+monotone, so an output lies between the roundings of both ends of that
+interval; e4m3 values are within half a step of theirs (2^-4 relative, 2^-10
+below 2^-6) of y / scale.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+REL = 64 * 2.0 ** -24
+
+
+def _reference(x, weight, residual, eps=1e-6):
+    h = x.double() + (0 if residual is None else residual.double())
+    return h, h / (h.square().mean(-1, keepdim=True) + eps).sqrt() * weight.double()
+
+
+def _close(got, want, dtype, rel=REL):
+    off = want.abs() * rel + 1e-40
+    inside = ((want - off).to(dtype) <= got) & (got <= (want + off).to(dtype))
+    assert bool(inside.all()), (got[~inside], want[~inside])
+
+
+def _blocks(y):
+    pad = torch.nn.functional.pad(y, (0, -y.shape[-1] % 128))
+    return pad.unflatten(-1, (-1, 128))
+
+
+def _close_fp8(q, scale, y):
+    want = _blocks(y).abs().amax(-1).clamp_min(1e-30) / 448
+    assert scale.shape == want.shape
+    assert bool(((scale.double() - want).abs() <= want * (REL + 2.0 ** -22)).all())
+    v = (_blocks(y) / want[..., None]).flatten(-2)[..., :y.shape[-1]]
+    limit = torch.clamp_min(v.abs() * 2.0 ** -4, 2.0 ** -10) + v.abs() * (2 * REL + 2.0 ** -21)
+    got = q.double()
+    assert bool(((got - v).abs() <= limit).all()), float(((got - v).abs() / limit).max())
+
+
+def _data(rows, hidden, dtype, seed=0):
+    gen = torch.Generator("cuda").manual_seed(seed)
+    rand = lambda *s: torch.randn(*s, generator=gen, device="cuda")  # noqa: E731
+    x = (rand(rows, hidden) * torch.where(rand(hidden).abs() > 2.5, 30.0, 1.0)).to(dtype)
+    return x, (rand(rows, hidden) * 3).to(dtype), (1 + 0.2 * rand(hidden)).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,hidden", [(1, 1), (3, 7), (2, 8), (5, 127), (9, 128), (17, 129), (8, 256), (33, 512), (4, 520),
+                                         (1, 5120), (3, 4100), (700, 1000), (601, 2056), (2, 8200), (600, 9001), (2, 65536)])
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_norm(rows, hidden, dtype, with_residual):
+    from stepquant_b200.kernels.norm import rms_norm, rms_norm_fp8
+    x, residual, weight = _data(rows, hidden, dtype)
+    residual = residual if with_residual else None
+    h, y = _reference(x, weight, residual)
+    got = rms_norm(x, weight, residual)
+    got8 = rms_norm_fp8(x, weight, residual)
+    if with_residual:
+        assert torch.equal(got[1], h.to(dtype) if dtype != torch.float32 else x + residual)
+        assert torch.equal(got8[2], got[1])
+    _close(got[0] if with_residual else got, y, dtype)
+    assert got8[0].dtype == torch.float8_e4m3fn and got8[0].shape == x.shape
+    _close_fp8(got8[0], got8[1], y)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,hidden", [(1, 1), (7, 130), (3, 4096), (640, 5120)])
+def test_quantize(rows, hidden, dtype):
+    from stepquant_b200.kernels.norm import quantize_fp8
+    x, _, _ = _data(rows, hidden, dtype, 1)
+    q, scale = quantize_fp8(x)
+    _close_fp8(q, scale, x.double())
+
+
+def test_weight_types_strides_and_batches():
+    """fp32 weights with bf16 rows; rows of a wider tensor, 16-byte aligned or
+    not; columns of a transposed one; more than two axes; a repeated row."""
+    from stepquant_b200.kernels.norm import rms_norm, rms_norm_fp8
+    x, residual, weight = _data(24, 1032, torch.bfloat16, 2)
+    wide = torch.randn(24, 2 * 1032 + 3, device="cuda").bfloat16()
+    for view in (wide[:, :1032], wide[:, 1032:2064], wide[:, 3:1035], torch.randn(1032, 24, device="cuda").bfloat16().T,
+                 x[:1].expand(24, -1)):
+        h, y = _reference(view, weight, residual)
+        out, total = rms_norm(view, weight.float(), residual)
+        _close(out, y, torch.bfloat16)
+        assert torch.equal(total, h.bfloat16())
+        q, scale, _ = rms_norm_fp8(view, weight.half().float(), residual)
+        _close_fp8(q, scale, _reference(view, weight.half(), residual)[1])
+    out = rms_norm(x.view(2, 3, 4, 1032), weight)
+    assert out.shape == (2, 3, 4, 1032)
+    _close(out.view(24, 1032), _reference(x, weight, None)[1], torch.bfloat16)
+    q, scale = rms_norm_fp8(x.view(2, 12, 1032), weight)
+    assert q.shape == (2, 12, 1032) and scale.shape == (2, 12, 9)
+
+
+def test_extremes():
+    """Zero rows, rows of the type's largest and smallest values, NaN and
+    infinity: each row by itself, no other row touched."""
+    from stepquant_b200.kernels.norm import quantize_fp8, rms_norm, rms_norm_fp8
+    x, _, weight = _data(8, 640, torch.bfloat16, 3)
+    x[1] = 0
+    x[2] = 1e-30
+    x[3] = 1e15
+    x[4, 100] = float("nan")
+    x[5, 639] = float("inf")
+    y = rms_norm(x, weight)
+    q, scale = rms_norm_fp8(x, weight)
+    assert bool((y[1] == 0).all()) and bool((q[1].float() == 0).all()) and bool((scale[1] == torch.tensor(1e-30) / 448).all())
+    assert bool(y[4].isnan().all()) and bool(q[4].float().isnan().all()) and bool(scale[4].isnan().all())
+    assert bool(y[5, 639].isnan()) and bool(q[5, 639].float().isnan())
+    for row in (0, 2, 3, 6, 7):
+        _close(y[row:row + 1], _reference(x[row:row + 1], weight, None)[1], torch.bfloat16)
+        _close_fp8(q[row:row + 1], scale[row:row + 1], _reference(x[row:row + 1], weight, None)[1])
+    q, scale = quantize_fp8(x)
+    assert bool(scale[4, 0].isnan()) and bool(scale[4, 1:].isfinite().all())
+    assert bool(scale[5, 4].isinf()) and bool((q[5, 512:639].float() == 0).all())
+
+
+def test_empty_and_refusals():
+    from stepquant_b200.kernels.norm import rms_norm, rms_norm_fp8
+    w = torch.ones(64, device="cuda")
+    assert rms_norm(torch.empty(0, 64, device="cuda"), w).shape == (0, 64)
+    assert rms_norm_fp8(torch.empty(0, 64, device="cuda"), w)[1].shape == (0, 1)
+    with pytest.raises(ValueError):
+        rms_norm(torch.ones(2, 64, device="cuda"), w.cpu())
+    with pytest.raises(NotImplementedError):
+        rms_norm(torch.ones(1, 65537, device="cuda"), torch.ones(65537, device="cuda"))
+
+
+def test_other_stream_and_graph():
+    """On a stream of the caller's, and replayed from a graph on new inputs."""
+    from stepquant_b200.kernels.norm import rms_norm_fp8
+    x, residual, weight = _data(16, 512, torch.bfloat16, 4)
+    want = [t.float() for t in rms_norm_fp8(x, weight, residual)]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = rms_norm_fp8(x, weight, residual)
+    side.synchronize()
+    assert all(torch.equal(g.float(), w) for g, w in zip(got, want))
+    still = torch.zeros_like(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = rms_norm_fp8(still, weight, residual)
+    still.copy_(x)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(g.float(), w) for g, w in zip(out, want))
