@@ -370,6 +370,35 @@ typedef struct sq_norm_args {
 int32_t sq_rms_norm(const sq_norm_args *args, sq_stream_t stream);
 
 /*
+ * Product of e4m3 matrices with block scales:
+ *   out[m, n] = residual[m, n] + sum_k (x[m, k] x_scale[m, k / 128]) (w[n, k] w_scale[n / 128, k / 128])
+ *   x        [rows, hidden] e4m3, rows x_stride bytes apart; w [width, hidden], w_stride
+ *   x_scale  [rows, ceil(hidden / 128)] fp32, w_scale [ceil(width / 128), ceil(hidden / 128)] fp32, contiguous
+ *   residual [rows, width] in dtype, rows residual_stride elements apart, or NULL
+ *   out      [rows, width] in dtype, contiguous; rounded once (may be residual's own contiguous buffer)
+ * hidden a multiple of 16; x, w 16-byte aligned, strides multiples of 16 and
+ * at least hidden.  status: SQ_STATUS_TIMEOUT if a bounded device wait gave up.
+ */
+typedef struct sq_matmul_args {
+    const void *x;
+    const float *x_scale;
+    const void *w;
+    const float *w_scale;
+    const void *residual;
+    void *out;
+    int32_t *status;
+    int64_t x_stride;
+    int64_t w_stride;
+    int64_t residual_stride;
+    int32_t rows;
+    int32_t width;
+    int32_t hidden;
+    int32_t dtype;
+} sq_matmul_args;
+
+int32_t sq_matmul_fp8(const sq_matmul_args *args, sq_stream_t stream);
+
+/*
  * Causal convolution of `taps` (2 to 4) inputs a channel over concatenated
  * sequences: y_t = act(bias + sum_j weight[:, j] x_{t - taps + 1 + j}), act =
  * SiLU or the identity.  Sequence n owns tokens [cu_seqlens[n],

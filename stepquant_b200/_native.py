@@ -51,6 +51,12 @@ class SqNormArgs(ctypes.Structure):
                 ("weight_dtype", _i32), ("normalize", _i32), ("eps", ctypes.c_float)]
 
 
+class SqMatmulArgs(ctypes.Structure):
+    _fields_ = [("x", _p), ("x_scale", _p), ("w", _p), ("w_scale", _p), ("residual", _p), ("out", _p), ("status", _p),
+                ("x_stride", _i64), ("w_stride", _i64), ("residual_stride", _i64), ("rows", _i32), ("width", _i32),
+                ("hidden", _i32), ("dtype", _i32)]
+
+
 class SqConvArgs(ctypes.Structure):
     _fields_ = [("x", _p), ("weight", _p), ("bias", _p), ("y", _p), ("initial_state", _p), ("final_state", _p),
                 ("slots", _p), ("cu_seqlens", _p), ("status", _p), ("x_stride", _i64), ("num_slots", _i64),
@@ -90,6 +96,7 @@ _SIGNATURES = {
     "sq_gdn_prefill_workspace_bytes": (_i64, [_i32, _i32, _i32]),
     "sq_kda_prefill": (_i32, [_p, _p]),
     "sq_rms_norm": (_i32, [_p, _p]),
+    "sq_matmul_fp8": (_i32, [_p, _p]),
     "sq_causal_conv": (_i32, [_p, _p]),
     "sq_causal_conv_step": (_i32, [_p, _p]),
     "sq_selective_scan": (_i32, [_p, _p]),

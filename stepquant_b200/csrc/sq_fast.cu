@@ -1355,6 +1355,16 @@ cudaError_t launch_fast_mode(const TileParams &p, int items, cudaStream_t stream
 
 }  // namespace
 
+// SMs that kernels launched on `stream` can run on, for the other persistent
+// kernels of the library; 0 when the device cannot be asked.
+int sms_of(cudaStream_t stream) {
+    int device = 0, sms = 0;
+    if (cudaGetDevice(&device) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+        return 0;
+    return stream_sms(stream, sms);
+}
+
 bool fast_eligible(const sq_plan &plan, const void *pages) {
     return plan.architecture == SQ_GDN && plan.storage == 0 && plan.keys == FK && plan.values == FV &&
            plan.heads <= kMaxHeads &&

@@ -14,6 +14,7 @@ from .. import _native as N
 
 FP8 = torch.float8_e4m3fn
 BLOCK = 128  # channels of a scale
+E4M3_MAX, SCALE_FLOOR = 448.0, 1e-30  # as in csrc/sq_norm.cu
 
 
 def _run(x, weight, residual, eps, fp8):
