@@ -5,6 +5,7 @@ fallback: if the library is missing every device operation raises.
 """
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -167,25 +168,51 @@ def require_cuda(*tensors):
             raise ValueError("stepquant_b200 operates on CUDA tensors only (no CPU fallback)")
 
 
-def launch(entry, args, device):
-    """Run a C entry point taking (args, stream) on ``device``'s current stream."""
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return check(entry(ctypes.byref(args), stream_handle()))
-    return check(entry(ctypes.byref(args), stream_handle()))
+# ---------------------------------------------------------------------------
+# the layer operators' calls (kernels/norm.py, matmul.py, conv.py, scan.py)
+# ---------------------------------------------------------------------------
+_FORMATS = {_p: "P", _i64: "q", _i32: "i", ctypes.c_float: "f"}
 
 
-def same_device(device, **tensors):
-    """The layer operators' operands lie on one CUDA device."""
-    require_cuda_device(device)
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name}: expected a tensor on {device}, got {t.device}")
+def packer(arguments):
+    """Function of a ctypes Structure's fields, in order, that returns its
+    bytes: a few microseconds less than building the Structure, on calls whose
+    kernels take about as long."""
+    fmt = struct.Struct("@" + "".join(_FORMATS[kind] for _, kind in arguments._fields_) + "0P")
+    assert fmt.size == ctypes.sizeof(arguments)
+    return fmt.pack
 
 
-def require_cuda_device(device):
-    if device.type != "cuda":
-        raise ValueError("stepquant_b200 operates on CUDA tensors only (no CPU fallback)")
+def launch(entry, packed, index):
+    """Run a C entry point of (arguments, stream) on the current stream of device ``index``."""
+    if index == torch._C._cuda_getDevice():
+        code = entry(packed, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            code = entry(packed, torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        check(code)
+
+
+def device_index(first, *others):
+    """Index of the CUDA device that ``first`` and the others (or None) lie on."""
+    index = first.get_device()
+    if index < 0:
+        require_cuda(first)
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"expected every tensor on {first.device}, got one on {t.device}")
+    return index
+
+
+def address(tensor):
+    return 0 if tensor is None else tensor.data_ptr()
+
+
+def aligned(x):
+    """x contiguous with a 16-byte aligned base (copied when it is not)."""
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
 def rows_of(x, name):
@@ -199,13 +226,3 @@ def rows_of(x, name):
     if x.stride(1) != 1 and x.shape[1] != 1:
         x = x.contiguous()
     return x
-
-
-def address(tensor):
-    return None if tensor is None else tensor.data_ptr()
-
-
-def aligned(x):
-    """x contiguous with a 16-byte aligned base (copied when it is not)."""
-    x = x.contiguous()
-    return x if x.data_ptr() % 16 == 0 else x.clone()

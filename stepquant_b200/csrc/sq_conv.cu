@@ -9,8 +9,12 @@
 // state are rounded to, or copied in, the input's type.
 //
 // Bound by bytes: x read once, y written once, the W - 1 inputs before a token
-// kept in registers.  A thread takes eight channels (16 bytes of a 16-bit row)
-// and walks a strip of tokens; strips overlap by their W - 1 leading inputs.
+// kept in registers.  A thread takes four channels (8 bytes of a 16-bit row)
+// and walks a strip of tokens, eight tokens in flight while the eight before are
+// worked on; strips overlap by their W - 1 leading inputs.
+#include <type_traits>
+
+#include "sq_rows.cuh"
 #include "sq_vec.cuh"
 
 namespace sq {
@@ -18,111 +22,130 @@ namespace {
 
 constexpr int kConvThreads = 128;
 
-// Strip `index` of the concatenated sequences: sequence n owns the indices from
-// cu[n] / strip + n on, at least as many as its strips, so a strip finds its
-// sequence by bisection and strip 0 exists for an empty sequence too.
-__device__ __forceinline__ int find_sequence(const int32_t *cu, int seqs, int tokens, int strip, int64_t index) {
-    int lo = 0, hi = seqs - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (max(0, min(cu[mid], tokens)) / strip + int64_t(mid) <= index) lo = mid;
-        else hi = mid - 1;
+// N values of VEC channels (a token's, or a state row's), by 8- or 16-byte accesses for four channels.
+template <class T, int N, int VEC>
+struct Run {
+    static constexpr int kPiece = VEC * sizeof(T) < 16 ? VEC * sizeof(T) : 16;
+    using Piece = std::conditional_t<kPiece == 16, uint4, uint2>;
+    alignas(16) T v[N];
+    __device__ __forceinline__ void load(const T *p) {
+        if (VEC > 1) {
+#pragma unroll
+            for (int i = 0; i < int(N * sizeof(T) / kPiece); ++i) reinterpret_cast<Piece *>(v)[i] = reinterpret_cast<const Piece *>(p)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = p[i];
+        }
     }
-    return lo;
-}
-
-// State row of request n: n itself, or slots[n].  -1: a padded request (slot
-// <= 0) or, flagged in status, a slot outside the pool.
-__device__ __forceinline__ int64_t state_row(const int64_t *slots, int n, int64_t num_slots, int32_t *status) {
-    if (!slots) return n;
-    const int64_t slot = slots[n];
-    if (slot >= num_slots) {
-        flag(status, SQ_STATUS_SLOT_RANGE);
-        return -1;
+    __device__ __forceinline__ void store(T *p) const {
+        if (VEC > 1) {
+#pragma unroll
+            for (int i = 0; i < int(N * sizeof(T) / kPiece); ++i) reinterpret_cast<Piece *>(p)[i] = reinterpret_cast<const Piece *>(v)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) p[i] = v[i];
+        }
     }
-    return slot <= 0 ? -1 : slot;
-}
+};
 
-template <class T, int VEC>
-__device__ __forceinline__ void load_vec(const T *p, float (&x)[VEC]) {
-    if (VEC == 8) load8(p, true, 8, *reinterpret_cast<float(*)[8]>(&x));
-    else x[0] = to_float(*p);
-}
-
-template <class T, int VEC>
-__device__ __forceinline__ void store_vec(T *p, const float (&x)[VEC]) {
-    if (VEC == 8) store8(p, true, 8, *reinterpret_cast<const float(*)[8]>(&x));
-    else *p = from_float<T>(x[0]);
-}
+// bias and weights of VEC channels, [channel][tap].
+template <int VEC, int W>
+struct Filter {
+    float w[VEC * W], bias[VEC];
+    __device__ __forceinline__ Filter(const sq_conv_args &a, int d0) {
+        Run<float, VEC * W, VEC> r;
+        r.load(a.weight + int64_t(d0) * W);
+        Run<float, VEC, VEC> s;
+        if (a.bias) s.load(a.bias + d0);
+#pragma unroll
+        for (int i = 0; i < VEC * W; ++i) w[i] = r.v[i];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) bias[i] = a.bias ? s.v[i] : 0.f;
+    }
+};
 
 template <class T, int VEC, int W>
 __global__ void __launch_bounds__(kConvThreads) conv_kernel(sq_conv_args a, int strip) {
+    using Token = Run<T, VEC, VEC>;
+    constexpr int BATCH = 8;  // tokens in flight a thread, while the batch before is worked on
     const int d0 = (blockIdx.y * kConvThreads + threadIdx.x) * VEC;
     if (d0 >= a.channels) return;
-    const int n = find_sequence(a.cu_seqlens, a.num_seqs, a.tokens, strip, blockIdx.x);
-    const int begin = max(0, min(a.cu_seqlens[n], a.tokens));
-    const int end = max(begin, min(a.cu_seqlens[n + 1], a.tokens));
+    const int n = sequence_of(a.cu_seqlens, a.num_seqs, a.tokens, strip, blockIdx.x);
+    const int2 seq = sequence_range(a.cu_seqlens, n, a.tokens);
+    const int begin = seq.x, end = seq.y;
     const int64_t part = blockIdx.x - (begin / strip + int64_t(n));  // strip of the sequence
     if (part < 0 || (part > 0 && part * strip >= end - begin)) return;
     const int t0 = begin + int(part) * strip, t1 = min(end, t0 + strip);
     const int64_t row = state_row(a.slots, n, a.num_slots, a.status);
     T *y = static_cast<T *>(a.y) + d0;
-    float zero[VEC] = {};
     if (row < 0) {
-        for (int t = t0; t < t1; ++t) store_vec<T, VEC>(y + int64_t(t) * a.channels, zero);
+        Token zero;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) zero.v[i] = from_float<T>(0.f);
+        for (int t = t0; t < t1; ++t) zero.store(y + int64_t(t) * a.channels);
         return;
     }
     const T *x = static_cast<const T *>(a.x) + d0;
-    const T *old = a.initial_state ? static_cast<const T *>(a.initial_state) + (row * a.channels + d0) * (W - 1) : nullptr;
-    float w[VEC][W], bias[VEC], kept[W - 1][VEC];  // kept[j]: input W - 1 - j tokens back
+    const int64_t state = (row * a.channels + d0) * (W - 1);
+    const T *old = a.initial_state ? static_cast<const T *>(a.initial_state) + state : nullptr;
+    Token next[BATCH], now[BATCH];
+    auto fetch = [&](int t) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-        bias[i] = a.bias ? a.bias[d0 + i] : 0.f;
-#pragma unroll
-        for (int j = 0; j < W; ++j) w[i][j] = a.weight[int64_t(d0 + i) * W + j];
-    }
+        for (int j = 0; j < BATCH; ++j)
+            if (t + j < t1) next[j].load(x + int64_t(t + j) * a.x_stride);
+    };
+    fetch(t0);
+    const Filter<VEC, W> f(a, d0);
     // Input of token t of the sequence, t < begin from the state.
-    auto input = [&](int64_t t, float(&v)[VEC]) {
+    auto input = [&](int64_t t, Token &v) {
         if (t >= begin) {
-            load_vec<T, VEC>(x + t * a.x_stride, v);
+            v.load(x + t * a.x_stride);
         } else {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) v[i] = old ? to_float(old[i * (W - 1) + int(t - begin) + W - 1]) : 0.f;
+            for (int i = 0; i < VEC; ++i) v.v[i] = old ? old[i * (W - 1) + int(t - begin) + W - 1] : from_float<T>(0.f);
         }
     };
+    float kept[W - 1][VEC];  // kept[j]: input W - 1 - j tokens back
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) input(int64_t(t0) - (W - 1) + j, kept[j]);
-    float last[W - 1][VEC];
-    if (part == 0 && a.final_state) {  // read before any write: the two states may be one buffer
+    for (int j = 0; j < W - 1; ++j) {
+        Token v;
+        input(int64_t(t0) - (W - 1) + j, v);
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) input(int64_t(end) - (W - 1) + j, last[j]);
+        for (int i = 0; i < VEC; ++i) kept[j][i] = to_float(v.v[i]);
     }
-#pragma unroll 4
-    for (int t = t0; t < t1; ++t) {
-        float now[VEC], out[VEC];
-        load_vec<T, VEC>(x + int64_t(t) * a.x_stride, now);
+    if (part == 0 && a.final_state) {  // the strip that reads the state writes it, after reading: they may be one buffer
+        Run<T, VEC * (W - 1), VEC> fin;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            float s = bias[i];
+        for (int j = 0; j < W - 1; ++j) {
+            Token v;
+            input(int64_t(end) - (W - 1) + j, v);
 #pragma unroll
-            for (int j = 0; j < W - 1; ++j) s = fmaf(w[i][j], kept[j][i], s);
-            s = fmaf(w[i][W - 1], now[i], s);
-            out[i] = a.silu ? silu(s) : s;
+            for (int i = 0; i < VEC; ++i) fin.v[i * (W - 1) + j] = v.v[i];
         }
-        store_vec<T, VEC>(y + int64_t(t) * a.channels, out);
-#pragma unroll
-        for (int j = 0; j + 1 < W - 1; ++j)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) kept[j][i] = kept[j + 1][i];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) kept[W - 2][i] = now[i];
+        fin.store(static_cast<T *>(a.final_state) + state);
     }
-    if (part == 0 && a.final_state) {
-        T *fin = static_cast<T *>(a.final_state) + (row * a.channels + d0) * (W - 1);
+    for (int t = t0; t < t1; t += BATCH) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i)
+        for (int j = 0; j < BATCH; ++j) now[j] = next[j];
+        fetch(t + BATCH);
 #pragma unroll
-            for (int j = 0; j < W - 1; ++j) fin[i * (W - 1) + j] = from_float<T>(last[j][i]);
+        for (int j = 0; j < BATCH; ++j) {
+            if (t + j >= t1) break;
+            Token out;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const float in = to_float(now[j].v[i]);
+                float s = f.bias[i];
+#pragma unroll
+                for (int k = 0; k < W - 1; ++k) s = fmaf(f.w[i * W + k], kept[k][i], s);
+                s = fmaf(f.w[i * W + W - 1], in, s);
+                out.v[i] = from_float<T>(a.silu ? silu(s) : s);
+#pragma unroll
+                for (int k = 0; k + 1 < W - 1; ++k) kept[k][i] = kept[k + 1][i];
+                kept[W - 2][i] = in;
+            }
+            out.store(y + int64_t(t + j) * a.channels);
+        }
     }
 }
 
@@ -133,30 +156,32 @@ __global__ void __launch_bounds__(kConvThreads) conv_step_kernel(sq_conv_args a)
     if (d0 >= a.channels) return;
     const int n = blockIdx.x;
     const int64_t row = state_row(a.slots, n, a.num_slots, a.status);
+    Run<T, VEC, VEC> in, out;
     T *y = static_cast<T *>(a.y) + int64_t(n) * a.channels + d0;
-    float now[VEC], out[VEC] = {};
     if (row < 0) {
-        store_vec<T, VEC>(y, out);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) out.v[i] = from_float<T>(0.f);
+        out.store(y);
         return;
     }
     T *state = static_cast<T *>(a.final_state) + (row * a.channels + d0) * (W - 1);
-    load_vec<T, VEC>(static_cast<const T *>(a.x) + int64_t(n) * a.x_stride + d0, now);
-    T kept[VEC * (W - 1)];
-#pragma unroll
-    for (int i = 0; i < VEC * (W - 1); ++i) kept[i] = state[i];
+    Run<T, VEC * (W - 1), VEC> kept;
+    in.load(static_cast<const T *>(a.x) + int64_t(n) * a.x_stride + d0);
+    kept.load(state);
+    const Filter<VEC, W> f(a, d0);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-        float s = a.bias ? a.bias[d0 + i] : 0.f;
+        float s = f.bias[i];
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) s = fmaf(a.weight[int64_t(d0 + i) * W + j], to_float(kept[i * (W - 1) + j]), s);
-        s = fmaf(a.weight[int64_t(d0 + i) * W + W - 1], now[i], s);
-        out[i] = a.silu ? silu(s) : s;
+        for (int j = 0; j < W - 1; ++j) s = fmaf(f.w[i * W + j], to_float(kept.v[i * (W - 1) + j]), s);
+        s = fmaf(f.w[i * W + W - 1], to_float(in.v[i]), s);
+        out.v[i] = from_float<T>(a.silu ? silu(s) : s);
+#pragma unroll
+        for (int j = 0; j + 1 < W - 1; ++j) kept.v[i * (W - 1) + j] = kept.v[i * (W - 1) + j + 1];
+        kept.v[i * (W - 1) + W - 2] = in.v[i];
     }
-    store_vec<T, VEC>(y, out);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i)
-#pragma unroll
-        for (int j = 0; j < W - 1; ++j) state[i * (W - 1) + j] = j + 1 < W - 1 ? kept[i * (W - 1) + j + 1] : from_float<T>(now[i]);
+    out.store(y);
+    kept.store(state);
 }
 
 template <class T, int VEC, int W>
@@ -175,12 +200,14 @@ cudaError_t launch_conv_as(const sq_conv_args &a, bool step, cudaStream_t s) {
 
 template <class T>
 cudaError_t launch_conv(const sq_conv_args &a, bool step, cudaStream_t s) {
-    const bool vec = a.channels % 8 == 0 && aligned16(a.x) && aligned16(a.y) && a.x_stride * int64_t(sizeof(T)) % 16 == 0 &&
-                     a.channels * int64_t(sizeof(T)) % 16 == 0;
+    const int64_t four = 4 * sizeof(T);
+    auto fits = [&](const void *p) { return reinterpret_cast<uintptr_t>(p) % four == 0; };
+    const bool vec = a.channels % 4 == 0 && a.x_stride % 4 == 0 && fits(a.x) && fits(a.y) && fits(a.initial_state) &&
+                     fits(a.final_state) && aligned16(a.weight) && aligned16(a.bias);
     switch (a.taps) {
-        case 2: return vec ? launch_conv_as<T, 8, 2>(a, step, s) : launch_conv_as<T, 1, 2>(a, step, s);
-        case 3: return vec ? launch_conv_as<T, 8, 3>(a, step, s) : launch_conv_as<T, 1, 3>(a, step, s);
-        default: return vec ? launch_conv_as<T, 8, 4>(a, step, s) : launch_conv_as<T, 1, 4>(a, step, s);
+        case 2: return vec ? launch_conv_as<T, 4, 2>(a, step, s) : launch_conv_as<T, 1, 2>(a, step, s);
+        case 3: return vec ? launch_conv_as<T, 4, 3>(a, step, s) : launch_conv_as<T, 1, 3>(a, step, s);
+        default: return vec ? launch_conv_as<T, 4, 4>(a, step, s) : launch_conv_as<T, 1, 4>(a, step, s);
     }
 }
 

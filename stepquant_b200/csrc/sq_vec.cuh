@@ -24,7 +24,7 @@ template <class T>
 __device__ __forceinline__ void load8(const T *p, bool whole, int n, float (&x)[8]) {
     if (whole) {
         constexpr int kPer = 16 / sizeof(T);
-        T v[8];
+        alignas(16) T v[8];
 #pragma unroll
         for (int i = 0; i < 8 / kPer; ++i)
             *reinterpret_cast<uint4 *>(v + i * kPer) = *reinterpret_cast<const uint4 *>(p + i * kPer);
@@ -40,7 +40,7 @@ template <class T>
 __device__ __forceinline__ void store8(T *p, bool whole, int n, const float (&x)[8]) {
     if (whole) {
         constexpr int kPer = 16 / sizeof(T);
-        T v[8];
+        alignas(16) T v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = from_float<T>(x[i]);
 #pragma unroll

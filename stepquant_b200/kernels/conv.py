@@ -12,6 +12,8 @@ import torch
 
 from .. import _native as N
 
+_pack = N.packer(N.SqConvArgs)
+
 
 def sequence_ends(cu_seqlens, tokens, device):
     """int32 boundaries on ``device`` (default: one sequence of all tokens)."""
@@ -19,6 +21,8 @@ def sequence_ends(cu_seqlens, tokens, device):
         return torch.tensor([0, tokens], dtype=torch.int32).to(device, non_blocking=True)
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
         raise ValueError("cu_seqlens: expected [sequences + 1]")
+    if cu_seqlens.dtype == torch.int32 and cu_seqlens.device == device and cu_seqlens.is_contiguous():
+        return cu_seqlens
     return cu_seqlens.to(device=device, dtype=torch.int32).contiguous()
 
 
@@ -26,9 +30,9 @@ def slot_rows(slots, count, device):
     """int64 state rows of ``count`` requests, or None."""
     if slots is None:
         return None
-    if slots.dim() != 1 or slots.numel() != count:
+    if slots.shape != (count,):
         raise ValueError(f"slots: expected [{count}]")
-    return slots.to(device=device, dtype=torch.int64).contiguous()
+    return slots if slots.dtype == torch.int64 and slots.device == device and slots.stride(0) == 1 else slots.to(device=device, dtype=torch.int64).contiguous()
 
 
 def _filter(weight, bias, channels):
@@ -38,7 +42,7 @@ def _filter(weight, bias, channels):
         raise ValueError(f"weight: expected [{channels}, taps]")
     if not 2 <= weight.shape[1] <= 4:
         raise NotImplementedError("the convolution is built for 2 to 4 taps")
-    if bias is not None and tuple(bias.shape) != (channels,):
+    if bias is not None and bias.shape != (channels,):
         raise ValueError(f"bias: expected [{channels}]")
     return weight.float().contiguous(), None if bias is None else bias.float().contiguous()
 
@@ -50,19 +54,18 @@ def _activation(name):
 
 
 def _state(state, rows, channels, taps, dtype, name):
-    if state.dim() != 3 or tuple(state.shape[1:]) != (channels, taps - 1) or (rows is not None and state.shape[0] != rows):
+    if state.dim() != 3 or state.shape[1:] != (channels, taps - 1) or (rows is not None and state.shape[0] != rows):
         raise ValueError(f"{name}: expected [{'rows' if rows is None else rows}, {channels}, {taps - 1}]")
     if state.dtype != dtype:
         raise ValueError(f"{name}: expected dtype {dtype}, got {state.dtype}")
     return state
 
 
-def _launch(entry, rows, y, weight, bias, initial, final, slots, cu, status, seqs, activation, device):
+def _launch(entry, rows, y, weight, bias, initial, final, slots, cu, status, seqs, activation, index):
     p = N.address
-    args = N.SqConvArgs(p(rows), p(weight), p(bias), p(y), p(initial), p(final), p(slots), p(cu), p(status),
-                        rows.stride(0), 0 if final is None else final.shape[0], rows.shape[0], seqs, rows.shape[1],
-                        weight.shape[1], N.dtype_code(rows.dtype), activation)
-    N.launch(entry, args, device)
+    N.launch(entry, _pack(p(rows), p(weight), p(bias), p(y), p(initial), p(final), p(slots), p(cu), p(status),
+                          rows.stride(0), 0 if final is None else final.shape[0], rows.shape[0], seqs, rows.shape[1],
+                          weight.shape[1], N.dtype_code(rows.dtype), activation), index)
 
 
 def causal_conv1d(x, weight, bias=None, *, initial_state=None, output_final_state=True, activation="silu",
@@ -84,15 +87,14 @@ def causal_conv1d(x, weight, bias=None, *, initial_state=None, output_final_stat
     tokens, channels = rows.shape
     weight, bias = _filter(weight, bias, channels)
     activation = _activation(activation)
-    device = x.device
-    N.same_device(device, weight=weight, bias=bias, initial_state=initial_state)
-    cu = sequence_ends(cu_seqlens, tokens, device)
+    index = N.device_index(x, weight, bias, initial_state)
+    cu = sequence_ends(cu_seqlens, tokens, x.device)
     seqs, taps = cu.numel() - 1, weight.shape[1]
     if initial_state is not None:
         initial_state = _state(initial_state, seqs, channels, taps, x.dtype, "initial_state").contiguous()
-    final = torch.empty(seqs, channels, taps - 1, device=device, dtype=x.dtype) if output_final_state else None
-    y = torch.empty(shape, device=device, dtype=x.dtype)
-    _launch(N.lib().sq_causal_conv, rows, y, weight, bias, initial_state, final, None, cu, None, seqs, activation, device)
+    final = x.new_empty((seqs, channels, taps - 1)) if output_final_state else None
+    y = x.new_empty(shape)
+    _launch(N.lib().sq_causal_conv, rows, y, weight, bias, initial_state, final, None, cu, None, seqs, activation, index)
     return y, final
 
 
@@ -104,14 +106,13 @@ def causal_conv1d_extend(x, state, weight, bias=None, *, slots, cu_seqlens=None,
     tokens, channels = rows.shape
     weight, bias = _filter(weight, bias, channels)
     activation = _activation(activation)
-    device = x.device
-    N.same_device(device, weight=weight, bias=bias, state=state, status=status)
-    cu = sequence_ends(cu_seqlens, tokens, device)
+    index = N.device_index(x, weight, bias, state, status)
+    cu = sequence_ends(cu_seqlens, tokens, x.device)
     seqs = cu.numel() - 1
     state = _pool_state(state, channels, weight.shape[1], x.dtype)
-    y = torch.empty(x.shape, device=device, dtype=x.dtype)
-    _launch(N.lib().sq_causal_conv, rows, y, weight, bias, state, state, slot_rows(slots, seqs, device), cu, status, seqs,
-            activation, device)
+    y = x.new_empty(x.shape)
+    _launch(N.lib().sq_causal_conv, rows, y, weight, bias, state, state, slot_rows(slots, seqs, x.device), cu, status, seqs,
+            activation, index)
     return y
 
 
@@ -133,12 +134,11 @@ def causal_conv1d_step(x, state, weight, bias=None, *, slots=None, activation="s
     batch, channels = rows.shape
     weight, bias = _filter(weight, bias, channels)
     activation = _activation(activation)
-    device = x.device
-    N.same_device(device, weight=weight, bias=bias, state=state, status=status)
+    index = N.device_index(x, weight, bias, state, status)
     state = _pool_state(state, channels, weight.shape[1], x.dtype)
     if slots is None and state.shape[0] != batch:
         raise ValueError(f"state: expected {batch} rows without slots")
-    y = torch.empty(batch, channels, device=device, dtype=x.dtype)
-    _launch(N.lib().sq_causal_conv_step, rows, y, weight, bias, None, state, slot_rows(slots, batch, device), None, status,
-            batch, activation, device)
+    y = x.new_empty((batch, channels))
+    _launch(N.lib().sq_causal_conv_step, rows, y, weight, bias, None, state, slot_rows(slots, batch, x.device), None, status,
+            batch, activation, index)
     return y

@@ -12,6 +12,8 @@ import torch
 from .. import _native as N
 from .norm import BLOCK, FP8, SCALE_FLOOR, E4M3_MAX
 
+_pack = N.packer(N.SqMatmulArgs)
+
 
 def quantize_weight_fp8(weight):
     """(w, scale) of weight [N, K]: float8_e4m3fn [N, K] and float32
@@ -38,7 +40,7 @@ def _operand(x, name):
 
 
 def _scales(scale, shape, name):
-    if scale.dtype != torch.float32 or tuple(scale.shape) != shape:
+    if scale.dtype != torch.float32 or scale.shape != shape:
         raise ValueError(f"{name}: expected float32 {list(shape)}, got {scale.dtype} {list(scale.shape)}")
     return scale.contiguous()
 
@@ -60,22 +62,21 @@ def matmul_fp8(x, x_scale, weight, weight_scale, *, residual=None, out_dtype=tor
     if hidden % 16:
         raise NotImplementedError("the product is built for a hidden size that is a multiple of 16")
     dtype = N.dtype_code(out_dtype)
-    device = x.device
-    N.same_device(device, weight=weight, x_scale=x_scale, weight_scale=weight_scale, residual=residual, status=status)
-    blocks = -(-hidden // BLOCK)
+    index = N.device_index(x, weight, x_scale, weight_scale, residual, status)
+    blocks = (hidden + BLOCK - 1) // BLOCK
     rows = _operand(x if x.dim() == 2 else x.reshape(-1, hidden), "x")
     weight = _operand(weight, "weight")
     x_scale = _scales(x_scale, (*lead, blocks), "x_scale")
-    weight_scale = _scales(weight_scale, (-(-width // BLOCK), blocks), "weight_scale")
+    weight_scale = _scales(weight_scale, ((width + BLOCK - 1) // BLOCK, blocks), "weight_scale")
     if residual is not None:
-        if tuple(residual.shape) != (*lead, width) or residual.dtype != out_dtype:
+        if residual.shape != (*lead, width) or residual.dtype != out_dtype:
             raise ValueError(f"residual: expected {out_dtype} {[*lead, width]}")
         residual = N.rows_of(residual, "residual")
-    out = torch.empty(*lead, width, device=device, dtype=out_dtype)
-    p = N.address
+    out = x_scale.new_empty((*lead, width), dtype=out_dtype)
     count = rows.shape[0]
-    args = N.SqMatmulArgs(p(rows), p(x_scale), p(weight), p(weight_scale), p(residual), p(out), p(status),
-                          rows.stride(0) if count > 1 else hidden, weight.stride(0) if width > 1 else hidden,
-                          0 if residual is None else residual.stride(0), count, width, hidden, dtype)
-    N.launch(N.lib().sq_matmul_fp8, args, device)
+    N.launch(N.lib().sq_matmul_fp8,
+             _pack(rows.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(), N.address(residual),
+                   out.data_ptr(), N.address(status), rows.stride(0) if count > 1 else hidden,
+                   weight.stride(0) if width > 1 else hidden, 0 if residual is None else residual.stride(0), count, width,
+                   hidden, dtype), index)
     return out

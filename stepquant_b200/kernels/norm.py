@@ -17,36 +17,35 @@ BLOCK = 128  # channels of a scale
 E4M3_MAX, SCALE_FLOOR = 448.0, 1e-30  # as in csrc/sq_norm.cu
 
 
+_pack = N.packer(N.SqNormArgs)
+
+
 def _run(x, weight, residual, eps, fp8):
-    if x.dim() < 1 or x.shape[-1] < 1:
+    shape = x.shape
+    if not shape or not shape[-1]:
         raise ValueError("x: expected [..., hidden] with hidden >= 1")
-    shape, hidden = x.shape, x.shape[-1]
-    rows = N.rows_of(x, "x")
-    if weight is not None and (weight.dim() != 1 or weight.shape[0] != hidden):
-        raise ValueError(f"weight: expected [{hidden}], got {tuple(weight.shape)}")
-    res = None
-    if residual is not None:
-        if residual.shape != shape or residual.dtype != x.dtype:
-            raise ValueError("residual: expected x's shape and dtype")
-        res = N.rows_of(residual, "residual")
-    if not eps >= 0:
-        raise ValueError("eps must not be negative")
-    device = x.device
-    N.same_device(device, weight=weight, residual=residual)
+    hidden = shape[-1]
+    rows, total, res_address, res_stride = N.rows_of(x, "x"), None, 0, 0
+    dtype, weight_dtype = N.dtype_code(x.dtype), N.SQ_F32
     if weight is not None:
+        if weight.shape != (hidden,):
+            raise ValueError(f"weight: expected [{hidden}], got {list(weight.shape)}")
         weight_dtype = N.dtype_code(weight.dtype)
         weight = weight.contiguous()
-    else:
-        weight_dtype = N.SQ_F32
-    count = rows.shape[0]
-    out = torch.empty(shape, device=device, dtype=FP8 if fp8 else x.dtype)
-    scale = torch.empty(*shape[:-1], -(-hidden // BLOCK), device=device, dtype=torch.float32) if fp8 else None
-    total = torch.empty(shape, device=device, dtype=x.dtype) if res is not None else None
-    args = N.SqNormArgs(rows.data_ptr(), None if res is None else res.data_ptr(), None if weight is None else weight.data_ptr(),
-                        None if total is None else total.data_ptr(), out.data_ptr(),
-                        None if scale is None else scale.data_ptr(), rows.stride(0), 0 if res is None else res.stride(0),
-                        count, hidden, N.dtype_code(x.dtype), weight_dtype, 0 if weight is None else 1, eps)
-    N.launch(N.lib().sq_rms_norm, args, device)
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
+        raise ValueError("residual: expected x's shape and dtype")
+    index = N.device_index(x, weight, residual)
+    if residual is not None:
+        res = N.rows_of(residual, "residual")
+        res_address, res_stride = res.data_ptr(), res.stride(0)
+        total = x.new_empty(shape)
+    out = x.new_empty(shape, dtype=FP8) if fp8 else x.new_empty(shape)
+    scale = x.new_empty((*shape[:-1], (hidden + BLOCK - 1) // BLOCK), dtype=torch.float32) if fp8 else None
+    N.launch(N.lib().sq_rms_norm, _pack(rows.data_ptr(), res_address, N.address(weight), N.address(total), out.data_ptr(),
+                                        N.address(scale), rows.stride(0), res_stride, rows.shape[0], hidden, dtype,
+                                        weight_dtype, weight is not None, eps), index)
     return out, scale, total
 
 

@@ -22,43 +22,68 @@ from .conv import causal_conv1d_extend, causal_conv1d_step, sequence_ends, slot_
 STATES = (4, 8, 16, 32, 64)
 
 
-def _inputs(u, dt, a, b, c, d, z, dt_bias):
-    """Checked rows and parameters, as (tensors by name, sizes)."""
-    rows = N.rows_of(u, "u")
-    tokens, channels = rows.shape
-    if a.dim() != 2 or a.shape[0] != channels or a.dtype != torch.float32:
-        raise ValueError(f"a: expected float32 [{channels}, states]")
-    states = a.shape[1]
-    if states not in STATES:
-        raise NotImplementedError(f"the scan is built for {STATES} states, got {states}")
-    t = {"u": rows, "a": N.aligned(a)}
-    for name, x in (("dt", dt), ("z", z)):
-        if x is not None and (x.shape != u.shape or x.dtype != u.dtype):
-            raise ValueError(f"{name}: expected u's shape and dtype")
-        t[name] = None if x is None else N.rows_of(x, name)
-    for name, x in (("b", b), ("c", c)):
-        if x.dim() == u.dim():  # one group
-            x = x.unsqueeze(-2)
-        if x.dim() == 4 and x.shape[0] == 1:
-            x = x[0]
-        if x.dim() != 3 or x.shape[0] != tokens or x.shape[2] != states or x.dtype != u.dtype:
-            raise ValueError(f"{name}: expected {u.dtype} [{tokens}, groups, {states}]")
-        if x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != states):
-            x = x.contiguous()
-        t[name] = x
-    groups = t["b"].shape[1]
-    if t["c"].shape[1] != groups or groups < 1 or channels % groups:
-        raise ValueError("b and c need the same groups, a divisor of the channels")
-    for name, x in (("d", d), ("dt_bias", dt_bias)):
-        if x is not None and tuple(x.shape) != (channels,):
-            raise ValueError(f"{name}: expected [{channels}]")
-        t[name] = None if x is None else x.float().contiguous()
-    N.same_device(u.device, **t)
-    return t, tokens, channels, states, groups
+_pack = N.packer(N.SqScanArgs)
+
+
+def _token_groups(x, u, states, name):
+    """b or c as [tokens, groups, states] with a token's groups contiguous."""
+    if x.dim() == u.dim():  # one group
+        x = x.unsqueeze(-2)
+    if x.dim() == 4 and x.shape[0] == 1:
+        x = x[0]
+    if x.dim() != 3 or x.shape[0] != u.shape[-2] or x.shape[2] != states or x.dtype != u.dtype:
+        raise ValueError(f"{name}: expected {u.dtype} [{u.shape[-2]}, groups, {states}]")
+    return x if x.stride(2) == 1 and (x.shape[1] == 1 or x.stride(1) == states) else x.contiguous()
+
+
+def _row_input(x, u, name):
+    if x.shape != u.shape or x.dtype != u.dtype:
+        raise ValueError(f"{name}: expected u's shape and dtype")
+    return N.rows_of(x, name)
+
+
+def _channel_vector(x, channels, name):
+    if x is None:
+        return None
+    if x.shape != (channels,):
+        raise ValueError(f"{name}: expected [{channels}]")
+    return x if x.dtype == torch.float32 and x.is_contiguous() else x.float().contiguous()
+
+
+class _Call:
+    """Checked operands of one call, and the launch of an entry point on them."""
+
+    def __init__(self, u, dt, a, b, c, d, z, dt_bias, softplus):
+        self.u = N.rows_of(u, "u")
+        self.tokens, self.channels = self.u.shape
+        if a.dim() != 2 or a.shape[0] != self.channels or a.dtype != torch.float32:
+            raise ValueError(f"a: expected float32 [{self.channels}, states]")
+        self.states = a.shape[1]
+        if self.states not in STATES:
+            raise NotImplementedError(f"the scan is built for {STATES} states, got {self.states}")
+        self.a = N.aligned(a)
+        self.dt = _row_input(dt, u, "dt")
+        self.z = None if z is None else _row_input(z, u, "z")
+        self.b, self.c = _token_groups(b, u, self.states, "b"), _token_groups(c, u, self.states, "c")
+        self.groups = self.b.shape[1]
+        if self.c.shape[1] != self.groups or self.groups < 1 or self.channels < 1 or self.channels % self.groups:
+            raise ValueError("b and c need the same groups, a divisor of the channels")
+        self.d, self.dt_bias = _channel_vector(d, self.channels, "d"), _channel_vector(dt_bias, self.channels, "dt_bias")
+        self.softplus = bool(softplus)
+        self.index = N.device_index(self.u, self.a, self.dt, self.z, self.b, self.c, self.d, self.dt_bias)
+
+    def launch(self, entry, y, initial, final, slots, cu, status, workspace, seqs):
+        p = N.address
+        N.launch(entry, _pack(self.u.data_ptr(), self.dt.data_ptr(), p(self.z), self.b.data_ptr(), self.c.data_ptr(),
+                              self.a.data_ptr(), p(self.d), p(self.dt_bias), y.data_ptr(), p(initial), p(final), p(slots),
+                              p(cu), p(status), p(workspace), 0 if workspace is None else workspace.numel(),
+                              self.u.stride(0), self.dt.stride(0), 0 if self.z is None else self.z.stride(0),
+                              self.b.stride(0), self.c.stride(0), 0 if final is None else final.shape[0], self.tokens, seqs,
+                              self.channels, self.states, self.groups, N.dtype_code(self.u.dtype), self.softplus), self.index)
 
 
 def _state(state, rows, channels, states, name):
-    if state.dim() != 3 or tuple(state.shape[1:]) != (channels, states) or (rows is not None and state.shape[0] != rows):
+    if state.dim() != 3 or state.shape[1:] != (channels, states) or (rows is not None and state.shape[0] != rows):
         raise ValueError(f"{name}: expected [{'rows' if rows is None else rows}, {channels}, {states}]")
     if state.dtype != torch.float32:
         raise ValueError(f"{name}: expected float32, got {state.dtype}")
@@ -72,42 +97,29 @@ def _pool_state(state, channels, states):
     return state
 
 
-def _launch(entry, t, sizes, y, initial, final, slots, cu, status, workspace, seqs, softplus, device):
-    tokens, channels, states, groups = sizes
-    p = N.address
-    args = N.SqScanArgs(p(t["u"]), p(t["dt"]), p(t["z"]), p(t["b"]), p(t["c"]), p(t["a"]), p(t["d"]), p(t["dt_bias"]), p(y),
-                        p(initial), p(final), p(slots), p(cu), p(status), p(workspace),
-                        0 if workspace is None else workspace.numel(), t["u"].stride(0), t["dt"].stride(0),
-                        0 if t["z"] is None else t["z"].stride(0), t["b"].stride(0), t["c"].stride(0),
-                        0 if final is None else final.shape[0], tokens, seqs, channels, states, groups,
-                        N.dtype_code(t["u"].dtype), 1 if softplus else 0)
-    N.launch(entry, args, device)
-
-
 def _prompts(u, dt, a, b, c, d, z, dt_bias, dt_softplus, cu_seqlens, initial, final, slots, status):
-    """The scan of concatenated prompts; ``final``: a pool, or a function of (seqs, channels, states)."""
+    """The scan of concatenated prompts; ``final``: with slots their pool, else whether to return the states."""
     if u.dim() == 3 and u.shape[0] != 1:
         raise ValueError("u: expected a leading batch of 1 (concatenated sequences)")
     if u.dim() not in (2, 3):
         raise ValueError("u: expected [tokens, channels]")
-    t, *sizes = _inputs(u, dt, a, b, c, d, z, dt_bias)
-    tokens, channels, states, groups = sizes
+    call = _Call(u, dt, a, b, c, d, z, dt_bias, dt_softplus)
     device = u.device
-    cu = sequence_ends(cu_seqlens, tokens, device)
+    cu = sequence_ends(cu_seqlens, call.tokens, device)
     seqs = cu.numel() - 1
     if slots is not None:
-        initial = final = _pool_state(final, channels, states)
+        initial = final = _pool_state(final, call.channels, call.states)
         slots = slot_rows(slots, seqs, device)
-        N.same_device(device, state=final, status=status)
+        N.device_index(u, final, status)
     else:
         if initial is not None:
-            initial = N.aligned(_state(initial, seqs, channels, states, "initial_state"))
-            N.same_device(device, initial_state=initial)
-        final = torch.empty(seqs, channels, states, device=device, dtype=torch.float32) if final else None
-    y = torch.empty(u.shape, device=device, dtype=u.dtype)
-    size = N.lib().sq_selective_scan_workspace_bytes(tokens, seqs, channels, states, groups)
-    workspace = torch.empty(size, device=device, dtype=torch.uint8) if size > 0 else None
-    _launch(N.lib().sq_selective_scan, t, sizes, y, initial, final, slots, cu, status, workspace, seqs, dt_softplus, device)
+            initial = N.aligned(_state(initial, seqs, call.channels, call.states, "initial_state"))
+            N.device_index(u, initial)
+        final = u.new_empty((seqs, call.channels, call.states), dtype=torch.float32) if final else None
+    y = u.new_empty(u.shape)
+    size = N.lib().sq_selective_scan_workspace_bytes(call.tokens, seqs, call.channels, call.states, call.groups)
+    workspace = u.new_empty(size, dtype=torch.uint8) if size > 0 else None
+    call.launch(N.lib().sq_selective_scan, y, initial, final, slots, cu, status, workspace, seqs)
     return y, final
 
 
@@ -141,16 +153,14 @@ def selective_scan_step(state, u, dt, a, b, c, *, d=None, z=None, dt_bias=None, 
     padding and slots outside the pool as in ``selective_scan_extend``."""
     if u.dim() != 2:
         raise ValueError("u: expected [batch, channels]")
-    t, *sizes = _inputs(u, dt, a, b, c, d, z, dt_bias)
-    batch, channels, states, _ = sizes
-    device = u.device
-    state = _pool_state(state, channels, states)
-    N.same_device(device, state=state, status=status)
+    call = _Call(u, dt, a, b, c, d, z, dt_bias, dt_softplus)
+    batch = call.tokens
+    state = _pool_state(state, call.channels, call.states)
+    N.device_index(u, state, status)
     if slots is None and state.shape[0] != batch:
         raise ValueError(f"state: expected {batch} rows without slots")
-    y = torch.empty(batch, channels, device=device, dtype=u.dtype)
-    _launch(N.lib().sq_selective_scan_step, t, sizes, y, None, state, slot_rows(slots, batch, device), None, status, None,
-            batch, dt_softplus, device)
+    y = u.new_empty((batch, call.channels))
+    call.launch(N.lib().sq_selective_scan_step, y, None, state, slot_rows(slots, batch, u.device), None, status, None, batch)
     return y
 
 
