@@ -7,20 +7,22 @@
 //
 // h, A and every intermediate are fp32; y is rounded once to the input's type.
 //
-// Prompts (scan_kernel): four states a lane, N / 4 lanes a channel; a CTA of 128
-// lanes walks its channels through the tokens in tiles of 32.  Per tile the CTA
-// forms dt' and dt' u once per (token, channel) in shared memory (two special
-// functions, against N exponentials), the lanes run the recurrence in registers,
-// four tokens at a time so that the loads and exponentials of a group do not wait
-// on its chain h, and the outputs leave through shared memory.  The next tile's
-// inputs are loaded before the recurrence of this one.
-// Bound by the special function unit: one exponential per (token, channel,
-// state) at 16 a clock and SM.
+// Prompts (scan_kernel): a lane holds up to 16 states of one channel and walks it
+// through the tokens, so dt', the gate and the sum over N are formed where they
+// are used and only more than 16 states need an exchange.  B and C, the same for
+// all channels of a group, are read from shared memory by broadcast.  A CTA of 128
+// lanes takes its tokens in tiles; the raw rows of the next tile are in flight
+// (cp.async of the 16-byte pieces that cover a row, so rows of any alignment take
+// one path) while a tile is worked on.  Four tokens at a time, so that the
+// exponentials and gates of one do not wait on the chain h of the others.
+// Bound by the special function unit (one exponential per token, channel and
+// state at 16 a clock and SM) and, next to it, by issue.
 //
 // Few channels and sequences: the tokens are cut into chunks.  A first pass gives
 // each chunk's state from zero and its sum of dt' (the decay of a chunk is
 // exp(A sum dt')), a second joins them along each sequence, the third is the scan
 // of every chunk from its state.  Twice the exponentials, on many more lanes.
+#include <type_traits>
 #include "sq_rows.cuh"
 #include "sq_vec.cuh"
 
@@ -28,20 +30,52 @@ namespace sq {
 namespace {
 
 constexpr int kScanThreads = 128;
-constexpr int kTile = 32;     // tokens of a tile
-constexpr int kPerLane = 4;   // states of a lane
-constexpr int kUnroll = 4;    // tokens of a group
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kPerLane = 4;   // states of a lane of the single-token kernel
+constexpr int kGroup = 4;     // tokens of a prompt worked on together
+constexpr float kLog2eRest = 1.92596299e-8f;  // log2(e) - kLog2e
 
-__device__ __forceinline__ float exp2_approx(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
+// dt_bias of a channel in units of log2(e), with the rounding of that product.
+struct Bias {
+    float value, high, low;
+    __device__ __forceinline__ explicit Bias(float b) : value(b), high(b * kLog2e), low(fmaf(b, kLog2e, -high) + b * kLog2eRest) {}
+};
+
+// log(1 + e^x), x = raw + bias, as max(x, 0) + log1p(e^-|x|), accurate to a few
+// units in the last place over the whole range: the step size scales every input
+// of the state, and far below zero softplus is the exponential alone.  So x
+// log2(e) is carried with its rounding error; log1p(e) = 2 atanh(e / (2 + e)) is
+// its series to the 13th power (the argument is at most 1/3).  NaN stays NaN, an
+// infinite x gives 0 or itself.
+__device__ __forceinline__ float softplus(float raw, const Bias &bias) {
+    const float y = fmaf(raw, kLog2e, bias.high);
+    float lost = fmaf(raw, kLog2e, bias.high - y) + fmaf(raw, kLog2eRest, bias.low);
+    lost = fminf(lost, 1.f);  // NaN where y is infinite
+    lost = __uint_as_float(__float_as_uint(lost) ^ (~__float_as_uint(y) & 0x80000000u));  // of -|y|
+    const float p = exp2_approx(-fminf(fabsf(y), 180.f)), e = fmaf(p, lost * 0.6931471806f, p);
+    const float q = e * reciprocal_approx(2.f + e), q2 = q * q;
+    float s = fmaf(q2, 1.f / 13.f, 1.f / 11.f);
+    s = fmaf(q2, s, 1.f / 9.f);
+    s = fmaf(q2, s, 1.f / 7.f);
+    s = fmaf(q2, s, 1.f / 5.f);
+    s = fmaf(q2, s, 1.f / 3.f);
+    s = fmaf(q2 * s, q, q);
+    float top;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(top) : "f"(raw + bias.value));
+    return fmaf(2.f, s, top);
 }
 
-// expf, not its fast form: far below zero softplus is the exponential, and the
-// step size scales every input of the state.
-__device__ __forceinline__ float softplus(float x) { return x > 20.f ? x : log1pf(expf(x)); }
+// Pairs of fp32 values, one instruction for both.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return reinterpret_cast<float2 &>(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(r) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)), "l"(reinterpret_cast<uint64_t &>(c)));
+    return reinterpret_cast<float2 &>(r);
+}
 
 // A lane's four entries of a state or A row (16-byte aligned: N is a multiple of 4).
 __device__ __forceinline__ void load4(const float *p, float (&x)[4]) {
@@ -49,32 +83,16 @@ __device__ __forceinline__ void load4(const float *p, float (&x)[4]) {
     x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
 }
 
-// Four channels of a token: one load of 8 or 16 bytes, or (rows not aligned for
-// it, or the last channels of a group) the first n singly.
-template <class T>
-struct Quad {
-    alignas(4 * sizeof(T)) T v[4];
-    __device__ __forceinline__ void load(const T *p, bool whole, int n) {
-        if (whole) {
-            if (sizeof(T) == 2) *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(p);
-            else *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(p);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = i < n ? p[i] : from_float<T>(0.f);
-        }
-    }
-    __device__ __forceinline__ void store(T *p, bool whole, int n) const {
-        if (whole) {
-            if (sizeof(T) == 2) *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(v);
-            else *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(v);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (i < n) p[i] = v[i];
-        }
-    }
-};
-
+// The 16-byte pieces that cover `bytes` bytes from p on, piece `i` into a row of
+// shared memory; nothing past the last byte is read (a piece may begin before p:
+// in the row before, or in the padding below a tensor's first row).
+__device__ __forceinline__ void cover(unsigned char *row, const void *p, int bytes, int i) {
+    const uintptr_t from = reinterpret_cast<uintptr_t>(p), piece = (from & ~uintptr_t(15)) + 16 * i;
+    const int64_t left = int64_t(from) + bytes - int64_t(piece);
+    if (left <= 0) return;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(static_cast<unsigned>(__cvta_generic_to_shared(row + 16 * i))),
+                 "l"(piece), "r"(int(left < 16 ? left : 16)) : "memory");
+}
 // Workspace of the chunked scan: a state per (chunk, channel), then a sum of dt'.
 struct Chunks {
     int length;     // tokens of a chunk; 0: whole sequences
@@ -84,16 +102,29 @@ struct Chunks {
 
 enum ScanPass { kWhole, kChunkState, kChunkScan };
 
-template <class T, int N, int PASS>
-__global__ void __launch_bounds__(kScanThreads) scan_kernel(sq_scan_args a, Chunks chunks, bool vec) {
-    constexpr int P = N / kPerLane;              // lanes of a channel
-    constexpr int CH = kScanThreads / P;         // channels of the CTA
-    constexpr int TILE = P > 1 ? kTile : kTile / 2;  // tokens of a tile (a lane a channel: shared memory for half)
-    constexpr int QUADS = CH / 4, ROWS = kScanThreads / QUADS;  // a thread's quad of channels, rows of a load
-    constexpr int EACH = TILE / ROWS > 0 ? TILE / ROWS : 1;
-    __shared__ float2 step[TILE][CH];           // dt', dt' u
-    __shared__ float ys[PASS == kChunkState ? 1 : TILE][PASS == kChunkState ? 1 : CH];
-    __shared__ float4 bs[TILE][P], cs[TILE][P];
+// Sizes of a CTA and its shared memory.
+template <class T, int N>
+struct ScanShape {
+    static constexpr int SN = N < 16 ? N : 16;     // states of a lane
+    static constexpr int P = N / SN;               // lanes of a channel
+    static constexpr int CH = kScanThreads / P;    // channels of the CTA
+    static constexpr int TILE = 16;           // tokens of a tile
+    static constexpr int kRow = CH * sizeof(T) + 16, kBcRow = N * sizeof(T) + 16;  // raw rows with their cover
+    static constexpr int kStage = TILE * (3 * kRow + 2 * kBcRow);                  // dt, u, z, B, C
+    static constexpr int kBc = TILE * N * 4;
+    static constexpr int kBytes = 2 * kBc + 2 * kStage;
+};
+
+// USUAL: softplus and (where there are outputs) a gate, known to the compiler so that the
+// tokens of a group have no branches between them; else as the arguments say.
+template <class T, int N, int PASS, bool USUAL>
+__global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(sq_scan_args a, Chunks chunks) {
+    using S = ScanShape<T, N>;
+    constexpr int SN = S::SN, P = S::P, CH = S::CH, TILE = S::TILE;
+    constexpr bool OUT = PASS != kChunkState;
+    extern __shared__ __align__(16) unsigned char smem[];
+    float4 *bs = reinterpret_cast<float4 *>(smem), *cs = reinterpret_cast<float4 *>(smem + S::kBc);  // [TILE][N]
+    unsigned char *raw = smem + 2 * S::kBc;
     const int tid = threadIdx.x, lane = tid % P, ch = tid / P;
     const int per = a.channels / a.groups, tiles = (per + CH - 1) / CH;  // CTAs of a group
     const int group = blockIdx.y / tiles, first = (blockIdx.y - group * tiles) * CH;
@@ -113,157 +144,159 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(sq_scan_args a, Chun
         if (PASS == kChunkState && end == seq.y) return;  // no chunk follows
     }
     T *y = static_cast<T *>(a.y) + d0;
-    const int64_t row = state_row(a.slots, n, a.num_slots, PASS == kChunkState ? nullptr : a.status);
+    const int64_t row = state_row(a.slots, n, a.num_slots, OUT ? a.status : nullptr);
     if (row < 0) {
-        if (PASS != kChunkState)
+        if (OUT)
             for (int64_t i = tid; i < (end - begin) * int64_t(CH); i += kScanThreads)
                 if (i % CH < live) y[(begin + i / CH) * a.channels + i % CH] = from_float<T>(0.f);
         return;
     }
 
-    // ---- this lane's states
-    const int mine = min(ch, live - 1);  // lanes past the group's channels follow its last
-    float A[4], h[4] = {0.f, 0.f, 0.f, 0.f};
-    load4(a.a + int64_t(d0 + mine) * N + lane * 4, A);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) A[i] *= kLog2e;
-    const int64_t at = (row * a.channels + d0 + mine) * N + lane * 4;
-    const int64_t kept = (int64_t(blockIdx.x) * a.channels + d0 + mine) * N + lane * 4;
-    if (PASS == kChunkScan && many) load4(chunks.state + kept, h);
-    else if (PASS != kChunkState && a.initial_state) load4(a.initial_state + at, h);
-    float total = 0.f;  // sum of dt' (first lane of the channel)
-
-    // ---- this thread's share of a tile's loads: rows r, r + ROWS, ... of one quad of channels
-    const int quad = tid % QUADS * 4, row0 = tid / QUADS, width = max(0, min(4, live - quad));
-    const bool whole = vec && width == 4;
-    const T *u = static_cast<const T *>(a.u) + d0 + quad, *dt = static_cast<const T *>(a.dt) + d0 + quad;
-    const T *z = a.z ? static_cast<const T *>(a.z) + d0 + quad : nullptr;
+    // ---- raw rows of a tile: a power of two of threads a row, its pieces among them
+    const T *u = static_cast<const T *>(a.u) + d0, *dt = static_cast<const T *>(a.dt) + d0;
+    const T *z = a.z ? static_cast<const T *>(a.z) + d0 : nullptr;
     const T *b = static_cast<const T *>(a.b) + group * N, *c = static_cast<const T *>(a.c) + group * N;
-    constexpr int BC = (TILE * N + kScanThreads - 1) / kScanThreads;  // entries of B (and C) a thread loads a tile
-    float bias[4], skip[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        bias[i] = a.dt_bias && i < width ? a.dt_bias[d0 + quad + i] : 0.f;
-        skip[i] = PASS != kChunkState && a.d && i < width ? a.d[d0 + quad + i] : 0.f;
-    }
-    Quad<T> next_dt[EACH], next_u[EACH], next_z[EACH];
-    T next_b[BC], next_c[BC];
-    auto fetch = [&](int t0) {
-#pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-            const int64_t t = t0 + row0 + e * ROWS;
-            if (row0 + e * ROWS < TILE && t < end) {
-                next_dt[e].load(dt + t * a.dt_stride, whole, width);
-                next_u[e].load(u + t * a.u_stride, whole, width);
-                if (PASS != kChunkState && z) next_z[e].load(z + t * a.z_stride, whole, width);
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < BC; ++e) {
-            const int i = e * kScanThreads + tid;
-            const int64_t t = t0 + i / N;
-            if (i >= TILE * N) continue;
-            next_b[e] = t < end ? b[t * a.b_stride + i % N] : from_float<T>(0.f);
-            if (PASS != kChunkState) next_c[e] = t < end ? c[t * a.c_stride + i % N] : from_float<T>(0.f);
-        }
-    };
-    // dt', dt' u, B and C of the fetched tile into shared memory; rows past the end leave the state alone.
-    auto put = [&](int t0) {
-#pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-            const int r = row0 + e * ROWS;
-            if (r >= TILE) continue;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = to_float(next_dt[e].v[i]) + bias[i];
-                const float s = t0 + r < end ? (a.softplus ? softplus(x) : x) : 0.f;
-                step[r][quad + i] = make_float2(s, t0 + r < end ? s * to_float(next_u[e].v[i]) : 0.f);
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < BC; ++e) {
-            const int i = e * kScanThreads + tid;
-            if (i >= TILE * N) continue;
-            reinterpret_cast<float *>(bs)[i] = to_float(next_b[e]);
-            if (PASS != kChunkState) reinterpret_cast<float *>(cs)[i] = to_float(next_c[e]);
-        }
-    };
-
-    if (begin < end) {
-        fetch(begin);
-        put(begin);
-    }
-    __syncthreads();
-    for (int t0 = begin; t0 < end; t0 += TILE) {
-        Quad<T> now_u[EACH], now_z[EACH];
-#pragma unroll
-        for (int e = 0; e < EACH; ++e) now_u[e] = next_u[e], now_z[e] = next_z[e];
-        if (t0 + TILE < end) fetch(t0 + TILE);
+    constexpr int kU = TILE * S::kRow, kZ = 2 * kU, kB = 3 * kU, kC = kB + TILE * S::kBcRow;  // offsets in a stage (dt at 0)
+    constexpr int PIECES = S::kRow / 16, LANES = PIECES <= 5 ? 4 : PIECES <= 9 ? 8 : PIECES <= 17 ? 16 : 32;
+    constexpr int BC_PIECES = S::kBcRow / 16, BC_LANES = BC_PIECES <= 4 ? 4 : BC_PIECES <= 8 ? 8 : BC_PIECES <= 16 ? 16 : 32;
+    constexpr int PASS_ROWS = kScanThreads / LANES, BC_ROWS = kScanThreads / BC_LANES;
+    const int bytes = live * int(sizeof(T)), bc_bytes = N * int(sizeof(T));
+    const T *fetch_dt = dt + (int64_t(begin) + tid / LANES) * a.dt_stride, *fetch_u = u + (int64_t(begin) + tid / LANES) * a.u_stride;
+    const T *fetch_z = OUT && z ? z + (int64_t(begin) + tid / LANES) * a.z_stride : nullptr;
+    const T *fetch_b = b + (int64_t(begin) + tid / BC_LANES) * a.b_stride, *fetch_c = c + (int64_t(begin) + tid / BC_LANES) * a.c_stride;
+    auto fetch = [&](int t0, int stage) {  // the tile after the one fetched before
         const int count = min(TILE, end - t0);
-        for (int t = 0; t < count; t += kUnroll) {  // rows past the end have dt' = 0
-            float2 s[kUnroll];
-            float4 bv[kUnroll], cv[kUnroll];
-            float decay[kUnroll][4], sum[kUnroll];
+        unsigned char *to = raw + stage * S::kStage + tid / LANES * S::kRow;
 #pragma unroll
-            for (int j = 0; j < kUnroll; ++j) {
-                s[j] = step[t + j][ch];
-                bv[j] = bs[t + j][lane];
-                if (PASS != kChunkState) cv[j] = cs[t + j][lane];
+        for (int r = 0; r < TILE; r += PASS_ROWS) {
+            if (r + tid / LANES < count) {
+#pragma unroll
+                for (int p = 0; p < PIECES; p += LANES)  // a cover is one piece longer than its row
+                    if (p == 0 || tid % LANES == 0) {
+                        cover(to + r * S::kRow, fetch_dt, bytes, tid % LANES + p);
+                        cover(to + kU + r * S::kRow, fetch_u, bytes, tid % LANES + p);
+                        if (OUT && (USUAL || z)) cover(to + kZ + r * S::kRow, fetch_z, bytes, tid % LANES + p);
+                    }
             }
+            constexpr int DONE = PASS_ROWS < TILE ? PASS_ROWS : TILE;
+            fetch_dt += DONE * a.dt_stride;
+            fetch_u += DONE * a.u_stride;
+            if (OUT && (USUAL || z)) fetch_z += DONE * a.z_stride;
+        }
+        to = raw + stage * S::kStage + tid / BC_LANES * S::kBcRow;
 #pragma unroll
-            for (int j = 0; j < kUnroll; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) decay[j][i] = exp2_approx(s[j].x * A[i]);
-#pragma unroll
-            for (int j = 0; j < kUnroll; ++j) {
-                const float bb[4] = {bv[j].x, bv[j].y, bv[j].z, bv[j].w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) h[i] = fmaf(decay[j][i], h[i], s[j].y * bb[i]);
-                if (PASS == kChunkState) {
-                    total += s[j].x;
-                } else {
-                    const float cc[4] = {cv[j].x, cv[j].y, cv[j].z, cv[j].w};
-                    sum[j] = fmaf(cc[3], h[3], fmaf(cc[2], h[2], fmaf(cc[1], h[1], cc[0] * h[0])));
-                }
+        for (int r = 0; r < TILE; r += BC_ROWS) {
+            if (r + tid / BC_LANES < count && tid % BC_LANES < BC_PIECES) {
+                cover(to + kB + r * S::kBcRow, fetch_b, bc_bytes, tid % BC_LANES);
+                if (OUT) cover(to + kC + r * S::kBcRow, fetch_c, bc_bytes, tid % BC_LANES);
             }
-            if (PASS != kChunkState) {
+            constexpr int DONE = BC_ROWS < TILE ? BC_ROWS : TILE;
+            fetch_b += DONE * a.b_stride;
+            if (OUT) fetch_c += DONE * a.c_stride;
+        }
+    };
+    auto commit = [] { asm volatile("cp.async.commit_group;\n" ::: "memory"); };
+    if (begin < end) fetch(begin, 0);
+    commit();
+
+    // ---- this lane's states, in pairs
+    const int k = min(ch, live - 1), d = d0 + k;  // lanes past the group's channels follow its last
+    const int64_t at = (row * a.channels + d) * N + lane * SN, kept = (int64_t(blockIdx.x) * a.channels + d) * N + lane * SN;
+    float2 A[SN / 2], h[SN / 2];
 #pragma unroll
-                for (int o = P / 2; o > 0; o >>= 1)
-#pragma unroll
-                    for (int j = 0; j < kUnroll; ++j) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], o);
-                if (lane == 0) {
-#pragma unroll
-                    for (int j = 0; j < kUnroll; ++j) ys[t + j][ch] = sum[j];
-                }
-            }
+    for (int i = 0; i < SN / 4; ++i) {
+        float v[4];
+        load4(a.a + int64_t(d) * N + lane * SN + 4 * i, v);
+        A[2 * i] = make_float2(v[0] * kLog2e, v[1] * kLog2e), A[2 * i + 1] = make_float2(v[2] * kLog2e, v[3] * kLog2e);
+        v[0] = v[1] = v[2] = v[3] = 0.f;
+        if (PASS == kChunkScan && many) load4(chunks.state + kept + 4 * i, v);
+        else if (OUT && a.initial_state) load4(a.initial_state + at + 4 * i, v);
+        h[2 * i] = make_float2(v[0], v[1]), h[2 * i + 1] = make_float2(v[2], v[3]);
+    }
+    const Bias bias(a.dt_bias ? a.dt_bias[d] : 0.f);
+    const float skip = OUT && a.d ? a.d[d] : 0.f;
+    float total = 0.f;  // sum of dt'
+
+    int stage = 0;
+    y += int64_t(begin) * a.channels + ch;
+    const bool stores = ch < live && lane == 0;
+    // Byte offsets of this lane's value in the raw rows: the alignment of row t within 16 bytes, plus the channel.
+    const uint32_t dt_low = uint32_t(reinterpret_cast<uintptr_t>(dt)), dt_step = uint32_t(a.dt_stride * sizeof(T));
+    const uint32_t u_low = uint32_t(reinterpret_cast<uintptr_t>(u)), u_step = uint32_t(a.u_stride * sizeof(T));
+    const uint32_t z_low = uint32_t(reinterpret_cast<uintptr_t>(z)), z_step = uint32_t(a.z_stride * sizeof(T));
+    const uint32_t b_low = uint32_t(reinterpret_cast<uintptr_t>(b)), b_step = uint32_t(a.b_stride * sizeof(T));
+    const uint32_t c_low = uint32_t(reinterpret_cast<uintptr_t>(c)), c_step = uint32_t(a.c_stride * sizeof(T));
+    auto value = [&](const unsigned char *rows, int row_bytes, uint32_t low, uint32_t step, int t0, int r, int i) {
+        return to_float(reinterpret_cast<const T *>(rows + r * row_bytes + ((low + uint32_t(t0 + r) * step) & 15))[i]);
+    };
+    for (int t0 = begin; t0 < end; t0 += TILE, stage ^= 1) {
+        const unsigned char *from = raw + stage * S::kStage;
+        asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+        __syncthreads();  // this tile's rows have landed; the tile before is done with B and C
+        const int count = min(TILE, end - t0);
+        for (int i = tid; i < count * N; i += kScanThreads) {
+            reinterpret_cast<float *>(bs)[i] = value(from + kB, S::kBcRow, b_low, b_step, t0, i / N, i % N);
+            if (OUT) reinterpret_cast<float *>(cs)[i] = value(from + kC, S::kBcRow, c_low, c_step, t0, i / N, i % N);
         }
         __syncthreads();
-        if (PASS != kChunkState) {
+        if (t0 + TILE < end) fetch(t0 + TILE, stage ^ 1);
+        commit();
+        auto tokens = [&](int t, auto group) {  // the next `group` tokens of the tile
+            constexpr int U = decltype(group)::value;
+            float s[U], in[U], un[U];
+            float2 decay[U][SN / 2];
 #pragma unroll
-            for (int e = 0; e < EACH; ++e) {
-                const int r = row0 + e * ROWS;
-                if (r >= count || width == 0) continue;
-                Quad<T> out;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float v = ys[r][quad + i];
-                    if (a.d) v = fmaf(skip[i], to_float(now_u[e].v[i]), v);
-                    if (z) v *= silu(to_float(now_z[e].v[i]));
-                    out.v[i] = from_float<T>(v);
-                }
-                out.store(y + quad + int64_t(t0 + r) * a.channels, whole, width);
+            for (int j = 0; j < U; ++j) {
+                const float x = value(from, S::kRow, dt_low, dt_step, t0, t + j, k);
+                un[j] = value(from + kU, S::kRow, u_low, u_step, t0, t + j, k);
+                s[j] = USUAL || a.softplus ? softplus(x, bias) : x + bias.value;
+                in[j] = s[j] * un[j];
+                if (!OUT) total += s[j];
             }
-        }
-        if (t0 + TILE < end) put(t0 + TILE);
-        __syncthreads();
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+#pragma unroll
+                for (int i = 0; i < SN / 2; ++i) {
+                    const float2 x = mul2(make_float2(s[j], s[j]), A[i]);
+                    decay[j][i] = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+                }
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                float2 sum = make_float2(0.f, 0.f);
+                const float2 both = make_float2(in[j], in[j]);
+#pragma unroll
+                for (int i = 0; i < SN / 4; ++i) {
+                    const float4 bv = bs[((t + j) * N + lane * SN) / 4 + i];
+                    h[2 * i] = fma2(decay[j][2 * i], h[2 * i], mul2(both, make_float2(bv.x, bv.y)));
+                    h[2 * i + 1] = fma2(decay[j][2 * i + 1], h[2 * i + 1], mul2(both, make_float2(bv.z, bv.w)));
+                    if (OUT) {
+                        const float4 cv = cs[((t + j) * N + lane * SN) / 4 + i];
+                        sum = fma2(make_float2(cv.x, cv.y), h[2 * i], sum);
+                        sum = fma2(make_float2(cv.z, cv.w), h[2 * i + 1], sum);
+                    }
+                }
+                if (!OUT) continue;
+                float v = sum.x + sum.y;
+#pragma unroll
+                for (int o = P / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                v = fmaf(skip, un[j], v);
+                if (USUAL || z) v *= silu(value(from + kZ, S::kRow, z_low, z_step, t0, t + j, k));
+                if (stores) *y = from_float<T>(v);
+                y += a.channels;
+            }
+        };
+        int t = 0;
+        for (; t + kGroup <= count; t += kGroup) tokens(t, std::integral_constant<int, kGroup>());
+        for (; t < count; ++t) tokens(t, std::integral_constant<int, 1>());
     }
     if (ch >= live) return;
-    if (PASS == kChunkState) {
-        *reinterpret_cast<float4 *>(chunks.state + kept) = make_float4(h[0], h[1], h[2], h[3]);
-        if (lane == 0) chunks.step_sum[int64_t(blockIdx.x) * a.channels + d0 + ch] = total;
-    } else if (a.final_state && end == seq.y) {
-        *reinterpret_cast<float4 *>(a.final_state + at) = make_float4(h[0], h[1], h[2], h[3]);
+#pragma unroll
+    for (int i = 0; i < SN / 4; ++i) {
+        const float4 v = make_float4(h[2 * i].x, h[2 * i].y, h[2 * i + 1].x, h[2 * i + 1].y);
+        if (!OUT) *reinterpret_cast<float4 *>(chunks.state + kept + 4 * i) = v;
+        else if (a.final_state && end == seq.y) *reinterpret_cast<float4 *>(a.final_state + at + 4 * i) = v;
     }
+    if (!OUT && lane == 0) chunks.step_sum[int64_t(blockIdx.x) * a.channels + d] = total;
 }
 
 // Along each sequence of several chunks: the state that every chunk starts from.
@@ -308,7 +341,8 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(sq_scan_args a)
     }
     load4(a.a + int64_t(k) * N + lane * 4, A);
     float dt_mine[SHARE], u_mine[SHARE], z_mine[SHARE];
-    const float bias = a.dt_bias ? a.dt_bias[k] : 0.f, skip = a.d ? a.d[k] : 0.f;
+    const Bias bias(a.dt_bias ? a.dt_bias[k] : 0.f);
+    const float skip = a.d ? a.d[k] : 0.f;
 #pragma unroll
     for (int q = 0; q < SHARE; ++q) {
         const int r = lane + q * P;
@@ -316,9 +350,9 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(sq_scan_args a)
         dt_mine[q] = u_mine[q] = z_mine[q] = 0.f;
         if (r < R && n < a.num_seqs) {
             u_mine[q] = to_float(static_cast<const T *>(a.u)[n * a.u_stride + k]);
-            const float raw = to_float(static_cast<const T *>(a.dt)[n * a.dt_stride + k]) + bias;
+            const float raw = to_float(static_cast<const T *>(a.dt)[n * a.dt_stride + k]);
             if (a.z) z_mine[q] = to_float(static_cast<const T *>(a.z)[n * a.z_stride + k]);
-            dt_mine[q] = a.softplus ? softplus(raw) : raw;
+            dt_mine[q] = a.softplus ? softplus(raw, bias) : raw + bias.value;
         }
     }
 #pragma unroll
@@ -349,46 +383,55 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(sq_scan_args a)
     }
 }
 
-// Tokens of a chunk, 0 for whole sequences: cut where the lanes of whole
-// sequences leave most of the 592 warp schedulers without a warp.
+// Tokens of a chunk, 0 for whole sequences.  A warp of 32 channels alone takes
+// 178 ns a token, a full GPU 0.2 ns a (warp, token), measured at 16 states.  Whole
+// sequences last as long as the longest (the host does not know the lengths: of
+// several, three times the mean is assumed); chunks cost 1.9 times the work.
+// Chunks of 192 to 256 tokens measured best at 2048 and 4096 channels (16 warps a
+// scheduler), 8 ragged prompts of 16384 tokens 779 us against 1103 us whole, one
+// of 8192 tokens 218 us against 1430 us.
 int chunk_length(int tokens, int seqs, int channels, int states) {
-    const int64_t warps = int64_t(channels) * (states / kPerLane) / 32 + 1;
-    if (seqs * warps >= 592 * 3 || tokens < 256) return 0;
-    const int64_t wanted = 592 * 6 / warps;  // chunks that fill them
-    int64_t length = (tokens / (wanted > 1 ? wanted : 1) + kTile - 1) / kTile * kTile;
-    if (length < 64) length = 64;
-    return length * 2 > tokens / seqs * int64_t(3) ? 0 : int(length);
+    const double warps = double(channels) * (states > 16 ? states / 16 : 1) / 32;
+    const double work = 0.2 * tokens * warps, alone = 178.0;
+    const double longest = seqs == 1 ? tokens : 3.0 * tokens / seqs < tokens ? 3.0 * tokens / seqs : tokens;
+    const double length = tokens * warps / (592 * 16);
+    const int chunk = length < 128 ? 128 : int(length + 15) / 16 * 16;
+    const double whole = longest * alone > work ? longest * alone : work;
+    const double cut = 10000.0 + (1.9 * work > 2 * chunk * alone ? 1.9 * work : 2 * chunk * alone);
+    return cut < whole ? chunk : 0;
 }
 
 template <class T, int N>
 cudaError_t launch_scan_as(const sq_scan_args &a, bool step, cudaStream_t s) {
-    constexpr int CH = kScanThreads / (N / kPerLane);
     if (step) {
-        const unsigned grid = unsigned((a.channels + CH - 1) / CH);
+        constexpr int P = N / kPerLane;
+        const unsigned grid = unsigned((int64_t(a.channels) * P + kScanThreads - 1) / kScanThreads);
         if (int64_t(a.num_seqs) * grid < 148 * 16) scan_step_kernel<T, N, 1><<<dim3(unsigned(a.num_seqs), grid), kScanThreads, 0, s>>>(a);
         else scan_step_kernel<T, N, 4><<<dim3(unsigned((a.num_seqs + 3) / 4), grid), kScanThreads, 0, s>>>(a);
         return cudaGetLastError();
     }
     const int per = a.channels / a.groups;
+    constexpr int CH = ScanShape<T, N>::CH;
     const unsigned columns = unsigned(a.groups * ((per + CH - 1) / CH));
-    const int64_t size = sizeof(T);
-    auto quads = [&](const void *p, int64_t stride) { return reinterpret_cast<uintptr_t>(p) % (4 * size) == 0 && stride % 4 == 0; };
-    const bool vec = per % 4 == 0 && quads(a.u, a.u_stride) && quads(a.dt, a.dt_stride) && (!a.z || quads(a.z, a.z_stride)) &&
-                     quads(a.y, a.channels);
     Chunks chunks{};
-    if (a.workspace) chunks.length = chunk_length(a.tokens, a.num_seqs, a.channels, a.states);
-    if (!chunks.length) {
-        scan_kernel<T, N, kWhole><<<dim3(unsigned(a.num_seqs), columns), kScanThreads, 0, s>>>(a, chunks, vec);
+    auto run = [&](auto kernel, int64_t rows) {
+        constexpr int bytes = ScanShape<T, N>::kBytes;
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != cudaSuccess) return e;
+        kernel<<<dim3(unsigned(rows), columns), kScanThreads, bytes, s>>>(a, chunks);
         return cudaGetLastError();
-    }
+    };
+    if (a.workspace) chunks.length = chunk_length(a.tokens, a.num_seqs, a.channels, a.states);
+    const bool usual = a.softplus && a.z;
+    if (!chunks.length) return usual ? run(scan_kernel<T, N, kWhole, true>, a.num_seqs) : run(scan_kernel<T, N, kWhole, false>, a.num_seqs);
     const int64_t count = a.tokens / chunks.length + a.num_seqs;
     chunks.state = static_cast<float *>(a.workspace);
     chunks.step_sum = chunks.state + count * a.channels * N;
-    const dim3 grid(unsigned(count), columns);
-    scan_kernel<T, N, kChunkState><<<grid, kScanThreads, 0, s>>>(a, chunks, vec);
+    cudaError_t e = a.softplus ? run(scan_kernel<T, N, kChunkState, true>, count) : run(scan_kernel<T, N, kChunkState, false>, count);
+    if (e != cudaSuccess) return e;
     join_kernel<<<dim3(unsigned(a.num_seqs), unsigned((int64_t(a.channels) * N + 255) / 256)), 256, 0, s>>>(a, chunks);
-    scan_kernel<T, N, kChunkScan><<<grid, kScanThreads, 0, s>>>(a, chunks, vec);
-    return cudaGetLastError();
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    return usual ? run(scan_kernel<T, N, kChunkScan, true>, count) : run(scan_kernel<T, N, kChunkScan, false>, count);
 }
 
 template <class T>

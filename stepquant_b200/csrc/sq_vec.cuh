@@ -53,10 +53,24 @@ __device__ __forceinline__ void store8(T *p, bool whole, int n, const float (&x)
     }
 }
 
-// x sigmoid(x) with the exponential and the reciprocal of the special function
-// unit (a few units in the last place of fp32; -inf gives 0 as its limit does
-// in the quotient form x / (1 + e^-x), NaN stays NaN).
-__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
+constexpr float kLog2e = 1.4426950408889634f;
+
+// The special function unit's 2^x and 1 / x (two and one units in the last
+// place), subnormals flushed to zero.
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float reciprocal_approx(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// x sigmoid(x) = x / (1 + e^-x).  Beyond -88 the exponential is infinite and the
+// result -0; -infinity and NaN give NaN as the quotient does.
+__device__ __forceinline__ float silu(float x) { return x * reciprocal_approx(1.f + exp2_approx(-kLog2e * x)); }
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
