@@ -3,19 +3,28 @@
 //   out[m, n] = residual[m, n] + sum_g sx[m, g] sw[n / 128, g] sum_{k in block g} x[m, k] w[n, k]
 //
 // x [M, K] has a scale per row and 128 columns, w [N, K] one per 128 rows and
-// 128 columns.  The tensor cores form each 128-deep block product exactly as
-// fp32 sums in tensor memory; the epilogue warps scale it and add it to fp32
-// registers while the next block's product runs into the other half of the
-// tensor memory.  One rounding, of the finished sum with the residual.
+// 128 columns.  The tensor cores form each 128-deep block product in fp32 tensor
+// memory; the epilogue warps scale it and add it to fp32 registers while the next
+// block's product runs into the other half of the tensor memory.  One rounding,
+// of the finished sum with the residual.
 //
 // Many rows (tile_kernel): tensor memory lanes are rows of x, columns are rows
-// of w, so a thread's scale is one number a block.  Persistent CTAs, one per SM.
+// of w, so a thread's scale is one number a block.  Persistent CTAs of 128 x TN
+// tiles, or pairs of CTAs (cta_group::2) of 256 x 256 tiles, each SM holding its
+// 128 rows of x and half of the rows of w: 32 instead of 48 KB a block from L2.
+// What bounds it is the turn of a half of the tensor memory: products (512 clocks
+// of 256 columns), their commit, the epilogue's read and its release; a read of
+// 256 columns also holds the products up by about 150 clocks.  Measured on the way
+// (16384 x 8256 x 5120): packed fp32 pairs in the epilogue 811 us, single ones with
+// the half released as soon as it is in registers, scales loaded four blocks ahead
+// and a release without cluster fence 695 us (1.99 PFLOP/s).
 // Few rows (split_kernel): the weights' bytes bound the call.  Lanes are 128
 // rows of w (one scale a block), columns the rows of x; the CTAs of a cluster
-// split K and add their sums in rank order through distributed shared memory.
+// split K and add their sums in rank order through distributed shared memory
+// (8 x 8256 x 5120: 11.9 us, 3.6 TB/s).
 //
 // Operands arrive by TMA (128-byte swizzle; zeros past K, M and N), one warp
-// issues the copies, one the products; every wait is bounded.
+// issues the copies, one or two the products; every wait is bounded.
 #include <cooperative_groups.h>
 #include <cudaTypedefs.h>
 
@@ -32,73 +41,112 @@ constexpr int kBlock = 128;                // depth of a scale block and of a pi
 constexpr int kEpilogueWarps = 8;
 constexpr int kCtaThreads = 32 * (kEpilogueWarps + 2);  // + copy warp, product warp
 constexpr int kRowTile = 128 * kBlock;     // bytes of a 128-row operand tile
+constexpr int kScaleGroup = 4;             // blocks whose scales are loaded together
 
 struct Sync {
     uint64_t full[8], empty[8];  // operand stages
-    uint64_t ready[2], free_[2]; // halves of the tensor memory
+    uint64_t ready[2][2], free_[2][2];  // halves of the tensor memory, column groups of each
     uint32_t tmem;
     int abort;
 };
 
-// A CTA that gives up leaves once what it issued has ended (again with a limit):
-// the copies of its last stages, the products of its last two blocks.
-__device__ __forceinline__ void drain_copies(Sync &s, int stages, int64_t count) {
+// Position in the ring of operand stages: the stage and the parity of its use.
+template <int STAGES>
+struct Ring {
+    int stage = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void next() {
+        if (++stage == STAGES) stage = 0, parity ^= 1;
+    }
+};
+
+// A copy warp that gives up leaves once the copies it issued have landed (with a
+// limit again): those of the last `count` <= STAGES stages before `at`.
+template <int STAGES>
+__device__ __forceinline__ void drain_copies(Sync &s, Ring<STAGES> at, int64_t count) {
     int never = 0;
-    for (int64_t i = max(int64_t(0), count - stages); i < count; ++i)
-        tc::bar_wait(&s.full[i % stages], uint32_t(i / stages) & 1, &never);
-}
-__device__ __forceinline__ void drain_products(Sync &s, int64_t count) {
-    int never = 0;
-    for (int64_t i = max(int64_t(0), count - 2); i < count; ++i) tc::bar_wait(&s.ready[i & 1], uint32_t(i >> 1) & 1, &never);
+    for (int i = 0; i < STAGES && i < count; ++i) {
+        if (--at.stage < 0) at.stage = STAGES - 1, at.parity ^= 1;
+        tc::bar_wait(&s.full[at.stage], at.parity, &never);
+    }
 }
 
+// G CTAs (one, or a pair) share the products, Q product warps issue them, each for
+// its group of the columns and with its share of the epilogue warps.
+template <int G, int Q>
 __device__ __forceinline__ void set_up(Sync &s, int stages, uint32_t columns, int warp) {
     if (threadIdx.x == 0) {
         for (int i = 0; i < stages; ++i) {
             tc::bar_init(&s.full[i], 1);
-            tc::bar_init(&s.empty[i], 1);
+            tc::bar_init(&s.empty[i], Q);
         }
-        for (int i = 0; i < 2; ++i) {
-            tc::bar_init(&s.ready[i], 1);
-            tc::bar_init(&s.free_[i], kEpilogueWarps);
-        }
+        for (int i = 0; i < 2; ++i)
+            for (int q = 0; q < Q; ++q) {
+                tc::bar_init(&s.ready[i][q], 1);
+                tc::bar_init(&s.free_[i][q], G * kEpilogueWarps / Q);
+            }
         s.abort = 0;
         tc::bar_init_fence();
     }
-    if (warp == kEpilogueWarps + 1) tc::tmem_alloc(&s.tmem, columns);
+    if (warp == kEpilogueWarps + 1) tc::tmem_alloc<G>(&s.tmem, columns);
     tc::fence_before();
-    __syncthreads();
+    if (G == 2) tc::cluster_sync();
+    else __syncthreads();
     tc::fence_after();
 }
 
-// The product warp's part of one block: 4 steps of 32 along K into buffer `half`.
-template <int N>
-__device__ __forceinline__ bool issue_block(Sync &s, int stages, int64_t it, uint32_t a, uint32_t b, uint32_t tmem) {
-    const int stage = int(it % stages), half = int(it & 1);
-    if (!tc::bar_wait(&s.full[stage], uint32_t(it / stages) & 1, &s.abort)) return false;
-    if (!tc::bar_wait(&s.free_[half], (uint32_t(it >> 1) & 1) ^ 1, &s.abort)) return false;
-    tc::fence_after();
+// Product warp q of Q: `count` blocks, each four steps of 32 along K into its N
+// columns of the halves of the tensor memory in turn.  The whole warp takes the
+// waits and one elected lane issues, which keeps the descriptors in uniform
+// registers.  base: shared address of the first stage's tile of x; w_rows: the
+// group's rows in the tile of w behind it.
+template <int G, int N, int STAGES, int STAGE_BYTES>
+__device__ __forceinline__ void issue_blocks(Sync &s, int q, int64_t count, uint32_t tmem, int half_columns, uint32_t base,
+                                             uint32_t w_rows) {
+    Ring<STAGES> at;
+    int64_t it = 0;
+    bool ok = true;
+    for (; it < count; ++it, at.next()) {
+        const int half = int(it) & 1;
+        const uint32_t use = uint32_t(it >> 1) & 1;
+        ok = tc::bar_wait(&s.full[at.stage], at.parity, &s.abort) && tc::bar_wait(&s.free_[half][q], use ^ 1, &s.abort);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        tc::fence_after();
+        if (tc::elected()) {
+            const uint32_t a = base + at.stage * STAGE_BYTES, b = a + kRowTile + w_rows * kBlock;
 #pragma unroll
-    for (int k = 0; k < kBlock / 32; ++k)
-        tc::mma_e4m3(tmem + half * N, tc::operand(a + 32 * k), tc::operand(b + 32 * k), tc::e4m3_product(N), k > 0);
-    tc::mma_commit(&s.empty[stage]);
-    tc::mma_commit(&s.ready[half]);
-    return true;
+            for (int k = 0; k < kBlock / 32; ++k)
+                tc::mma_e4m3<G>(tmem + half * half_columns + q * N, tc::operand(a + 32 * k), tc::operand(b + 32 * k),
+                                tc::e4m3_product(128 * G, N), k > 0);
+            tc::mma_commit<G>(&s.ready[half][q]);
+            tc::mma_commit<G>(&s.empty[at.stage]);
+        }
+        __syncwarp();
+    }
+    // A warp that gives up leaves once its last products have ended (with a limit again).
+    if (!ok) {
+        int never = 0;
+        for (int64_t i = it > 2 ? it - 2 : 0; i < it; ++i) tc::bar_wait(&s.ready[i & 1][q], uint32_t(i >> 1) & 1, &never);
+        __syncwarp();
+    }
 }
 
 // ---------------------------------------------------------------------------
 // many rows
 // ---------------------------------------------------------------------------
-constexpr int kGroupRows = 16;  // row tiles that share a sweep over the columns (operands stay in L2)
+// A third warpgroup (copy warp, two product warps and an idle one) hands registers to the two of the epilogue.
+constexpr int kTileThreads = 384, kEpilogueRegisters = 216, kIssueRegisters = 56;  // 2 x 216 + 56 <= 3 x 168
+constexpr int kGroupRows = 8;  // row tiles that share a sweep over the columns (operands stay in L2)
 
-template <int TN>
+// A CTA holds 128 rows of x and, of a pair (G = 2), half of the TN rows of w.
+template <int TN, int G>
 struct TileShape {
-    static constexpr int kStage = kRowTile + TN * kBlock;
+    static constexpr int kStage = kRowTile + TN / G * kBlock;
     static constexpr int kStaging = kEpilogueWarps * 32 * 16 * 4;
-    static constexpr int kStages = (226 * 1024 - kStaging - 1024 - int(sizeof(Sync))) / kStage > 8
-                                       ? 8 : (226 * 1024 - kStaging - 1024 - int(sizeof(Sync))) / kStage;
+    static constexpr int kRoom = (226 * 1024 - kStaging - 1024 - int(sizeof(Sync))) / kStage;
+    static constexpr int kStages = kRoom > 8 ? 8 : kRoom;
     static constexpr int kBytes = kStages * kStage + kStaging + 1024 + int(sizeof(Sync));
-    static constexpr int kColumns = 2 * TN <= 64 ? 64 : 2 * TN <= 128 ? 128 : 2 * TN <= 256 ? 256 : 512;
+    static constexpr int kColumns = 2 * TN <= 128 ? 128 : 2 * TN <= 256 ? 256 : 512;
 };
 
 // Tile `i` of the sweep: groups of kGroupRows row tiles, rows fastest within a group.
@@ -109,140 +157,205 @@ __device__ __forceinline__ int2 tile_at(int64_t i, int row_tiles, int column_til
     return make_int2(first + int(in % rows), int(in / rows));
 }
 
-template <class T, int TN>
-__global__ void __launch_bounds__(kCtaThreads, 1)
+// Four consecutive values of a row of out or residual: one access where `wide`, else the first n singly.
+template <class T>
+struct Four {
+    alignas(4 * sizeof(T)) T v[4];
+    __device__ __forceinline__ void load(const T *p, bool wide, int n) {
+        if (wide) {
+            if (sizeof(T) == 2) *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(p);
+            else *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(p);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = i < n ? p[i] : from_float<T>(0.f);
+        }
+    }
+    __device__ __forceinline__ void store(T *p, bool wide, int n) const {
+        if (wide) {
+            if (sizeof(T) == 2) *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(v);
+            else *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < n) p[i] = v[i];
+        }
+    }
+};
+
+template <class T, int TN, int G>
+__global__ void __launch_bounds__(kTileThreads, 1)
     tile_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, sq_matmul_args a,
                 bool wide) {
-    using S = TileShape<TN>;
+    using S = TileShape<TN, G>;
     extern __shared__ unsigned char raw[];
     unsigned char *base = raw + ((1024u - (tc::smem_u32(raw) & 1023u)) & 1023u);
     float *staging = reinterpret_cast<float *>(base + S::kStages * S::kStage);
-    Sync &s = *reinterpret_cast<Sync *>(base + S::kStages * S::kStage + S::kStaging);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    Sync &s = *reinterpret_cast<Sync *>(staging + S::kStaging / 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x % G;
     const int blocks = (a.hidden + kBlock - 1) / kBlock;
-    const int row_tiles = (a.rows + 127) / 128, column_tiles = (a.width + TN - 1) / TN;
-    const int64_t tiles = int64_t(row_tiles) * column_tiles;
-    set_up(s, S::kStages, S::kColumns, warp);
+    constexpr int ROWS = 128 * G;
+    const int row_tiles = (a.rows + ROWS - 1) / ROWS, column_tiles = (a.width + TN - 1) / TN;
+    const int64_t tiles = int64_t(row_tiles) * column_tiles, first = blockIdx.x / G, step = gridDim.x / G;
+    set_up<G, G>(s, S::kStages, S::kColumns, warp);
     const uint32_t tmem = s.tmem;
 
-    if (warp == kEpilogueWarps) {  // copies
-        if (lane == 0) {
-            int64_t it = 0;
-            bool ok = true;
-            for (int64_t i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
-                const int2 at = tile_at(i, row_tiles, column_tiles);
-                for (int g = 0; g < blocks; ++g, ++it) {
-                    const int stage = int(it % S::kStages);
-                    if (!(ok = tc::bar_wait(&s.empty[stage], (uint32_t(it / S::kStages) & 1) ^ 1, &s.abort))) break;
-                    unsigned char *to = base + stage * S::kStage;
-                    tc::bar_expect(&s.full[stage], S::kStage);
-                    tc::tma_load(to, &xmap, g * kBlock, at.x * 128, &s.full[stage]);
-                    tc::tma_load(to + kRowTile, &wmap, g * kBlock, at.y * TN, &s.full[stage]);
+    if (warp >= kEpilogueWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kIssueRegisters));
+        if (warp == kEpilogueWarps) {  // copies of both CTAs complete on the first one's barriers
+            if (lane == 0) {
+                Ring<S::kStages> at;
+                int64_t count = 0;
+                bool ok = true;
+                for (int64_t i = first; i < tiles && ok; i += step) {
+                    const int2 tile = tile_at(i, row_tiles, column_tiles);
+                    const int x_row = tile.x * ROWS + rank * 128, w_row = tile.y * TN + rank * (TN / 4);
+                    for (int g = 0; g < blocks; ++g, ++count, at.next()) {
+                        if (!(ok = tc::bar_wait(&s.empty[at.stage], at.parity ^ 1, &s.abort))) break;
+                        unsigned char *to = base + at.stage * S::kStage;
+                        if (rank == 0) tc::bar_expect(&s.full[at.stage], G * S::kStage);
+                        if (G == 1) {
+                            tc::tma_load(to, &xmap, g * kBlock, x_row, &s.full[at.stage]);
+                            tc::tma_load(to + kRowTile, &wmap, g * kBlock, w_row, &s.full[at.stage]);
+                        } else {
+                            const uint32_t bar = tc::in_first(&s.full[at.stage]);
+                            tc::tma_load_pair(to, &xmap, g * kBlock, x_row, bar);
+                            tc::tma_load_pair(to + kRowTile, &wmap, g * kBlock, w_row, bar);
+                            tc::tma_load_pair(to + kRowTile + TN / 4 * kBlock, &wmap, g * kBlock, w_row + TN / 2, bar);
+                        }
+                    }
                 }
+                if (!ok && rank == 0) drain_copies(s, at, count);
             }
-            if (!ok) drain_copies(s, S::kStages, it);
+            __syncwarp();
+        } else if (warp < kEpilogueWarps + 1 + G) {  // products: of a pair issued by its first CTA, a warp for each half of the columns
+            const int64_t mine = first < tiles ? (tiles - first + step - 1) / step : 0;
+            const int q = warp - kEpilogueWarps - 1;
+            if (rank == 0)
+                issue_blocks<G, TN / G, S::kStages, S::kStage>(s, q, mine * blocks, tmem, TN, tc::smem_u32(base), q * (TN / 4));
         }
-        __syncwarp();
-    } else if (warp == kEpilogueWarps + 1) {  // products
-        if (lane == 0) {
-            int64_t it = 0;
-            bool ok = true;
-            for (int64_t i = blockIdx.x; i < tiles && ok; i += gridDim.x)
-                for (int g = 0; g < blocks; ++g, ++it) {
-                    const uint32_t to = tc::smem_u32(base + int(it % S::kStages) * S::kStage);
-                    if (!(ok = issue_block<TN>(s, S::kStages, it, to, to + kRowTile, tmem))) break;
-                }
-            if (!ok) drain_products(s, it);
-        }
-        __syncwarp();
-    } else {  // scales and sums: warp w holds lanes 32 (w % 4) .. + 31, half w / 4 of the columns
+    } else {  // scales and sums: warp w holds lanes 32 (w % 4) .. + 31, half q = w / 4 of the columns
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kEpilogueRegisters));
         constexpr int C = TN / 2, CHUNKS = C / 16;
-        const uint32_t mine = tmem + (uint32_t(32 * (warp & 3)) << 16) + (warp >> 2) * C;
+        const int q = warp >> 2;  // the half of the columns
+        const uint32_t mine = tmem + (uint32_t(32 * (warp & 3)) << 16) + q * C;
+        const int group = G == 1 ? 0 : q;  // of the products
+        const uint32_t released[2] = {tc::in_first(&s.free_[0][group]), tc::in_first(&s.free_[1][group])};
         float *stage = staging + warp * 32 * 16;
+        // Scales of kScaleGroup blocks from g on, loaded that many blocks before their use (a load's way
+        // from L2 is longer than a block): the lane's row of x, and the two 128-row blocks of w that the
+        // C <= 128 columns can meet.
+        const int last = (a.width - 1) / kBlock;
+        const float *sx = nullptr, *sw0 = nullptr, *sw1 = nullptr;
+        float next_x[kScaleGroup], next_0[kScaleGroup], next_1[kScaleGroup];
+        auto aim = [&](int64_t i) {
+            const int2 at = tile_at(i, row_tiles, column_tiles);
+            const int n0 = at.y * TN + q * C;
+            sx = a.x_scale + int64_t(min(at.x * ROWS + rank * 128 + 32 * (warp & 3) + lane, a.rows - 1)) * blocks;
+            sw0 = a.w_scale + int64_t(min(n0 / kBlock, last)) * blocks;
+            sw1 = a.w_scale + int64_t(min((n0 + C - 1) / kBlock, last)) * blocks;
+        };
+        auto fetch_scales = [&](int g) {
+#pragma unroll
+            for (int q = 0; q < kScaleGroup; ++q) {
+                const int at = min(g + q, blocks - 1);
+                next_x[q] = sx[at], next_0[q] = sw0[at], next_1[q] = sw1[at];
+            }
+        };
+        if (first < tiles) {
+            aim(first);
+            fetch_scales(0);
+        }
         int64_t it = 0;
         bool ok = true;
-        for (int64_t i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
+        for (int64_t i = first; i < tiles && ok; i += step) {
             const int2 at = tile_at(i, row_tiles, column_tiles);
-            const int m0 = at.x * 128 + 32 * (warp & 3), n0 = at.y * TN + (warp >> 2) * C;
-            const float *sx = a.x_scale + int64_t(min(m0 + lane, a.rows - 1)) * blocks;
-            // The C <= 128 columns cross at most one boundary of 128-row weight blocks.
-            const int last = (a.width - 1) / kBlock;
-            const float *sw0 = a.w_scale + int64_t(min(n0 / kBlock, last)) * blocks;
-            const float *sw1 = a.w_scale + int64_t(min((n0 + C - 1) / kBlock, last)) * blocks;
-            const int cross = (kBlock - n0 % kBlock) / 16;  // first chunk of the second block
-            uint64_t acc[C / 2];
+            const int m0 = at.x * ROWS + rank * 128 + 32 * (warp & 3), n0 = at.y * TN + q * C;
+            const int cross = (kBlock - n0 % kBlock) / 16;  // first chunk of the second block of w
+            float acc[C];
 #pragma unroll
-            for (int j = 0; j < C / 2; ++j) acc[j] = 0;
-            float fx = sx[0], f0 = sw0[0], f1 = sw1[0];
+            for (int j = 0; j < C; ++j) acc[j] = 0.f;
+            float s0[kScaleGroup], s1[kScaleGroup];
             for (int g = 0; g < blocks; ++g, ++it) {
-                const float s0 = fx * f0, s1 = fx * f1;
-                if (g + 1 < blocks) fx = sx[g + 1], f0 = sw0[g + 1], f1 = sw1[g + 1];
-                ok = __all_sync(0xffffffffu, tc::bar_wait(&s.ready[it & 1], uint32_t(it >> 1) & 1, &s.abort));
+                if (g % kScaleGroup == 0) {
+#pragma unroll
+                    for (int q = 0; q < kScaleGroup; ++q) s0[q] = next_x[q] * next_0[q], s1[q] = next_x[q] * next_1[q];
+                    fetch_scales(g + kScaleGroup);
+                }
+                const float f0 = s0[0], f1 = s1[0];
+#pragma unroll
+                for (int q = 0; q + 1 < kScaleGroup; ++q) s0[q] = s0[q + 1], s1[q] = s1[q + 1];
+                ok = __all_sync(0xffffffffu, tc::bar_wait(&s.ready[it & 1][group], uint32_t(it >> 1) & 1, &s.abort));
                 if (!ok) break;
                 tc::fence_after();
                 const uint32_t from = mine + int(it & 1) * TN;
+                // The next 16 columns are on their way while 16 are added; the half is free once all are in registers.
                 uint32_t r[2][16];
                 tc::tmem_load(from, r[0]);
 #pragma unroll
                 for (int c = 0; c < CHUNKS; ++c) {
                     tc::tmem_wait(r[c & 1]);
-                    if (c + 1 < CHUNKS) tc::tmem_load(from + 16 * (c + 1), r[(c + 1) & 1]);
-                    const float f = c < cross ? s0 : s1;
-                    const uint64_t ff = tc::pair(f, f);
+                    if (c + 1 < CHUNKS) {
+                        tc::tmem_load(from + 16 * (c + 1), r[(c + 1) & 1]);
+                    } else {
+                        tc::fence_before();
+                        __syncwarp();
+                        if (lane == 0) tc::bar_arrive_cluster(released[it & 1]);
+                    }
+                    const float f = c < cross ? f0 : f1;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) tc::fma2(acc[8 * c + j], r[c & 1][2 * j], r[c & 1][2 * j + 1], ff);
+                    for (int j = 0; j < 16; ++j) acc[16 * c + j] = fmaf(__uint_as_float(r[c & 1][j]), f, acc[16 * c + j]);
                 }
-                tc::fence_before();
-                __syncwarp();
-                if (lane == 0) tc::bar_arrive(&s.free_[it & 1]);
             }
             if (!ok) break;
-            // Out through shared memory, 16 columns at a time: a row's 16 values leave by four lanes.
+            if (i + step < tiles) {
+                aim(i + step);
+                fetch_scales(0);
+            }
+            // Out through shared memory, 16 columns at a time: a row's 16 values leave by four lanes
+            // (four rows of eight per access), the residual's next 16 columns on their way meanwhile.
             // 16-byte pieces of row r are rotated by r / 2 so that neither side meets bank conflicts.
+            const T *residual = static_cast<const T *>(a.residual);
+            Four<T> old[4];
+            auto fetch = [&](int c) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int m = m0 + q * 8 + (lane >> 2), n = n0 + 16 * c + 4 * (lane & 3);
+                    if (residual && m < a.rows && n < a.width)
+                        old[q].load(residual + int64_t(m) * a.residual_stride + n, wide, a.width - n);
+                }
+            };
+            fetch(0);
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c) {
                 __syncwarp();
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float2 lo = tc::unpair(acc[8 * c + 2 * j]), hi = tc::unpair(acc[8 * c + 2 * j + 1]);
-                    *reinterpret_cast<float4 *>(stage + lane * 16 + ((j + (lane >> 1)) & 3) * 4) = make_float4(lo.x, lo.y, hi.x, hi.y);
+                    const float *v = acc + 16 * c + 4 * j;
+                    *reinterpret_cast<float4 *>(stage + lane * 16 + ((j + (lane >> 1)) & 3) * 4) = make_float4(v[0], v[1], v[2], v[3]);
                 }
                 __syncwarp();
+                Four<T> add[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) add[q] = old[q];
+                if (c + 1 < CHUNKS) fetch(c + 1);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int row = q * 8 + (lane >> 2), m = m0 + row, n = n0 + 16 * c + 4 * (lane & 3);
                     const float4 v = *reinterpret_cast<const float4 *>(stage + row * 16 + (((lane & 3) + (row >> 1)) & 3) * 4);
-                    float x[4] = {v.x, v.y, v.z, v.w};
-                    if (m >= a.rows || n >= a.width) continue;
-                    const T *res = a.residual ? static_cast<const T *>(a.residual) + int64_t(m) * a.residual_stride + n : nullptr;
-                    T *out = static_cast<T *>(a.out) + int64_t(m) * a.width + n;
-                    if (wide) {
-                        T y[4];
-                        if (res) {
-                            T old[4];
-                            if (sizeof(T) == 2) *reinterpret_cast<uint2 *>(old) = *reinterpret_cast<const uint2 *>(res);
-                            else *reinterpret_cast<uint4 *>(old) = *reinterpret_cast<const uint4 *>(res);
+                    const float x[4] = {v.x, v.y, v.z, v.w};
+                    Four<T> y;
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) x[j] += to_float(old[j]);
-                        }
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) y[j] = from_float<T>(x[j]);
-                        if (sizeof(T) == 2) *reinterpret_cast<uint2 *>(out) = *reinterpret_cast<const uint2 *>(y);
-                        else *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<const uint4 *>(y);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (n + j < a.width) out[j] = from_float<T>(res ? x[j] + to_float(res[j]) : x[j]);
-                    }
+                    for (int j = 0; j < 4; ++j) y.v[j] = from_float<T>(residual ? x[j] + to_float(add[q].v[j]) : x[j]);
+                    if (m < a.rows && n < a.width) y.store(static_cast<T *>(a.out) + int64_t(m) * a.width + n, wide, a.width - n);
                 }
             }
         }
     }
     tc::fence_before();
-    __syncthreads();
+    tc::cluster_sync();  // the pair's last arrivals and products are over
     tc::fence_after();
     if (s.abort && threadIdx.x == 0) flag(a.status, SQ_STATUS_TIMEOUT);
-    if (warp == kEpilogueWarps + 1) tc::tmem_free(tmem, S::kColumns);
+    if (warp == kEpilogueWarps + 1) tc::tmem_free<G>(tmem, S::kColumns);
 }
 
 // ---------------------------------------------------------------------------
@@ -252,118 +365,130 @@ template <int TM>
 struct SplitShape {
     static constexpr int kStage = kRowTile + TM * kBlock;
     static constexpr int kStages = 98304 / kStage;  // 5, 4, 4, 3: two CTAs an SM
-    static constexpr int kBytes = kStages * kStage + 2 * TM * 4 + 1024 + int(sizeof(Sync));
+    static constexpr int kScales = 2 * kScaleGroup * TM * 4;  // of two groups of blocks
+    static constexpr int kBytes = kStages * kStage + kScales + 1024 + int(sizeof(Sync));
     static constexpr int kColumns = 2 * TM;
 };
 
 template <class T, int TM>
 __global__ void __launch_bounds__(kCtaThreads, 2)
-    split_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, sq_matmul_args a) {
+    split_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, sq_matmul_args a,
+                 bool wide) {
     using S = SplitShape<TM>;
     namespace cg = cooperative_groups;
     extern __shared__ unsigned char raw[];
     unsigned char *base = raw + ((1024u - (tc::smem_u32(raw) & 1023u)) & 1023u);
-    float *factor = reinterpret_cast<float *>(base + S::kStages * S::kStage);  // [2][TM]
-    Sync &s = *reinterpret_cast<Sync *>(factor + 2 * TM);
+    float *ring = reinterpret_cast<float *>(base + S::kStages * S::kStage);  // [2][kScaleGroup][TM]
+    Sync &s = *reinterpret_cast<Sync *>(ring + S::kScales / 4);
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = int(cluster.num_blocks()), rank = int(cluster.block_rank());
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int blocks = (a.hidden + kBlock - 1) / kBlock;
     const int g0 = int(int64_t(blocks) * rank / ranks), g1 = int(int64_t(blocks) * (rank + 1) / ranks);
     const int n0 = int(blockIdx.x) / ranks * 128, m0 = blockIdx.y * TM;
-    set_up(s, S::kStages, S::kColumns, warp);
+    set_up<1, 1>(s, S::kStages, S::kColumns, warp);
     const uint32_t tmem = s.tmem;
     float *sums = reinterpret_cast<float *>(base);  // [TM][128], once the operands are consumed
 
     if (warp == kEpilogueWarps) {
         if (lane == 0) {
+            Ring<S::kStages> at;
             bool ok = true;
-            int it = 0;
-            for (; it < g1 - g0; ++it) {
-                const int stage = it % S::kStages;
-                if (!(ok = tc::bar_wait(&s.empty[stage], (uint32_t(it / S::kStages) & 1) ^ 1, &s.abort))) break;
-                unsigned char *to = base + stage * S::kStage;
-                tc::bar_expect(&s.full[stage], S::kStage);
-                tc::tma_load(to, &wmap, (g0 + it) * kBlock, n0, &s.full[stage]);
-                tc::tma_load(to + kRowTile, &xmap, (g0 + it) * kBlock, m0, &s.full[stage]);
+            int g = g0;
+            for (; g < g1; ++g, at.next()) {
+                if (!(ok = tc::bar_wait(&s.empty[at.stage], at.parity ^ 1, &s.abort))) break;
+                unsigned char *to = base + at.stage * S::kStage;
+                tc::bar_expect(&s.full[at.stage], S::kStage);
+                tc::tma_load(to, &wmap, g * kBlock, n0, &s.full[at.stage]);
+                tc::tma_load(to + kRowTile, &xmap, g * kBlock, m0, &s.full[at.stage]);
             }
-            if (!ok) drain_copies(s, S::kStages, it);
+            if (!ok) drain_copies(s, at, g - g0);
         }
         __syncwarp();
-    } else if (warp == kEpilogueWarps + 1) {
-        if (lane == 0) {
-            bool ok = true;
-            int it = 0;
-            for (; it < g1 - g0; ++it) {
-                const uint32_t to = tc::smem_u32(base + it % S::kStages * S::kStage);
-                if (!(ok = issue_block<TM>(s, S::kStages, it, to, to + kRowTile, tmem))) break;
-            }
-            if (!ok) drain_products(s, it);
-        }
-        __syncwarp();
+    } else if (warp > kEpilogueWarps) {
+        issue_blocks<1, TM, S::kStages, S::kStage>(s, 0, g1 - g0, tmem, TM, tc::smem_u32(base), 0);
     } else {
         constexpr int C = TM / 2, W = C < 16 ? C : 16, CHUNKS = C / W;
         const int tid = threadIdx.x, half = warp >> 2;
         const uint32_t mine = tmem + (uint32_t(32 * (warp & 3)) << 16) + half * C;
+        // Scales of kScaleGroup blocks, a column of a block each: loaded while the group before is worked on.
+        constexpr int EACH = (kScaleGroup * TM + 32 * kEpilogueWarps - 1) / (32 * kEpilogueWarps);
         const float *sw = a.w_scale + int64_t(n0 / kBlock) * blocks;
-        const float *sx = a.x_scale + int64_t(min(m0 + tid % TM, a.rows - 1)) * blocks;
-        uint64_t acc[C / 2];
+        float next[EACH];
+        auto fetch_scales = [&](int g) {
 #pragma unroll
-        for (int j = 0; j < C / 2; ++j) acc[j] = 0;
-        float next = tid < TM && g0 < g1 ? sx[g0] * sw[g0] : 0.f;
-        for (int it = 0; it < g1 - g0; ++it) {
-            // Scales of the block's columns, one thread each; the barrier also says that every warp
-            // has left the buffer of two blocks ago.
-            if (tid < TM) {
-                factor[(it & 1) * TM + tid] = next;
-                if (g0 + it + 1 < g1) next = sx[g0 + it + 1] * sw[g0 + it + 1];
+            for (int e = 0; e < EACH; ++e) {
+                const int i = e * 32 * kEpilogueWarps + tid, at = min(g + i / TM, blocks - 1);
+                if (i < kScaleGroup * TM) next[e] = a.x_scale[int64_t(min(m0 + i % TM, a.rows - 1)) * blocks + at] * sw[at];
             }
-            asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kEpilogueWarps) : "memory");
-            tc::bar_wait(&s.ready[it & 1], uint32_t(it >> 1) & 1, &s.abort);  // giving up: the sums are not used
+        };
+        fetch_scales(g0);
+        float acc[C];
+#pragma unroll
+        for (int j = 0; j < C; ++j) acc[j] = 0.f;
+        for (int it = 0; it < g1 - g0; ++it) {
+            const float *group = ring + (it / kScaleGroup & 1) * kScaleGroup * TM;
+            if (it % kScaleGroup == 0) {
+#pragma unroll
+                for (int e = 0; e < EACH; ++e) {
+                    const int i = e * 32 * kEpilogueWarps + tid;
+                    if (i < kScaleGroup * TM) const_cast<float *>(group)[i] = next[e];
+                }
+                fetch_scales(g0 + it + kScaleGroup);
+                // The group's scales are there for all, and all are done with those of two groups ago.
+                asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kEpilogueWarps) : "memory");
+            }
+            tc::bar_wait(&s.ready[it & 1][0], uint32_t(it >> 1) & 1, &s.abort);  // giving up: the sums are not used
             __syncwarp();
             tc::fence_after();
             const uint32_t from = mine + (it & 1) * TM;
-            const float *f = factor + (it & 1) * TM + half * C;
-            uint32_t r[2][W];
-            tc::tmem_load(from, r[0]);
+            const float *f = group + it % kScaleGroup * TM + half * C;
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c) {
-                tc::tmem_wait(r[c & 1]);
-                if (c + 1 < CHUNKS) tc::tmem_load(from + W * (c + 1), r[(c + 1) & 1]);
+                uint32_t r[W];
+                tc::tmem_load(from + W * c, r);
+                tc::tmem_wait(r);
 #pragma unroll
-                for (int j = 0; j < W / 4; ++j) {
-                    const float4 v = *reinterpret_cast<const float4 *>(f + W * c + 4 * j);
-                    tc::fma2(acc[W / 2 * c + 2 * j], r[c & 1][4 * j], r[c & 1][4 * j + 1], tc::pair(v.x, v.y));
-                    tc::fma2(acc[W / 2 * c + 2 * j + 1], r[c & 1][4 * j + 2], r[c & 1][4 * j + 3], tc::pair(v.z, v.w));
+                for (int j = 0; j < W; j += 4) {
+                    const float4 v = *reinterpret_cast<const float4 *>(f + W * c + j);
+                    float *sum = acc + W * c + j;
+                    sum[0] = fmaf(__uint_as_float(r[j]), v.x, sum[0]);
+                    sum[1] = fmaf(__uint_as_float(r[j + 1]), v.y, sum[1]);
+                    sum[2] = fmaf(__uint_as_float(r[j + 2]), v.z, sum[2]);
+                    sum[3] = fmaf(__uint_as_float(r[j + 3]), v.w, sum[3]);
                 }
             }
             tc::fence_before();
             __syncwarp();
-            if (lane == 0) tc::bar_arrive(&s.free_[it & 1]);
+            if (lane == 0) tc::bar_arrive(&s.free_[it & 1][0]);
         }
         // Every product has been read from tensor memory, hence every operand by the tensor cores.
         if (!s.abort) {
 #pragma unroll
-            for (int j = 0; j < C / 2; ++j) {
-                const float2 v = tc::unpair(acc[j]);
-                sums[(half * C + 2 * j) * 128 + 32 * (warp & 3) + lane] = v.x;
-                sums[(half * C + 2 * j + 1) * 128 + 32 * (warp & 3) + lane] = v.y;
-            }
+            for (int j = 0; j < C; ++j) sums[(half * C + j) * 128 + 32 * (warp & 3) + lane] = acc[j];
         }
     }
     tc::fence_before();
     cluster.sync();
     tc::fence_after();
-    if (warp == kEpilogueWarps + 1) tc::tmem_free(tmem, S::kColumns);
-    // The sums of the ranks, in their order; each rank finishes its share of the rows of x.
-    const int first = TM * rank / ranks, count = TM * (rank + 1) / ranks - first;
-    for (int i = threadIdx.x; i < count * 128; i += kCtaThreads) {
-        const int m = m0 + first + i / 128, n = n0 + i % 128;
+    if (warp == kEpilogueWarps + 1) tc::tmem_free<1>(tmem, S::kColumns);
+    // The sums of the ranks, in their order; each rank finishes its share of the rows of x, four columns a thread.
+    const int share = TM * rank / ranks, count = TM * (rank + 1) / ranks - share;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < count * 32; i += kCtaThreads) {
+        const int m = m0 + share + i / 32, n = n0 + i % 32 * 4;
         if (m >= a.rows || n >= a.width) continue;
-        float v = 0.f;
-        for (int q = 0; q < ranks; ++q) v += cluster.map_shared_rank(sums, q)[first * 128 + i];
-        if (a.residual) v += to_float(static_cast<const T *>(a.residual)[int64_t(m) * a.residual_stride + n]);
-        static_cast<T *>(a.out)[int64_t(m) * a.width + n] = from_float<T>(v);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int q = 0; q < ranks; ++q) {
+            const float4 part = reinterpret_cast<const float4 *>(cluster.map_shared_rank(sums, q))[share * 32 + i];
+            v.x += part.x, v.y += part.y, v.z += part.z, v.w += part.w;
+        }
+        const float x[4] = {v.x, v.y, v.z, v.w};
+        Four<T> old, y;
+        if (a.residual) old.load(static_cast<const T *>(a.residual) + int64_t(m) * a.residual_stride + n, wide, a.width - n);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y.v[j] = from_float<T>(a.residual ? x[j] + to_float(old.v[j]) : x[j]);
+        y.store(static_cast<T *>(a.out) + int64_t(m) * a.width + n, wide, a.width - n);
     }
     if (s.abort && threadIdx.x == 0) flag(a.status, SQ_STATUS_TIMEOUT);
     cluster.sync();
@@ -396,21 +521,36 @@ bool byte_map(CUtensorMap *map, const void *p, int hidden, int rows, int64_t str
                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class T, int TN>
+template <class K, class... A>
+int32_t launch_clusters(K kernel, dim3 grid, int threads, int cluster, int bytes, cudaStream_t s, A... args) {
+    cudaLaunchConfig_t c{};
+    c.gridDim = grid;
+    c.blockDim = dim3(unsigned(threads));
+    c.dynamicSmemBytes = bytes;
+    c.stream = s;
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = unsigned(cluster);
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    c.attrs = &attribute;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, args...) == cudaSuccess ? SQ_OK : SQ_ERR_CUDA;
+}
+
+template <class T, int TN, int G>
 int32_t launch_tile(const sq_matmul_args &a, bool wide, int sms, cudaStream_t s) {
-    using S = TileShape<TN>;
+    using S = TileShape<TN, G>;
     CUtensorMap x, w;
-    if (!byte_map(&x, a.x, a.hidden, a.rows, a.x_stride, 128) || !byte_map(&w, a.w, a.hidden, a.width, a.w_stride, TN))
+    if (!byte_map(&x, a.x, a.hidden, a.rows, a.x_stride, 128) || !byte_map(&w, a.w, a.hidden, a.width, a.w_stride, G == 1 ? TN : TN / 4))
         return SQ_ERR_CUDA;
-    if (cudaFuncSetAttribute(tile_kernel<T, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess)
+    if (cudaFuncSetAttribute(tile_kernel<T, TN, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess)
         return SQ_ERR_CUDA;
-    const int64_t tiles = int64_t((a.rows + 127) / 128) * ((a.width + TN - 1) / TN);
-    tile_kernel<T, TN><<<unsigned(tiles < sms ? tiles : sms), kCtaThreads, S::kBytes, s>>>(x, w, a, wide);
-    return cudaGetLastError() == cudaSuccess ? SQ_OK : SQ_ERR_CUDA;
+    const int64_t tiles = int64_t((a.rows + 128 * G - 1) / (128 * G)) * ((a.width + TN - 1) / TN), most = sms > G ? sms / G : 1;
+    return launch_clusters(tile_kernel<T, TN, G>, dim3(unsigned(G * (tiles < most ? tiles : most))), kTileThreads, G, S::kBytes, s, x, w, a, wide);
 }
 
 template <class T, int TM>
-int32_t launch_split(const sq_matmul_args &a, int sms, cudaStream_t s) {
+int32_t launch_split(const sq_matmul_args &a, bool wide, int sms, cudaStream_t s) {
     using S = SplitShape<TM>;
     CUtensorMap x, w;
     if (!byte_map(&x, a.x, a.hidden, a.rows, a.x_stride, TM) || !byte_map(&w, a.w, a.hidden, a.width, a.w_stride, 128))
@@ -421,18 +561,7 @@ int32_t launch_split(const sq_matmul_args &a, int sms, cudaStream_t s) {
     // K is split while two CTAs an SM are not in use and each keeps two blocks.
     int split = 8;
     while (split > 1 && (int64_t(columns) * rows * split > 2 * sms || blocks < 2 * split)) split /= 2;
-    cudaLaunchConfig_t c{};
-    c.gridDim = dim3(unsigned(columns * split), unsigned(rows));
-    c.blockDim = dim3(kCtaThreads);
-    c.dynamicSmemBytes = S::kBytes;
-    c.stream = s;
-    cudaLaunchAttribute cluster;
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = unsigned(split);
-    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-    c.attrs = &cluster;
-    c.numAttrs = 1;
-    return cudaLaunchKernelEx(&c, split_kernel<T, TM>, x, w, a) == cudaSuccess ? SQ_OK : SQ_ERR_CUDA;
+    return launch_clusters(split_kernel<T, TM>, dim3(unsigned(columns * split), unsigned(rows)), kCtaThreads, split, S::kBytes, s, x, w, a, wide);
 }
 
 template <class T>
@@ -440,24 +569,27 @@ int32_t launch_matmul(const sq_matmul_args &a, int sms, cudaStream_t s) {
     const int64_t size = sizeof(T);
     auto rows4 = [&](const void *p, int64_t stride) { return reinterpret_cast<uintptr_t>(p) % (4 * size) == 0 && stride % 4 == 0; };
     const bool wide = a.width % 4 == 0 && rows4(a.out, a.width) && (!a.residual || rows4(a.residual, a.residual_stride));
-    if (a.rows <= 16) return launch_split<T, 16>(a, sms, s);
-    if (a.rows <= 32) return launch_split<T, 32>(a, sms, s);
-    if (a.rows <= 64) return launch_split<T, 64>(a, sms, s);
-    if (a.rows <= 128) return launch_split<T, 128>(a, sms, s);
-    // The column tile whose waves of tiles cost least, a tile costing its operand bytes.
-    int best = 256;
+    if (a.rows <= 16) return launch_split<T, 16>(a, wide, sms, s);
+    if (a.rows <= 32) return launch_split<T, 32>(a, wide, sms, s);
+    if (a.rows <= 64) return launch_split<T, 64>(a, wide, sms, s);
+    if (a.rows <= 128) return launch_split<T, 128>(a, wide, sms, s);
+    // The tile whose waves take least: a block of 128 x TN (or, of a pair, 256 x TN) took 288 + 1.3 TN ns
+    // a wave, measured from TN = 64 (371) to 256 (620; the pair 598, so it has the tie).
+    int best = 0;
     int64_t least = INT64_MAX;
-    for (int tn : {256, 192, 160, 128, 96, 64}) {
-        const int64_t tiles = int64_t((a.rows + 127) / 128) * ((a.width + tn - 1) / tn), cost = (tiles + sms - 1) / sms * (128 + tn);
-        if (cost < least) least = cost, best = tn;
+    for (int tile : {512, 256, 192, 160, 128, 64}) {
+        const int group = tile == 512 ? 2 : 1, tn = tile == 512 ? 256 : tile, room = sms > group ? sms / group : 1;
+        const int64_t tiles = int64_t((a.rows + 128 * group - 1) / (128 * group)) * ((a.width + tn - 1) / tn);
+        const int64_t cost = (tiles + room - 1) / room * (2880 + 13 * tn);
+        if (cost < least) least = cost, best = tile;
     }
     switch (best) {
-        case 256: return launch_tile<T, 256>(a, wide, sms, s);
-        case 192: return launch_tile<T, 192>(a, wide, sms, s);
-        case 160: return launch_tile<T, 160>(a, wide, sms, s);
-        case 128: return launch_tile<T, 128>(a, wide, sms, s);
-        case 96: return launch_tile<T, 96>(a, wide, sms, s);
-        default: return launch_tile<T, 64>(a, wide, sms, s);
+        case 512: return launch_tile<T, 256, 2>(a, wide, sms, s);
+        case 256: return launch_tile<T, 256, 1>(a, wide, sms, s);
+        case 192: return launch_tile<T, 192, 1>(a, wide, sms, s);
+        case 160: return launch_tile<T, 160, 1>(a, wide, sms, s);
+        case 128: return launch_tile<T, 128, 1>(a, wide, sms, s);
+        default: return launch_tile<T, 64, 1>(a, wide, sms, s);
     }
 }
 

@@ -8,7 +8,7 @@
 namespace sq {
 namespace tc {
 
-constexpr uint64_t kWaitNs = 2000000000;  // a wait gives up after two seconds
+constexpr int64_t kWaitClocks = int64_t(1) << 32;  // a wait gives up after about two seconds
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
@@ -22,29 +22,32 @@ __device__ __forceinline__ void bar_expect(uint64_t *bar, uint32_t bytes) {
 __device__ __forceinline__ void bar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ uint64_t now_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %globaltimer;\n" : "=l"(t));
-    return t;
-}
-// Waits for the phase of `parity`; false when kWaitNs ran out (sets `abort`) or another warp set `abort`.
+// Waits for the phase of `parity`; false when kWaitClocks ran out (sets `abort`) or another warp set `abort`.
+// (The cycle counter bounds it: a read of the global timer takes longer than a block's products.)
 __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatile int *abort) {
-    uint64_t since = 0;
-    for (uint32_t it = 0;; ++it) {
+    int64_t since = 0;
+    for (uint32_t it = 1;; ++it) {
         uint32_t done;
         asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
                      : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
         if (done) return true;
-        if (*abort) return false;
         if ((it & 15) == 0) {
-            const uint64_t now = now_ns();
+            if (*abort) return false;
+            const int64_t now = clock64();
             if (since == 0) since = now;
-            if (now - since > kWaitNs) {
+            if (now - since > kWaitClocks) {
                 *abort = 1;
                 return false;
             }
         }
     }
+}
+
+// One lane of the (converged) warp.
+__device__ __forceinline__ bool elected() {
+    uint32_t r;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r != 0;
 }
 
 // Box of a 2-D tensor map at (x, y) into shared memory, completing on `bar`.
@@ -53,26 +56,64 @@ __device__ __forceinline__ void tma_load(void *dst, const CUtensorMap *map, int 
                  ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
 }
 
+// Address of the same barrier in the first CTA of the cluster.
+__device__ __forceinline__ uint32_t in_first(const uint64_t *bar) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(bar)));
+    return r;
+}
+__device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+// The same load by either CTA of a pair, completing on a barrier of the first.
+__device__ __forceinline__ void tma_load_pair(void *dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+
 // K-major operand tile of 128-byte rows under the 128-byte swizzle, 8-row groups of 1024 bytes.
 __device__ __forceinline__ uint64_t operand(uint32_t addr) {
     return uint64_t((addr >> 4) & 0x3FFF) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-// e4m3 x e4m3 -> fp32, M = 128, both operands K-major.
-__device__ __forceinline__ constexpr uint32_t e4m3_product(int n) { return (1u << 4) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24); }
+// e4m3 x e4m3 -> fp32, both operands K-major.
+__device__ __forceinline__ constexpr uint32_t e4m3_product(int m, int n) { return (1u << 4) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24); }
 
+// G = 2: one lane of the pair's first CTA issues for both; a commit arrives on both CTAs' barriers.
+template <int G>
 __device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)) : "memory");
+    if (G == 1)
+        asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)) : "memory");
+    else
+        asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)) : "memory");
 }
+template <int G>
 __device__ __forceinline__ void mma_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar)) : "memory");
+    if (G == 1)
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar)) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
+                     ::"r"(smem_u32(bar)), "h"(uint16_t(3)) : "memory");
 }
+template <int G>
 __device__ __forceinline__ void tmem_alloc(uint32_t *slot, uint32_t columns) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(slot)), "r"(columns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+    if (G == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(slot)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(slot)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n");
+    }
 }
+template <int G>
 __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t columns) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(addr), "r"(columns));
+    if (G == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(addr), "r"(columns));
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(addr), "r"(columns));
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
@@ -94,23 +135,6 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&r)[N]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
     for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
-}
-
-// Two fp32 multiply-adds: (a.lo, a.hi) += (x, y) * (f, g).
-__device__ __forceinline__ void fma2(uint64_t &acc, uint32_t x, uint32_t y, uint64_t factors) {
-    uint64_t v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(x), "r"(y));
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(v), "l"(factors));
-}
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-    uint64_t v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-    return v;
-}
-__device__ __forceinline__ float2 unpair(uint64_t v) {
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-    return f;
 }
 
 }  // namespace tc
