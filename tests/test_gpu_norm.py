@@ -68,6 +68,25 @@ def test_norm(rows, hidden, dtype, with_residual):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,hidden", [(2047, 1024), (2048, 520), (2049, 1000), (3001, 5120), (2500, 8192), (2100, 8200),
+                                         (2100, 16384), (2100, 2052)])
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_many_rows(rows, hidden, dtype, with_residual):
+    """Batches that take the persistent kernel (16-byte aligned rows) and those beside it, rows of a wider tensor."""
+    from stepquant_b200.kernels.norm import rms_norm, rms_norm_fp8
+    x, residual, weight = _data(rows, hidden + 8, dtype, 5)
+    x, weight = x[:, 8:], weight[8:].float()
+    residual = residual[:, :hidden] if with_residual else None
+    h, y = _reference(x, weight, residual)
+    got, got8 = rms_norm(x, weight, residual), rms_norm_fp8(x, weight, residual)
+    if with_residual:
+        want = h.to(dtype) if dtype != torch.float32 else x + residual
+        assert torch.equal(got[1], want) and torch.equal(got8[2], want)
+    _close(got[0] if with_residual else got, y, dtype)
+    _close_fp8(got8[0], got8[1], y)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("rows,hidden", [(1, 1), (7, 130), (3, 4096), (640, 5120)])
 def test_quantize(rows, hidden, dtype):
     from stepquant_b200.kernels.norm import quantize_fp8
