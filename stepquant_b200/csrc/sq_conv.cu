@@ -64,7 +64,7 @@ struct Filter {
     }
 };
 
-template <class T, int VEC, int W>
+template <class T, int VEC, int W, bool SILU>
 __global__ void __launch_bounds__(kConvThreads) conv_kernel(sq_conv_args a, int strip) {
     using Token = Run<T, VEC, VEC>;
     constexpr int BATCH = 8;  // tokens in flight a thread, while the batch before is worked on
@@ -90,9 +90,10 @@ __global__ void __launch_bounds__(kConvThreads) conv_kernel(sq_conv_args a, int 
     const T *old = a.initial_state ? static_cast<const T *>(a.initial_state) + state : nullptr;
     Token next[BATCH], now[BATCH];
     auto fetch = [&](int t) {
+        const T *from = x + int64_t(t) * a.x_stride;
 #pragma unroll
-        for (int j = 0; j < BATCH; ++j)
-            if (t + j < t1) next[j].load(x + int64_t(t + j) * a.x_stride);
+        for (int j = 0; j < BATCH; ++j, from += a.x_stride)
+            if (t + j < t1) next[j].load(from);
     };
     fetch(t0);
     const Filter<VEC, W> f(a, d0);
@@ -124,27 +125,33 @@ __global__ void __launch_bounds__(kConvThreads) conv_kernel(sq_conv_args a, int 
         }
         fin.store(static_cast<T *>(a.final_state) + state);
     }
+    auto token = [&](int t, const Token &in) {
+        Token out;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const float x_t = to_float(in.v[i]);
+            float s = f.bias[i];
+#pragma unroll
+            for (int k = 0; k < W - 1; ++k) s = fmaf(f.w[i * W + k], kept[k][i], s);
+            s = fmaf(f.w[i * W + W - 1], x_t, s);
+            out.v[i] = from_float<T>(SILU ? silu(s) : s);
+#pragma unroll
+            for (int k = 0; k + 1 < W - 1; ++k) kept[k][i] = kept[k + 1][i];
+            kept[W - 2][i] = x_t;
+        }
+        out.store(y + int64_t(t) * a.channels);
+    };
     for (int t = t0; t < t1; t += BATCH) {
 #pragma unroll
         for (int j = 0; j < BATCH; ++j) now[j] = next[j];
         fetch(t + BATCH);
+        if (t + BATCH <= t1) {  // no branch between the tokens of a whole batch
 #pragma unroll
-        for (int j = 0; j < BATCH; ++j) {
-            if (t + j >= t1) break;
-            Token out;
+            for (int j = 0; j < BATCH; ++j) token(t + j, now[j]);
+        } else {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float in = to_float(now[j].v[i]);
-                float s = f.bias[i];
-#pragma unroll
-                for (int k = 0; k < W - 1; ++k) s = fmaf(f.w[i * W + k], kept[k][i], s);
-                s = fmaf(f.w[i * W + W - 1], in, s);
-                out.v[i] = from_float<T>(a.silu ? silu(s) : s);
-#pragma unroll
-                for (int k = 0; k + 1 < W - 1; ++k) kept[k][i] = kept[k + 1][i];
-                kept[W - 2][i] = in;
-            }
-            out.store(y + int64_t(t + j) * a.channels);
+            for (int j = 0; j < BATCH; ++j)
+                if (t + j < t1) token(t + j, now[j]);
         }
     }
 }
@@ -194,7 +201,9 @@ cudaError_t launch_conv_as(const sq_conv_args &a, bool step, cudaStream_t s) {
     // Strips of 64 tokens; shorter ones while the grid would leave SMs idle.
     int strip = 64;
     while (strip > 8 && int64_t(a.tokens / strip + a.num_seqs) * columns < 148 * 8) strip /= 2;
-    conv_kernel<T, VEC, W><<<dim3(unsigned(a.tokens / strip + a.num_seqs), columns), kConvThreads, 0, s>>>(a, strip);
+    const dim3 grid(unsigned(a.tokens / strip + a.num_seqs), columns);
+    if (a.silu) conv_kernel<T, VEC, W, true><<<grid, kConvThreads, 0, s>>>(a, strip);
+    else conv_kernel<T, VEC, W, false><<<grid, kConvThreads, 0, s>>>(a, strip);
     return cudaGetLastError();
 }
 
