@@ -159,9 +159,10 @@ __global__ void __launch_bounds__(kConvThreads) conv_kernel(sq_conv_args a, int 
 // One token of each request: the state row shifts by one input.
 template <class T, int VEC, int W>
 __global__ void __launch_bounds__(kConvThreads) conv_step_kernel(sq_conv_args a) {
-    const int d0 = (blockIdx.y * kConvThreads + threadIdx.x) * VEC;
+    // Neighbouring CTAs take neighbouring channels of a request.
+    const unsigned columns = (unsigned(a.channels) + kConvThreads * VEC - 1) / (kConvThreads * VEC), n = blockIdx.x / columns;
+    const int d0 = ((blockIdx.x - n * columns) * kConvThreads + threadIdx.x) * VEC;
     if (d0 >= a.channels) return;
-    const int n = blockIdx.x;
     const int64_t row = state_row(a.slots, n, a.num_slots, a.status);
     Run<T, VEC, VEC> in, out;
     T *y = static_cast<T *>(a.y) + int64_t(n) * a.channels + d0;
@@ -195,7 +196,8 @@ template <class T, int VEC, int W>
 cudaError_t launch_conv_as(const sq_conv_args &a, bool step, cudaStream_t s) {
     const unsigned columns = unsigned((int64_t(a.channels) + kConvThreads * VEC - 1) / (kConvThreads * VEC));
     if (step) {
-        conv_step_kernel<T, VEC, W><<<dim3(unsigned(a.num_seqs), columns), kConvThreads, 0, s>>>(a);
+        if (int64_t(a.num_seqs) * columns > 0x7fffffff) return cudaErrorInvalidConfiguration;
+        conv_step_kernel<T, VEC, W><<<unsigned(a.num_seqs) * columns, kConvThreads, 0, s>>>(a);
         return cudaGetLastError();
     }
     // Strips of 64 tokens; shorter ones while the grid would leave SMs idle.

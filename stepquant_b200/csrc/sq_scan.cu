@@ -313,47 +313,88 @@ __global__ void join_kernel(sq_scan_args a, Chunks chunks) {
     const float A = a.a[i] * kLog2e;
     float h = a.initial_state ? a.initial_state[row * size + i] : 0.f;
     const int64_t base = seq.x / chunks.length + int64_t(n);
-    for (int k = 0; k < count; ++k) {
-        float *at = chunks.state + (base + k) * size + i;
-        const float own = k + 1 < count ? *at : 0.f, sum = k + 1 < count ? chunks.step_sum[(base + k) * a.channels + d] : 0.f;
-        *at = h;
-        h = fmaf(exp2_approx(A * sum), h, own);
+    constexpr int B = 8;  // chunks whose loads are in flight together
+    for (int k = 0; k < count; k += B) {
+        float own[B], sum[B];
+#pragma unroll
+        for (int j = 0; j < B; ++j) {
+            const bool in = k + j + 1 < count;  // of the last chunk nothing was kept
+            own[j] = in ? chunks.state[(base + k + j) * size + i] : 0.f;
+            sum[j] = in ? chunks.step_sum[(base + k + j) * a.channels + d] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < B; ++j)
+            if (k + j < count) {
+                chunks.state[(base + k + j) * size + i] = h;
+                h = fmaf(exp2_approx(A * sum[j]), h, own[j]);
+            }
     }
 }
 
+// Four values of a row, by one access where `whole`.
+template <class T>
+struct Quad {
+    alignas(4 * sizeof(T)) T v[4];
+    __device__ __forceinline__ void load(const T *p, bool whole) {
+        if (whole) {
+            if (sizeof(T) == 2) *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(p);
+            else *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(p);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = p[i];
+        }
+    }
+};
+
 // One token of each request: N / 4 lanes a channel, the state read and written
-// once.  A lane takes R requests, their states in flight together; of the R
-// steps and gates of its channel each lane forms its share.
-template <class T, int N, int R>
-__global__ void __launch_bounds__(kScanThreads) scan_step_kernel(sq_scan_args a) {
+// once.  A lane takes R requests, their states (and B and C) in flight together;
+// of the R steps and gates of its channel each lane forms its share.  Bound by the
+// states' bytes (8 a channel and state); `whole`: B and C rows are aligned for one
+// access of four.
+template <class T, int N, int R, bool USUAL>
+__global__ void __launch_bounds__(kScanThreads) scan_step_kernel(sq_scan_args a, bool whole) {
     constexpr int P = N / kPerLane;
     constexpr int SHARE = R > P ? R / P : 1;  // requests whose scalars a lane forms
-    const int lane = threadIdx.x % P, n0 = blockIdx.x * R;
-    const int d = (blockIdx.y * kScanThreads + threadIdx.x) / P;
+    // Neighbouring CTAs take neighbouring channels: a request's state row is read through.
+    const unsigned tiles = (unsigned(a.channels) * P + kScanThreads - 1) / kScanThreads, request = blockIdx.x / tiles;
+    const int lane = threadIdx.x % P, n0 = request * R;
+    const int d = ((blockIdx.x - request * tiles) * kScanThreads + threadIdx.x) / P;
     const bool live = d < a.channels;
     const int k = live ? d : a.channels - 1, group = k / (a.channels / a.groups);
     int64_t rows[R];
-    float h[R][4], A[4];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        rows[r] = n0 + r < a.num_seqs ? state_row(a.slots, n0 + r, a.num_slots, a.status) : -1;
+    for (int r = 0; r < R; ++r) rows[r] = n0 + r < a.num_seqs ? state_row(a.slots, n0 + r, a.num_slots, a.status) : -1;
+    float A[4], h[R][4];
+    Quad<T> b[R], c[R];
+    T dt_raw[SHARE], u_raw[SHARE], z_raw[SHARE];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
         if (rows[r] >= 0) load4(a.final_state + (rows[r] * a.channels + k) * N + lane * 4, h[r]);
-    }
-    load4(a.a + int64_t(k) * N + lane * 4, A);
-    float dt_mine[SHARE], u_mine[SHARE], z_mine[SHARE];
-    const Bias bias(a.dt_bias ? a.dt_bias[k] : 0.f);
-    const float skip = a.d ? a.d[k] : 0.f;
 #pragma unroll
     for (int q = 0; q < SHARE; ++q) {
-        const int r = lane + q * P;
-        const int64_t n = n0 + r;
-        dt_mine[q] = u_mine[q] = z_mine[q] = 0.f;
-        if (r < R && n < a.num_seqs) {
-            u_mine[q] = to_float(static_cast<const T *>(a.u)[n * a.u_stride + k]);
-            const float raw = to_float(static_cast<const T *>(a.dt)[n * a.dt_stride + k]);
-            if (a.z) z_mine[q] = to_float(static_cast<const T *>(a.z)[n * a.z_stride + k]);
-            dt_mine[q] = a.softplus ? softplus(raw, bias) : raw + bias.value;
-        }
+        const int64_t n = min(n0 + lane + q * P, a.num_seqs - 1);  // lanes past R or the batch follow the last
+        dt_raw[q] = static_cast<const T *>(a.dt)[n * a.dt_stride + k];
+        u_raw[q] = static_cast<const T *>(a.u)[n * a.u_stride + k];
+        if (USUAL || a.z) z_raw[q] = static_cast<const T *>(a.z)[n * a.z_stride + k];
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int64_t n = min(n0 + r, a.num_seqs - 1);
+        b[r].load(static_cast<const T *>(a.b) + n * a.b_stride + group * N + lane * 4, whole);
+        c[r].load(static_cast<const T *>(a.c) + n * a.c_stride + group * N + lane * 4, whole);
+    }
+    load4(a.a + int64_t(k) * N + lane * 4, A);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) A[i] *= kLog2e;
+    const Bias bias(a.dt_bias ? a.dt_bias[k] : 0.f);
+    const float skip = a.d ? a.d[k] : 0.f;
+    float dt_mine[SHARE], u_mine[SHARE], gate_mine[SHARE];
+#pragma unroll
+    for (int q = 0; q < SHARE; ++q) {
+        const float raw = to_float(dt_raw[q]);
+        dt_mine[q] = USUAL || a.softplus ? softplus(raw, bias) : raw + bias.value;
+        u_mine[q] = to_float(u_raw[q]);
+        gate_mine[q] = USUAL || a.z ? silu(to_float(z_raw[q])) : 1.f;
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -362,12 +403,10 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(sq_scan_args a)
         const int64_t n = n0 + r;
         float sum = 0.f;
         if (rows[r] >= 0) {
-            const T *b = static_cast<const T *>(a.b) + n * a.b_stride + group * N + lane * 4;
-            const T *c = static_cast<const T *>(a.c) + n * a.c_stride + group * N + lane * 4;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                h[r][i] = fmaf(exp2_approx(dt * (A[i] * kLog2e)), h[r][i], dt * u * to_float(b[i]));
-                sum = fmaf(to_float(c[i]), h[r][i], sum);
+                h[r][i] = fmaf(exp2_approx(dt * A[i]), h[r][i], dt * u * to_float(b[r].v[i]));
+                sum = fmaf(to_float(c[r].v[i]), h[r][i], sum);
             }
             if (live)
                 *reinterpret_cast<float4 *>(a.final_state + (rows[r] * a.channels + k) * N + lane * 4) =
@@ -375,11 +414,9 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(sq_scan_args a)
         }
 #pragma unroll
         for (int o = P / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (live && lane == r % P && n < a.num_seqs) {
-            if (a.d) sum = fmaf(skip, u, sum);
-            if (a.z) sum *= silu(z_mine[r / P % SHARE]);
-            static_cast<T *>(a.y)[n * a.channels + d] = from_float<T>(rows[r] >= 0 ? sum : 0.f);
-        }
+        if (live && lane == r % P && n < a.num_seqs)
+            static_cast<T *>(a.y)[n * a.channels + d] =
+                from_float<T>(rows[r] >= 0 ? fmaf(skip, u, sum) * gate_mine[r / P % SHARE] : 0.f);
     }
 }
 
@@ -406,8 +443,16 @@ cudaError_t launch_scan_as(const sq_scan_args &a, bool step, cudaStream_t s) {
     if (step) {
         constexpr int P = N / kPerLane;
         const unsigned grid = unsigned((int64_t(a.channels) * P + kScanThreads - 1) / kScanThreads);
-        if (int64_t(a.num_seqs) * grid < 148 * 16) scan_step_kernel<T, N, 1><<<dim3(unsigned(a.num_seqs), grid), kScanThreads, 0, s>>>(a);
-        else scan_step_kernel<T, N, 4><<<dim3(unsigned((a.num_seqs + 3) / 4), grid), kScanThreads, 0, s>>>(a);
+        if (int64_t(a.num_seqs) * grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
+        constexpr int64_t four = 4 * sizeof(T);
+        auto fours = [&](const void *p, int64_t stride) { return reinterpret_cast<uintptr_t>(p) % four == 0 && stride % 4 == 0; };
+        const bool whole = fours(a.b, a.b_stride) && fours(a.c, a.c_stride), usual = a.softplus && a.z;
+        auto run = [&](auto kernel, int each) {
+            kernel<<<unsigned((a.num_seqs + each - 1) / each) * grid, kScanThreads, 0, s>>>(a, whole);
+        };
+        // Few requests: one a lane, for the CTAs' number.
+        if (int64_t(a.num_seqs) * grid < 148 * 16) usual ? run(scan_step_kernel<T, N, 1, true>, 1) : run(scan_step_kernel<T, N, 1, false>, 1);
+        else usual ? run(scan_step_kernel<T, N, 4, true>, 4) : run(scan_step_kernel<T, N, 4, false>, 4);
         return cudaGetLastError();
     }
     const int per = a.channels / a.groups;
