@@ -21,6 +21,7 @@ namespace sq {
 namespace {
 
 constexpr int kConvThreads = 128;
+constexpr unsigned kGridRows = 32768;  // requests along a grid's second axis, the rest along its third
 
 // N values of VEC channels (a token's, or a state row's), by 8- or 16-byte accesses for four channels.
 template <class T, int N, int VEC>
@@ -160,9 +161,8 @@ __global__ void __launch_bounds__(kConvThreads) conv_kernel(sq_conv_args a, int 
 template <class T, int VEC, int W>
 __global__ void __launch_bounds__(kConvThreads) conv_step_kernel(sq_conv_args a) {
     // Neighbouring CTAs take neighbouring channels of a request.
-    const unsigned columns = (unsigned(a.channels) + kConvThreads * VEC - 1) / (kConvThreads * VEC), n = blockIdx.x / columns;
-    const int d0 = ((blockIdx.x - n * columns) * kConvThreads + threadIdx.x) * VEC;
-    if (d0 >= a.channels) return;
+    const int n = blockIdx.z * kGridRows + blockIdx.y, d0 = (blockIdx.x * kConvThreads + threadIdx.x) * VEC;
+    if (d0 >= a.channels || n >= a.num_seqs) return;
     const int64_t row = state_row(a.slots, n, a.num_slots, a.status);
     Run<T, VEC, VEC> in, out;
     T *y = static_cast<T *>(a.y) + int64_t(n) * a.channels + d0;
@@ -196,8 +196,9 @@ template <class T, int VEC, int W>
 cudaError_t launch_conv_as(const sq_conv_args &a, bool step, cudaStream_t s) {
     const unsigned columns = unsigned((int64_t(a.channels) + kConvThreads * VEC - 1) / (kConvThreads * VEC));
     if (step) {
-        if (int64_t(a.num_seqs) * columns > 0x7fffffff) return cudaErrorInvalidConfiguration;
-        conv_step_kernel<T, VEC, W><<<unsigned(a.num_seqs) * columns, kConvThreads, 0, s>>>(a);
+        const unsigned rows = unsigned(a.num_seqs);
+        const dim3 grid(columns, rows < kGridRows ? rows : kGridRows, (rows + kGridRows - 1) / kGridRows);
+        conv_step_kernel<T, VEC, W><<<grid, kConvThreads, 0, s>>>(a);
         return cudaGetLastError();
     }
     // Strips of 64 tokens; shorter ones while the grid would leave SMs idle.
@@ -229,7 +230,7 @@ int32_t conv_entry(const sq_conv_args *args, bool step, sq_stream_t stream) {
     if (a.dtype < SQ_F32 || a.dtype > SQ_F16) return SQ_ERR_ARGUMENT;
     if (a.taps < 2 || a.taps > 4) return SQ_ERR_UNSUPPORTED;
     if (a.x_stride < 0) return SQ_ERR_SHAPE;
-    if (a.channels > (1 << 22)) return SQ_ERR_UNSUPPORTED;
+    if (a.channels > (1 << 22) || a.num_seqs > (1 << 30)) return SQ_ERR_UNSUPPORTED;
     if (a.num_seqs == 0) return SQ_OK;
     if (!a.weight || (a.tokens > 0 && (!a.x || !a.y))) return SQ_ERR_ARGUMENT;
     if (step ? !a.final_state : !a.cu_seqlens) return SQ_ERR_ARGUMENT;

@@ -32,6 +32,7 @@ namespace {
 constexpr int kScanThreads = 128;
 constexpr int kPerLane = 4;   // states of a lane of the single-token kernel
 constexpr int kGroup = 4;     // tokens of a prompt worked on together
+constexpr unsigned kGridRows = 32768;  // groups of requests along a grid's second axis, the rest along its third
 constexpr float kLog2eRest = 1.92596299e-8f;  // log2(e) - kLog2e
 
 // dt_bias of a channel in units of log2(e), with the rounding of that product.
@@ -356,32 +357,46 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(sq_scan_args a,
     constexpr int P = N / kPerLane;
     constexpr int SHARE = R > P ? R / P : 1;  // requests whose scalars a lane forms
     // Neighbouring CTAs take neighbouring channels: a request's state row is read through.
-    const unsigned tiles = (unsigned(a.channels) * P + kScanThreads - 1) / kScanThreads, request = blockIdx.x / tiles;
-    const int lane = threadIdx.x % P, n0 = request * R;
-    const int d = ((blockIdx.x - request * tiles) * kScanThreads + threadIdx.x) / P;
+    const int lane = threadIdx.x % P, n0 = (blockIdx.z * kGridRows + blockIdx.y) * R;
+    const int d = (blockIdx.x * kScanThreads + threadIdx.x) / P;
     const bool live = d < a.channels;
-    const int k = live ? d : a.channels - 1, group = k / (a.channels / a.groups);
+    const int k = live ? d : a.channels - 1, group = a.groups == 1 ? 0 : k / (a.channels / a.groups);
+    // The requests' places, formed once a CTA: state (-1: none), u, dt, z, B, C, y.
+    __shared__ int64_t place[7][R];
+    if (threadIdx.x < R) {
+        const int n = n0 + threadIdx.x;
+        const int64_t row = n < a.num_seqs ? state_row(a.slots, n, a.num_slots, a.status) : -1;
+        const int64_t in = min(n, a.num_seqs - 1);  // past the batch: read the last request's, write nothing
+        place[0][threadIdx.x] = row < 0 ? -1 : row * a.channels * N;
+        place[1][threadIdx.x] = in * a.u_stride;
+        place[2][threadIdx.x] = in * a.dt_stride;
+        place[3][threadIdx.x] = in * a.z_stride;
+        place[4][threadIdx.x] = in * a.b_stride;
+        place[5][threadIdx.x] = in * a.c_stride;
+        place[6][threadIdx.x] = n < a.num_seqs ? int64_t(n) * a.channels : -1;
+    }
+    __syncthreads();
     int64_t rows[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) rows[r] = n0 + r < a.num_seqs ? state_row(a.slots, n0 + r, a.num_slots, a.status) : -1;
+    for (int r = 0; r < R; ++r) rows[r] = place[0][r];
+    const int own = k * N + lane * 4, bc = group * N + lane * 4;  // below 2^24 and 2^20
     float A[4], h[R][4];
     Quad<T> b[R], c[R];
     T dt_raw[SHARE], u_raw[SHARE], z_raw[SHARE];
 #pragma unroll
     for (int r = 0; r < R; ++r)
-        if (rows[r] >= 0) load4(a.final_state + (rows[r] * a.channels + k) * N + lane * 4, h[r]);
+        if (rows[r] >= 0) load4(a.final_state + rows[r] + own, h[r]);
 #pragma unroll
     for (int q = 0; q < SHARE; ++q) {
-        const int64_t n = min(n0 + lane + q * P, a.num_seqs - 1);  // lanes past R or the batch follow the last
-        dt_raw[q] = static_cast<const T *>(a.dt)[n * a.dt_stride + k];
-        u_raw[q] = static_cast<const T *>(a.u)[n * a.u_stride + k];
-        if (USUAL || a.z) z_raw[q] = static_cast<const T *>(a.z)[n * a.z_stride + k];
+        const int r = min(lane + q * P, R - 1);  // lanes past R follow the last
+        u_raw[q] = static_cast<const T *>(a.u)[place[1][r] + k];
+        dt_raw[q] = static_cast<const T *>(a.dt)[place[2][r] + k];
+        if (USUAL || a.z) z_raw[q] = static_cast<const T *>(a.z)[place[3][r] + k];
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int64_t n = min(n0 + r, a.num_seqs - 1);
-        b[r].load(static_cast<const T *>(a.b) + n * a.b_stride + group * N + lane * 4, whole);
-        c[r].load(static_cast<const T *>(a.c) + n * a.c_stride + group * N + lane * 4, whole);
+        b[r].load(static_cast<const T *>(a.b) + place[4][r] + bc, whole);
+        c[r].load(static_cast<const T *>(a.c) + place[5][r] + bc, whole);
     }
     load4(a.a + int64_t(k) * N + lane * 4, A);
 #pragma unroll
@@ -400,7 +415,6 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(sq_scan_args a,
     for (int r = 0; r < R; ++r) {
         const int from = (threadIdx.x & 31) / P * P + r % P;
         const float dt = __shfl_sync(0xffffffffu, dt_mine[r / P % SHARE], from), u = __shfl_sync(0xffffffffu, u_mine[r / P % SHARE], from);
-        const int64_t n = n0 + r;
         float sum = 0.f;
         if (rows[r] >= 0) {
 #pragma unroll
@@ -409,14 +423,13 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(sq_scan_args a,
                 sum = fmaf(to_float(c[r].v[i]), h[r][i], sum);
             }
             if (live)
-                *reinterpret_cast<float4 *>(a.final_state + (rows[r] * a.channels + k) * N + lane * 4) =
-                    make_float4(h[r][0], h[r][1], h[r][2], h[r][3]);
+                *reinterpret_cast<float4 *>(a.final_state + rows[r] + own) = make_float4(h[r][0], h[r][1], h[r][2], h[r][3]);
         }
 #pragma unroll
         for (int o = P / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (live && lane == r % P && n < a.num_seqs)
-            static_cast<T *>(a.y)[n * a.channels + d] =
-                from_float<T>(rows[r] >= 0 ? fmaf(skip, u, sum) * gate_mine[r / P % SHARE] : 0.f);
+        const int64_t at = place[6][r];
+        if (live && lane == r % P && at >= 0)
+            static_cast<T *>(a.y)[at + k] = from_float<T>(rows[r] >= 0 ? fmaf(skip, u, sum) * gate_mine[r / P % SHARE] : 0.f);
     }
 }
 
@@ -443,12 +456,12 @@ cudaError_t launch_scan_as(const sq_scan_args &a, bool step, cudaStream_t s) {
     if (step) {
         constexpr int P = N / kPerLane;
         const unsigned grid = unsigned((int64_t(a.channels) * P + kScanThreads - 1) / kScanThreads);
-        if (int64_t(a.num_seqs) * grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
         constexpr int64_t four = 4 * sizeof(T);
         auto fours = [&](const void *p, int64_t stride) { return reinterpret_cast<uintptr_t>(p) % four == 0 && stride % 4 == 0; };
         const bool whole = fours(a.b, a.b_stride) && fours(a.c, a.c_stride), usual = a.softplus && a.z;
         auto run = [&](auto kernel, int each) {
-            kernel<<<unsigned((a.num_seqs + each - 1) / each) * grid, kScanThreads, 0, s>>>(a, whole);
+            const unsigned rows = unsigned((int64_t(a.num_seqs) + each - 1) / each);
+            kernel<<<dim3(grid, rows < kGridRows ? rows : kGridRows, (rows + kGridRows - 1) / kGridRows), kScanThreads, 0, s>>>(a, whole);
         };
         // Few requests: one a lane, for the CTAs' number.
         if (int64_t(a.num_seqs) * grid < 148 * 16) usual ? run(scan_step_kernel<T, N, 1, true>, 1) : run(scan_step_kernel<T, N, 1, false>, 1);
@@ -498,7 +511,7 @@ int32_t scan_entry(const sq_scan_args *args, bool step, sq_stream_t stream) {
     if (a.channels % a.groups || a.u_stride < 0 || a.dt_stride < 0 || a.z_stride < 0 || a.b_stride < 0 || a.c_stride < 0)
         return SQ_ERR_SHAPE;
     if (a.states != 4 && a.states != 8 && a.states != 16 && a.states != 32 && a.states != 64) return SQ_ERR_UNSUPPORTED;
-    if (a.channels > (1 << 18) || a.groups > (1 << 14)) return SQ_ERR_UNSUPPORTED;
+    if (a.channels > (1 << 18) || a.groups > (1 << 14) || a.num_seqs > (1 << 30)) return SQ_ERR_UNSUPPORTED;
     if (a.num_seqs == 0) return SQ_OK;
     if (!a.a || (a.tokens > 0 && (!a.u || !a.dt || !a.b || !a.c || !a.y))) return SQ_ERR_ARGUMENT;
     if (step ? !a.final_state : !a.cu_seqlens) return SQ_ERR_ARGUMENT;
