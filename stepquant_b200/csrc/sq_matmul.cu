@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(kCtaThreads, 2)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int blocks = (a.hidden + kBlock - 1) / kBlock;
     const int g0 = int(int64_t(blocks) * rank / ranks), g1 = int(int64_t(blocks) * (rank + 1) / ranks);
-    const int n0 = int(blockIdx.x) / ranks * 128, m0 = blockIdx.y * TM;
+    const int n0 = int(blockIdx.x) / ranks * 128;  // and all rows of x: TM or fewer
     set_up<1, 1>(s, S::kStages, S::kColumns, warp);
     const uint32_t tmem = s.tmem;
     float *sums = reinterpret_cast<float *>(base);  // [TM][128], once the operands are consumed
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(kCtaThreads, 2)
                 unsigned char *to = base + at.stage * S::kStage;
                 tc::bar_expect(&s.full[at.stage], S::kStage);
                 tc::tma_load(to, &wmap, g * kBlock, n0, &s.full[at.stage]);
-                tc::tma_load(to + kRowTile, &xmap, g * kBlock, m0, &s.full[at.stage]);
+                tc::tma_load(to + kRowTile, &xmap, g * kBlock, 0, &s.full[at.stage]);
             }
             if (!ok) drain_copies(s, at, g - g0);
         }
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(kCtaThreads, 2)
 #pragma unroll
             for (int e = 0; e < EACH; ++e) {
                 const int i = e * 32 * kEpilogueWarps + tid, at = min(g + i / TM, blocks - 1);
-                if (i < kScaleGroup * TM) next[e] = a.x_scale[int64_t(min(m0 + i % TM, a.rows - 1)) * blocks + at] * sw[at];
+                if (i < kScaleGroup * TM) next[e] = a.x_scale[int64_t(min(i % TM, a.rows - 1)) * blocks + at] * sw[at];
             }
         };
         fetch_scales(g0);
@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(kCtaThreads, 2)
     const int share = TM * rank / ranks, count = TM * (rank + 1) / ranks - share;
 #pragma unroll 4
     for (int i = threadIdx.x; i < count * 32; i += kCtaThreads) {
-        const int m = m0 + share + i / 32, n = n0 + i % 32 * 4;
+        const int m = share + i / 32, n = n0 + i % 32 * 4;
         if (m >= a.rows || n >= a.width) continue;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int q = 0; q < ranks; ++q) {
@@ -557,11 +557,11 @@ int32_t launch_split(const sq_matmul_args &a, bool wide, int sms, cudaStream_t s
         return SQ_ERR_CUDA;
     if (cudaFuncSetAttribute(split_kernel<T, TM>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess)
         return SQ_ERR_CUDA;
-    const int columns = (a.width + 127) / 128, rows = (a.rows + TM - 1) / TM, blocks = (a.hidden + kBlock - 1) / kBlock;
+    const int columns = (a.width + 127) / 128, blocks = (a.hidden + kBlock - 1) / kBlock;
     // K is split while two CTAs an SM are not in use and each keeps two blocks.
     int split = 8;
-    while (split > 1 && (int64_t(columns) * rows * split > 2 * sms || blocks < 2 * split)) split /= 2;
-    return launch_clusters(split_kernel<T, TM>, dim3(unsigned(columns * split), unsigned(rows)), kCtaThreads, split, S::kBytes, s, x, w, a, wide);
+    while (split > 1 && (int64_t(columns) * split > 2 * sms || blocks < 2 * split)) split /= 2;
+    return launch_clusters(split_kernel<T, TM>, dim3(unsigned(columns * split)), kCtaThreads, split, S::kBytes, s, x, w, a, wide);
 }
 
 template <class T>
