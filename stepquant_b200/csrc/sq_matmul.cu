@@ -10,14 +10,15 @@
 //
 // Many rows (tile_kernel): tensor memory lanes are rows of x, columns are rows
 // of w, so a thread's scale is one number a block.  Persistent CTAs of 128 x TN
-// tiles, or pairs of CTAs (cta_group::2) of 256 x 256 tiles, each SM holding its
-// 128 rows of x and half of the rows of w: 32 instead of 48 KB a block from L2.
-// What bounds it is the turn of a half of the tensor memory: products (512 clocks
-// of 256 columns), their commit, the epilogue's read and its release; a read of
-// 256 columns also holds the products up by about 150 clocks.  Measured on the way
-// (16384 x 8256 x 5120): packed fp32 pairs in the epilogue 811 us, single ones with
-// the half released as soon as it is in registers, scales loaded four blocks ahead
-// and a release without cluster fence 695 us (1.99 PFLOP/s).
+// tiles, the block products in 2 to 4 parts of the tensor memory.  What bounds it
+// short of the power limit is the turn of a part (products, 512 clocks of 256
+// columns, and the epilogue's read, which holds the products up by about 150)
+// and the operands' way from L2 (48 KB a block of 128 x 256, 11 TB/s measured);
+// in a loop of seconds the GPU runs at its 1000 W limit, 1.53 GHz.  Measured on the
+// way at 16384 x 8256 x 5120: packed fp32 pairs in the epilogue 811 us, single ones,
+// a part released as soon as it is in registers, scales loaded four blocks ahead
+// and two product warps in turn 698 us (1.98 PFLOP/s; 814 us at the power limit).
+// Pairs of CTAs (256 x 256 tiles, 32 KB a block and SM) measured 705 and 827 us.
 // Few rows (split_kernel): the weights' bytes bound the call.  Lanes are 128
 // rows of w (one scale a block), columns the rows of x; the CTAs of a cluster
 // split K and add their sums in rank order through distributed shared memory
@@ -39,24 +40,27 @@ namespace {
 
 constexpr int kBlock = 128;                // depth of a scale block and of a pipeline stage
 constexpr int kEpilogueWarps = 8;
-constexpr int kCtaThreads = 32 * (kEpilogueWarps + 2);  // + copy warp, product warp
+constexpr int kMostParts = 4;              // blocks in tensor memory at a time
 constexpr int kRowTile = 128 * kBlock;     // bytes of a 128-row operand tile
 constexpr int kScaleGroup = 4;             // blocks whose scales are loaded together
 
 struct Sync {
     uint64_t full[8], empty[8];  // operand stages
-    uint64_t ready[2][2], free_[2][2];  // halves of the tensor memory, column groups of each
+    uint64_t ready[kMostParts], free_[kMostParts];  // parts of the tensor memory
     uint32_t tmem;
     int abort;
 };
 
-// Position in the ring of operand stages: the stage and the parity of its use.
+// Position in a ring (of operand stages, of parts of the tensor memory) and the parity of its use.
 template <int STAGES>
 struct Ring {
     int stage = 0;
     uint32_t parity = 0;
     __device__ __forceinline__ void next() {
         if (++stage == STAGES) stage = 0, parity ^= 1;
+    }
+    __device__ __forceinline__ void back() {
+        if (--stage < 0) stage = STAGES - 1, parity ^= 1;
     }
 };
 
@@ -66,67 +70,67 @@ template <int STAGES>
 __device__ __forceinline__ void drain_copies(Sync &s, Ring<STAGES> at, int64_t count) {
     int never = 0;
     for (int i = 0; i < STAGES && i < count; ++i) {
-        if (--at.stage < 0) at.stage = STAGES - 1, at.parity ^= 1;
+        at.back();
         tc::bar_wait(&s.full[at.stage], at.parity, &never);
     }
 }
 
-// G CTAs (one, or a pair) share the products, Q product warps issue them, each for
-// its group of the columns and with its share of the epilogue warps.
-template <int G, int Q>
 __device__ __forceinline__ void set_up(Sync &s, int stages, uint32_t columns, int warp) {
     if (threadIdx.x == 0) {
         for (int i = 0; i < stages; ++i) {
             tc::bar_init(&s.full[i], 1);
-            tc::bar_init(&s.empty[i], Q);
+            tc::bar_init(&s.empty[i], 1);
         }
-        for (int i = 0; i < 2; ++i)
-            for (int q = 0; q < Q; ++q) {
-                tc::bar_init(&s.ready[i][q], 1);
-                tc::bar_init(&s.free_[i][q], G * kEpilogueWarps / Q);
-            }
+        for (int i = 0; i < kMostParts; ++i) {
+            tc::bar_init(&s.ready[i], 1);
+            tc::bar_init(&s.free_[i], kEpilogueWarps);
+        }
         s.abort = 0;
         tc::bar_init_fence();
     }
-    if (warp == kEpilogueWarps + 1) tc::tmem_alloc<G>(&s.tmem, columns);
+    if (warp == kEpilogueWarps + 1) tc::tmem_alloc(&s.tmem, columns);
     tc::fence_before();
-    if (G == 2) tc::cluster_sync();
-    else __syncthreads();
+    __syncthreads();
     tc::fence_after();
 }
 
-// Product warp q of Q: `count` blocks, each four steps of 32 along K into its N
-// columns of the halves of the tensor memory in turn.  The whole warp takes the
-// waits and one elected lane issues, which keeps the descriptors in uniform
-// registers.  base: shared address of the first stage's tile of x; w_rows: the
-// group's rows in the tile of w behind it.
-template <int G, int N, int STAGES, int STAGE_BYTES>
-__device__ __forceinline__ void issue_blocks(Sync &s, int q, int64_t count, uint32_t tmem, int half_columns, uint32_t base,
-                                             uint32_t w_rows) {
+// Product warp: blocks w, w + W, ... of `count`, each four steps of 32 along K into
+// N columns of the tensor memory, its PARTS parts in turn.  The whole warp takes
+// the waits and one elected lane issues, which keeps the descriptors in uniform
+// registers; two waits, four products and two commits took a warp about 900 clocks,
+// so two warps alternate (W = 2) where there are registers for them.  base: shared
+// address of the first stage, its two operand tiles kRowTile apart.
+template <int N, int W, int PARTS, int STAGES, int STAGE_BYTES>
+__device__ __forceinline__ void issue_blocks(Sync &s, int w, int64_t count, uint32_t tmem, uint32_t base) {
     Ring<STAGES> at;
-    int64_t it = 0;
+    Ring<PARTS> part;
+    int64_t it = w;
     bool ok = true;
-    for (; it < count; ++it, at.next()) {
-        const int half = int(it) & 1;
-        const uint32_t use = uint32_t(it >> 1) & 1;
-        ok = tc::bar_wait(&s.full[at.stage], at.parity, &s.abort) && tc::bar_wait(&s.free_[half][q], use ^ 1, &s.abort);
+    if (w) at.next(), part.next();
+    for (; it < count; it += W) {
+        ok = tc::bar_wait(&s.full[at.stage], at.parity, &s.abort) && tc::bar_wait(&s.free_[part.stage], part.parity ^ 1, &s.abort);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc::fence_after();
         if (tc::elected()) {
-            const uint32_t a = base + at.stage * STAGE_BYTES, b = a + kRowTile + w_rows * kBlock;
+            const uint32_t a = base + at.stage * STAGE_BYTES, b = a + kRowTile;
 #pragma unroll
             for (int k = 0; k < kBlock / 32; ++k)
-                tc::mma_e4m3<G>(tmem + half * half_columns + q * N, tc::operand(a + 32 * k), tc::operand(b + 32 * k),
-                                tc::e4m3_product(128 * G, N), k > 0);
-            tc::mma_commit<G>(&s.ready[half][q]);
-            tc::mma_commit<G>(&s.empty[at.stage]);
+                tc::mma_e4m3(tmem + part.stage * N, tc::operand(a + 32 * k), tc::operand(b + 32 * k), tc::e4m3_product(N), k > 0);
+            tc::mma_commit(&s.ready[part.stage]);
+            tc::mma_commit(&s.empty[at.stage]);
         }
         __syncwarp();
+#pragma unroll
+        for (int i = 0; i < W; ++i) at.next(), part.next();
     }
     // A warp that gives up leaves once its last products have ended (with a limit again).
     if (!ok) {
         int never = 0;
-        for (int64_t i = it > 2 ? it - 2 : 0; i < it; ++i) tc::bar_wait(&s.ready[i & 1][q], uint32_t(i >> 1) & 1, &never);
+        for (int i = 0; i < PARTS && it >= W; ++i, it -= W) {
+#pragma unroll
+            for (int k = 0; k < W; ++k) part.back();
+            tc::bar_wait(&s.ready[part.stage], part.parity, &never);
+        }
         __syncwarp();
     }
 }
@@ -138,15 +142,15 @@ __device__ __forceinline__ void issue_blocks(Sync &s, int q, int64_t count, uint
 constexpr int kTileThreads = 384, kEpilogueRegisters = 216, kIssueRegisters = 56;  // 2 x 216 + 56 <= 3 x 168
 constexpr int kGroupRows = 8;  // row tiles that share a sweep over the columns (operands stay in L2)
 
-// A CTA holds 128 rows of x and, of a pair (G = 2), half of the TN rows of w.
-template <int TN, int G>
+template <int TN>
 struct TileShape {
-    static constexpr int kStage = kRowTile + TN / G * kBlock;
+    static constexpr int kStage = kRowTile + TN * kBlock;
     static constexpr int kStaging = kEpilogueWarps * 32 * 16 * 4;
     static constexpr int kRoom = (226 * 1024 - kStaging - 1024 - int(sizeof(Sync))) / kStage;
     static constexpr int kStages = kRoom > 8 ? 8 : kRoom;
     static constexpr int kBytes = kStages * kStage + kStaging + 1024 + int(sizeof(Sync));
-    static constexpr int kColumns = 2 * TN <= 128 ? 128 : 2 * TN <= 256 ? 256 : 512;
+    static constexpr int kParts = 512 / TN < kMostParts ? 512 / TN : kMostParts;
+    static constexpr int kColumns = kParts * TN <= 256 ? 256 : 512;
 };
 
 // Tile `i` of the sweep: groups of kGroupRows row tiles, rows fastest within a group.
@@ -182,64 +186,52 @@ struct Four {
     }
 };
 
-template <class T, int TN, int G>
+template <class T, int TN>
 __global__ void __launch_bounds__(kTileThreads, 1)
     tile_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, sq_matmul_args a,
                 bool wide) {
-    using S = TileShape<TN, G>;
+    using S = TileShape<TN>;
     extern __shared__ unsigned char raw[];
     unsigned char *base = raw + ((1024u - (tc::smem_u32(raw) & 1023u)) & 1023u);
     float *staging = reinterpret_cast<float *>(base + S::kStages * S::kStage);
     Sync &s = *reinterpret_cast<Sync *>(staging + S::kStaging / 4);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x % G;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int blocks = (a.hidden + kBlock - 1) / kBlock;
-    constexpr int ROWS = 128 * G;
-    const int row_tiles = (a.rows + ROWS - 1) / ROWS, column_tiles = (a.width + TN - 1) / TN;
-    const int64_t tiles = int64_t(row_tiles) * column_tiles, first = blockIdx.x / G, step = gridDim.x / G;
-    set_up<G, G>(s, S::kStages, S::kColumns, warp);
+    const int row_tiles = (a.rows + 127) / 128, column_tiles = (a.width + TN - 1) / TN;
+    const int64_t tiles = int64_t(row_tiles) * column_tiles, first = blockIdx.x, step = gridDim.x;
+    set_up(s, S::kStages, S::kColumns, warp);
     const uint32_t tmem = s.tmem;
 
     if (warp >= kEpilogueWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kIssueRegisters));
-        if (warp == kEpilogueWarps) {  // copies of both CTAs complete on the first one's barriers
+        if (warp == kEpilogueWarps) {  // copies
             if (lane == 0) {
                 Ring<S::kStages> at;
                 int64_t count = 0;
                 bool ok = true;
                 for (int64_t i = first; i < tiles && ok; i += step) {
                     const int2 tile = tile_at(i, row_tiles, column_tiles);
-                    const int x_row = tile.x * ROWS + rank * 128, w_row = tile.y * TN + rank * (TN / 4);
+                    const int x_row = tile.x * 128, w_row = tile.y * TN;
                     for (int g = 0; g < blocks; ++g, ++count, at.next()) {
                         if (!(ok = tc::bar_wait(&s.empty[at.stage], at.parity ^ 1, &s.abort))) break;
                         unsigned char *to = base + at.stage * S::kStage;
-                        if (rank == 0) tc::bar_expect(&s.full[at.stage], G * S::kStage);
-                        if (G == 1) {
-                            tc::tma_load(to, &xmap, g * kBlock, x_row, &s.full[at.stage]);
-                            tc::tma_load(to + kRowTile, &wmap, g * kBlock, w_row, &s.full[at.stage]);
-                        } else {
-                            const uint32_t bar = tc::in_first(&s.full[at.stage]);
-                            tc::tma_load_pair(to, &xmap, g * kBlock, x_row, bar);
-                            tc::tma_load_pair(to + kRowTile, &wmap, g * kBlock, w_row, bar);
-                            tc::tma_load_pair(to + kRowTile + TN / 4 * kBlock, &wmap, g * kBlock, w_row + TN / 2, bar);
-                        }
+                        tc::bar_expect(&s.full[at.stage], S::kStage);
+                        tc::tma_load(to, &xmap, g * kBlock, x_row, &s.full[at.stage]);
+                        tc::tma_load(to + kRowTile, &wmap, g * kBlock, w_row, &s.full[at.stage]);
                     }
                 }
-                if (!ok && rank == 0) drain_copies(s, at, count);
+                if (!ok) drain_copies(s, at, count);
             }
             __syncwarp();
-        } else if (warp < kEpilogueWarps + 1 + G) {  // products: of a pair issued by its first CTA, a warp for each half of the columns
+        } else if (warp < kEpilogueWarps + 3) {  // products
             const int64_t mine = first < tiles ? (tiles - first + step - 1) / step : 0;
-            const int q = warp - kEpilogueWarps - 1;
-            if (rank == 0)
-                issue_blocks<G, TN / G, S::kStages, S::kStage>(s, q, mine * blocks, tmem, TN, tc::smem_u32(base), q * (TN / 4));
+            issue_blocks<TN, 2, S::kParts, S::kStages, S::kStage>(s, warp - kEpilogueWarps - 1, mine * blocks, tmem, tc::smem_u32(base));
         }
     } else {  // scales and sums: warp w holds lanes 32 (w % 4) .. + 31, half q = w / 4 of the columns
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kEpilogueRegisters));
         constexpr int C = TN / 2, CHUNKS = C / 16;
         const int q = warp >> 2;  // the half of the columns
         const uint32_t mine = tmem + (uint32_t(32 * (warp & 3)) << 16) + q * C;
-        const int group = G == 1 ? 0 : q;  // of the products
-        const uint32_t released[2] = {tc::in_first(&s.free_[0][group]), tc::in_first(&s.free_[1][group])};
         float *stage = staging + warp * 32 * 16;
         // Scales of kScaleGroup blocks from g on, loaded that many blocks before their use (a load's way
         // from L2 is longer than a block): the lane's row of x, and the two 128-row blocks of w that the
@@ -250,7 +242,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         auto aim = [&](int64_t i) {
             const int2 at = tile_at(i, row_tiles, column_tiles);
             const int n0 = at.y * TN + q * C;
-            sx = a.x_scale + int64_t(min(at.x * ROWS + rank * 128 + 32 * (warp & 3) + lane, a.rows - 1)) * blocks;
+            sx = a.x_scale + int64_t(min(at.x * 128 + 32 * (warp & 3) + lane, a.rows - 1)) * blocks;
             sw0 = a.w_scale + int64_t(min(n0 / kBlock, last)) * blocks;
             sw1 = a.w_scale + int64_t(min((n0 + C - 1) / kBlock, last)) * blocks;
         };
@@ -265,17 +257,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             aim(first);
             fetch_scales(0);
         }
-        int64_t it = 0;
+        Ring<S::kParts> part;
         bool ok = true;
         for (int64_t i = first; i < tiles && ok; i += step) {
             const int2 at = tile_at(i, row_tiles, column_tiles);
-            const int m0 = at.x * ROWS + rank * 128 + 32 * (warp & 3), n0 = at.y * TN + q * C;
+            const int m0 = at.x * 128 + 32 * (warp & 3), n0 = at.y * TN + q * C;
             const int cross = (kBlock - n0 % kBlock) / 16;  // first chunk of the second block of w
             float acc[C];
 #pragma unroll
             for (int j = 0; j < C; ++j) acc[j] = 0.f;
             float s0[kScaleGroup], s1[kScaleGroup];
-            for (int g = 0; g < blocks; ++g, ++it) {
+            for (int g = 0; g < blocks; ++g, part.next()) {
                 if (g % kScaleGroup == 0) {
 #pragma unroll
                     for (int q = 0; q < kScaleGroup; ++q) s0[q] = next_x[q] * next_0[q], s1[q] = next_x[q] * next_1[q];
@@ -284,11 +276,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 const float f0 = s0[0], f1 = s1[0];
 #pragma unroll
                 for (int q = 0; q + 1 < kScaleGroup; ++q) s0[q] = s0[q + 1], s1[q] = s1[q + 1];
-                ok = __all_sync(0xffffffffu, tc::bar_wait(&s.ready[it & 1][group], uint32_t(it >> 1) & 1, &s.abort));
+                ok = __all_sync(0xffffffffu, tc::bar_wait(&s.ready[part.stage], part.parity, &s.abort));
                 if (!ok) break;
                 tc::fence_after();
-                const uint32_t from = mine + int(it & 1) * TN;
-                // The next 16 columns are on their way while 16 are added; the half is free once all are in registers.
+                const uint32_t from = mine + part.stage * TN;
+                // The next 16 columns are on their way while 16 are added; the part is free once all are in registers.
                 uint32_t r[2][16];
                 tc::tmem_load(from, r[0]);
 #pragma unroll
@@ -299,7 +291,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     } else {
                         tc::fence_before();
                         __syncwarp();
-                        if (lane == 0) tc::bar_arrive_cluster(released[it & 1]);
+                        if (lane == 0) tc::bar_arrive(&s.free_[part.stage]);
                     }
                     const float f = c < cross ? f0 : f1;
 #pragma unroll
@@ -352,10 +344,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
     }
     tc::fence_before();
-    tc::cluster_sync();  // the pair's last arrivals and products are over
+    __syncthreads();
     tc::fence_after();
     if (s.abort && threadIdx.x == 0) flag(a.status, SQ_STATUS_TIMEOUT);
-    if (warp == kEpilogueWarps + 1) tc::tmem_free<G>(tmem, S::kColumns);
+    if (warp == kEpilogueWarps + 1) tc::tmem_free(tmem, S::kColumns);
 }
 
 // ---------------------------------------------------------------------------
@@ -367,11 +359,14 @@ struct SplitShape {
     static constexpr int kStages = 98304 / kStage;  // 5, 4, 4, 3: two CTAs an SM
     static constexpr int kScales = 2 * kScaleGroup * TM * 4;  // of two groups of blocks
     static constexpr int kBytes = kStages * kStage + kScales + 1024 + int(sizeof(Sync));
-    static constexpr int kColumns = 2 * TM;
+    static constexpr int kParts = 256 / TM < kMostParts ? 256 / TM : kMostParts;  // 256 columns: two CTAs an SM
+    static constexpr int kColumns = kParts * TM;
+    static constexpr int kProductWarps = TM <= 32 ? 2 : 1;  // more rows have no registers for a second
+    static constexpr int kThreads = 32 * (kEpilogueWarps + 1 + kProductWarps);
 };
 
 template <class T, int TM>
-__global__ void __launch_bounds__(kCtaThreads, 2)
+__global__ void __launch_bounds__(SplitShape<TM>::kThreads, 2)
     split_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, sq_matmul_args a,
                  bool wide) {
     using S = SplitShape<TM>;
@@ -386,7 +381,7 @@ __global__ void __launch_bounds__(kCtaThreads, 2)
     const int blocks = (a.hidden + kBlock - 1) / kBlock;
     const int g0 = int(int64_t(blocks) * rank / ranks), g1 = int(int64_t(blocks) * (rank + 1) / ranks);
     const int n0 = int(blockIdx.x) / ranks * 128;  // and all rows of x: TM or fewer
-    set_up<1, 1>(s, S::kStages, S::kColumns, warp);
+    set_up(s, S::kStages, S::kColumns, warp);
     const uint32_t tmem = s.tmem;
     float *sums = reinterpret_cast<float *>(base);  // [TM][128], once the operands are consumed
 
@@ -406,7 +401,7 @@ __global__ void __launch_bounds__(kCtaThreads, 2)
         }
         __syncwarp();
     } else if (warp > kEpilogueWarps) {
-        issue_blocks<1, TM, S::kStages, S::kStage>(s, 0, g1 - g0, tmem, TM, tc::smem_u32(base), 0);
+        issue_blocks<TM, S::kProductWarps, S::kParts, S::kStages, S::kStage>(s, warp - kEpilogueWarps - 1, g1 - g0, tmem, tc::smem_u32(base));
     } else {
         constexpr int C = TM / 2, W = C < 16 ? C : 16, CHUNKS = C / W;
         const int tid = threadIdx.x, half = warp >> 2;
@@ -426,7 +421,8 @@ __global__ void __launch_bounds__(kCtaThreads, 2)
         float acc[C];
 #pragma unroll
         for (int j = 0; j < C; ++j) acc[j] = 0.f;
-        for (int it = 0; it < g1 - g0; ++it) {
+        Ring<S::kParts> part;
+        for (int it = 0; it < g1 - g0; ++it, part.next()) {
             const float *group = ring + (it / kScaleGroup & 1) * kScaleGroup * TM;
             if (it % kScaleGroup == 0) {
 #pragma unroll
@@ -438,10 +434,10 @@ __global__ void __launch_bounds__(kCtaThreads, 2)
                 // The group's scales are there for all, and all are done with those of two groups ago.
                 asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kEpilogueWarps) : "memory");
             }
-            tc::bar_wait(&s.ready[it & 1][0], uint32_t(it >> 1) & 1, &s.abort);  // giving up: the sums are not used
+            tc::bar_wait(&s.ready[part.stage], part.parity, &s.abort);  // giving up: the sums are not used
             __syncwarp();
             tc::fence_after();
-            const uint32_t from = mine + (it & 1) * TM;
+            const uint32_t from = mine + part.stage * TM;
             const float *f = group + it % kScaleGroup * TM + half * C;
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c) {
@@ -460,7 +456,7 @@ __global__ void __launch_bounds__(kCtaThreads, 2)
             }
             tc::fence_before();
             __syncwarp();
-            if (lane == 0) tc::bar_arrive(&s.free_[it & 1][0]);
+            if (lane == 0) tc::bar_arrive(&s.free_[part.stage]);
         }
         // Every product has been read from tensor memory, hence every operand by the tensor cores.
         if (!s.abort) {
@@ -471,11 +467,11 @@ __global__ void __launch_bounds__(kCtaThreads, 2)
     tc::fence_before();
     cluster.sync();
     tc::fence_after();
-    if (warp == kEpilogueWarps + 1) tc::tmem_free<1>(tmem, S::kColumns);
+    if (warp == kEpilogueWarps + 1) tc::tmem_free(tmem, S::kColumns);
     // The sums of the ranks, in their order; each rank finishes its share of the rows of x, four columns a thread.
     const int share = TM * rank / ranks, count = TM * (rank + 1) / ranks - share;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < count * 32; i += kCtaThreads) {
+    for (int i = threadIdx.x; i < count * 32; i += S::kThreads) {
         const int m = share + i / 32, n = n0 + i % 32 * 4;
         if (m >= a.rows || n >= a.width) continue;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -521,32 +517,17 @@ bool byte_map(CUtensorMap *map, const void *p, int hidden, int rows, int64_t str
                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class K, class... A>
-int32_t launch_clusters(K kernel, dim3 grid, int threads, int cluster, int bytes, cudaStream_t s, A... args) {
-    cudaLaunchConfig_t c{};
-    c.gridDim = grid;
-    c.blockDim = dim3(unsigned(threads));
-    c.dynamicSmemBytes = bytes;
-    c.stream = s;
-    cudaLaunchAttribute attribute;
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = unsigned(cluster);
-    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-    c.attrs = &attribute;
-    c.numAttrs = 1;
-    return cudaLaunchKernelEx(&c, kernel, args...) == cudaSuccess ? SQ_OK : SQ_ERR_CUDA;
-}
-
-template <class T, int TN, int G>
+template <class T, int TN>
 int32_t launch_tile(const sq_matmul_args &a, bool wide, int sms, cudaStream_t s) {
-    using S = TileShape<TN, G>;
+    using S = TileShape<TN>;
     CUtensorMap x, w;
-    if (!byte_map(&x, a.x, a.hidden, a.rows, a.x_stride, 128) || !byte_map(&w, a.w, a.hidden, a.width, a.w_stride, G == 1 ? TN : TN / 4))
+    if (!byte_map(&x, a.x, a.hidden, a.rows, a.x_stride, 128) || !byte_map(&w, a.w, a.hidden, a.width, a.w_stride, TN))
         return SQ_ERR_CUDA;
-    if (cudaFuncSetAttribute(tile_kernel<T, TN, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess)
+    if (cudaFuncSetAttribute(tile_kernel<T, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess)
         return SQ_ERR_CUDA;
-    const int64_t tiles = int64_t((a.rows + 128 * G - 1) / (128 * G)) * ((a.width + TN - 1) / TN), most = sms > G ? sms / G : 1;
-    return launch_clusters(tile_kernel<T, TN, G>, dim3(unsigned(G * (tiles < most ? tiles : most))), kTileThreads, G, S::kBytes, s, x, w, a, wide);
+    const int64_t tiles = int64_t((a.rows + 127) / 128) * ((a.width + TN - 1) / TN);
+    tile_kernel<T, TN><<<unsigned(tiles < sms ? tiles : sms), kTileThreads, S::kBytes, s>>>(x, w, a, wide);
+    return cudaGetLastError() == cudaSuccess ? SQ_OK : SQ_ERR_CUDA;
 }
 
 template <class T, int TM>
@@ -561,7 +542,18 @@ int32_t launch_split(const sq_matmul_args &a, bool wide, int sms, cudaStream_t s
     // K is split while two CTAs an SM are not in use and each keeps two blocks.
     int split = 8;
     while (split > 1 && (int64_t(columns) * split > 2 * sms || blocks < 2 * split)) split /= 2;
-    return launch_clusters(split_kernel<T, TM>, dim3(unsigned(columns * split)), kCtaThreads, split, S::kBytes, s, x, w, a, wide);
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3(unsigned(columns * split));
+    c.blockDim = dim3(unsigned(S::kThreads));
+    c.dynamicSmemBytes = S::kBytes;
+    c.stream = s;
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = unsigned(split);
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    c.attrs = &cluster;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, split_kernel<T, TM>, x, w, a, wide) == cudaSuccess ? SQ_OK : SQ_ERR_CUDA;
 }
 
 template <class T>
@@ -573,23 +565,21 @@ int32_t launch_matmul(const sq_matmul_args &a, int sms, cudaStream_t s) {
     if (a.rows <= 32) return launch_split<T, 32>(a, wide, sms, s);
     if (a.rows <= 64) return launch_split<T, 64>(a, wide, sms, s);
     if (a.rows <= 128) return launch_split<T, 128>(a, wide, sms, s);
-    // The tile whose waves take least: a block of 128 x TN (or, of a pair, 256 x TN) took 288 + 1.3 TN ns
-    // a wave, measured from TN = 64 (371) to 256 (620; the pair 598, so it has the tie).
+    // The tile whose waves take least; ns of a block of 128 x TN with every SM at it, measured.
+    constexpr int kTile[5] = {256, 192, 160, 128, 64}, kTime[5] = {590, 470, 410, 330, 270};
     int best = 0;
     int64_t least = INT64_MAX;
-    for (int tile : {512, 256, 192, 160, 128, 64}) {
-        const int group = tile == 512 ? 2 : 1, tn = tile == 512 ? 256 : tile, room = sms > group ? sms / group : 1;
-        const int64_t tiles = int64_t((a.rows + 128 * group - 1) / (128 * group)) * ((a.width + tn - 1) / tn);
-        const int64_t cost = (tiles + room - 1) / room * (2880 + 13 * tn);
-        if (cost < least) least = cost, best = tile;
+    for (int i = 0; i < 5; ++i) {
+        const int64_t tiles = int64_t((a.rows + 127) / 128) * ((a.width + kTile[i] - 1) / kTile[i]);
+        const int64_t time = (tiles + sms - 1) / sms * kTime[i];
+        if (time < least) least = time, best = kTile[i];
     }
     switch (best) {
-        case 512: return launch_tile<T, 256, 2>(a, wide, sms, s);
-        case 256: return launch_tile<T, 256, 1>(a, wide, sms, s);
-        case 192: return launch_tile<T, 192, 1>(a, wide, sms, s);
-        case 160: return launch_tile<T, 160, 1>(a, wide, sms, s);
-        case 128: return launch_tile<T, 128, 1>(a, wide, sms, s);
-        default: return launch_tile<T, 64, 1>(a, wide, sms, s);
+        case 256: return launch_tile<T, 256>(a, wide, sms, s);
+        case 192: return launch_tile<T, 192>(a, wide, sms, s);
+        case 160: return launch_tile<T, 160>(a, wide, sms, s);
+        case 128: return launch_tile<T, 128>(a, wide, sms, s);
+        default: return launch_tile<T, 64>(a, wide, sms, s);
     }
 }
 
