@@ -22,29 +22,37 @@ _pack = N.packer(N.SqNormArgs)
 
 def _run(x, weight, residual, eps, fp8):
     shape = x.shape
-    if not shape or not shape[-1]:
+    hidden = shape[-1] if shape else 0
+    if not hidden:
         raise ValueError("x: expected [..., hidden] with hidden >= 1")
-    hidden = shape[-1]
-    rows, total, res_address, res_stride = N.rows_of(x, "x"), None, 0, 0
-    dtype, weight_dtype = N.dtype_code(x.dtype), N.SQ_F32
+    dtype = N.dtype_code(x.dtype)
+    rows, total, res_address, res_stride, weight_dtype, weight_address = N.rows_of(x, "x"), None, 0, 0, N.SQ_F32, 0
     if weight is not None:
         if weight.shape != (hidden,):
             raise ValueError(f"weight: expected [{hidden}], got {list(weight.shape)}")
         weight_dtype = N.dtype_code(weight.dtype)
         weight = weight.contiguous()
+        weight_address = weight.data_ptr()
     if not eps >= 0:
         raise ValueError("eps must not be negative")
     if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
         raise ValueError("residual: expected x's shape and dtype")
     index = N.device_index(x, weight, residual)
+    count = rows.shape[0]
+    # empty_like is the quicker allocation, of the right layout only for contiguous rows.
+    like = x if x.is_contiguous() else None
     if residual is not None:
         res = N.rows_of(residual, "residual")
         res_address, res_stride = res.data_ptr(), res.stride(0)
-        total = x.new_empty(shape)
-    out = x.new_empty(shape, dtype=FP8) if fp8 else x.new_empty(shape)
-    scale = x.new_empty((*shape[:-1], (hidden + BLOCK - 1) // BLOCK), dtype=torch.float32) if fp8 else None
-    N.launch(N.lib().sq_rms_norm, _pack(rows.data_ptr(), res_address, N.address(weight), N.address(total), out.data_ptr(),
-                                        N.address(scale), rows.stride(0), res_stride, rows.shape[0], hidden, dtype,
+        total = x.new_empty(shape) if like is None else torch.empty_like(x)
+    if fp8:
+        out = x.new_empty(shape, dtype=FP8) if like is None else torch.empty_like(x, dtype=FP8)
+        scale = x.new_empty((*shape[:-1], (hidden + BLOCK - 1) // BLOCK), dtype=torch.float32)
+        scale_address = scale.data_ptr()
+    else:
+        out, scale, scale_address = x.new_empty(shape) if like is None else torch.empty_like(x), None, 0
+    N.launch(N.lib().sq_rms_norm, _pack(rows.data_ptr(), res_address, weight_address, 0 if total is None else total.data_ptr(),
+                                        out.data_ptr(), scale_address, rows.stride(0), res_stride, count, hidden, dtype,
                                         weight_dtype, weight is not None, eps), index)
     return out, scale, total
 

@@ -25,15 +25,21 @@ STATES = (4, 8, 16, 32, 64)
 _pack = N.packer(N.SqScanArgs)
 
 
-def _token_groups(x, u, states, name):
+def _token_groups(x, tokens, states, dtype, name):
     """b or c as [tokens, groups, states] with a token's groups contiguous."""
-    if x.dim() == u.dim():  # one group
-        x = x.unsqueeze(-2)
-    if x.dim() == 4 and x.shape[0] == 1:
-        x = x[0]
-    if x.dim() != 3 or x.shape[0] != u.shape[-2] or x.shape[2] != states or x.dtype != u.dtype:
-        raise ValueError(f"{name}: expected {u.dtype} [{u.shape[-2]}, groups, {states}]")
-    return x if x.stride(2) == 1 and (x.shape[1] == 1 or x.stride(1) == states) else x.contiguous()
+    shape = x.shape
+    if len(shape) != 3 or shape[0] != tokens:
+        if len(shape) == 2:  # one group
+            x = x.unsqueeze(1)
+        elif len(shape) == 4 and shape[0] == 1:
+            x = x[0]
+        elif len(shape) == 3 and shape[0] == 1 and shape[1] == tokens:  # a leading batch of 1, one group
+            x = x[0].unsqueeze(1)
+        shape = x.shape
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != states or x.dtype != dtype:
+        raise ValueError(f"{name}: expected {dtype} [{tokens}, groups, {states}]")
+    stride = x.stride()
+    return x if stride[2] == 1 and (shape[1] == 1 or stride[1] == states) else x.contiguous()
 
 
 def _row_input(x, u, name):
@@ -53,33 +59,37 @@ def _channel_vector(x, channels, name):
 class _Call:
     """Checked operands of one call, and the launch of an entry point on them."""
 
+    __slots__ = ("tokens", "channels", "states", "groups", "index", "kept", "pointers", "strides", "tail")
+
     def __init__(self, u, dt, a, b, c, d, z, dt_bias, softplus):
-        self.u = N.rows_of(u, "u")
-        self.tokens, self.channels = self.u.shape
-        if a.dim() != 2 or a.shape[0] != self.channels or a.dtype != torch.float32:
-            raise ValueError(f"a: expected float32 [{self.channels}, states]")
-        self.states = a.shape[1]
-        if self.states not in STATES:
-            raise NotImplementedError(f"the scan is built for {STATES} states, got {self.states}")
-        self.a = N.aligned(a)
-        self.dt = _row_input(dt, u, "dt")
-        self.z = None if z is None else _row_input(z, u, "z")
-        self.b, self.c = _token_groups(b, u, self.states, "b"), _token_groups(c, u, self.states, "c")
-        self.groups = self.b.shape[1]
-        if self.c.shape[1] != self.groups or self.groups < 1 or self.channels < 1 or self.channels % self.groups:
+        rows = N.rows_of(u, "u")
+        tokens, channels = rows.shape
+        if a.dim() != 2 or a.shape[0] != channels or a.dtype != torch.float32:
+            raise ValueError(f"a: expected float32 [{channels}, states]")
+        states = a.shape[1]
+        if states not in STATES:
+            raise NotImplementedError(f"the scan is built for {STATES} states, got {states}")
+        a, dtype = N.aligned(a), u.dtype
+        dt = _row_input(dt, u, "dt")
+        z = None if z is None else _row_input(z, u, "z")
+        b, c = _token_groups(b, tokens, states, dtype, "b"), _token_groups(c, tokens, states, dtype, "c")
+        groups = b.shape[1]
+        if c.shape[1] != groups or groups < 1 or channels < 1 or channels % groups:
             raise ValueError("b and c need the same groups, a divisor of the channels")
-        self.d, self.dt_bias = _channel_vector(d, self.channels, "d"), _channel_vector(dt_bias, self.channels, "dt_bias")
-        self.softplus = bool(softplus)
-        self.index = N.device_index(self.u, self.a, self.dt, self.z, self.b, self.c, self.d, self.dt_bias)
+        d, dt_bias = _channel_vector(d, channels, "d"), _channel_vector(dt_bias, channels, "dt_bias")
+        self.index = N.device_index(rows, a, dt, z, b, c, d, dt_bias)
+        self.tokens, self.channels, self.states, self.groups = tokens, channels, states, groups
+        p = N.address
+        self.kept = (rows, dt, z, b, c, a, d, dt_bias)  # copies made above live until the launch
+        self.pointers = (rows.data_ptr(), dt.data_ptr(), p(z), b.data_ptr(), c.data_ptr(), a.data_ptr(), p(d), p(dt_bias))
+        self.strides = (rows.stride(0), dt.stride(0), 0 if z is None else z.stride(0), b.stride(0), c.stride(0))
+        self.tail = (channels, states, groups, N.dtype_code(dtype), bool(softplus))
 
     def launch(self, entry, y, initial, final, slots, cu, status, workspace, seqs):
         p = N.address
-        N.launch(entry, _pack(self.u.data_ptr(), self.dt.data_ptr(), p(self.z), self.b.data_ptr(), self.c.data_ptr(),
-                              self.a.data_ptr(), p(self.d), p(self.dt_bias), y.data_ptr(), p(initial), p(final), p(slots),
-                              p(cu), p(status), p(workspace), 0 if workspace is None else workspace.numel(),
-                              self.u.stride(0), self.dt.stride(0), 0 if self.z is None else self.z.stride(0),
-                              self.b.stride(0), self.c.stride(0), 0 if final is None else final.shape[0], self.tokens, seqs,
-                              self.channels, self.states, self.groups, N.dtype_code(self.u.dtype), self.softplus), self.index)
+        N.launch(entry, _pack(*self.pointers, y.data_ptr(), p(initial), p(final), p(slots), p(cu), p(status), p(workspace),
+                              0 if workspace is None else workspace.numel(), *self.strides,
+                              0 if final is None else final.shape[0], self.tokens, seqs, *self.tail), self.index)
 
 
 def _state(state, rows, channels, states, name):
