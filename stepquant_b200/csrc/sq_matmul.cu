@@ -17,12 +17,12 @@
 // in a loop of seconds the GPU runs at its 1000 W limit, 1.53 GHz.  Measured on the
 // way at 16384 x 8256 x 5120: packed fp32 pairs in the epilogue 811 us, single ones,
 // a part released as soon as it is in registers, scales loaded four blocks ahead
-// and two product warps in turn 698 us (1.98 PFLOP/s; 814 us at the power limit).
+// and two product warps in turn 685 us (2.02 PFLOP/s; 814 us at the power limit).
 // Pairs of CTAs (256 x 256 tiles, 32 KB a block and SM) measured 705 and 827 us.
 // Few rows (split_kernel): the weights' bytes bound the call.  Lanes are 128
 // rows of w (one scale a block), columns the rows of x; the CTAs of a cluster
 // split K and add their sums in rank order through distributed shared memory
-// (8 x 8256 x 5120: 11.9 us, 3.6 TB/s).
+// (8 x 8256 x 5120: 11.4 us, 3.7 TB/s).
 //
 // Operands arrive by TMA (128-byte swizzle; zeros past K, M and N), one warp
 // issues the copies, one or two the products; every wait is bounded.
@@ -102,13 +102,18 @@ __device__ __forceinline__ void set_up(Sync &s, int stages, uint32_t columns, in
 // address of the first stage, its two operand tiles kRowTile apart.
 template <int N, int W, int PARTS, int STAGES, int STAGE_BYTES>
 __device__ __forceinline__ void issue_blocks(Sync &s, int w, int64_t count, uint32_t tmem, uint32_t base) {
+    // A wait knows its phase from the one before by parity alone, so it may only begin when the phase two
+    // before has ended.  Copies land in any order: with the stages even each warp has its own, and waits
+    // for every use of them.  Parts are released in order, so the other warp's are no trouble; free_ first,
+    // so that a block's stage is asked about only when the blocks before it are.
+    static_assert(STAGES % W == 0, "two product warps must not share a stage");
     Ring<STAGES> at;
     Ring<PARTS> part;
     int64_t it = w;
     bool ok = true;
     if (w) at.next(), part.next();
     for (; it < count; it += W) {
-        ok = tc::bar_wait(&s.full[at.stage], at.parity, &s.abort) && tc::bar_wait(&s.free_[part.stage], part.parity ^ 1, &s.abort);
+        ok = tc::bar_wait(&s.free_[part.stage], part.parity ^ 1, &s.abort) && tc::bar_wait(&s.full[at.stage], at.parity, &s.abort);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc::fence_after();
         if (tc::elected()) {
@@ -147,7 +152,7 @@ struct TileShape {
     static constexpr int kStage = kRowTile + TN * kBlock;
     static constexpr int kStaging = kEpilogueWarps * 32 * 16 * 4;
     static constexpr int kRoom = (226 * 1024 - kStaging - 1024 - int(sizeof(Sync))) / kStage;
-    static constexpr int kStages = kRoom > 8 ? 8 : kRoom;
+    static constexpr int kStages = kRoom > 8 ? 8 : kRoom & ~1;  // even, for the two product warps
     static constexpr int kBytes = kStages * kStage + kStaging + 1024 + int(sizeof(Sync));
     static constexpr int kParts = 512 / TN < kMostParts ? 512 / TN : kMostParts;
     static constexpr int kColumns = kParts * TN <= 256 ? 256 : 512;
@@ -356,12 +361,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 template <int TM>
 struct SplitShape {
     static constexpr int kStage = kRowTile + TM * kBlock;
-    static constexpr int kStages = 98304 / kStage;  // 5, 4, 4, 3: two CTAs an SM
+    static constexpr int kProductWarps = TM <= 32 ? 2 : 1;  // more rows have no registers for a second
+    static constexpr int kStages = 112640 / kStage / kProductWarps * kProductWarps;  // 6, 4, 4, 3: two CTAs an SM
     static constexpr int kScales = 2 * kScaleGroup * TM * 4;  // of two groups of blocks
     static constexpr int kBytes = kStages * kStage + kScales + 1024 + int(sizeof(Sync));
     static constexpr int kParts = 256 / TM < kMostParts ? 256 / TM : kMostParts;  // 256 columns: two CTAs an SM
     static constexpr int kColumns = kParts * TM;
-    static constexpr int kProductWarps = TM <= 32 ? 2 : 1;  // more rows have no registers for a second
     static constexpr int kThreads = 32 * (kEpilogueWarps + 1 + kProductWarps);
 };
 

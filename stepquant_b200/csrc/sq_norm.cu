@@ -11,7 +11,10 @@
 //
 // Bound by bytes (6 flops a value): the row is read once into registers, eight
 // values a thread and step, so a block of 128 channels is the eight values of
-// half a warp and its maximum four shuffles.
+// half a warp and its maximum four shuffles.  Measured, bf16 with residual and
+// e4m3 output: 65536 x 5120 in 397 us (5.9 TB/s, 0.92 of the measured copy; with a
+// CTA a row and nothing on its way 560 us), one row of 5120 in 2.7 us, of launch
+// and two trips to memory; 777 x 4100 f16 (rows on 8-byte boundaries) 6.0 us.
 #include <cuda_fp8.h>
 
 #include "sq_vec.cuh"

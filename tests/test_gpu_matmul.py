@@ -49,6 +49,24 @@ SHAPES = [(1, 1, 16), (1, 128, 128), (3, 130, 144), (16, 300, 256), (17, 100, 20
           (1000, 1500, 640), (140, 20000, 96), (2500, 260, 128), (4, 9000, 640), (1, 5120, 4096)]
 
 
+@pytest.mark.parametrize("rows,width,hidden", [(8, 16384, 8192), (16, 9000, 8192), (32, 16384, 4096), (64, 5000, 8192),
+                                               (128, 5120, 8192), (512, 5120, 8192), (512, 6500, 8192), (700, 8200, 8192)])
+def test_deep_products(rows, width, hidden):
+    """Many blocks a CTA, weights that do not stay in L2: the copies of different blocks land in any order."""
+    from stepquant_b200.kernels.matmul import matmul_fp8
+    x, sx, w, sw = _data(rows, width, hidden, 7)
+    status = torch.zeros(1, device="cuda", dtype=torch.int32)
+    flush = torch.empty(1 << 26, device="cuda")
+    want = None
+    for _ in range(6):
+        flush.zero_()
+        got = matmul_fp8(x, sx, w, sw, status=status)
+        want = got if want is None else want
+        assert torch.equal(got, want)
+    _close(want, x, sx, w, sw)
+    assert int(status) == 0
+
+
 @pytest.mark.parametrize("rows,width,hidden", SHAPES)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_product(rows, width, hidden, dtype):
