@@ -5,8 +5,8 @@
 // x [M, K] has a scale per row and 128 columns, w [N, K] one per 128 rows and
 // 128 columns.  The tensor cores form each 128-deep block product in fp32 tensor
 // memory; the epilogue warps scale it and add it to fp32 registers while the next
-// block's product runs into the other half of the tensor memory.  One rounding,
-// of the finished sum with the residual.
+// blocks' products run into other parts of the tensor memory.  One rounding, of
+// the finished sum with the residual.
 //
 // Many rows (tile_kernel): tensor memory lanes are rows of x, columns are rows
 // of w, so a thread's scale is one number a block.  Persistent CTAs of 128 x TN
