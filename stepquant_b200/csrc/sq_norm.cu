@@ -12,10 +12,12 @@
 // Bound by bytes (6 flops a value): the row is read once into registers, eight
 // values a thread and step, so a block of 128 channels is the eight values of
 // half a warp and its maximum four shuffles.  Measured, bf16 with residual and
-// e4m3 output: 65536 x 5120 in 397 us (5.9 TB/s, 0.92 of the measured copy; with a
-// CTA a row and nothing on its way 560 us), one row of 5120 in 2.7 us, of launch
-// and two trips to memory; 777 x 4100 f16 (rows on 8-byte boundaries) 6.0 us.
+// e4m3 output: 65536 x 5120 in 391 us (6.0 TB/s, 0.94 of the measured copy; with a
+// CTA a row and nothing on its way 560 us), one row of 5120 in 2.8 us, of launch
+// and two trips to memory; 777 x 4100 f16 (rows on 8-byte boundaries) 5.9 us.
 #include <cuda_fp8.h>
+
+#include <type_traits>
 
 #include "sq_vec.cuh"
 
@@ -32,113 +34,212 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// Sum over the TPR threads of a row: one warp, or the whole CTA.
-template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float *scratch) {
+// Sum over a group of LANES neighbouring lanes.
+template <int LANES>
+__device__ __forceinline__ float lane_sum(float v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (TPR == 32) return v;
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// Sum over the CTA.
+__device__ __forceinline__ float cta_sum(float v, float *scratch) {
+    v = lane_sum<32>(v);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (lane == 0) scratch[warp] = v;
     __syncthreads();
-    const int warps = blockDim.x >> 5;
-    v = lane < warps ? scratch[lane] : 0.f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    return lane_sum<32>(lane < int(blockDim.x >> 5) ? scratch[lane] : 0.f);
 }
 
-// Eight weights from `at` on.
-__device__ __forceinline__ void load_weights(const sq_norm_args &a, int at, int width, int n, float (&w)[8]) {
-    if (a.weight_dtype == SQ_F32) load8(static_cast<const float *>(a.weight) + at, width, n, w);
-    else if (a.weight_dtype == SQ_BF16) load8(static_cast<const __nv_bfloat16 *>(a.weight) + at, width, n, w);
-    else load8(static_cast<const __half *>(a.weight) + at, width, n, w);
+// A row is cut in units of 8 LANES channels, eight a lane: neighbours where an
+// access takes WIDTH (8 or 4) of them; LANES apart where rows are aligned for
+// single ones only, so that the lanes of an access are neighbours: 32768 rows of 5119
+// in 314 us, 777 x 4099 f16 in 8 us (eight neighbours a lane there too: 586 and 22 us).
+template <int WIDTH, int LANES>
+struct Place {
+    static constexpr int kStep = WIDTH == 1 ? LANES : 1;
+    int at, n;  // the lane's first channel, and how many of its eight are in the row (<= 0: none)
+    Place() = default;
+    __device__ __forceinline__ Place(int unit, int lane, int hidden) {
+        at = unit * LANES * 8 + (WIDTH == 1 ? lane : lane * 8);
+        n = min(8, (hidden - at + kStep - 1) / kStep);
+        if (at >= hidden) n = 0;
+    }
+    template <class T>
+    __device__ __forceinline__ void load(const T *row, T (&v)[8]) const {
+        const T *p = row + at;
+        constexpr int kPer = WIDTH * sizeof(T) < 16 ? WIDTH : 16 / sizeof(T);
+        using Piece = std::conditional_t<kPer * sizeof(T) == 16, uint4, std::conditional_t<kPer * sizeof(T) == 8, uint2, T>>;
+#pragma unroll
+        for (int i = 0; i < 8; i += kPer)
+            *reinterpret_cast<Piece *>(v + i) = i < n ? *reinterpret_cast<const Piece *>(p + i * kStep) : Piece{};
+    }
+    template <class T>
+    __device__ __forceinline__ void store(T *row, const T (&v)[8]) const {
+        T *p = row + at;
+        constexpr int kPer = WIDTH * sizeof(T) < 16 ? WIDTH : 16 / sizeof(T);
+        using Piece = std::conditional_t<kPer * sizeof(T) == 16, uint4,
+                                         std::conditional_t<kPer * sizeof(T) == 8, uint2,
+                                                            std::conditional_t<kPer * sizeof(T) == 4, uint32_t, T>>>;
+#pragma unroll
+        for (int i = 0; i < 8; i += kPer)
+            if (i < n) *reinterpret_cast<Piece *>(p + i * kStep) = *reinterpret_cast<const Piece *>(v + i);
+    }
+    __device__ __forceinline__ void load_weights(const sq_norm_args &a, float (&w)[8]) const {
+        auto from = [&](auto *p) {
+            alignas(16) std::remove_const_t<std::remove_pointer_t<decltype(p)>> v[8];
+            load(p, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = to_float(v[i]);
+        };
+        if (a.weight_dtype == SQ_F32) from(static_cast<const float *>(a.weight));
+        else if (a.weight_dtype == SQ_BF16) from(static_cast<const __nv_bfloat16 *>(a.weight));
+        else from(static_cast<const __half *>(a.weight));
+    }
+    template <class T>
+    __device__ __forceinline__ void round(T *row, const float (&x)[8]) const {
+        alignas(16) T v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = from_float<T>(x[i]);
+        store(row, v);
+    }
+    // Eight outputs: in T, or e4m3 with the scale of their 128 channels (every lane of the
+    // warp calls; `mine`: there is such a row).
+    template <class T>
+    __device__ __forceinline__ void put(const sq_norm_args &a, int64_t row, bool mine, const float (&y)[8]) const {
+        if (!a.scale) {
+            if (mine) round(static_cast<T *>(a.out) + row * a.hidden, y);
+            return;
+        }
+        // Blocks of 128: the eight neighbours of 16 lanes, or 128 / LANES of the eight of the group.
+        constexpr int kBlocks = WIDTH == 1 ? LANES / 16 : 1, kEach = 8 / kBlocks;
+        alignas(8) uint8_t q[8];
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) top = max_nan(top, fabsf(y[b * kEach + i]));
+#pragma unroll
+            for (int o = WIDTH == 1 ? LANES / 2 : 8; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float scale = max_nan(top, kScaleFloor) / kE4m3Max, inverse = 1.f / scale;
+            const int first = at + b * 128;  // of the block, for its first lane
+            if (first % 128 == 0 && first < a.hidden && mine) a.scale[row * ((a.hidden + 127) / 128) + first / 128] = scale;
+#pragma unroll
+            for (int i = b * kEach; i < (b + 1) * kEach; i += 2)
+                *reinterpret_cast<uint16_t *>(q + i) =
+                    __nv_cvt_float2_to_fp8x2(make_float2(y[i] * inverse, y[i + 1] * inverse), __NV_SATFINITE, __NV_E4M3);
+        }
+        if (mine) store(static_cast<uint8_t *>(a.out) + row * a.hidden, q);
+    }
+};
+
+// Short rows: a group of LANES lanes a row, CH units each, the group's next row on
+// its way; the weights stay in registers and nothing is shared between warps.
+// 100000 bf16 rows of 336 to e4m3: 39 us (a grid of all rows, each warp ending after
+// its own, 61 us; two rows a turn, 142 registers, 69 us).
+template <class T, int CH, int LANES, int WIDTH>
+__global__ void __launch_bounds__(256, CH == 1 ? 4 : 3) norm_lanes_kernel(sq_norm_args a) {
+    const int lane = threadIdx.x % LANES;
+    const int groups = int(gridDim.x) * (256 / LANES);
+    // The row of the warp's first group: the loop's, the same for a warp's lanes.
+    const int64_t first = (int64_t(blockIdx.x) * 256 + (threadIdx.x & ~31)) / LANES;
+    int64_t row = first + (threadIdx.x & 31) / LANES;
+    alignas(16) T x[CH][8], res[CH][8];
+    Place<WIDTH, LANES> place[CH];
+    float w[CH][8];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) place[c] = Place<WIDTH, LANES>(c, lane, a.hidden);
+    auto fetch = [&](int64_t from) {
+        if (from >= a.rows) return;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) place[c].load(static_cast<const T *>(a.x) + from * a.x_stride, x[c]);
+        if (!a.residual) return;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) place[c].load(static_cast<const T *>(a.residual) + from * a.residual_stride, res[c]);
+    };
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            x[c][i] = from_float<T>(0.f);
+            w[c][i] = 1.f;
+        }
+    fetch(row);
+    if (a.weight) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) place[c].load_weights(a, w[c]);
+    }
+    for (int64_t turn = first; turn < a.rows; turn += groups, row += groups) {
+        float h[CH][8], squares = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[c][i] = to_float(x[c][i]);
+        if (a.residual) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) h[c][i] += to_float(res[c][i]);
+        }
+        fetch(row + groups);
+        const bool mine = row < a.rows;
+        if (a.residual && mine) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) place[c].round(static_cast<T *>(a.residual_out) + row * a.hidden, h[c]);
+        }
+        if (a.normalize) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) squares += h[c][i] * h[c][i];
+            const float factor = rsqrtf(lane_sum<LANES>(squares) / float(a.hidden) + a.eps);
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) h[c][i] = h[c][i] * factor * w[c][i];
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) place[c].template put<T>(a, row, mine, h[c]);
+    }
 }
 
-// Eight outputs of a row: in T, or e4m3 with the scale of their 128 channels
-// (the eight values of 16 neighbouring lanes; every lane of the warp calls).
-template <class T>
-__device__ __forceinline__ void put(const sq_norm_args &a, int64_t row, int at, int width, int n, const float (&y)[8]) {
-    if (!a.scale) {
-        if (n > 0) store8(static_cast<T *>(a.out) + row * a.hidden + at, width, n, y);
-        return;
-    }
-    float top = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(y[i]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float scale = max_nan(top, kScaleFloor) / kE4m3Max, inverse = 1.f / scale;
-    if (n <= 0) return;
-    if ((threadIdx.x & 15) == 0) a.scale[row * ((a.hidden + 127) / 128) + at / 128] = scale;
-    uint32_t q[2];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * i] * inverse, y[2 * i + 1] * inverse), __NV_SATFINITE, __NV_E4M3);
-        q[i / 2] = i % 2 ? q[i / 2] | two << 16 : two;
-    }
-    uint8_t *out = static_cast<uint8_t *>(a.out) + row * a.hidden + at;
-    if (width == 8 && n == 8) {
-        *reinterpret_cast<uint2 *>(out) = make_uint2(q[0], q[1]);
-    } else if (width >= 4) {
-        reinterpret_cast<uint32_t *>(out)[0] = q[0];
-        if (n > 4) reinterpret_cast<uint32_t *>(out)[1] = q[1];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n) out[i] = uint8_t(q[i / 4] >> (8 * (i % 4)));
-    }
-}
-
-// TPR threads a row (32: a warp each; 0: the CTA), each with CH steps of 8 values.
-template <class T, int CH, int TPR>
-__global__ void __launch_bounds__(TPR ? 256 : 1024) norm_kernel(sq_norm_args a, int width) {
+// A CTA a row, each thread with CH steps of 8 values.
+template <class T, int CH, int WIDTH>
+__global__ void __launch_bounds__(1024) norm_kernel(sq_norm_args a) {
     __shared__ float scratch[32];
-    const int tpr = TPR ? TPR : blockDim.x;
-    const int64_t row = TPR ? int64_t(blockIdx.x) * (blockDim.x / 32) + (threadIdx.x >> 5) : blockIdx.x;
-    const int t = TPR ? threadIdx.x & 31 : threadIdx.x;
-    if (TPR && row >= a.rows) return;  // whole warps
-    const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
-    const T *res = a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
+    const int64_t row = blockIdx.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     float h[CH][8];
-    float squares = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int at = (c * tpr + t) * 8, n = min(8, a.hidden - at);
-        if (n > 0) {
-            load8(x + at, width, n, h[c]);
-            if (res) {
-                float r[8];
-                load8(res + at, width, n, r);
+        const Place<WIDTH, 32> place(c * warps + warp, lane, a.hidden);
+        alignas(16) T x[8], res[8];
+        place.load(static_cast<const T *>(a.x) + row * a.x_stride, x);
+        if (a.residual) place.load(static_cast<const T *>(a.residual) + row * a.residual_stride, res);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) h[c][i] += r[i];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) h[c][i] = 0.f;
+        for (int i = 0; i < 8; ++i) {
+            h[c][i] = to_float(x[i]);
+            if (a.residual) h[c][i] += to_float(res[i]);
         }
     }
-    float factor = 1.f;
-    if (a.normalize) {
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int at = (c * tpr + t) * 8, n = min(8, a.hidden - at);
-            if (res && n > 0) store8(static_cast<T *>(a.residual_out) + row * a.hidden + at, width, n, h[c]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) squares += h[c][i] * h[c][i];
-        }
-        factor = rsqrtf(row_sum<TPR>(squares, scratch) / float(a.hidden) + a.eps);
-    }
+    float squares = 0.f, factor = 1.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int at = (c * tpr + t) * 8, n = min(8, a.hidden - at);
-        if (a.weight && n > 0) {
+        if (a.residual)
+            Place<WIDTH, 32>(c * warps + warp, lane, a.hidden).round(static_cast<T *>(a.residual_out) + row * a.hidden, h[c]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) squares += h[c][i] * h[c][i];
+    }
+    if (a.normalize) factor = rsqrtf(cta_sum(squares, scratch) / float(a.hidden) + a.eps);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const Place<WIDTH, 32> place(c * warps + warp, lane, a.hidden);
+        if (a.weight) {
             float w[8];
-            load_weights(a, at, width, n, w);
+            place.load_weights(a, w);
 #pragma unroll
             for (int i = 0; i < 8; ++i) h[c][i] = h[c][i] * factor * w[i];
         }
-        put<T>(a, row, at, width, n, h[c]);
+        place.template put<T>(a, row, true, h[c]);
     }
 }
 
@@ -159,7 +260,7 @@ __global__ void __launch_bounds__(512) norm_rows_kernel(sq_norm_args a) {
         const int at = (c * threads + t) * 8;
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[c][i] = 0.f;
-        if (at < a.hidden) load_weights(a, at, 8, 8, w[c]);
+        if (at < a.hidden) Place<8, 32>(c * (threads / 32) + t / 32, t % 32, a.hidden).load_weights(a, w[c]);
     }
     auto slot = [&](int stage, int which, int c) { return ring + int64_t((((stage * 2 + which) * CH + c) * threads + t)) * kPiece; };
     auto fetch = [&](int64_t row, int stage) {
@@ -192,28 +293,30 @@ __global__ void __launch_bounds__(512) norm_rows_kernel(sq_norm_args a) {
         float h[CH][8], squares = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const int at = (c * threads + t) * 8;
+            const Place<8, 32> place(c * (threads / 32) + t / 32, t % 32, a.hidden);
 #pragma unroll
             for (int i = 0; i < 8; ++i) h[c][i] = 0.f;
-            if (at >= a.hidden) continue;
-            load8(reinterpret_cast<const T *>(slot(stage, 0, c)), 8, 8, h[c]);
-            if (a.residual) {
-                float r[8];
-                load8(reinterpret_cast<const T *>(slot(stage, 1, c)), 8, 8, r);
+            if (place.n <= 0) continue;
+            const T *x = reinterpret_cast<const T *>(slot(stage, 0, c)), *res = reinterpret_cast<const T *>(slot(stage, 1, c));
+            alignas(16) T v[8];
+            Place<8, 32>(0, 0, 8).load(x, v);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) h[c][i] += r[i];
-                store8(static_cast<T *>(a.residual_out) + row * a.hidden + at, 8, 8, h[c]);
+            for (int i = 0; i < 8; ++i) h[c][i] = to_float(v[i]);
+            if (a.residual) {
+                Place<8, 32>(0, 0, 8).load(res, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) h[c][i] += to_float(v[i]);
+                place.round(static_cast<T *>(a.residual_out) + row * a.hidden, h[c]);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) squares += h[c][i] * h[c][i];
         }
-        const float factor = rsqrtf(row_sum<0>(squares, scratch[turn]) / float(a.hidden) + a.eps);
+        const float factor = rsqrtf(cta_sum(squares, scratch[turn]) / float(a.hidden) + a.eps);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const int at = (c * threads + t) * 8;
 #pragma unroll
             for (int i = 0; i < 8; ++i) h[c][i] = h[c][i] * factor * w[c][i];
-            put<T>(a, row, at, 8, min(8, a.hidden - at), h[c]);
+            Place<8, 32>(c * (threads / 32) + t / 32, t % 32, a.hidden).template put<T>(a, row, true, h[c]);
         }
         stage = stage + 1 == kRows ? 0 : stage + 1;
         turn ^= 1;
@@ -231,27 +334,30 @@ cudaError_t launch_rows(const sq_norm_args &a, int threads, int bytes, cudaStrea
     return cudaGetLastError();
 }
 
-template <class T>
-cudaError_t launch_norm(const sq_norm_args &a, cudaStream_t s) {
-    const int64_t size = sizeof(T);
-    auto fits = [&](int n) {  // rows of pieces of n values, each by one access
-        auto on = [&](const void *p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % (bytes < 16 ? bytes : 16) == 0; };
-        return a.hidden % n == 0 && a.x_stride % n == 0 && on(a.x, n * size) &&
-               (!a.residual || (a.residual_stride % n == 0 && on(a.residual, n * size) && on(a.residual_out, n * size))) &&
-               on(a.weight, n * (a.weight_dtype == SQ_F32 ? 4 : 2)) && on(a.out, n * (a.scale ? 1 : size));
-    };
-    const int width = fits(8) ? 8 : fits(4) ? 4 : 1;
-    const int steps = (a.hidden + 7) / 8;
-    if (steps <= 64) {  // up to 512 channels: a warp a row, no barrier
-        const unsigned grid = unsigned((int64_t(a.rows) + 7) / 8);
-        if (steps <= 32) norm_kernel<T, 1, 32><<<grid, 256, 0, s>>>(a, width);
-        else norm_kernel<T, 2, 32><<<grid, 256, 0, s>>>(a, width);
-        return cudaGetLastError();
+template <class T, int CH, int LANES, int WIDTH>
+cudaError_t launch_lanes(const sq_norm_args &a, cudaStream_t s) {
+    const int64_t need = (int64_t(a.rows) * LANES + 255) / 256;
+    int64_t room = sms_of(s);
+    if (need > room) {
+        int each = 0;
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, norm_lanes_kernel<T, CH, LANES, WIDTH>, 256, 0);
+        if (e != cudaSuccess) return e;
+        room *= each > 0 ? each : 1;
     }
+    norm_lanes_kernel<T, CH, LANES, WIDTH><<<unsigned(need < room ? need : room), 256, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+template <class T, int WIDTH>
+cudaError_t launch_width(const sq_norm_args &a, cudaStream_t s) {
+    const int steps = (a.hidden + 7) / 8;
+    if (steps <= 16) return launch_lanes<T, 1, 16, WIDTH>(a, s);
+    if (steps <= 32) return launch_lanes<T, 1, 32, WIDTH>(a, s);
+    if (steps <= 64) return launch_lanes<T, 2, 32, WIDTH>(a, s);
     // Rows on their way while others are worked on, once each resident CTA has several.
-    if (width == 8 && a.normalize && a.rows >= 2048 && steps <= 2048) {
+    if (WIDTH == 8 && a.normalize && a.rows >= 2048 && steps <= 2048) {
         const int ch = steps <= 1024 ? 2 : 4, threads = ((steps + ch - 1) / ch + 31) / 32 * 32;
-        const int bytes = kRows * 2 * ch * threads * 8 * int(size);
+        const int bytes = kRows * 2 * ch * threads * 8 * int(sizeof(T));
         if (bytes <= 200 * 1024)
             return ch == 2 ? launch_rows<T, 2>(a, threads, bytes, s) : launch_rows<T, 4>(a, threads, bytes, s);
     }
@@ -261,12 +367,24 @@ cudaError_t launch_norm(const sq_norm_args &a, cudaStream_t s) {
     const int threads = ((steps + ch - 1) / ch + 31) / 32 * 32;
     const unsigned grid = unsigned(a.rows);
     switch (ch) {
-        case 1: norm_kernel<T, 1, 0><<<grid, threads, 0, s>>>(a, width); break;
-        case 2: norm_kernel<T, 2, 0><<<grid, threads, 0, s>>>(a, width); break;
-        case 4: norm_kernel<T, 4, 0><<<grid, threads, 0, s>>>(a, width); break;
-        default: norm_kernel<T, 8, 0><<<grid, threads, 0, s>>>(a, width); break;
+        case 1: norm_kernel<T, 1, WIDTH><<<grid, threads, 0, s>>>(a); break;
+        case 2: norm_kernel<T, 2, WIDTH><<<grid, threads, 0, s>>>(a); break;
+        case 4: norm_kernel<T, 4, WIDTH><<<grid, threads, 0, s>>>(a); break;
+        default: norm_kernel<T, 8, WIDTH><<<grid, threads, 0, s>>>(a); break;
     }
     return cudaGetLastError();
+}
+
+template <class T>
+cudaError_t launch_norm(const sq_norm_args &a, cudaStream_t s) {
+    const int64_t size = sizeof(T);
+    auto fits = [&](int n) {  // rows of pieces of n values, each by one access
+        auto on = [&](const void *p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % (bytes < 16 ? bytes : 16) == 0; };
+        return a.hidden % n == 0 && a.x_stride % n == 0 && on(a.x, n * size) &&
+               (!a.residual || (a.residual_stride % n == 0 && on(a.residual, n * size) && on(a.residual_out, n * size))) &&
+               on(a.weight, n * (a.weight_dtype == SQ_F32 ? 4 : 2)) && on(a.out, n * (a.scale ? 1 : size));
+    };
+    return fits(8) ? launch_width<T, 8>(a, s) : fits(4) ? launch_width<T, 4>(a, s) : launch_width<T, 1>(a, s);
 }
 
 }  // namespace

@@ -1,5 +1,5 @@
-// Typed access to eight consecutive values, shared by the layer operators
-// (norm, convolution, scan, block-scaled product).
+// Conversions and approximate functions shared by the layer operators (norm,
+// convolution, scan, block-scaled product).
 #pragma once
 
 #include "sq_common.cuh"
@@ -17,58 +17,6 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 template <>
 __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
-
-// Eight values starting at p, of which n exist.  width: how many of them one
-// access takes, by p's alignment (8: 16-byte accesses, n = 8; 4: four values each,
-// n = 4 or 8; 1: singly).  Missing values read as zero.
-template <class T>
-__device__ __forceinline__ void load8(const T *p, int width, int n, float (&x)[8]) {
-    constexpr int kPer = 16 / sizeof(T);
-    alignas(16) T v[8];
-    if (width == 8 && n == 8) {
-#pragma unroll
-        for (int i = 0; i < 8; i += kPer) *reinterpret_cast<uint4 *>(v + i) = *reinterpret_cast<const uint4 *>(p + i);
-    } else if (width >= 4) {
-#pragma unroll
-        for (int i = 0; i < 8; i += 4) {
-            if (i < n) {
-                if (sizeof(T) == 2) *reinterpret_cast<uint2 *>(v + i) = *reinterpret_cast<const uint2 *>(p + i);
-                else *reinterpret_cast<uint4 *>(v + i) = *reinterpret_cast<const uint4 *>(p + i);
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[i + k] = from_float<T>(0.f);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : from_float<T>(0.f);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_float(v[i]);
-}
-
-template <class T>
-__device__ __forceinline__ void store8(T *p, int width, int n, const float (&x)[8]) {
-    constexpr int kPer = 16 / sizeof(T);
-    alignas(16) T v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = from_float<T>(x[i]);
-    if (width == 8 && n == 8) {
-#pragma unroll
-        for (int i = 0; i < 8; i += kPer) *reinterpret_cast<uint4 *>(p + i) = *reinterpret_cast<const uint4 *>(v + i);
-    } else if (width >= 4) {
-#pragma unroll
-        for (int i = 0; i < 8; i += 4)
-            if (i < n) {
-                if (sizeof(T) == 2) *reinterpret_cast<uint2 *>(p + i) = *reinterpret_cast<const uint2 *>(v + i);
-                else *reinterpret_cast<uint4 *>(p + i) = *reinterpret_cast<const uint4 *>(v + i);
-            }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n) p[i] = v[i];
-    }
-}
 
 constexpr float kLog2e = 1.4426950408889634f;
 

@@ -87,6 +87,23 @@ def test_many_rows(rows, hidden, dtype, with_residual):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,hidden", [(40003, 128), (40003, 96), (40003, 100), (40003, 127), (20001, 256), (20001, 204),
+                                         (20001, 255), (20001, 512), (20001, 300), (20001, 509), (20001, 1)])
+def test_many_short_rows(rows, hidden, dtype):
+    """Short rows, half a warp or a warp each, more than the grid takes at once, the last turn not full."""
+    from stepquant_b200.kernels.norm import quantize_fp8, rms_norm, rms_norm_fp8
+    x, residual, weight = _data(rows, hidden, dtype, 7)
+    h, y = _reference(x, weight, residual)
+    want = h.to(dtype) if dtype != torch.float32 else x + residual
+    got, got8 = rms_norm(x, weight, residual), rms_norm_fp8(x, weight, residual)
+    assert torch.equal(got[1], want) and torch.equal(got8[2], want)
+    _close(got[0], y, dtype)
+    _close_fp8(got8[0], got8[1], y)
+    _close_fp8(*quantize_fp8(x), x.double())
+    _close(rms_norm(x, weight), _reference(x, weight, None)[1], dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("rows,hidden", [(1, 1), (7, 130), (3, 4096), (640, 5120)])
 def test_quantize(rows, hidden, dtype):
     from stepquant_b200.kernels.norm import quantize_fp8
