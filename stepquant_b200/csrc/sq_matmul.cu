@@ -17,7 +17,7 @@
 // in a loop of seconds the GPU runs at its 1000 W limit, 1.53 GHz.  Measured on the
 // way at 16384 x 8256 x 5120: packed fp32 pairs in the epilogue 811 us, single ones,
 // a part released as soon as it is in registers, scales loaded four blocks ahead
-// and two product warps in turn 685 us (2.02 PFLOP/s; 814 us at the power limit).
+// and two product warps in turn 685 to 700 us (2.0 PFLOP/s; 814 us at the power limit).
 // Pairs of CTAs (256 x 256 tiles, 32 KB a block and SM) measured 705 and 827 us.
 // Few rows (split_kernel): the weights' bytes bound the call.  Lanes are 128
 // rows of w (one scale a block), columns the rows of x; the CTAs of a cluster
@@ -30,6 +30,8 @@
 #include <cudaTypedefs.h>
 
 #include <mutex>
+
+#include <type_traits>
 
 #include "sq_tc.cuh"
 #include "sq_vec.cuh"
@@ -308,44 +310,65 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 aim(i + step);
                 fetch_scales(0);
             }
-            // Out through shared memory, 16 columns at a time: a row's 16 values leave by four lanes
-            // (four rows of eight per access), the residual's next 16 columns on their way meanwhile.
-            // 16-byte pieces of row r are rotated by r / 2 so that neither side meets bank conflicts.
-            const T *residual = static_cast<const T *>(a.residual);
-            Four<T> old[4];
-            auto fetch = [&](int c) {
+            // Out through shared memory, 16 columns at a time, the residual's next 16 columns on their way
+            // meanwhile: a row's 16 values leave by four lanes (four rows of eight per access), or singly
+            // where rows are not aligned for that (two rows per access, every value in a register of its
+            // own: packed on arrival, as fours would be, each load was waited for, 4096 x 8255 x 5120 with
+            // residual in 336 us for 232).  16-byte pieces of row r are rotated by r / 2 so that neither side
+            // meets bank conflicts.
+            auto put = [&](auto four) {
+                constexpr bool kFour = decltype(four)::value;
+                using Value = std::conditional_t<kFour, Four<T>, T>;
+                constexpr int kEach = kFour ? 4 : 1, kAccesses = 16 / kEach, kLanes = 16 / kEach;
+                const int r0 = lane / kLanes, c0 = lane % kLanes * kEach;  // within the rows of an access
+                constexpr int kRows = 32 / kLanes;
+                const int rows = a.rows - m0 - r0, columns = a.width - n0 - c0;  // that exist from the lane's first on
+                const int64_t out_step = int64_t(kRows) * a.width, residual_step = int64_t(kRows) * a.residual_stride;
+                const T *residual = a.residual ? static_cast<const T *>(a.residual) + int64_t(m0 + r0) * a.residual_stride + n0 + c0 : nullptr;
+                T *out = static_cast<T *>(a.out) + int64_t(m0 + r0) * a.width + n0 + c0;
+                Value old[kAccesses];
+                auto fetch = [&](int c) {
+                    if (!residual || 16 * c >= columns) return;
+                    const T *from = residual + 16 * c;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int m = m0 + q * 8 + (lane >> 2), n = n0 + 16 * c + 4 * (lane & 3);
-                    if (residual && m < a.rows && n < a.width)
-                        old[q].load(residual + int64_t(m) * a.residual_stride + n, wide, a.width - n);
+                    for (int i = 0; i < kAccesses; ++i, from += residual_step)
+                        if (i * kRows < rows) old[i] = *reinterpret_cast<const Value *>(from);
+                };
+                if (kFour) fetch(0);
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c) {
+                    if (!kFour) fetch(c);
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float *v = acc + 16 * c + 4 * j;
+                        *reinterpret_cast<float4 *>(stage + lane * 16 + ((j + (lane >> 1)) & 3) * 4) = make_float4(v[0], v[1], v[2], v[3]);
+                    }
+                    __syncwarp();
+                    Value add[kAccesses];
+#pragma unroll
+                    for (int i = 0; i < kAccesses; ++i) add[i] = old[i];
+                    if (kFour && c + 1 < CHUNKS) fetch(c + 1);
+                    T *to = out + 16 * c;
+#pragma unroll
+                    for (int i = 0; i < kAccesses; ++i, to += out_step) {
+                        const int row = i * kRows + r0;
+                        const float *from = stage + row * 16 + (((c0 >> 2) + (row >> 1)) & 3) * 4 + (c0 & 3);
+                        Value y;
+                        if constexpr (kFour) {
+                            const float4 v = *reinterpret_cast<const float4 *>(from);
+                            const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) y.v[j] = from_float<T>(residual ? x[j] + to_float(add[i].v[j]) : x[j]);
+                        } else {
+                            y = from_float<T>(residual ? *from + to_float(add[i]) : *from);
+                        }
+                        if (i * kRows < rows && 16 * c < columns) *reinterpret_cast<Value *>(to) = y;
+                    }
                 }
             };
-            fetch(0);
-#pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) {
-                __syncwarp();
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float *v = acc + 16 * c + 4 * j;
-                    *reinterpret_cast<float4 *>(stage + lane * 16 + ((j + (lane >> 1)) & 3) * 4) = make_float4(v[0], v[1], v[2], v[3]);
-                }
-                __syncwarp();
-                Four<T> add[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) add[q] = old[q];
-                if (c + 1 < CHUNKS) fetch(c + 1);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int row = q * 8 + (lane >> 2), m = m0 + row, n = n0 + 16 * c + 4 * (lane & 3);
-                    const float4 v = *reinterpret_cast<const float4 *>(stage + row * 16 + (((lane & 3) + (row >> 1)) & 3) * 4);
-                    const float x[4] = {v.x, v.y, v.z, v.w};
-                    Four<T> y;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) y.v[j] = from_float<T>(residual ? x[j] + to_float(add[q].v[j]) : x[j]);
-                    if (m < a.rows && n < a.width) y.store(static_cast<T *>(a.out) + int64_t(m) * a.width + n, wide, a.width - n);
-                }
-            }
+            if (wide) put(std::true_type());
+            else put(std::false_type());
         }
     }
     tc::fence_before();
