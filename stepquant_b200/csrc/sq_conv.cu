@@ -14,7 +14,9 @@
 // worked on; strips overlap by their W - 1 leading inputs.  Measured at 8192 bf16
 // channels: 32768 tokens in 184 us (5.8 TB/s, 0.91 of the measured copy); eight
 // channels a thread 431 us (loads held behind stores, half the threads), a branch
-// between the tokens of a batch 218 us.  One token of 256 requests 8.5 us (4 TB/s).
+// between the tokens of a batch 218 us.  One token of 256 requests 8.7 us (4 TB/s).
+// Rows aligned for two channels or one take them so, with more instructions a byte:
+// 8190 channels 234 us (singly 312), 8191 in 302 us; one token 9.1 and 12.2 us.
 #include <type_traits>
 
 #include "sq_rows.cuh"
@@ -26,11 +28,11 @@ namespace {
 constexpr int kConvThreads = 128;
 constexpr unsigned kGridRows = 32768;  // requests along a grid's second axis, the rest along its third
 
-// N values of VEC channels (a token's, or a state row's), by 8- or 16-byte accesses for four channels.
+// N values of VEC channels (a token's, or a state row's), by accesses of VEC channels, at most 16 bytes.
 template <class T, int N, int VEC>
 struct Run {
     static constexpr int kPiece = VEC * sizeof(T) < 16 ? VEC * sizeof(T) : 16;
-    using Piece = std::conditional_t<kPiece == 16, uint4, uint2>;
+    using Piece = std::conditional_t<kPiece == 16, uint4, std::conditional_t<kPiece == 8, uint2, uint32_t>>;
     alignas(16) T v[N];
     __device__ __forceinline__ void load(const T *p) {
         if (VEC > 1) {
@@ -95,9 +97,14 @@ __global__ void __launch_bounds__(kConvThreads) conv_kernel(sq_conv_args a, int 
     Token next[BATCH], now[BATCH];
     auto fetch = [&](int t) {
         const T *from = x + int64_t(t) * a.x_stride;
+        if (t + BATCH <= t1) {
 #pragma unroll
-        for (int j = 0; j < BATCH; ++j, from += a.x_stride)
-            if (t + j < t1) next[j].load(from);
+            for (int j = 0; j < BATCH; ++j, from += a.x_stride) next[j].load(from);
+        } else {
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j, from += a.x_stride)
+                if (t + j < t1) next[j].load(from);
+        }
     };
     fetch(t0);
     const Filter<VEC, W> f(a, d0);
@@ -129,7 +136,8 @@ __global__ void __launch_bounds__(kConvThreads) conv_kernel(sq_conv_args a, int 
         }
         fin.store(static_cast<T *>(a.final_state) + state);
     }
-    auto token = [&](int t, const Token &in) {
+    T *to = y + int64_t(t0) * a.channels;
+    auto token = [&](const Token &in) {
         Token out;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
@@ -143,7 +151,8 @@ __global__ void __launch_bounds__(kConvThreads) conv_kernel(sq_conv_args a, int 
             for (int k = 0; k + 1 < W - 1; ++k) kept[k][i] = kept[k + 1][i];
             kept[W - 2][i] = x_t;
         }
-        out.store(y + int64_t(t) * a.channels);
+        out.store(to);
+        to += a.channels;
     };
     for (int t = t0; t < t1; t += BATCH) {
 #pragma unroll
@@ -151,11 +160,11 @@ __global__ void __launch_bounds__(kConvThreads) conv_kernel(sq_conv_args a, int 
         fetch(t + BATCH);
         if (t + BATCH <= t1) {  // no branch between the tokens of a whole batch
 #pragma unroll
-            for (int j = 0; j < BATCH; ++j) token(t + j, now[j]);
+            for (int j = 0; j < BATCH; ++j) token(now[j]);
         } else {
 #pragma unroll
             for (int j = 0; j < BATCH; ++j)
-                if (t + j < t1) token(t + j, now[j]);
+                if (t + j < t1) token(now[j]);
         }
     }
 }
@@ -213,17 +222,23 @@ cudaError_t launch_conv_as(const sq_conv_args &a, bool step, cudaStream_t s) {
     return cudaGetLastError();
 }
 
+template <class T, int VEC>
+cudaError_t launch_taps(const sq_conv_args &a, bool step, cudaStream_t s) {
+    switch (a.taps) {
+        case 2: return launch_conv_as<T, VEC, 2>(a, step, s);
+        case 3: return launch_conv_as<T, VEC, 3>(a, step, s);
+        default: return launch_conv_as<T, VEC, 4>(a, step, s);
+    }
+}
+
 template <class T>
 cudaError_t launch_conv(const sq_conv_args &a, bool step, cudaStream_t s) {
-    const int64_t four = 4 * sizeof(T);
-    auto fits = [&](const void *p) { return reinterpret_cast<uintptr_t>(p) % four == 0; };
-    const bool vec = a.channels % 4 == 0 && a.x_stride % 4 == 0 && fits(a.x) && fits(a.y) && fits(a.initial_state) &&
-                     fits(a.final_state) && aligned16(a.weight) && aligned16(a.bias);
-    switch (a.taps) {
-        case 2: return vec ? launch_conv_as<T, 4, 2>(a, step, s) : launch_conv_as<T, 1, 2>(a, step, s);
-        case 3: return vec ? launch_conv_as<T, 4, 3>(a, step, s) : launch_conv_as<T, 1, 3>(a, step, s);
-        default: return vec ? launch_conv_as<T, 4, 4>(a, step, s) : launch_conv_as<T, 1, 4>(a, step, s);
-    }
+    auto fits = [&](int n) {  // rows of pieces of n channels
+        auto on = [&](const void *p) { return reinterpret_cast<uintptr_t>(p) % (n * sizeof(T)) == 0; };
+        return a.channels % n == 0 && a.x_stride % n == 0 && on(a.x) && on(a.y) && on(a.initial_state) && on(a.final_state) &&
+               aligned16(a.weight) && aligned16(a.bias);
+    };
+    return fits(4) ? launch_taps<T, 4>(a, step, s) : fits(2) ? launch_taps<T, 2>(a, step, s) : launch_taps<T, 1>(a, step, s);
 }
 
 int32_t conv_entry(const sq_conv_args *args, bool step, sq_stream_t stream) {

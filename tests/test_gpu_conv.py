@@ -101,6 +101,25 @@ def test_step(taps, channels, batch, dtype):
     assert torch.equal(again, kept)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("taps", [2, 3, 4])
+@pytest.mark.parametrize("channels", [2, 258, 770, 771])
+def test_rows_aligned_for_pairs(channels, taps, dtype):
+    """Channels that four do not divide, by pairs or singly; prompts, then a token of each."""
+    from stepquant_b200.kernels.conv import causal_conv1d, causal_conv1d_step
+    cu = [0, 1, 1, 71, 72, 300]
+    x, weight, bias, initial = _data(cu[-1], channels, taps, dtype, len(cu) - 1, 9)
+    y, final = causal_conv1d(x, weight, bias, initial_state=initial, cu_seqlens=torch.tensor(cu, device="cuda"))
+    want, size, kept = _reference(x, weight, bias, cu, initial)
+    _close(y, want, size)
+    assert torch.equal(final, kept)
+    x, pool = x[:5], kept.clone()
+    y = causal_conv1d_step(x, pool, weight, bias)
+    want, size, kept = _reference(x, weight, bias, list(range(6)), kept)
+    _close(y, want, size)
+    assert torch.equal(pool, kept)
+
+
 def test_prompt_in_parts_and_tokens():
     """A prompt in one pass = in two passes = a pass and single tokens, bit for bit."""
     from stepquant_b200.kernels.conv import causal_conv1d, causal_conv1d_extend, causal_conv1d_step
