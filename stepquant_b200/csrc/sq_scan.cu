@@ -116,7 +116,9 @@ struct ScanShape {
     static constexpr int P = N / SN;               // lanes of a channel
     static constexpr int CH = kScanThreads / P;    // channels of the CTA
     static constexpr int TILE = 16;           // tokens of a tile
-    static constexpr int kRow = CH * sizeof(T) + 16, kBcRow = N * sizeof(T) + 16;  // raw rows with their cover
+    // Raw rows with their cover, whole 16-byte pieces (4 states of 16 bits are half a piece).
+    static constexpr int kRow = CH * sizeof(T) + 16, kBcRow = (N * sizeof(T) + 15) / 16 * 16 + 16;
+    static_assert(kRow % 16 == 0 && kBcRow % 16 == 0, "cp.async writes 16-byte aligned pieces");
     static constexpr int kStage = TILE * (3 * kRow + 2 * kBcRow);                  // dt, u, z, B, C
     static constexpr int kBc = TILE * N * 4;
     static constexpr int kBytes = 2 * kBc + 2 * kStage;

@@ -92,6 +92,23 @@ def test_prompts(channels, states, groups, cu, dtype):
         _close(y, final, _reference(t, ends, start))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("channels,groups,batch", [(40, 1, 1), (70, 2, 5), (300, 3, 40), (2048, 1, 9)])
+def test_four_states(channels, groups, batch, dtype):
+    """Rows of B and C of half a 16-byte piece, many tokens; a token of many requests."""
+    from stepquant_b200.kernels.scan import selective_scan, selective_scan_step
+    t = _data(90, channels, 4, groups, dtype, 12)
+    cu = [0, 33, 34, 90]
+    initial = torch.randn(3, channels, 4, device="cuda")
+    y, final = selective_scan(*_core(t), **_options(t), initial_state=initial, cu_seqlens=torch.tensor(cu, device="cuda"))
+    _close(y, final, _reference(t, cu, initial))
+    t = _data(batch, channels, 4, groups, dtype, 13)
+    pool = torch.randn(batch, channels, 4, device="cuda")
+    before = pool.clone()
+    y = selective_scan_step(pool, *_core(t), **_options(t))
+    _close(y, pool, _reference(t, list(range(batch + 1)), before))
+
+
 def test_without_gate_skip_bias_softplus():
     from stepquant_b200.kernels.scan import selective_scan
     t = _data(50, 96, 16, 1, torch.float32, 1, plain=True)
