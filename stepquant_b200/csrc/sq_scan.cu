@@ -322,7 +322,7 @@ __global__ void join_kernel(sq_scan_args a, Chunks chunks) {
     const float A = a.a[i] * kLog2e;
     float h = a.initial_state ? a.initial_state[row * size + i] : 0.f;
     const int64_t base = seq.x / chunks.length + int64_t(n);
-    constexpr int B = 8;  // chunks whose loads are in flight together
+    constexpr int B = 16;  // chunks whose loads are in flight together
     for (int k = 0; k < count; k += B) {
         float own[B], sum[B];
 #pragma unroll
@@ -442,22 +442,38 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(sq_scan_args a,
     }
 }
 
-// Tokens of a chunk, 0 for whole sequences.  A warp of 32 channels alone takes
-// 178 ns a token, a full GPU 0.2 ns a (warp, token), measured at 16 states.  Whole
-// sequences last as long as the longest (the host does not know the lengths: of
-// several, three times the mean is assumed); chunks cost 1.9 times the work.
-// Chunks of 192 to 256 tokens measured best at 2048 and 4096 channels (16 warps a
-// scheduler), 8 ragged prompts of 16384 tokens 705 us against 1103 us whole, one
-// of 8192 tokens 199 us against 1430 us.
-int chunk_length(int tokens, int seqs, int channels, int states) {
-    const double warps = double(channels) * (states > 16 ? states / 16 : 1) / 32;
-    const double work = 0.2 * tokens * warps, alone = 178.0;
-    const double longest = seqs == 1 ? tokens : 3.0 * tokens / seqs < tokens ? 3.0 * tokens / seqs : tokens;
-    const double length = tokens * warps / (592 * 16);
-    const int chunk = length < 128 ? 128 : int(length + 15) / 16 * 16;
-    const double whole = longest * alone > work ? longest * alone : work;
-    const double cut = 10000.0 + (1.9 * work > 2 * chunk * alone ? 1.9 * work : 2 * chunk * alone);
-    return cut < whole ? chunk : 0;
+// Tokens of a chunk, 0 for whole sequences: the least of the estimated times, in ns.
+// A warp alone takes `alone` for a token and a scheduler `turn` for a token of one
+// of its warps, by the states of a lane (16: 178 and 118 measured; 8: 119 and 71);
+// 64 states spread over four lanes cost half as much again.  Four CTAs an SM are
+// resident.  Whole sequences last as long as the longest (the host does not know
+// the lengths: of several, three times the mean is assumed); chunks take 0.75 of
+// the work twice, two launches and the join, whose steps of 16 chunks are one trip
+// to memory.  Measured, whole against chunks: 8 ragged prompts of 16384 tokens x
+// 4096 channels 1103 and 706 us, one of 8192 x 2048 1430 and 197 us, one of 300 x
+// 1024 55 and 18 us, 58 ones of 14223 x 1736 even 197 and
+// 308 us, ragged 380 and 335.
+int chunk_length(int tokens, int seqs, int channels, int states, int groups) {
+    const int own = states < 16 ? states : 16, lanes = states > 16 ? states / 16 : 1;
+    const int each = kScanThreads / (lanes < kScanThreads ? lanes : kScanThreads), per = (channels + groups - 1) / groups;
+    const double columns = double(groups) * ((per + each - 1) / each), slow = states > 32 ? 1.5 : 1.0;
+    const double turn = 5.9 * (own + 4) * slow, alone = (60 + 7.4 * own) * (slow > 1.0 ? 1.3 : 1.0);
+    auto pass = [&](double length, double count) {
+        const double ctas = columns * count, busy = ctas > 148 * 3 ? 4 : ctas > 148 * 2 ? 3 : ctas > 148 ? 2 : 1;
+        const double one = 4000 + length * (alone > busy * turn ? alone : busy * turn), work = tokens * columns * turn / 148;
+        return ctas <= 148 * 4 ? one : (work > one ? work : one) + 0.25 * length * alone;  // the rounds' end
+    };
+    const double mean = double(tokens) / seqs, longest = seqs == 1 || 3 * mean > tokens ? tokens : 3 * mean;
+    const double together = pass(mean, seqs), whole = together > longest * alone ? together : longest * alone;
+    double best = whole;
+    int chosen = 0;
+    for (int64_t length = 32; length < longest; length += 16 + length / 128 * 16) {
+        const double count = double(tokens) / length + seqs;
+        const double trips = (1 + longest / length / 16) * 1700, bytes = count * channels * states * 8 / 5000;
+        const double cut = 8000 + (trips > bytes ? trips : bytes) + 1.75 * pass(length, count);
+        if (cut < best) best = cut, chosen = int(length);
+    }
+    return chosen;
 }
 
 template <class T, int N>
@@ -488,7 +504,7 @@ cudaError_t launch_scan_as(const sq_scan_args &a, bool step, cudaStream_t s) {
         kernel<<<dim3(unsigned(rows), columns), kScanThreads, bytes, s>>>(a, chunks);
         return cudaGetLastError();
     };
-    if (a.workspace) chunks.length = chunk_length(a.tokens, a.num_seqs, a.channels, a.states);
+    if (a.workspace) chunks.length = chunk_length(a.tokens, a.num_seqs, a.channels, a.states, a.groups);
     const bool usual = a.softplus && a.z;
     if (!chunks.length) return usual ? run(scan_kernel<T, N, kWhole, true>, a.num_seqs) : run(scan_kernel<T, N, kWhole, false>, a.num_seqs);
     const int64_t count = a.tokens / chunks.length + a.num_seqs;
@@ -541,7 +557,7 @@ int32_t scan_entry(const sq_scan_args *args, bool step, sq_stream_t stream) {
 extern "C" int64_t sq_selective_scan_workspace_bytes(int32_t tokens, int32_t num_seqs, int32_t channels, int32_t states,
                                                      int32_t groups) {
     if (tokens < 0 || num_seqs < 0 || channels < 1 || states < 1 || groups < 1) return -1;
-    const int length = num_seqs ? sq::chunk_length(tokens, num_seqs, channels, states) : 0;
+    const int length = num_seqs ? sq::chunk_length(tokens, num_seqs, channels, states, groups) : 0;
     if (!length) return 0;
     return (int64_t(tokens / length) + num_seqs) * channels * (states + 1) * int64_t(sizeof(float));
 }

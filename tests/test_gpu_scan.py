@@ -132,6 +132,29 @@ def test_long_prompts_of_few_channels(channels, states, groups, cu):
     _close(y, final, _reference(t, cu, initial))
 
 
+@pytest.mark.parametrize("channels,states,groups,cu", [
+    (1032, 16, 1, [0, 200]), (70, 4, 2, [0, 500]), (99, 8, 3, [0, 31, 63, 96, 160, 161, 161, 450]),
+    (224, 64, 4, [0, 400, 700]), (146, 32, 1, [0, 64, 129, 460]), (36, 16, 4, [0, 32, 64, 600])])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_short_chunks(channels, states, groups, cu, dtype):
+    """Prompts of a few hundred tokens, cut into chunks too; into a pool's rows, one request padding."""
+    from stepquant_b200.kernels.scan import selective_scan, selective_scan_extend
+    t = _data(cu[-1], channels, states, groups, dtype, 11)
+    t["a"] *= torch.logspace(-3, 0, channels, device="cuda")[:, None]
+    ends = torch.tensor(cu, device="cuda")
+    want = _reference(t, cu, None)
+    y, final = selective_scan(*_core(t), **_options(t), cu_seqlens=ends)
+    _close(y, final, want)
+    y2, none = selective_scan(*_core(t), **_options(t), cu_seqlens=ends, output_final_state=False)
+    assert none is None and torch.equal(y2, y)
+    pool = torch.zeros(len(cu) + 1, channels, states, device="cuda")
+    slots = torch.arange(len(cu) - 1, 0, -1, device="cuda")
+    slots[0] = 0
+    y3 = selective_scan_extend(pool, *_core(t), **_options(t), slots=slots, cu_seqlens=ends)
+    assert torch.equal(y3[cu[1]:], y[cu[1]:]) and not y3[:cu[1]].any()
+    assert torch.equal(pool[slots[1:]], final[1:]) and not pool[0].any()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("channels,states,groups,batch", [(1, 4, 1, 1), (33, 8, 1, 5), (128, 16, 2, 300), (60, 32, 4, 3),
                                                           (21, 64, 3, 2), (4096, 16, 1, 9)])
