@@ -12,7 +12,7 @@
 // kept in registers.  A thread takes four channels (8 bytes of a 16-bit row)
 // and walks a strip of tokens, eight tokens in flight while the eight before are
 // worked on; strips overlap by their W - 1 leading inputs.  Measured at 8192 bf16
-// channels: 32768 tokens in 184 us (5.8 TB/s, 0.91 of the measured copy); eight
+// channels: 32768 tokens in 183 us (5.9 TB/s, 0.91 of the measured copy); eight
 // channels a thread 431 us (loads held behind stores, half the threads), a branch
 // between the tokens of a batch 218 us.  One token of 256 requests 8.7 us (4 TB/s).
 // Rows aligned for two channels or one take them so, with more instructions a byte:
