@@ -71,19 +71,6 @@ __device__ __forceinline__ float softplus(float raw, const Bias &bias) {
     return fmaf(2.f, s, top);
 }
 
-// Pairs of fp32 values, one instruction for both.
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
-    return reinterpret_cast<float2 &>(r);
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(r) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)), "l"(reinterpret_cast<uint64_t &>(c)));
-    return reinterpret_cast<float2 &>(r);
-}
-
 // A lane's four entries of a state or A row (16-byte aligned: N is a multiple of 4).
 __device__ __forceinline__ void load4(const float *p, float (&x)[4]) {
     const float4 v = *reinterpret_cast<const float4 *>(p);

@@ -186,3 +186,26 @@ def test_other_stream_and_graph():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(g.float(), w) for g, w in zip(out, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,hidden", [(4100, 2048), (4099, 2051), (30000, 300), (30000, 128)])
+def test_codes_are_rounded_quotients(rows, hidden, dtype):
+    """Every code is e4m3 of y over the stored scale, a quotient rounded to fp32
+    once (a product with the rounded reciprocal differs at some ties), and the
+    same on every run.  y: x itself, or what the norm of fp32 rows returns."""
+    from stepquant_b200.kernels.norm import quantize_fp8, rms_norm, rms_norm_fp8
+    x, _, weight = _data(rows, hidden, dtype, 9)
+    most = torch.full((), 448.0, device="cuda")  # a quotient of tensors: by a number, torch multiplies with its reciprocal
+
+    def same(q, scale, y):
+        wide = scale.repeat_interleave(128, 1)[:, :hidden]
+        assert torch.equal(scale, torch.clamp_min(_blocks(y).abs().amax(-1), 1e-30) / most)
+        assert torch.equal(q.view(torch.uint8), (y / wide).to(torch.float8_e4m3fn).view(torch.uint8))
+
+    first = quantize_fp8(x)
+    same(*first, x.float())
+    again = quantize_fp8(x)
+    assert torch.equal(first[0].view(torch.uint8), again[0].view(torch.uint8)) and torch.equal(first[1], again[1])
+    if dtype == torch.float32:
+        same(*rms_norm_fp8(x, weight), rms_norm(x, weight))
