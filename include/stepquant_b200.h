@@ -409,8 +409,9 @@ int32_t sq_matmul_fp8(const sq_matmul_args *args, sq_stream_t stream);
  *   initial_state, final_state  [num_seqs or num_slots, channels, taps - 1] in
  *           dtype, oldest input first: the inputs before the first token (NULL:
  *           zeros) and the last taps - 1 ones (NULL: not kept); may be one buffer
- *   slots   [num_seqs] rows of the states, or NULL for row n.  A slot <= 0 or
- *           >= num_slots (flagged in status) gives zero outputs and no state.
+ *   slots   [num_seqs] rows of the states, or NULL for row n (then num_slots is
+ *           0 or at least num_seqs).  A slot <= 0 or >= num_slots (flagged in
+ *           status) gives zero outputs and no state.
  * sq_causal_conv_step: one token of each of num_seqs = tokens requests;
  * final_state is read and updated in place (cu_seqlens, initial_state unused).
  */

@@ -252,6 +252,7 @@ int32_t conv_entry(const sq_conv_args *args, bool step, sq_stream_t stream) {
     if (a.num_seqs == 0) return SQ_OK;
     if (!a.weight || (a.tokens > 0 && (!a.x || !a.y))) return SQ_ERR_ARGUMENT;
     if (step ? !a.final_state : !a.cu_seqlens) return SQ_ERR_ARGUMENT;
+    if (!a.slots && a.num_slots > 0 && a.num_slots < a.num_seqs) return SQ_ERR_CAPACITY;  // state row n of a smaller pool
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const cudaError_t e = a.dtype == SQ_F32    ? launch_conv<float>(a, step, s)
                           : a.dtype == SQ_BF16 ? launch_conv<__nv_bfloat16>(a, step, s)

@@ -527,6 +527,7 @@ int32_t scan_entry(const sq_scan_args *args, bool step, sq_stream_t stream) {
     if (a.num_seqs == 0) return SQ_OK;
     if (!a.a || (a.tokens > 0 && (!a.u || !a.dt || !a.b || !a.c || !a.y))) return SQ_ERR_ARGUMENT;
     if (step ? !a.final_state : !a.cu_seqlens) return SQ_ERR_ARGUMENT;
+    if (!a.slots && a.num_slots > 0 && a.num_slots < a.num_seqs) return SQ_ERR_CAPACITY;  // state row n of a smaller pool
     if (!aligned16(a.a) || !aligned16(a.initial_state) || !aligned16(a.final_state) || !aligned16(a.workspace)) return SQ_ERR_SHAPE;
     if (!step && a.workspace &&
         a.workspace_bytes < sq_selective_scan_workspace_bytes(a.tokens, a.num_seqs, a.channels, a.states, a.groups))

@@ -102,6 +102,8 @@ def causal_conv1d_extend(x, state, weight, bias=None, *, slots, cu_seqlens=None,
     """``causal_conv1d`` on a pool of states [S, D, W - 1]: sequence n continues
     from, and updates in place, row slots[n].  A slot <= 0 (padding) or outside
     the pool (flagged in ``status``, an int32 word) gives zero outputs."""
+    if slots is None:
+        raise ValueError("slots: required, the pool's row of each sequence")
     rows = N.rows_of(x, "x")
     tokens, channels = rows.shape
     weight, bias = _filter(weight, bias, channels)

@@ -153,6 +153,8 @@ def selective_scan_extend(state, u, dt, a, b, c, *, slots, d=None, z=None, dt_bi
     """``selective_scan`` on a pool of states [S, D, N]: sequence n continues
     from, and updates in place, row slots[n].  A slot <= 0 (padding) or outside
     the pool (flagged in ``status``, an int32 word) gives zero outputs."""
+    if slots is None:
+        raise ValueError("slots: required, the pool's row of each sequence")
     return _prompts(u, dt, a, b, c, d, z, dt_bias, dt_softplus, cu_seqlens, None, state, slots, status)[0]
 
 

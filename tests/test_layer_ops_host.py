@@ -110,3 +110,26 @@ def test_c_entries_refuse_before_launch():
     assert lib.sq_selective_scan_workspace_bytes(-1, 1, 8, 16, 1) == -1
     assert lib.sq_selective_scan_workspace_bytes(8192, 1, 2048, 16, 1) > 0
     assert lib.sq_selective_scan_workspace_bytes(16, 1, 2048, 16, 1) == 0
+
+
+def test_pool_forms_need_slots():
+    """Without slots a sequence's row would be its number, which may lie past the pool."""
+    x, state, ends = ones(5, 6), torch.zeros(2, 6, 3), torch.tensor([0, 1, 3, 5])
+    with pytest.raises(ValueError, match="slots"):
+        causal_conv1d_extend(x, state, ones(6, 4), slots=None, cu_seqlens=ends)
+    a, b = -ones(6, 8), ones(5, 1, 8)
+    with pytest.raises(ValueError, match="slots"):
+        selective_scan_extend(torch.zeros(2, 6, 8), x, x, a, b, b, slots=None, cu_seqlens=ends)
+    pool = SelectiveStatePool(2, 6, 8, dtype=torch.float32, device="cpu")
+    with pytest.raises(ValueError, match="slots"):
+        pool.convolve(x, ones(6, 4), slots=None, cu_seqlens=ends)
+    with pytest.raises(ValueError, match="slots"):
+        pool.extend(x, x, a, b, b, None, ends)
+    lib, fake = N.lib(), 4096
+    conv = dict(x=fake, weight=fake, y=fake, cu_seqlens=fake, initial_state=fake, final_state=fake, x_stride=6, tokens=5,
+                num_seqs=3, channels=6, taps=4, num_slots=2)
+    scan = dict(u=fake, dt=fake, b=fake, c=fake, a=fake, y=fake, cu_seqlens=fake, initial_state=fake, final_state=fake, tokens=5,
+                num_seqs=3, channels=6, states=8, groups=1, num_slots=2)
+    for entry, kind, fields in ((lib.sq_causal_conv, N.SqConvArgs, conv), (lib.sq_causal_conv_step, N.SqConvArgs, conv),
+                                (lib.sq_selective_scan, N.SqScanArgs, scan), (lib.sq_selective_scan_step, N.SqScanArgs, scan)):
+        assert entry(ctypes.byref(kind(**fields)), None) == N.SQ_ERR_CAPACITY
