@@ -16,9 +16,11 @@ _pack = N.packer(N.SqConvArgs)
 
 
 def sequence_ends(cu_seqlens, tokens, device):
-    """int32 boundaries on ``device`` (default: one sequence of all tokens)."""
+    """int32 boundaries on ``device`` (default: one sequence of all tokens, written
+    there: a copy from the host could not be captured)."""
     if cu_seqlens is None:
-        return torch.tensor([0, tokens], dtype=torch.int32).to(device, non_blocking=True)
+        return torch.arange(0, 2 * tokens, tokens, dtype=torch.int32, device=device) if tokens else torch.zeros(
+            2, dtype=torch.int32, device=device)
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
         raise ValueError("cu_seqlens: expected [sequences + 1]")
     if cu_seqlens.dtype == torch.int32 and cu_seqlens.device == device and cu_seqlens.is_contiguous():

@@ -166,3 +166,21 @@ def test_no_tokens_and_extremes():
     assert float(y[3, 5]) == 1e30 or abs(float(y[3, 5]) / 1e30 - 1) < 1e-6
     assert float(y[4, 7].abs()) == 0.0
     assert bool(y[:, :3].isfinite().all())
+
+
+def test_default_boundaries_under_capture():
+    """One sequence without cu_seqlens, captured and replayed on new inputs: no copy from the host."""
+    from stepquant_b200.kernels.conv import causal_conv1d, sequence_ends
+    for tokens in (0, 1, 77, 2 ** 31 - 1):
+        ends = sequence_ends(None, tokens, torch.device("cuda", 0))
+        assert ends.tolist() == [0, tokens] and ends.dtype == torch.int32
+    x, weight, bias, _ = _data(77, 264, 4, torch.bfloat16, 1, 11)
+    want = causal_conv1d(x, weight, bias)
+    still = torch.zeros_like(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = causal_conv1d(still, weight, bias)
+    still.copy_(x)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

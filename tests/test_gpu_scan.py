@@ -271,3 +271,19 @@ def test_large_steps():
     t["dt"][1::3] = -30.0
     y, final = selective_scan(*_core(t), **_options(t))
     _close(y, final, _reference(t, [0, 40], None))
+
+
+@pytest.mark.parametrize("tokens", [40, 600])
+def test_default_boundaries_under_capture(tokens):
+    """One sequence without cu_seqlens, whole and in chunks, captured and replayed on new inputs."""
+    from stepquant_b200.kernels.scan import selective_scan
+    t = _data(tokens, 64, 16, 1, torch.bfloat16, 14)
+    want = selective_scan(*_core(t), **_options(t))
+    still = torch.zeros_like(t["u"])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = selective_scan(still, *_core(t)[1:], **_options(t))
+    still.copy_(t["u"])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
