@@ -70,6 +70,15 @@ def _launch(entry, rows, y, weight, bias, initial, final, slots, cu, status, seq
                           weight.shape[1], N.dtype_code(rows.dtype), activation), index)
 
 
+def _token_rows(x):
+    """[tokens, channels] of concatenated sequences."""
+    if x.dim() == 3 and x.shape[0] != 1:
+        raise ValueError("x: expected a leading batch of 1 (concatenated sequences)")
+    if x.dim() not in (2, 3) or x.shape[-1] < 1:
+        raise ValueError("x: expected [tokens, channels]")
+    return N.rows_of(x, "x")
+
+
 def causal_conv1d(x, weight, bias=None, *, initial_state=None, output_final_state=True, activation="silu",
                   cu_seqlens=None):
     """Convolution of concatenated sequences: (y, final_state).
@@ -80,12 +89,7 @@ def causal_conv1d(x, weight, bias=None, *, initial_state=None, output_final_stat
     x's dtype, or None (zeros).  y has x's shape and dtype; final_state [N, D,
     W - 1] or None when ``output_final_state`` is false.
     """
-    shape = x.shape
-    if x.dim() == 3 and shape[0] != 1:
-        raise ValueError("x: expected a leading batch of 1 (concatenated sequences)")
-    if x.dim() not in (2, 3) or shape[-1] < 1:
-        raise ValueError("x: expected [tokens, channels]")
-    rows = N.rows_of(x, "x")
+    rows = _token_rows(x)
     tokens, channels = rows.shape
     weight, bias = _filter(weight, bias, channels)
     activation = _activation(activation)
@@ -95,7 +99,7 @@ def causal_conv1d(x, weight, bias=None, *, initial_state=None, output_final_stat
     if initial_state is not None:
         initial_state = _state(initial_state, seqs, channels, taps, x.dtype, "initial_state").contiguous()
     final = x.new_empty((seqs, channels, taps - 1)) if output_final_state else None
-    y = x.new_empty(shape)
+    y = x.new_empty(x.shape)
     _launch(N.lib().sq_causal_conv, rows, y, weight, bias, initial_state, final, None, cu, None, seqs, activation, index)
     return y, final
 
@@ -106,7 +110,7 @@ def causal_conv1d_extend(x, state, weight, bias=None, *, slots, cu_seqlens=None,
     the pool (flagged in ``status``, an int32 word) gives zero outputs."""
     if slots is None:
         raise ValueError("slots: required, the pool's row of each sequence")
-    rows = N.rows_of(x, "x")
+    rows = _token_rows(x)
     tokens, channels = rows.shape
     weight, bias = _filter(weight, bias, channels)
     activation = _activation(activation)

@@ -133,3 +133,13 @@ def test_pool_forms_need_slots():
     for entry, kind, fields in ((lib.sq_causal_conv, N.SqConvArgs, conv), (lib.sq_causal_conv_step, N.SqConvArgs, conv),
                                 (lib.sq_selective_scan, N.SqScanArgs, scan), (lib.sq_selective_scan_step, N.SqScanArgs, scan)):
         assert entry(ctypes.byref(kind(**fields)), None) == N.SQ_ERR_CAPACITY
+
+
+def test_batches_are_not_one_stream():
+    """Prompts are concatenated: a batch of several would run on from one into the next."""
+    state, slots, ends = torch.zeros(3, 6, 3), torch.tensor([1, 2]), torch.tensor([0, 5, 10])
+    for x in (ones(2, 5, 6), ones(2, 1, 5, 6), ones(6)):
+        for call in (lambda: causal_conv1d(x, ones(6, 4), cu_seqlens=ends),
+                     lambda: causal_conv1d_extend(x, state, ones(6, 4), slots=slots, cu_seqlens=ends)):
+            with pytest.raises(ValueError, match="x: expected"):
+                call()
