@@ -402,8 +402,8 @@ int32_t sq_matmul_fp8(const sq_matmul_args *args, sq_stream_t stream);
  * Causal convolution of `taps` (2 to 4) inputs a channel over concatenated
  * sequences: y_t = act(bias + sum_j weight[:, j] x_{t - taps + 1 + j}), act =
  * SiLU or the identity.  Sequence n owns tokens [cu_seqlens[n],
- * cu_seqlens[n + 1]), clamped to [0, tokens); tokens of no sequence are left
- * unwritten.
+ * cu_seqlens[n + 1]), clamped to [0, tokens); y is zero for tokens before the
+ * first and past the last (nothing is written where num_seqs is 0).
  *   x       [tokens, channels] in dtype; y the same, contiguous
  *   weight  [channels, taps] fp32, bias [channels] fp32 or NULL
  *   initial_state, final_state  [num_seqs or num_slots, channels, taps - 1] in

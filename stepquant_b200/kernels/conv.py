@@ -70,6 +70,11 @@ def _launch(entry, rows, y, weight, bias, initial, final, slots, cu, status, seq
                           weight.shape[1], N.dtype_code(rows.dtype), activation), index)
 
 
+def _outputs(x, seqs):
+    """y of concatenated sequences; without any there is no launch that writes its zeros."""
+    return x.new_empty(x.shape) if seqs else x.new_zeros(x.shape)
+
+
 def _token_rows(x):
     """[tokens, channels] of concatenated sequences."""
     if x.dim() == 3 and x.shape[0] != 1:
@@ -86,8 +91,8 @@ def causal_conv1d(x, weight, bias=None, *, initial_state=None, output_final_stat
     x: [T, D] or [1, T, D] float32, bfloat16 or float16, rows any stride apart;
     weight: [D, W] (or [D, 1, W]), bias: [D], both used in fp32; cu_seqlens:
     [N + 1] boundaries (default: one sequence); initial_state: [N, D, W - 1] in
-    x's dtype, or None (zeros).  y has x's shape and dtype; final_state [N, D,
-    W - 1] or None when ``output_final_state`` is false.
+    x's dtype, or None (zeros).  y has x's shape and dtype, zero for tokens of no
+    sequence; final_state [N, D, W - 1] or None when ``output_final_state`` is false.
     """
     rows = _token_rows(x)
     tokens, channels = rows.shape
@@ -99,7 +104,7 @@ def causal_conv1d(x, weight, bias=None, *, initial_state=None, output_final_stat
     if initial_state is not None:
         initial_state = _state(initial_state, seqs, channels, taps, x.dtype, "initial_state").contiguous()
     final = x.new_empty((seqs, channels, taps - 1)) if output_final_state else None
-    y = x.new_empty(x.shape)
+    y = _outputs(x, seqs)
     _launch(N.lib().sq_causal_conv, rows, y, weight, bias, initial_state, final, None, cu, None, seqs, activation, index)
     return y, final
 
@@ -118,7 +123,7 @@ def causal_conv1d_extend(x, state, weight, bias=None, *, slots, cu_seqlens=None,
     cu = sequence_ends(cu_seqlens, tokens, x.device)
     seqs = cu.numel() - 1
     state = _pool_state(state, channels, weight.shape[1], x.dtype)
-    y = x.new_empty(x.shape)
+    y = _outputs(x, seqs)
     _launch(N.lib().sq_causal_conv, rows, y, weight, bias, state, state, slot_rows(slots, seqs, x.device), cu, status, seqs,
             activation, index)
     return y

@@ -184,3 +184,23 @@ def test_default_boundaries_under_capture():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("channels", [264, 131])
+@pytest.mark.parametrize("cu,tokens", [([0, 30, 41], 41), ([0, 30, 41], 300), ([5, 30, 30, 99], 99), ([131, 131, 402], 5000),
+                                       ([0], 50), ([7], 7), ([0, 0], 333), ([300, 300, 300], 300), ([77, 78], 79)])
+def test_tokens_of_no_sequence_are_zero(cu, tokens, channels, dtype):
+    """Tokens before the first boundary and past the last, as a padded batch has them, in memory that held NaN."""
+    from stepquant_b200.kernels.conv import causal_conv1d
+    x, weight, bias, _ = _data(tokens, channels, 4, dtype, 1, 12)
+    x[:cu[0]] = x[cu[-1]:] = float("nan")
+    want = torch.zeros(tokens, channels, device="cuda", dtype=dtype)
+    if len(cu) > 1:
+        inner = torch.tensor(cu, device="cuda") - cu[0]
+        want[cu[0]:cu[-1]], kept = causal_conv1d(x[cu[0]:cu[-1]], weight, bias, cu_seqlens=inner)
+    for _ in range(3):
+        torch.full((tokens, channels), float("nan"), device="cuda", dtype=dtype)  # freed at once: the next output's memory
+        y, final = causal_conv1d(x, weight, bias, cu_seqlens=torch.tensor(cu, device="cuda"))
+        assert torch.equal(y, want)
+        assert len(cu) == 1 or torch.equal(final, kept)
