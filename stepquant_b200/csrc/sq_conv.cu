@@ -70,36 +70,18 @@ struct Filter {
     }
 };
 
-// Rows of zeros.
-template <class T, int VEC>
-__device__ __forceinline__ void clear(T *y, int64_t from, int64_t to, int64_t step, int channels) {
-    Run<T, VEC, VEC> zero;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) zero.v[i] = from_float<T>(0.f);
-    for (int64_t t = from; t < to; t += step) zero.store(y + t * channels);
-}
-
-// Tokens of no sequence, by `step` CTAs a column.  Not inlined: beside it the schedule of the
-// tokens' loop gets worse (32768 x 8192 in 187 us for 180).
-template <class T, int VEC>
-__device__ __noinline__ void clear_outside(T *y, const int32_t *cu, int seqs, int tokens, int channels, unsigned first, unsigned step) {
-    const int begin = sequence_range(cu, 0, tokens).x, end = sequence_range(cu, seqs - 1, tokens).y;
-    clear<T, VEC>(y, first, begin, step, channels);
-    clear<T, VEC>(y, int64_t(end) + first, tokens, step, channels);
-}
-
 // The CTAs past `strips` clear the tokens of no sequence.
 template <class T, int VEC, int W, bool SILU>
 __global__ void __launch_bounds__(kConvThreads) conv_kernel(sq_conv_args a, int strip, unsigned strips) {
     using Token = Run<T, VEC, VEC>;
     constexpr int BATCH = 8;  // tokens in flight a thread, while the batch before is worked on
-    const int d0 = (blockIdx.y * kConvThreads + threadIdx.x) * VEC;
-    if (d0 >= a.channels) return;
-    T *y = static_cast<T *>(a.y) + d0;
     if (blockIdx.x >= strips) {
-        clear_outside<T, VEC>(y, a.cu_seqlens, a.num_seqs, a.tokens, a.channels, blockIdx.x - strips, gridDim.x - strips);
+        clear_outside(a.y, int64_t(a.channels) * sizeof(T), a.cu_seqlens, a.num_seqs, a.tokens,
+                      (blockIdx.x - strips) * gridDim.y + blockIdx.y, (gridDim.x - strips) * gridDim.y);
         return;
     }
+    const int d0 = (blockIdx.y * kConvThreads + threadIdx.x) * VEC;
+    if (d0 >= a.channels) return;
     const int n = sequence_of(a.cu_seqlens, a.num_seqs, a.tokens, strip, blockIdx.x);
     const int2 seq = sequence_range(a.cu_seqlens, n, a.tokens);
     const int begin = seq.x, end = seq.y;
@@ -107,8 +89,12 @@ __global__ void __launch_bounds__(kConvThreads) conv_kernel(sq_conv_args a, int 
     if (part < 0 || (part > 0 && part * strip >= end - begin)) return;
     const int t0 = begin + int(part) * strip, t1 = min(end, t0 + strip);
     const int64_t row = state_row(a.slots, n, a.num_slots, a.status);
+    T *y = static_cast<T *>(a.y) + d0;
     if (row < 0) {
-        clear<T, VEC>(y, t0, t1, 1, a.channels);
+        Token zero;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) zero.v[i] = from_float<T>(0.f);
+        for (int t = t0; t < t1; ++t) zero.store(y + int64_t(t) * a.channels);
         return;
     }
     const T *x = static_cast<const T *>(a.x) + d0;

@@ -112,9 +112,10 @@ struct ScanShape {
 };
 
 // USUAL: softplus and (where there are outputs) a gate, known to the compiler so that the
-// tokens of a group have no branches between them; else as the arguments say.
+// tokens of a group have no branches between them; else as the arguments say.  Whole
+// sequences: the CTAs past `parts` clear the tokens of no sequence.
 template <class T, int N, int PASS, bool USUAL>
-__global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(sq_scan_args a, Chunks chunks) {
+__global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(sq_scan_args a, Chunks chunks, unsigned parts) {
     using S = ScanShape<T, N>;
     constexpr int SN = S::SN, P = S::P, CH = S::CH, TILE = S::TILE;
     constexpr bool OUT = PASS != kChunkState;
@@ -125,6 +126,12 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(sq_scan_args a, C
     const int per = a.channels / a.groups, tiles = (per + CH - 1) / CH;  // CTAs of a group
     const int group = blockIdx.y / tiles, first = (blockIdx.y - group * tiles) * CH;
     const int live = min(CH, per - first), d0 = group * per + first;
+    if (PASS == kWhole && blockIdx.x >= parts) {
+        clear_outside(a.y, int64_t(a.channels) * sizeof(T), a.cu_seqlens, a.num_seqs, a.tokens,
+                      (blockIdx.x - parts) * gridDim.y + blockIdx.y, (gridDim.x - parts) * gridDim.y);
+        return;
+    }
+    T *y = static_cast<T *>(a.y) + d0;
 
     // ---- the tokens of this CTA
     const int n = PASS == kWhole ? blockIdx.x : sequence_of(a.cu_seqlens, a.num_seqs, a.tokens, chunks.length, blockIdx.x);
@@ -139,7 +146,6 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(sq_scan_args a, C
         end = min(seq.y, begin + chunks.length);
         if (PASS == kChunkState && end == seq.y) return;  // no chunk follows
     }
-    T *y = static_cast<T *>(a.y) + d0;
     const int64_t row = state_row(a.slots, n, a.num_slots, OUT ? a.status : nullptr);
     if (row < 0) {
         if (OUT)
@@ -295,10 +301,15 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(sq_scan_args a, C
     if (!OUT && lane == 0) chunks.step_sum[int64_t(blockIdx.x) * a.channels + d] = total;
 }
 
-// Along each sequence of several chunks: the state that every chunk starts from.
+// Along each sequence of several chunks: the state that every chunk starts from.  The CTAs
+// past the sequences clear the tokens of none.
 __global__ void join_kernel(sq_scan_args a, Chunks chunks) {
     const int64_t i = int64_t(blockIdx.y) * blockDim.x + threadIdx.x;  // (channel, state)
     const int n = blockIdx.x;
+    if (n == a.num_seqs) {
+        clear_outside(a.y, int64_t(a.channels) * (a.dtype == SQ_F32 ? 4 : 2), a.cu_seqlens, a.num_seqs, a.tokens, blockIdx.y, gridDim.y);
+        return;
+    }
     if (i >= int64_t(a.channels) * a.states) return;
     const int2 seq = sequence_range(a.cu_seqlens, n, a.tokens);
     const int count = (seq.y - seq.x + chunks.length - 1) / chunks.length;
@@ -484,24 +495,27 @@ cudaError_t launch_scan_as(const sq_scan_args &a, bool step, cudaStream_t s) {
     constexpr int CH = ScanShape<T, N>::CH;
     const unsigned columns = unsigned(a.groups * ((per + CH - 1) / CH));
     Chunks chunks{};
-    auto run = [&](auto kernel, int64_t rows) {
+    auto run = [&](auto kernel, int64_t parts, unsigned more) {
         constexpr int bytes = ScanShape<T, N>::kBytes;
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
         if (e != cudaSuccess) return e;
-        kernel<<<dim3(unsigned(rows), columns), kScanThreads, bytes, s>>>(a, chunks);
+        kernel<<<dim3(unsigned(parts) + more, columns), kScanThreads, bytes, s>>>(a, chunks, unsigned(parts));
         return cudaGetLastError();
     };
     if (a.workspace) chunks.length = chunk_length(a.tokens, a.num_seqs, a.channels, a.states, a.groups);
     const bool usual = a.softplus && a.z;
-    if (!chunks.length) return usual ? run(scan_kernel<T, N, kWhole, true>, a.num_seqs) : run(scan_kernel<T, N, kWhole, false>, a.num_seqs);
+    if (!chunks.length) {
+        const unsigned more = (37 + columns) / columns;
+        return usual ? run(scan_kernel<T, N, kWhole, true>, a.num_seqs, more) : run(scan_kernel<T, N, kWhole, false>, a.num_seqs, more);
+    }
     const int64_t count = a.tokens / chunks.length + a.num_seqs;
     chunks.state = static_cast<float *>(a.workspace);
     chunks.step_sum = chunks.state + count * a.channels * N;
-    cudaError_t e = a.softplus ? run(scan_kernel<T, N, kChunkState, true>, count) : run(scan_kernel<T, N, kChunkState, false>, count);
+    cudaError_t e = a.softplus ? run(scan_kernel<T, N, kChunkState, true>, count, 0) : run(scan_kernel<T, N, kChunkState, false>, count, 0);
     if (e != cudaSuccess) return e;
-    join_kernel<<<dim3(unsigned(a.num_seqs), unsigned((int64_t(a.channels) * N + 255) / 256)), 256, 0, s>>>(a, chunks);
+    join_kernel<<<dim3(unsigned(a.num_seqs) + 1, unsigned((int64_t(a.channels) * N + 255) / 256)), 256, 0, s>>>(a, chunks);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    return usual ? run(scan_kernel<T, N, kChunkScan, true>, count) : run(scan_kernel<T, N, kChunkScan, false>, count);
+    return usual ? run(scan_kernel<T, N, kChunkScan, true>, count, 0) : run(scan_kernel<T, N, kChunkScan, false>, count, 0);
 }
 
 template <class T>

@@ -70,7 +70,7 @@ def _launch(entry, rows, y, weight, bias, initial, final, slots, cu, status, seq
                           weight.shape[1], N.dtype_code(rows.dtype), activation), index)
 
 
-def _outputs(x, seqs):
+def outputs(x, seqs):
     """y of concatenated sequences; without any there is no launch that writes its zeros."""
     return x.new_empty(x.shape) if seqs else x.new_zeros(x.shape)
 
@@ -104,7 +104,7 @@ def causal_conv1d(x, weight, bias=None, *, initial_state=None, output_final_stat
     if initial_state is not None:
         initial_state = _state(initial_state, seqs, channels, taps, x.dtype, "initial_state").contiguous()
     final = x.new_empty((seqs, channels, taps - 1)) if output_final_state else None
-    y = _outputs(x, seqs)
+    y = outputs(x, seqs)
     _launch(N.lib().sq_causal_conv, rows, y, weight, bias, initial_state, final, None, cu, None, seqs, activation, index)
     return y, final
 
@@ -123,7 +123,7 @@ def causal_conv1d_extend(x, state, weight, bias=None, *, slots, cu_seqlens=None,
     cu = sequence_ends(cu_seqlens, tokens, x.device)
     seqs = cu.numel() - 1
     state = _pool_state(state, channels, weight.shape[1], x.dtype)
-    y = _outputs(x, seqs)
+    y = outputs(x, seqs)
     _launch(N.lib().sq_causal_conv, rows, y, weight, bias, state, state, slot_rows(slots, seqs, x.device), cu, status, seqs,
             activation, index)
     return y

@@ -17,7 +17,7 @@ States are fp32.  Asynchronous on the current stream.
 import torch
 
 from .. import _native as N
-from .conv import causal_conv1d_extend, causal_conv1d_step, sequence_ends, slot_rows
+from .conv import causal_conv1d_extend, causal_conv1d_step, outputs, sequence_ends, slot_rows
 
 STATES = (4, 8, 16, 32, 64)
 
@@ -126,7 +126,7 @@ def _prompts(u, dt, a, b, c, d, z, dt_bias, dt_softplus, cu_seqlens, initial, fi
             initial = N.aligned(_state(initial, seqs, call.channels, call.states, "initial_state"))
             N.device_index(u, initial)
         final = u.new_empty((seqs, call.channels, call.states), dtype=torch.float32) if final else None
-    y = u.new_empty(u.shape)
+    y = outputs(u, seqs)
     size = N.lib().sq_selective_scan_workspace_bytes(call.tokens, seqs, call.channels, call.states, call.groups)
     workspace = u.new_empty(size, dtype=torch.uint8) if size > 0 else None
     call.launch(N.lib().sq_selective_scan, y, initial, final, slots, cu, status, workspace, seqs)
@@ -142,8 +142,8 @@ def selective_scan(u, dt, a, b, c, *, d=None, z=None, dt_bias=None, dt_softplus=
     one group) in u's dtype; d, dt_bias: [D] or None, used in fp32; rows any
     stride apart.  cu_seqlens: [S + 1] boundaries (default: one sequence);
     initial_state: [S, D, N] float32 or None (zeros).  y has u's shape and
-    dtype; final_state [S, D, N] float32, None when ``output_final_state`` is
-    false.
+    dtype, zero for tokens of no sequence; final_state [S, D, N] float32, None
+    when ``output_final_state`` is false.
     """
     return _prompts(u, dt, a, b, c, d, z, dt_bias, dt_softplus, cu_seqlens, initial_state, bool(output_final_state), None, None)
 

@@ -287,3 +287,29 @@ def test_default_boundaries_under_capture(tokens):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("channels", [48, 200])
+@pytest.mark.parametrize("cu,tokens", [([0, 30, 41], 41), ([0, 30, 41], 70), ([5, 30, 30, 99], 99), ([131, 131, 402], 1500),
+                                       ([0, 700, 1400], 2001), ([0], 50), ([0, 0], 333), ([300, 300, 300], 300), ([77, 78], 79),
+                                       ([600, 1600], 1611)])
+def test_tokens_of_no_sequence_are_zero(cu, tokens, channels, dtype):
+    """Tokens before the first boundary and past the last, whole sequences and chunks, in memory that held NaN."""
+    from stepquant_b200.kernels.scan import selective_scan
+    t = _data(tokens, channels, 16, 1, dtype, 15)
+    for k in ("u", "dt", "z", "b", "c"):
+        t[k][:cu[0]] = t[k][cu[-1]:] = float("nan")
+    want = torch.zeros(tokens, channels, device="cuda", dtype=torch.float64)
+    limit = torch.zeros_like(want)
+    states = state_limits = torch.zeros(0, channels, 16, device="cuda", dtype=torch.float64)
+    if len(cu) > 1:
+        inner = {k: v[cu[0]:cu[-1]] if k in ("u", "dt", "z", "b", "c") else v for k, v in t.items()}
+        want[cu[0]:cu[-1]], limit[cu[0]:cu[-1]], states, state_limits = _reference(inner, [at - cu[0] for at in cu], None)
+    for _ in range(3):
+        torch.full((tokens, channels), float("nan"), device="cuda", dtype=dtype)  # freed at once: the next output's memory
+        y, final = selective_scan(*_core(t), **_options(t), cu_seqlens=torch.tensor(cu, device="cuda"))
+        outside = torch.ones(tokens, device="cuda", dtype=torch.bool)
+        outside[cu[0]:cu[-1]] = False
+        assert not bool(y[outside].isnan().any()) and not bool(y[outside].any())
+        _close(y, final, (want, limit, states, state_limits))
