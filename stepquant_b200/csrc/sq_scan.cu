@@ -41,24 +41,19 @@ constexpr int kGroup = 4;     // tokens of a prompt worked on together
 constexpr unsigned kGridRows = 32768;  // groups of requests along a grid's second axis, the rest along its third
 constexpr float kLog2eRest = 1.92596299e-8f;  // log2(e) - kLog2e
 
-// dt_bias of a channel in units of log2(e), with the rounding of that product.
-struct Bias {
-    float value, high, low;
-    __device__ __forceinline__ explicit Bias(float b) : value(b), high(b * kLog2e), low(fmaf(b, kLog2e, -high) + b * kLog2eRest) {}
-};
-
-// log(1 + e^x), x = raw + bias, as max(x, 0) + log1p(e^-|x|), accurate to a few
-// units in the last place over the whole range: the step size scales every input
-// of the state, and far below zero softplus is the exponential alone.  So x
-// log2(e) is carried with its rounding error; log1p(e) = 2 atanh(e / (2 + e)) is
-// its series to the 13th power (the argument is at most 1/3).  NaN stays NaN, an
-// infinite x gives 0 or itself.
-__device__ __forceinline__ float softplus(float raw, const Bias &bias) {
-    const float y = fmaf(raw, kLog2e, bias.high);
-    float lost = fmaf(raw, kLog2e, bias.high - y) + fmaf(raw, kLog2eRest, bias.low);
-    lost = fminf(lost, 1.f);  // NaN where y is infinite
-    lost = __uint_as_float(__float_as_uint(lost) ^ (~__float_as_uint(y) & 0x80000000u));  // of -|y|
-    const float p = exp2_approx(-fminf(fabsf(y), 180.f)), e = fmaf(p, lost * 0.6931471806f, p);
+// log(1 + e^x), x = raw + bias, as max(x, 0) + log1p(e^-|x|), off by less than 16 * 2^-24 of
+// itself (4 measured; zero below 2^-126): the step size scales every input of the state, and far
+// below zero softplus is the exponential alone.  So the rounding errors of the sum (two-sum: the
+// larger of the two may be either) and of its product with log2(e) are carried into the
+// exponential to first order; log1p(e) = 2 atanh(e / (2 + e)) is its series to the 13th power
+// (the argument is at most 1/3).  NaN stays NaN, an infinite x gives 0 or itself.
+__device__ __forceinline__ float softplus(float raw, float bias) {
+    const float x = raw + bias, part = x - raw;
+    const float lost = fminf((raw - (x - part)) + (bias - part), 1.f);  // of x; NaN where x is infinite
+    const float m = fminf(fabsf(x), 128.f), y = m * kLog2e;
+    const float rest = fmaf(m, kLog2eRest, fmaf(m, kLog2e, -y));
+    const float off = fmaf(rest, 0.6931471806f, __uint_as_float(__float_as_uint(lost) ^ (__float_as_uint(x) & 0x80000000u)));  // of |x|
+    const float p = exp2_approx(-y), e = fmaf(-p, off, p);
     const float q = e * reciprocal_approx(2.f + e), q2 = q * q;
     float s = fmaf(q2, 1.f / 13.f, 1.f / 11.f);
     s = fmaf(q2, s, 1.f / 9.f);
@@ -67,7 +62,7 @@ __device__ __forceinline__ float softplus(float raw, const Bias &bias) {
     s = fmaf(q2, s, 1.f / 3.f);
     s = fmaf(q2 * s, q, q);
     float top;
-    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(top) : "f"(raw + bias.value));
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(top) : "f"(x));
     return fmaf(2.f, s, top);
 }
 
@@ -215,7 +210,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(sq_scan_args a, C
         else if (OUT && a.initial_state) load4(a.initial_state + at + 4 * i, v);
         h[2 * i] = make_float2(v[0], v[1]), h[2 * i + 1] = make_float2(v[2], v[3]);
     }
-    const Bias bias(a.dt_bias ? a.dt_bias[d] : 0.f);
+    const float bias = a.dt_bias ? a.dt_bias[d] : 0.f;
     const float skip = OUT && a.d ? a.d[d] : 0.f;
     float total = 0.f;  // sum of dt'
 
@@ -251,7 +246,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(sq_scan_args a, C
             for (int j = 0; j < U; ++j) {
                 const float x = value(from, S::kRow, dt_low, dt_step, t0, t + j, k);
                 un[j] = value(from + kU, S::kRow, u_low, u_step, t0, t + j, k);
-                s[j] = USUAL || a.softplus ? softplus(x, bias) : x + bias.value;
+                s[j] = USUAL || a.softplus ? softplus(x, bias) : x + bias;
                 in[j] = s[j] * un[j];
                 if (!OUT) total += s[j];
             }
@@ -408,13 +403,13 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(sq_scan_args a,
     load4(a.a + int64_t(k) * N + lane * 4, A);
 #pragma unroll
     for (int i = 0; i < 4; ++i) A[i] *= kLog2e;
-    const Bias bias(a.dt_bias ? a.dt_bias[k] : 0.f);
+    const float bias = a.dt_bias ? a.dt_bias[k] : 0.f;
     const float skip = a.d ? a.d[k] : 0.f;
     float dt_mine[SHARE], u_mine[SHARE], gate_mine[SHARE];
 #pragma unroll
     for (int q = 0; q < SHARE; ++q) {
         const float raw = to_float(dt_raw[q]);
-        dt_mine[q] = USUAL || a.softplus ? softplus(raw, bias) : raw + bias.value;
+        dt_mine[q] = USUAL || a.softplus ? softplus(raw, bias) : raw + bias;
         u_mine[q] = to_float(u_raw[q]);
         gate_mine[q] = USUAL || a.z ? silu(to_float(z_raw[q])) : 1.f;
     }

@@ -313,3 +313,31 @@ def test_tokens_of_no_sequence_are_zero(cu, tokens, channels, dtype):
         outside[cu[0]:cu[-1]] = False
         assert not bool(y[outside].isnan().any()) and not bool(y[outside].any())
         _close(y, final, (want, limit, states, state_limits))
+
+
+@pytest.mark.parametrize("single", [False, True])
+def test_step_sizes_alone(single):
+    """softplus(dt + dt_bias) by itself: u = b = 1, one token from a state of zero, so that the
+    state is dt'.  Off by at most 16 * 2^-24 of itself: the exponential 4, the first order
+    correction of its argument, its product and the quotient's sum 1 each, the reciprocal 2, the
+    quotient, its square, the series and the sum with max(x, 0) 1 each, with room for what the
+    argument's own rounding error was rounded to.  Values below 2^-126 may be flushed to zero."""
+    from stepquant_b200.kernels.scan import selective_scan, selective_scan_step
+    raw = torch.cat([torch.linspace(-80, 30, 100001), torch.linspace(-1, 1, 20001), torch.linspace(-100, -85, 301),
+                     torch.tensor([0.0, 1e-30, -1e-30, 1e4, 3e38])])
+    raw = torch.nn.functional.pad(raw, (0, -len(raw) % 1000)).cuda().view(-1, 1000)
+    for bias in (0.0, -0.03, 0.07, -1.0, -2.7, -4.6, -6.9, 5.3, 40.0, -60.0):
+        t = dict(a=torch.zeros(1000, 4, device="cuda"), b=torch.ones(len(raw), 1, 4, device="cuda"), u=torch.ones_like(raw),
+                 dt_bias=torch.full((1000,), bias, device="cuda"))
+        if single:
+            state = torch.zeros(len(raw), 1000, 4, device="cuda")
+            selective_scan_step(state, t["u"], raw, t["a"], t["b"], t["b"], dt_bias=t["dt_bias"])
+        else:
+            state = selective_scan(t["u"], raw, t["a"], t["b"], t["b"], dt_bias=t["dt_bias"],
+                                   cu_seqlens=torch.arange(len(raw) + 1, device="cuda", dtype=torch.int32))[1]
+        x = raw.double() + t["dt_bias"].double()
+        want = torch.clamp_min(x, 0) + torch.log1p(torch.exp(-x.abs()))
+        error = (state[:, :, 0].double() - want).abs()
+        limit = 16 * E24 * want + torch.where(want < 2.0 ** -125, want, 0.0)
+        assert bool((error <= limit).all()), (bias, float((error / want.clamp_min(2.0 ** -125)).max() / E24))
+        assert bool((state == state[:, :, :1]).all())
