@@ -343,7 +343,8 @@ int32_t sq_kda_prefill(const sq_prefill_args *args, sq_stream_t stream);
  *   x, residual  [rows, hidden] in dtype; residual may be NULL
  *   weight       [hidden] in weight_dtype
  *   residual_out [rows, hidden] in dtype, contiguous: x + residual rounded
- *                once (may be residual's own contiguous buffer); NULL without residual
+ *                once (may be residual's own contiguous buffer: then rows with |h|
+ *                above 1.8e19 may take h rounded below); NULL without residual
  *   out          [rows, hidden] contiguous: h / sqrt(mean(h^2) + eps) * weight
  *                with h = x + residual unrounded; in dtype, or e4m3 when scale is given
  *   scale        [rows, ceil(hidden / 128)] fp32 or NULL: per 128 channels

@@ -6,8 +6,10 @@
 //   s = max(max |y| over 128 channels, 1e-30) / 448,  q = e4m3(y / s)
 //
 // h and every statistic stay in fp32; y is rounded once, to the output type.
-// The floor of s keeps 1 / s finite for an all-zero block.  A NaN or infinity
-// makes its row's y NaN, hence its scales and codes too.
+// The floor of s keeps 1 / s finite for an all-zero block.  Rows whose squares
+// overflow (|h| above 1.8e19) take them of h times 2^-80.  A NaN makes its row's y
+// NaN, an infinity its own channel's, with the scale and codes of their blocks; the
+// other channels of an infinite row are 0.
 //
 // Bound by bytes (6 flops a value): the row is read once into registers, eight
 // values a thread and step, so a block of 128 channels is the eight values of
@@ -151,6 +153,46 @@ struct Place {
     }
 };
 
+// A row whose squares overflow takes them of h times 2^-80: the largest h is above 2^55 (65536 of
+// them overflow no earlier), so nothing that counts underflows; none comes above 2^48, so nothing
+// overflows; and eps is nothing beside it.
+constexpr float kShrink = 0x1p-80f;
+
+// 1 / sqrt(mean h^2) of such a row, held by groups of LANES lanes of a warp (scratch null) or by the
+// CTA.  Passed by value and not inlined: the registers of the usual path stay as they are (inlined,
+// 32768 x 5119 took 383 us for 311).
+template <int CH>
+struct Values {
+    float h[CH][8];
+};
+template <int CH, int LANES>
+__device__ __noinline__ float large_factor(Values<CH> v, int hidden, float *scratch) {
+    float squares = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float h = v.h[c][i] * kShrink;
+            squares += h * h;
+        }
+    if (scratch) {
+        __syncthreads();  // all have read the first sum
+        squares = cta_sum(squares, scratch);
+    } else {
+        squares = lane_sum<LANES>(squares);
+    }
+    return rsqrtf(squares / float(hidden)) * kShrink;
+}
+template <int CH, int LANES>
+__device__ __forceinline__ float large_factor_of(const float (&h)[CH][8], int hidden, float *scratch) {
+    Values<CH> v;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v.h[c][i] = h[c][i];
+    return large_factor<CH, LANES>(v, hidden, scratch);
+}
+
 // Short rows: a group of LANES lanes a row, CH units each, the group's next row on
 // its way; the weights stay in registers and nothing is shared between warps.
 // 100000 bf16 rows of 336 to e4m3: 39 us (a grid of all rows, each warp ending after
@@ -210,7 +252,12 @@ __global__ void __launch_bounds__(256, CH == 1 ? 4 : 3) norm_lanes_kernel(sq_nor
             for (int c = 0; c < CH; ++c)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) squares += h[c][i] * h[c][i];
-            const float factor = rsqrtf(lane_sum<LANES>(squares) / float(a.hidden) + a.eps);
+            squares = lane_sum<LANES>(squares);
+            float factor = rsqrtf(squares / float(a.hidden) + a.eps);
+            if (__any_sync(0xffffffffu, squares == INFINITY)) {  // in a row of the warp
+                const float large = large_factor_of<CH, LANES>(h, a.hidden, nullptr);
+                if (squares == INFINITY) factor = large;
+            }
 #pragma unroll
             for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -248,7 +295,11 @@ __global__ void __launch_bounds__(1024) norm_kernel(sq_norm_args a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) squares += h[c][i] * h[c][i];
     }
-    if (a.normalize) factor = rsqrtf(cta_sum(squares, scratch) / float(a.hidden) + a.eps);
+    if (a.normalize) {
+        squares = cta_sum(squares, scratch);
+        factor = rsqrtf(squares / float(a.hidden) + a.eps);
+        if (squares == INFINITY) factor = large_factor_of<CH, 32>(h, a.hidden, scratch);
+    }
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const Place<WIDTH, 32> place(c * warps + warp, lane, a.hidden);
@@ -266,6 +317,51 @@ __global__ void __launch_bounds__(1024) norm_kernel(sq_norm_args a) {
 // Each thread copies (cp.async) what it will itself read, so the only barrier of
 // a row is its sum's; the weights stay in registers.
 constexpr int kRows = 3;
+
+// The CTA's rows first, first + gridDim.x, ... again, those whose squares overflow (or come near),
+// after all of them: any branch between the sum and the outputs below costs (65536 x 5120 in 417 to
+// 520 us for 387).  Where residual_out is residual's own buffer, it holds the rounded h by now.
+template <class T>
+__device__ __noinline__ void redo_large(const sq_norm_args &a, int64_t first) {
+    __shared__ float scratch[32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const bool held = a.residual && a.residual == a.residual_out;
+    for (int64_t row = first; row < a.rows; row += gridDim.x) {
+        const T *x = held ? static_cast<const T *>(a.residual_out) + row * a.hidden : static_cast<const T *>(a.x) + row * a.x_stride;
+        const T *res = a.residual && !held ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
+        auto value = [&](int i) { return (to_float(x[i]) + (res ? to_float(res[i]) : 0.f)) * kShrink; };
+        __syncthreads();  // the row's outputs are written, and the scratch of the row before is read
+        float squares = 0.f;
+        for (int i = threadIdx.x; i < a.hidden; i += blockDim.x) squares += value(i) * value(i);
+        squares = cta_sum(squares, scratch);
+        if (squares < 0x1p-34f) continue;
+        const float factor = rsqrtf(squares / float(a.hidden));
+        auto normed = [&](int i) {
+            const float w = a.weight_dtype == SQ_F32    ? static_cast<const float *>(a.weight)[i]
+                            : a.weight_dtype == SQ_BF16 ? to_float(static_cast<const __nv_bfloat16 *>(a.weight)[i])
+                                                        : to_float(static_cast<const __half *>(a.weight)[i]);
+            return value(i) * factor * w;
+        };
+        for (int block = warp; block * 128 < a.hidden; block += warps) {
+            float y[4], top = 0.f;
+            for (int k = 0; k < 4; ++k) {
+                const int i = block * 128 + k * 32 + lane;
+                y[k] = i < a.hidden ? normed(i) : 0.f;
+                top = max_nan(top, fabsf(y[k]));
+                if (!a.scale && i < a.hidden) static_cast<T *>(a.out)[row * a.hidden + i] = from_float<T>(y[k]);
+            }
+            if (!a.scale) continue;
+            for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float scale = over_most(max_nan(top, kScaleFloor));
+            if (lane == 0) a.scale[row * ((a.hidden + 127) / 128) + block] = scale;
+            for (int k = 0; k < 4; ++k) {
+                const int i = block * 128 + k * 32 + lane;
+                if (i < a.hidden)
+                    static_cast<uint8_t *>(a.out)[row * a.hidden + i] = __nv_cvt_float_to_fp8(y[k] / scale, __NV_SATFINITE, __NV_E4M3);
+            }
+        }
+    }
+}
 
 template <class T, int CH>
 __global__ void __launch_bounds__(512) norm_rows_kernel(sq_norm_args a) {
@@ -306,6 +402,7 @@ __global__ void __launch_bounds__(512) norm_rows_kernel(sq_norm_args a) {
 #pragma unroll
     for (int i = 0; i + 1 < kRows; ++i) fetch(blockIdx.x + int64_t(i) * gridDim.x, i);
     int stage = 0, turn = 0;
+    bool large = false;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         fetch(row + int64_t(kRows - 1) * gridDim.x, (stage + kRows - 1) % kRows);
         asm volatile("cp.async.wait_group %0;\n" ::"n"(kRows - 1) : "memory");
@@ -330,7 +427,9 @@ __global__ void __launch_bounds__(512) norm_rows_kernel(sq_norm_args a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) squares += h[c][i] * h[c][i];
         }
-        const float factor = rsqrtf(cta_sum(squares, scratch[turn]) / float(a.hidden) + a.eps);
+        squares = cta_sum(squares, scratch[turn]);
+        large |= squares == INFINITY;
+        const float factor = rsqrtf(squares / float(a.hidden) + a.eps);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
 #pragma unroll
@@ -340,6 +439,7 @@ __global__ void __launch_bounds__(512) norm_rows_kernel(sq_norm_args a) {
         stage = stage + 1 == kRows ? 0 : stage + 1;
         turn ^= 1;
     }
+    if (large) redo_large<T>(a, blockIdx.x);
 }
 
 template <class T, int CH>

@@ -209,3 +209,55 @@ def test_codes_are_rounded_quotients(rows, hidden, dtype):
     assert torch.equal(first[0].view(torch.uint8), again[0].view(torch.uint8)) and torch.equal(first[1], again[1])
     if dtype == torch.float32:
         same(*rms_norm_fp8(x, weight), rms_norm(x, weight))
+
+
+@pytest.mark.parametrize("rows,hidden", [(5, 96), (5, 256), (40001, 300), (5, 509), (3, 1003), (700, 5120), (2100, 5120), (2, 65536)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_whose_squares_overflow(rows, hidden, dtype):
+    """Finite rows up to the type's largest values are normed as any other; a row with an
+    infinity is NaN there (and in its block's codes and scale) and 0 elsewhere; a NaN is all of its row."""
+    from stepquant_b200.kernels.norm import rms_norm, rms_norm_fp8
+    x, residual, weight = _data(rows, hidden, torch.float32, 21)
+    x[0], x[1] = x[0].clamp(-40, 40) * 1e25, x[1].clamp(-40, 40) / 50 * 3e38
+    x[-1], x[-1, -1] = x[-1].clamp(-40, 40), 2e38  # one large value
+    x = x.to(dtype)
+    weight = weight.clamp(0.5, 1.0).to(dtype)
+    _, y = _reference(x, weight, None)
+    y = torch.where(y.abs() < 2.0 ** -120, 0.0, y)  # below: no longer normal
+    got, (q, scale) = rms_norm(x, weight), rms_norm_fp8(x, weight)
+    off = y.abs() * REL + 2.0 ** -119
+    inside = ((y - off).to(dtype) <= got) & (got <= (y + off).to(dtype))
+    assert bool(inside.all()), (got[~inside], y[~inside])
+    _close_fp8(q, scale, y)
+    if rows == 2:
+        return
+    x[0, hidden // 2], x[2, hidden - 1] = float("inf"), float("nan")
+    before = got
+    got, (q, scale) = rms_norm(x, weight), rms_norm_fp8(x, weight)
+    at = torch.arange(hidden, device="cuda")
+    block = torch.arange(scale.shape[1], device="cuda") == hidden // 2 // 128
+    assert bool(got[0, hidden // 2].isnan()) and not bool(got[0, at != hidden // 2].any())
+    assert bool(q[0].float().isnan()[hidden // 2]) and not bool(q[0].float()[at // 128 != hidden // 2 // 128].any())
+    assert bool(scale[0][block].isnan().all()) and bool((scale[0][~block] == torch.tensor(1e-30) / 448).all())
+    assert bool(got[2].isnan().all()) and bool(q[2].float().isnan().all()) and bool(scale[2].isnan().all())
+    assert torch.equal(got[1], before[1]) and torch.equal(got[3:], before[3:])
+
+
+@pytest.mark.parametrize("rows", [3, 2100])
+def test_residual_updated_in_place(rows):
+    """The C entry with residual_out in residual's own buffer, ordinary and overflowing rows."""
+    import ctypes
+    from stepquant_b200 import _native as N
+    from stepquant_b200.kernels.norm import rms_norm
+    hidden = 1024
+    x, residual, weight = _data(rows, hidden, torch.float32, 23)
+    x[1] *= 1e22
+    h, (y, _) = x + residual, rms_norm(x, weight, residual)
+    assert bool(y[1].abs().amax() > 0.5)
+    out = torch.empty_like(x)
+    args = N.SqNormArgs(x.data_ptr(), residual.data_ptr(), weight.data_ptr(), residual.data_ptr(), out.data_ptr(), None, hidden,
+                        hidden, rows, hidden, N.SQ_F32, N.SQ_F32, 1, 1e-6)
+    N.check(N.lib().sq_rms_norm(ctypes.byref(args), N.stream_handle()))
+    assert torch.equal(residual, h)
+    assert torch.equal(out, y)
+
