@@ -378,7 +378,9 @@ int32_t sq_rms_norm(const sq_norm_args *args, sq_stream_t stream);
  *   residual [rows, width] in dtype, rows residual_stride elements apart, or NULL
  *   out      [rows, width] in dtype, contiguous; rounded once (may be residual's own contiguous buffer)
  * hidden a multiple of 16; x, w 16-byte aligned, strides multiples of 16 and
- * at least hidden.  status: SQ_STATUS_TIMEOUT if a bounded device wait gave up.
+ * at least hidden.  status: SQ_STATUS_TIMEOUT if a bounded device wait gave up;
+ * the outputs it left undone are NaN.  wait_clocks: how many clocks a wait may
+ * take, 0 for 2^32 (about two seconds), negative for one try.
  */
 typedef struct sq_matmul_args {
     const void *x;
@@ -395,6 +397,7 @@ typedef struct sq_matmul_args {
     int32_t width;
     int32_t hidden;
     int32_t dtype;
+    int64_t wait_clocks;
 } sq_matmul_args;
 
 int32_t sq_matmul_fp8(const sq_matmul_args *args, sq_stream_t stream);

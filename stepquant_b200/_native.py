@@ -55,7 +55,7 @@ class SqNormArgs(ctypes.Structure):
 class SqMatmulArgs(ctypes.Structure):
     _fields_ = [("x", _p), ("x_scale", _p), ("w", _p), ("w_scale", _p), ("residual", _p), ("out", _p), ("status", _p),
                 ("x_stride", _i64), ("w_stride", _i64), ("residual_stride", _i64), ("rows", _i32), ("width", _i32),
-                ("hidden", _i32), ("dtype", _i32)]
+                ("hidden", _i32), ("dtype", _i32), ("wait_clocks", _i64)]
 
 
 class SqConvArgs(ctypes.Structure):

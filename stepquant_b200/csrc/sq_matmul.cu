@@ -25,7 +25,9 @@
 // (8 x 8256 x 5120: 11.4 us, 3.7 TB/s).
 //
 // Operands arrive by TMA (128-byte swizzle; zeros past K, M and N), one warp
-// issues the copies, one or two the products; every wait is bounded.
+// issues the copies, one or two the products.  Every wait is bounded: outputs whose
+// sums a wait gave up on are NaN, and status says so.  No warp leaves before the
+// copies and products it issued have ended.
 #include <cooperative_groups.h>
 #include <cudaTypedefs.h>
 
@@ -49,6 +51,7 @@ constexpr int kScaleGroup = 4;             // blocks whose scales are loaded tog
 struct Sync {
     uint64_t full[8], empty[8];  // operand stages
     uint64_t ready[kMostParts], free_[kMostParts];  // parts of the tensor memory
+    uint64_t done[2];                               // all products of a product warp
     uint32_t tmem;
     int abort;
 };
@@ -66,14 +69,14 @@ struct Ring {
     }
 };
 
-// A copy warp that gives up leaves once the copies it issued have landed (with a
-// limit again): those of the last `count` <= STAGES stages before `at`.
+// A copy warp leaves once the copies it issued have landed (with a limit again), also where another
+// warp gave up on them: those of the last `count` <= STAGES stages before `at`.
 template <int STAGES>
 __device__ __forceinline__ void drain_copies(Sync &s, Ring<STAGES> at, int64_t count) {
     int never = 0;
     for (int i = 0; i < STAGES && i < count; ++i) {
         at.back();
-        tc::bar_wait(&s.full[at.stage], at.parity, &never);
+        tc::bar_wait(&s.full[at.stage], at.parity, &never, tc::kWaitClocks);
     }
 }
 
@@ -87,6 +90,7 @@ __device__ __forceinline__ void set_up(Sync &s, int stages, uint32_t columns, in
             tc::bar_init(&s.ready[i], 1);
             tc::bar_init(&s.free_[i], kEpilogueWarps);
         }
+        for (int i = 0; i < 2; ++i) tc::bar_init(&s.done[i], 1);
         s.abort = 0;
         tc::bar_init_fence();
     }
@@ -96,14 +100,24 @@ __device__ __forceinline__ void set_up(Sync &s, int stages, uint32_t columns, in
     tc::fence_after();
 }
 
+// Waits (with a limit again) until the products that product warp w issued have ended, once.
+__device__ __forceinline__ void end_products(Sync &s, int w) {
+    if (tc::elected()) tc::mma_commit(&s.done[w]);
+    __syncwarp();
+    int never = 0;
+    tc::bar_wait(&s.done[w], 0, &never, tc::kWaitClocks);
+    __syncwarp();
+}
+
 // Product warp: blocks w, w + W, ... of `count`, each four steps of 32 along K into
 // N columns of the tensor memory, its PARTS parts in turn.  The whole warp takes
 // the waits and one elected lane issues, which keeps the descriptors in uniform
 // registers; two waits, four products and two commits took a warp about 900 clocks,
 // so two warps alternate (W = 2) where there are registers for them.  base: shared
-// address of the first stage, its two operand tiles kRowTile apart.
+// address of the first stage, its two operand tiles kRowTile apart.  False: it gave up,
+// and its products have ended; else they have when the epilogue has read them.
 template <int N, int W, int PARTS, int STAGES, int STAGE_BYTES>
-__device__ __forceinline__ void issue_blocks(Sync &s, int w, int64_t count, uint32_t tmem, uint32_t base) {
+__device__ __forceinline__ bool issue_blocks(Sync &s, int w, int64_t count, uint32_t tmem, uint32_t base, int64_t limit) {
     // A wait knows its phase from the one before by parity alone, so it may only begin when the phase two
     // before has ended.  Copies land in any order: with the stages even each warp has its own, and waits
     // for every use of them.  Parts are released in order, so the other warp's are no trouble; free_ first,
@@ -115,7 +129,8 @@ __device__ __forceinline__ void issue_blocks(Sync &s, int w, int64_t count, uint
     bool ok = true;
     if (w) at.next(), part.next();
     for (; it < count; it += W) {
-        ok = tc::bar_wait(&s.free_[part.stage], part.parity ^ 1, &s.abort) && tc::bar_wait(&s.full[at.stage], at.parity, &s.abort);
+        ok = tc::bar_wait(&s.free_[part.stage], part.parity ^ 1, &s.abort, limit) &&
+             tc::bar_wait(&s.full[at.stage], at.parity, &s.abort, limit);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc::fence_after();
         if (tc::elected()) {
@@ -130,16 +145,8 @@ __device__ __forceinline__ void issue_blocks(Sync &s, int w, int64_t count, uint
 #pragma unroll
         for (int i = 0; i < W; ++i) at.next(), part.next();
     }
-    // A warp that gives up leaves once its last products have ended (with a limit again).
-    if (!ok) {
-        int never = 0;
-        for (int i = 0; i < PARTS && it >= W; ++i, it -= W) {
-#pragma unroll
-            for (int k = 0; k < W; ++k) part.back();
-            tc::bar_wait(&s.ready[part.stage], part.parity, &never);
-        }
-        __syncwarp();
-    }
+    if (!ok) end_products(s, w);
+    return ok;
 }
 
 // ---------------------------------------------------------------------------
@@ -208,6 +215,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int64_t tiles = int64_t(row_tiles) * column_tiles, first = blockIdx.x, step = gridDim.x;
     set_up(s, S::kStages, S::kColumns, warp);
     const uint32_t tmem = s.tmem;
+    bool issued = false;
 
     if (warp >= kEpilogueWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kIssueRegisters));
@@ -220,19 +228,20 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     const int2 tile = tile_at(i, row_tiles, column_tiles);
                     const int x_row = tile.x * 128, w_row = tile.y * TN;
                     for (int g = 0; g < blocks; ++g, ++count, at.next()) {
-                        if (!(ok = tc::bar_wait(&s.empty[at.stage], at.parity ^ 1, &s.abort))) break;
+                        if (!(ok = tc::bar_wait(&s.empty[at.stage], at.parity ^ 1, &s.abort, a.wait_clocks))) break;
                         unsigned char *to = base + at.stage * S::kStage;
                         tc::bar_expect(&s.full[at.stage], S::kStage);
                         tc::tma_load(to, &xmap, g * kBlock, x_row, &s.full[at.stage]);
                         tc::tma_load(to + kRowTile, &wmap, g * kBlock, w_row, &s.full[at.stage]);
                     }
                 }
-                if (!ok) drain_copies(s, at, count);
+                drain_copies(s, at, count);
             }
             __syncwarp();
         } else if (warp < kEpilogueWarps + 3) {  // products
             const int64_t mine = first < tiles ? (tiles - first + step - 1) / step : 0;
-            issue_blocks<TN, 2, S::kParts, S::kStages, S::kStage>(s, warp - kEpilogueWarps - 1, mine * blocks, tmem, tc::smem_u32(base));
+            issued = issue_blocks<TN, 2, S::kParts, S::kStages, S::kStage>(s, warp - kEpilogueWarps - 1, mine * blocks, tmem, tc::smem_u32(base),
+                                                                       a.wait_clocks);
         }
     } else {  // scales and sums: warp w holds lanes 32 (w % 4) .. + 31, half q = w / 4 of the columns
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kEpilogueRegisters));
@@ -266,7 +275,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         Ring<S::kParts> part;
         bool ok = true;
-        for (int64_t i = first; i < tiles && ok; i += step) {
+        int64_t i = first;
+        for (; i < tiles; i += step) {
             const int2 at = tile_at(i, row_tiles, column_tiles);
             const int m0 = at.x * 128 + 32 * (warp & 3), n0 = at.y * TN + q * C;
             const int cross = (kBlock - n0 % kBlock) / 16;  // first chunk of the second block of w
@@ -283,7 +293,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 const float f0 = s0[0], f1 = s1[0];
 #pragma unroll
                 for (int q = 0; q + 1 < kScaleGroup; ++q) s0[q] = s0[q + 1], s1[q] = s1[q + 1];
-                ok = __all_sync(0xffffffffu, tc::bar_wait(&s.ready[part.stage], part.parity, &s.abort));
+                ok = __all_sync(0xffffffffu, tc::bar_wait(&s.ready[part.stage], part.parity, &s.abort, a.wait_clocks));
                 if (!ok) break;
                 tc::fence_after();
                 const uint32_t from = mine + part.stage * TN;
@@ -370,11 +380,22 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (wide) put(std::true_type());
             else put(std::false_type());
         }
+        for (; i < tiles; i += step) {  // given up
+            const int2 at = tile_at(i, row_tiles, column_tiles);
+            const int m0 = at.x * 128 + 32 * (warp & 3), n0 = at.y * TN + q * C;
+            for (int m = m0; m < min(m0 + 32, a.rows); ++m)
+                for (int n = n0 + lane; n < min(n0 + C, a.width); n += 32)
+                    static_cast<T *>(a.out)[int64_t(m) * a.width + n] = from_float<T>(NAN);
+        }
     }
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    if (s.abort && threadIdx.x == 0) flag(a.status, SQ_STATUS_TIMEOUT);
+    if (s.abort) {  // by all or none
+        if (threadIdx.x == 0) flag(a.status, SQ_STATUS_TIMEOUT);
+        if (issued) end_products(s, warp - kEpilogueWarps - 1);
+        __syncthreads();
+    }
     if (warp == kEpilogueWarps + 1) tc::tmem_free(tmem, S::kColumns);
 }
 
@@ -412,6 +433,7 @@ __global__ void __launch_bounds__(SplitShape<TM>::kThreads, 2)
     set_up(s, S::kStages, S::kColumns, warp);
     const uint32_t tmem = s.tmem;
     float *sums = reinterpret_cast<float *>(base);  // [TM][128], once the operands are consumed
+    bool issued = false;
 
     if (warp == kEpilogueWarps) {
         if (lane == 0) {
@@ -419,17 +441,18 @@ __global__ void __launch_bounds__(SplitShape<TM>::kThreads, 2)
             bool ok = true;
             int g = g0;
             for (; g < g1; ++g, at.next()) {
-                if (!(ok = tc::bar_wait(&s.empty[at.stage], at.parity ^ 1, &s.abort))) break;
+                if (!(ok = tc::bar_wait(&s.empty[at.stage], at.parity ^ 1, &s.abort, a.wait_clocks))) break;
                 unsigned char *to = base + at.stage * S::kStage;
                 tc::bar_expect(&s.full[at.stage], S::kStage);
                 tc::tma_load(to, &wmap, g * kBlock, n0, &s.full[at.stage]);
                 tc::tma_load(to + kRowTile, &xmap, g * kBlock, 0, &s.full[at.stage]);
             }
-            if (!ok) drain_copies(s, at, g - g0);
+            drain_copies(s, at, g - g0);
         }
         __syncwarp();
     } else if (warp > kEpilogueWarps) {
-        issue_blocks<TM, S::kProductWarps, S::kParts, S::kStages, S::kStage>(s, warp - kEpilogueWarps - 1, g1 - g0, tmem, tc::smem_u32(base));
+        issued = issue_blocks<TM, S::kProductWarps, S::kParts, S::kStages, S::kStage>(s, warp - kEpilogueWarps - 1, g1 - g0, tmem, tc::smem_u32(base),
+                                                                                 a.wait_clocks);
     } else {
         constexpr int C = TM / 2, W = C < 16 ? C : 16, CHUNKS = C / W;
         const int tid = threadIdx.x, half = warp >> 2;
@@ -462,7 +485,7 @@ __global__ void __launch_bounds__(SplitShape<TM>::kThreads, 2)
                 // The group's scales are there for all, and all are done with those of two groups ago.
                 asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kEpilogueWarps) : "memory");
             }
-            tc::bar_wait(&s.ready[part.stage], part.parity, &s.abort);  // giving up: the sums are not used
+            tc::bar_wait(&s.ready[part.stage], part.parity, &s.abort, a.wait_clocks);  // giving up: the sums are not used
             __syncwarp();
             tc::fence_after();
             const uint32_t from = mine + part.stage * TM;
@@ -495,18 +518,26 @@ __global__ void __launch_bounds__(SplitShape<TM>::kThreads, 2)
     tc::fence_before();
     cluster.sync();
     tc::fence_after();
+    if (s.abort) {  // by all or none of the CTA
+        if (threadIdx.x == 0) flag(a.status, SQ_STATUS_TIMEOUT);
+        if (issued) end_products(s, warp - kEpilogueWarps - 1);
+        __syncthreads();
+    }
     if (warp == kEpilogueWarps + 1) tc::tmem_free(tmem, S::kColumns);
-    // The sums of the ranks, in their order; each rank finishes its share of the rows of x, four columns a thread.
+    // The sums of the ranks (NaN where one gave up), in their order; each rank finishes its share of the rows of x, four columns a thread.
     const int share = TM * rank / ranks, count = TM * (rank + 1) / ranks - share;
 #pragma unroll 4
     for (int i = threadIdx.x; i < count * 32; i += S::kThreads) {
         const int m = share + i / 32, n = n0 + i % 32 * 4;
         if (m >= a.rows || n >= a.width) continue;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        int gone = 0;
         for (int q = 0; q < ranks; ++q) {
             const float4 part = reinterpret_cast<const float4 *>(cluster.map_shared_rank(sums, q))[share * 32 + i];
+            gone |= *cluster.map_shared_rank(&s.abort, q);
             v.x += part.x, v.y += part.y, v.z += part.z, v.w += part.w;
         }
+        if (gone) v = make_float4(NAN, NAN, NAN, NAN);
         const float x[4] = {v.x, v.y, v.z, v.w};
         Four<T> old, y;
         if (a.residual) old.load(static_cast<const T *>(a.residual) + int64_t(m) * a.residual_stride + n, wide, a.width - n);
@@ -514,7 +545,6 @@ __global__ void __launch_bounds__(SplitShape<TM>::kThreads, 2)
         for (int j = 0; j < 4; ++j) y.v[j] = from_float<T>(a.residual ? x[j] + to_float(old.v[j]) : x[j]);
         y.store(static_cast<T *>(a.out) + int64_t(m) * a.width + n, wide, a.width - n);
     }
-    if (s.abort && threadIdx.x == 0) flag(a.status, SQ_STATUS_TIMEOUT);
     cluster.sync();
 }
 
@@ -616,7 +646,7 @@ int32_t launch_matmul(const sq_matmul_args &a, int sms, cudaStream_t s) {
 
 extern "C" int32_t sq_matmul_fp8(const sq_matmul_args *args, sq_stream_t stream) {
     if (!args) return SQ_ERR_ARGUMENT;
-    const sq_matmul_args &a = *args;
+    sq_matmul_args a = *args;
     if (a.rows < 0 || a.width < 1 || a.hidden < 1) return SQ_ERR_ARGUMENT;
     if (a.dtype < SQ_F32 || a.dtype > SQ_F16) return SQ_ERR_ARGUMENT;
     if (a.hidden % 16) return SQ_ERR_UNSUPPORTED;
@@ -625,6 +655,7 @@ extern "C" int32_t sq_matmul_fp8(const sq_matmul_args *args, sq_stream_t stream)
     if (!sq::aligned16(a.x) || !sq::aligned16(a.w) || a.x_stride < a.hidden || a.w_stride < a.hidden || a.x_stride % 16 ||
         a.w_stride % 16 || a.residual_stride < 0)
         return SQ_ERR_SHAPE;
+    if (a.wait_clocks == 0) a.wait_clocks = sq::tc::kWaitClocks;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int sms = sq::sms_of(s);
     if (sms < 1) return SQ_ERR_CUDA;

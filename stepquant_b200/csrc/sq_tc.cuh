@@ -8,7 +8,7 @@
 namespace sq {
 namespace tc {
 
-constexpr int64_t kWaitClocks = int64_t(1) << 32;  // a wait gives up after about two seconds
+constexpr int64_t kWaitClocks = int64_t(1) << 32;  // a wait gives up after about two seconds, unless the call says otherwise
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
@@ -22,20 +22,23 @@ __device__ __forceinline__ void bar_expect(uint64_t *bar, uint32_t bytes) {
 __device__ __forceinline__ void bar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bar)) : "memory");
 }
-// Waits for the phase of `parity`; false when kWaitClocks ran out (sets `abort`) or another warp set `abort`.
-// (The cycle counter bounds it: a read of the global timer takes longer than a block's products.)
-__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatile int *abort) {
+// Waits for the phase of `parity`; false when `limit` clocks ran out (sets `abort`) or another warp
+// set `abort`.  Both are looked at after the first try that fails and every 16th from there (a
+// negative limit: never again).  A try suspends the thread for a while that the hardware chooses: an
+// explicit time made the products 3 to 8 % slower, and so did a look after every try.  (The cycle
+// counter bounds it: a read of the global timer takes longer than a block's products.)
+__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatile int *abort, int64_t limit) {
     int64_t since = 0;
     for (uint32_t it = 1;; ++it) {
         uint32_t done;
         asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
                      : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
         if (done) return true;
-        if ((it & 15) == 0) {
+        if ((it & 15) == 1) {
             if (*abort) return false;
             const int64_t now = clock64();
             if (since == 0) since = now;
-            if (now - since > kWaitClocks) {
+            if (now - since > limit) {
                 *abort = 1;
                 return false;
             }

@@ -51,8 +51,8 @@ def matmul_fp8(x, x_scale, weight, weight_scale, *, residual=None, out_dtype=tor
     x: [..., K] and weight: [N, K] float8_e4m3fn, K a multiple of 16; x_scale:
     [..., ceil(K / 128)], weight_scale: [ceil(N / 128), ceil(K / 128)] float32;
     residual: [..., N] in out_dtype (float32, bfloat16 or float16), or None.
-    ``status``: an int32 word for SQ_STATUS_TIMEOUT, should a bounded device
-    wait give up (the output is then incomplete).
+    Should a bounded device wait give up, the outputs left undone are NaN and
+    ``status`` (an int32 word, or None) has SQ_STATUS_TIMEOUT.
     """
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError("x and weight: expected [..., hidden] and [width, hidden]")
@@ -78,5 +78,5 @@ def matmul_fp8(x, x_scale, weight, weight_scale, *, residual=None, out_dtype=tor
              _pack(rows.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(), N.address(residual),
                    out.data_ptr(), N.address(status), rows.stride(0) if count > 1 else hidden,
                    weight.stride(0) if width > 1 else hidden, 0 if residual is None else residual.stride(0), count, width,
-                   hidden, dtype), index)
+                   hidden, dtype, 0), index)
     return out

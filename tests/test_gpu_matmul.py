@@ -175,3 +175,30 @@ def test_weight_quantization():
     assert q.shape == w.shape and scale.shape == (2, 3) and bool(scale[1, 2] > 0)
     back = q.double() * _expand(scale, 128, w.shape)
     assert bool(((back - w.double()).abs() <= torch.clamp_min(w.double().abs() * 2.0 ** -4, 1e-4)).all())
+
+
+@pytest.mark.parametrize("rows,width,hidden", [(8, 16384, 8192), (30, 5000, 4096), (60, 2000, 8192), (128, 9001, 4096), (129, 700, 8192),
+                                               (300, 2050, 8192), (512, 6500, 8192), (700, 8200, 4096), (4096, 5120, 1024)])
+def test_waits_that_run_out(rows, width, hidden):
+    """Device waits limited to one try or a few clocks give up in the middle of copies and products: every
+    output is what it should be or NaN, NaN exactly where the status is flagged, and the calls
+    after it are whole."""
+    import ctypes
+    from stepquant_b200 import _native as N
+    from stepquant_b200.kernels.matmul import matmul_fp8
+    x, sx, w, sw = _data(rows, width, hidden, 31)
+    want = matmul_fp8(x, sx, w, sw)
+    flush = torch.empty(1 << 26, device="cuda")
+    seen = 0
+    for limit in (-1, -1, 1, 300, 1000, 3000, 10000, 100000):
+        out, status = torch.zeros_like(want), torch.zeros(1, device="cuda", dtype=torch.int32)
+        flush.zero_()  # the operands leave L2: the first copies take longer than a try
+        args = N.SqMatmulArgs(x.data_ptr(), sx.data_ptr(), w.data_ptr(), sw.data_ptr(), None, out.data_ptr(), status.data_ptr(),
+                              hidden, hidden, 0, rows, width, hidden, N.SQ_BF16, limit)
+        N.check(N.lib().sq_matmul_fp8(ctypes.byref(args), N.stream_handle()))
+        gone = out.isnan()
+        assert torch.equal(out[~gone], want[~gone])
+        assert int(status) == (N.SQ_STATUS_TIMEOUT if bool(gone.any()) else 0)
+        seen += bool(gone.any())
+        assert torch.equal(matmul_fp8(x, sx, w, sw, status=status.zero_()), want) and int(status) == 0
+    assert seen or width * hidden < 1 << 25  # thousands of waits with one try each
