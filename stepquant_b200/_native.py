@@ -205,6 +205,13 @@ def device_index(first, *others):
     return index
 
 
+def status_word(status):
+    """``status`` (or None): four bytes that a kernel sets bits in."""
+    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
+        raise ValueError(f"status: expected an int32 word, got {status.dtype} {list(status.shape)}")
+    return status
+
+
 def address(tensor):
     return 0 if tensor is None else tensor.data_ptr()
 

@@ -119,7 +119,7 @@ def causal_conv1d_extend(x, state, weight, bias=None, *, slots, cu_seqlens=None,
     tokens, channels = rows.shape
     weight, bias = _filter(weight, bias, channels)
     activation = _activation(activation)
-    index = N.device_index(x, weight, bias, state, status)
+    index = N.device_index(x, weight, bias, state, N.status_word(status))
     cu = sequence_ends(cu_seqlens, tokens, x.device)
     seqs = cu.numel() - 1
     state = _pool_state(state, channels, weight.shape[1], x.dtype)
@@ -147,7 +147,7 @@ def causal_conv1d_step(x, state, weight, bias=None, *, slots=None, activation="s
     batch, channels = rows.shape
     weight, bias = _filter(weight, bias, channels)
     activation = _activation(activation)
-    index = N.device_index(x, weight, bias, state, status)
+    index = N.device_index(x, weight, bias, state, N.status_word(status))
     state = _pool_state(state, channels, weight.shape[1], x.dtype)
     if slots is None and state.shape[0] != batch:
         raise ValueError(f"state: expected {batch} rows without slots")

@@ -62,7 +62,7 @@ def matmul_fp8(x, x_scale, weight, weight_scale, *, residual=None, out_dtype=tor
     if hidden % 16:
         raise NotImplementedError("the product is built for a hidden size that is a multiple of 16")
     dtype = N.dtype_code(out_dtype)
-    index = N.device_index(x, weight, x_scale, weight_scale, residual, status)
+    index = N.device_index(x, weight, x_scale, weight_scale, residual, N.status_word(status))
     blocks = (hidden + BLOCK - 1) // BLOCK
     rows = _operand(x if x.dim() == 2 else x.reshape(-1, hidden), "x")
     weight = _operand(weight, "weight")

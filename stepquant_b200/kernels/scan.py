@@ -120,7 +120,7 @@ def _prompts(u, dt, a, b, c, d, z, dt_bias, dt_softplus, cu_seqlens, initial, fi
     if slots is not None:
         initial = final = _pool_state(final, call.channels, call.states)
         slots = slot_rows(slots, seqs, device)
-        N.device_index(u, final, status)
+        N.device_index(u, final, N.status_word(status))
     else:
         if initial is not None:
             initial = N.aligned(_state(initial, seqs, call.channels, call.states, "initial_state"))
@@ -168,7 +168,7 @@ def selective_scan_step(state, u, dt, a, b, c, *, d=None, z=None, dt_bias=None, 
     call = _Call(u, dt, a, b, c, d, z, dt_bias, dt_softplus)
     batch = call.tokens
     state = _pool_state(state, call.channels, call.states)
-    N.device_index(u, state, status)
+    N.device_index(u, state, N.status_word(status))
     if slots is None and state.shape[0] != batch:
         raise ValueError(f"state: expected {batch} rows without slots")
     y = u.new_empty((batch, call.channels))

@@ -73,3 +73,25 @@ def test_product_with_rows_past_32_bits():
     want = matmul_fp8(x[-2:], scale[-2:], w, sw)
     torch.testing.assert_close(got[-2:], want, rtol=2 ** -7, atol=1e-3)
     assert not bool(got[-300:-2].any())
+
+
+def test_status_is_an_int32_word():
+    """A word of another size would be written past its end."""
+    from stepquant_b200.kernels.conv import causal_conv1d_extend, causal_conv1d_step
+    from stepquant_b200.kernels.matmul import matmul_fp8, quantize_weight_fp8
+    from stepquant_b200.kernels.norm import quantize_fp8
+    from stepquant_b200.kernels.scan import selective_scan_extend, selective_scan_step
+    x, slots = torch.randn(2, 32, device="cuda"), torch.tensor([1, 2], device="cuda")
+    ends, filters = torch.tensor([0, 1, 2], device="cuda"), torch.ones(32, 4, device="cuda")
+    conv, state = torch.zeros(3, 32, 3, device="cuda"), torch.zeros(3, 32, 16, device="cuda")
+    a, b = -torch.ones(32, 16, device="cuda"), torch.ones(2, 1, 16, device="cuda")
+    operands = (*quantize_fp8(x), *quantize_weight_fp8(torch.ones(8, 32, device="cuda")))
+    for status in (torch.zeros(1, device="cuda", dtype=torch.int8), torch.zeros(0, device="cuda", dtype=torch.int32),
+                   torch.zeros(1, device="cuda", dtype=torch.int64)):
+        for call in (lambda: causal_conv1d_step(x, conv, filters, slots=slots, status=status),
+                     lambda: causal_conv1d_extend(x, conv, filters, slots=slots, cu_seqlens=ends, status=status),
+                     lambda: selective_scan_step(state, x, x, a, b, b, slots=slots, status=status),
+                     lambda: selective_scan_extend(state, x, x, a, b, b, slots=slots, cu_seqlens=ends, status=status),
+                     lambda: matmul_fp8(*operands, status=status)):
+            with pytest.raises(ValueError, match="status"):
+                call()
