@@ -180,7 +180,14 @@ def packer(arguments):
     kernels take about as long."""
     fmt = struct.Struct("@" + "".join(_FORMATS[kind] for _, kind in arguments._fields_) + "0P")
     assert fmt.size == ctypes.sizeof(arguments)
-    return fmt.pack
+
+    def pack(*values):
+        try:
+            return fmt.pack(*values)
+        except struct.error:
+            raise ValueError(f"a size or a stride is out of the C structure's range: {values}") from None
+
+    return pack
 
 
 def launch(entry, packed, index):

@@ -255,7 +255,7 @@ int32_t conv_entry(const sq_conv_args *args, bool step, sq_stream_t stream) {
     if (a.dtype < SQ_F32 || a.dtype > SQ_F16) return SQ_ERR_ARGUMENT;
     if (a.taps < 2 || a.taps > 4) return SQ_ERR_UNSUPPORTED;
     if (a.x_stride < 0) return SQ_ERR_SHAPE;
-    if (a.channels > (1 << 22) || a.num_seqs > (1 << 30)) return SQ_ERR_UNSUPPORTED;
+    if (a.channels > (1 << 22) || a.num_seqs > (1 << 30) || a.tokens > kMostTokens) return SQ_ERR_UNSUPPORTED;
     if (a.num_seqs == 0) return SQ_OK;
     if (!a.weight || (a.tokens > 0 && (!a.x || !a.y))) return SQ_ERR_ARGUMENT;
     if (step ? !a.final_state : !a.cu_seqlens) return SQ_ERR_ARGUMENT;

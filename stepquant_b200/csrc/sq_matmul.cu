@@ -47,6 +47,7 @@ constexpr int kEpilogueWarps = 8;
 constexpr int kMostParts = 4;              // blocks in tensor memory at a time
 constexpr int kRowTile = 128 * kBlock;     // bytes of a 128-row operand tile
 constexpr int kScaleGroup = 4;             // blocks whose scales are loaded together
+constexpr int kMostRows = 0x7fff0000;      // of either operand: the end of a tile is an int too
 
 struct Sync {
     uint64_t full[8], empty[8];  // operand stages
@@ -649,7 +650,7 @@ extern "C" int32_t sq_matmul_fp8(const sq_matmul_args *args, sq_stream_t stream)
     sq_matmul_args a = *args;
     if (a.rows < 0 || a.width < 1 || a.hidden < 1) return SQ_ERR_ARGUMENT;
     if (a.dtype < SQ_F32 || a.dtype > SQ_F16) return SQ_ERR_ARGUMENT;
-    if (a.hidden % 16) return SQ_ERR_UNSUPPORTED;
+    if (a.hidden % 16 || a.rows > sq::kMostRows || a.width > sq::kMostRows || a.hidden > sq::kMostRows) return SQ_ERR_UNSUPPORTED;
     if (a.rows == 0) return SQ_OK;
     if (!a.x || !a.x_scale || !a.w || !a.w_scale || !a.out) return SQ_ERR_ARGUMENT;
     if (!sq::aligned16(a.x) || !sq::aligned16(a.w) || a.x_stride < a.hidden || a.w_stride < a.hidden || a.x_stride % 16 ||

@@ -6,6 +6,10 @@
 
 namespace sq {
 
+// A strip, a chunk's tile or a batch of tokens may begin anywhere before the last token, and its end
+// is an int too.
+constexpr int kMostTokens = 0x7fff0000;
+
 // Token range of sequence n, clamped to [0, tokens).
 __device__ __forceinline__ int2 sequence_range(const int32_t *cu, int n, int tokens) {
     const int b = max(0, min(cu[n], tokens));

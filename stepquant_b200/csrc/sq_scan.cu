@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(sq_scan_args a, C
         if (part < 0 || (part > 0 && part * chunks.length >= seq.y - seq.x)) return;
         many = seq.y - seq.x > chunks.length;
         begin = seq.x + int(part) * chunks.length;
-        end = min(seq.y, begin + chunks.length);
+        end = int(min(int64_t(seq.y), int64_t(begin) + chunks.length));
         if (PASS == kChunkState && end == seq.y) return;  // no chunk follows
     }
     const int64_t row = state_row(a.slots, n, a.num_slots, OUT ? a.status : nullptr);
@@ -307,7 +307,7 @@ __global__ void join_kernel(sq_scan_args a, Chunks chunks) {
     }
     if (i >= int64_t(a.channels) * a.states) return;
     const int2 seq = sequence_range(a.cu_seqlens, n, a.tokens);
-    const int count = (seq.y - seq.x + chunks.length - 1) / chunks.length;
+    const int count = int((int64_t(seq.y) - seq.x + chunks.length - 1) / chunks.length);
     if (count < 2) return;
     const int64_t row = state_row(a.slots, n, a.num_slots, nullptr);
     if (row < 0) return;
@@ -532,7 +532,8 @@ int32_t scan_entry(const sq_scan_args *args, bool step, sq_stream_t stream) {
     if (a.channels % a.groups || a.u_stride < 0 || a.dt_stride < 0 || a.z_stride < 0 || a.b_stride < 0 || a.c_stride < 0)
         return SQ_ERR_SHAPE;
     if (a.states != 4 && a.states != 8 && a.states != 16 && a.states != 32 && a.states != 64) return SQ_ERR_UNSUPPORTED;
-    if (a.channels > (1 << 18) || a.groups > (1 << 14) || a.num_seqs > (1 << 30)) return SQ_ERR_UNSUPPORTED;
+    if (a.channels > (1 << 18) || a.groups > (1 << 14) || a.num_seqs > (1 << 30) || a.tokens > kMostTokens)
+        return SQ_ERR_UNSUPPORTED;
     if (a.num_seqs == 0) return SQ_OK;
     if (!a.a || (a.tokens > 0 && (!a.u || !a.dt || !a.b || !a.c || !a.y))) return SQ_ERR_ARGUMENT;
     if (step ? !a.final_state : !a.cu_seqlens) return SQ_ERR_ARGUMENT;

@@ -143,3 +143,23 @@ def test_batches_are_not_one_stream():
                      lambda: causal_conv1d_extend(x, state, ones(6, 4), slots=slots, cu_seqlens=ends)):
             with pytest.raises(ValueError, match="x: expected"):
                 call()
+
+
+def test_sizes_near_2_31():
+    """Counts whose last tile would end past an int are refused, and those an int cannot hold are a ValueError."""
+    lib, fake, near = N.lib(), 4096, 2 ** 31 - 64
+
+    def code(entry, kind, **fields):
+        return entry(ctypes.byref(kind(**fields)), None)
+
+    matmul = dict(x=fake, x_scale=fake, w=fake, w_scale=fake, out=fake, x_stride=32, w_stride=32, rows=2, width=3, hidden=32)
+    for change in (dict(rows=near), dict(width=near), dict(hidden=near, x_stride=near, w_stride=near)):
+        assert code(lib.sq_matmul_fp8, N.SqMatmulArgs, **{**matmul, **change}) == N.SQ_ERR_UNSUPPORTED, change
+    conv = dict(x=fake, weight=fake, y=fake, cu_seqlens=fake, final_state=fake, x_stride=8, tokens=near, num_seqs=1, channels=8, taps=4)
+    assert code(lib.sq_causal_conv, N.SqConvArgs, **conv) == N.SQ_ERR_UNSUPPORTED
+    scan = dict(u=fake, dt=fake, b=fake, c=fake, a=fake, y=fake, cu_seqlens=fake, tokens=near, num_seqs=1, channels=8, states=16, groups=1)
+    assert code(lib.sq_selective_scan, N.SqScanArgs, **scan) == N.SQ_ERR_UNSUPPORTED
+    for kind in (N.SqNormArgs, N.SqMatmulArgs, N.SqConvArgs, N.SqScanArgs):
+        names = [name for name, _ in kind._fields_]
+        with pytest.raises(ValueError, match="range"):
+            N.packer(kind)(*[2 ** 31 if n in ("rows", "tokens") else 1 for n in names])
