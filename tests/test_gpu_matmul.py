@@ -202,3 +202,19 @@ def test_waits_that_run_out(rows, width, hidden):
         seen += bool(gone.any())
         assert torch.equal(matmul_fp8(x, sx, w, sw, status=status.zero_()), want) and int(status) == 0
     assert seen or width * hidden < 1 << 25  # thousands of waits with one try each
+
+
+@pytest.mark.parametrize("rows,width,hidden", [(5, 1000, 4096), (16, 128, 8192), (30, 5120, 2048), (60, 300, 4096), (100, 9000, 1024)])
+def test_few_rows_on_few_sms(rows, width, hidden):
+    """Clusters on a stream of 16 SMs, K split over fewer CTAs than on the whole GPU: the same bounds."""
+    from stepquant_b200.kernels.matmul import matmul_fp8
+    from stepquant_b200.kernels.resources import writeback_resources
+    x, sx, w, sw = _data(rows, width, hidden, 6)
+    status = torch.zeros(1, device="cuda", dtype=torch.int32)
+    torch.cuda.synchronize()
+    stream = writeback_resources("cuda", 16).stream
+    with torch.cuda.stream(stream):
+        got = matmul_fp8(x, sx, w, sw, out_dtype=torch.float32, status=status)
+    stream.synchronize()
+    _close(got, x, sx, w, sw)
+    assert int(status) == 0
