@@ -12,11 +12,11 @@
 // kept in registers.  A thread takes four channels (8 bytes of a 16-bit row)
 // and walks a strip of tokens, eight tokens in flight while the eight before are
 // worked on; strips overlap by their W - 1 leading inputs.  Measured at 8192 bf16
-// channels: 32768 tokens in 183 us (5.9 TB/s, 0.91 of the measured copy); eight
+// channels: 32768 tokens in 181 us (5.9 TB/s, 0.92 of the measured copy); eight
 // channels a thread 431 us (loads held behind stores, half the threads), a branch
-// between the tokens of a batch 218 us.  One token of 256 requests 8.7 us (4 TB/s).
+// between the tokens of a batch 218 us.  One token of 256 requests 8.6 us (4 TB/s).
 // Rows aligned for two channels or one take them so, with more instructions a byte:
-// 8190 channels 234 us (singly 312), 8191 in 302 us; one token 9.1 and 12.2 us.
+// 8190 channels 232 us (singly 312), 8191 in 297 us; one token 8.7 and 11.6 us.
 #include <type_traits>
 
 #include "sq_rows.cuh"
@@ -219,7 +219,8 @@ cudaError_t launch_conv_as(const sq_conv_args &a, bool step, cudaStream_t s) {
         conv_step_kernel<T, VEC, W><<<grid, kConvThreads, 0, s>>>(a);
         return cudaGetLastError();
     }
-    // Strips of 64 tokens; shorter ones while the grid would leave SMs idle.
+    // Strips of 64 tokens; shorter ones while the grid would leave SMs idle (of a whole GPU's 148:
+    // a stream of fewer takes the same strips).
     int strip = 64;
     while (strip > 8 && int64_t(a.tokens / strip + a.num_seqs) * columns < 148 * 8) strip /= 2;
     const unsigned strips = unsigned(a.tokens / strip + a.num_seqs);

@@ -1355,8 +1355,7 @@ cudaError_t launch_fast_mode(const TileParams &p, int items, cudaStream_t stream
 
 }  // namespace
 
-// SMs that kernels launched on `stream` can run on, for the other persistent
-// kernels of the library; 0 when the device cannot be asked.
+// For the layer operators (sq_vec.cuh).
 int sms_of(cudaStream_t stream) {
     int device = 0, sms = 0;
     if (cudaGetDevice(&device) != cudaSuccess ||

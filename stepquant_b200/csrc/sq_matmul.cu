@@ -11,18 +11,24 @@
 // Many rows (tile_kernel): tensor memory lanes are rows of x, columns are rows
 // of w, so a thread's scale is one number a block.  Persistent CTAs of 128 x TN
 // tiles, the block products in 2 to 4 parts of the tensor memory.  What bounds it
-// short of the power limit is the turn of a part (products, 512 clocks of 256
-// columns, and the epilogue's read, which holds the products up by about 150)
-// and the operands' way from L2 (48 KB a block of 128 x 256, 11 TB/s measured);
-// in a loop of seconds the GPU runs at its 1000 W limit, 1.53 GHz.  Measured on the
-// way at 16384 x 8256 x 5120: packed fp32 pairs in the epilogue 811 us, single ones,
-// a part released as soon as it is in registers, scales loaded four blocks ahead
-// and two product warps in turn 685 to 700 us (2.0 PFLOP/s; 814 us at the power limit).
-// Pairs of CTAs (256 x 256 tiles, 32 KB a block and SM) measured 705 and 827 us.
+// short of the power limit are the products with their barriers, 500 ns of a 620 ns
+// block of 128 x 256 (512 clocks of tensor pipe), and then, each as much, the
+// operands' way from L2 beside them and the epilogue's reads, which hold them up:
+// at 4096 x 8256 x 5120, 198 us, copies alone take 144, products alone 162, reads
+// alone 149, products with either of the others 190 (at 512 x 5120 x 4096, 18.6:
+// 14.2, 16.6, 15.5, with reads 18.4, with copies 17.2).  In a loop of seconds the GPU
+// runs at its 1000 W limit, 1.53 GHz.  Measured on the way at 16384 x 8256 x 5120:
+// packed fp32 pairs in the epilogue 811 us, single ones, a part released as soon as
+// it is in registers, scales loaded four blocks ahead and two product warps in turn
+// 685 to 700 us (2.0 PFLOP/s; 794 to 814 us at the power limit).  Pairs of CTAs
+// (256 x 256 tiles, 32 KB a block and SM) measured 705 and 827 us.
 // Few rows (split_kernel): the weights' bytes bound the call.  Lanes are 128
 // rows of w (one scale a block), columns the rows of x; the CTAs of a cluster
-// split K and add their sums in rank order through distributed shared memory
-// (8 x 8256 x 5120: 11.4 us, 3.7 TB/s).
+// split K and add their sums in rank order through distributed shared memory.
+// Weights from memory (several sets in turn): 8 x 16384 x 8192 25.6 us (5.2 TB/s),
+// 8 to 32 x 8256 x 5120 12.1 to 12.5 us (3.5 TB/s, start and end of ten blocks a CTA
+// the rest), 64 rows 14.0, 128 rows 20.7, of 5120 x 4096 9.9, 12.1 and 17.6 us at 32,
+// 64 and 128; with one set of 42 MB in L2 8 rows take 9.0 us.
 //
 // Operands arrive by TMA (128-byte swizzle; zeros past K, M and N), one warp
 // issues the copies, one or two the products.  Every wait is bounded: outputs whose
@@ -39,7 +45,6 @@
 #include "sq_vec.cuh"
 
 namespace sq {
-int sms_of(cudaStream_t stream);  // sq_fast.cu
 namespace {
 
 constexpr int kBlock = 128;                // depth of a scale block and of a pipeline stage
@@ -624,7 +629,8 @@ int32_t launch_matmul(const sq_matmul_args &a, int sms, cudaStream_t s) {
     if (a.rows <= 32) return launch_split<T, 32>(a, wide, sms, s);
     if (a.rows <= 64) return launch_split<T, 64>(a, wide, sms, s);
     if (a.rows <= 128) return launch_split<T, 128>(a, wide, sms, s);
-    // The tile whose waves take least; ns of a block of 128 x TN with every SM at it, measured.
+    // The tile whose waves take least; ns of a block of 128 x TN with every SM at it, measured (start and
+    // end of a call, about 6 us, are the same for all).
     constexpr int kTile[5] = {256, 192, 160, 128, 64}, kTime[5] = {590, 470, 410, 330, 270};
     int best = 0;
     int64_t least = INT64_MAX;

@@ -14,9 +14,10 @@
 // Bound by bytes (6 flops a value): the row is read once into registers, eight
 // values a thread and step, so a block of 128 channels is the eight values of
 // half a warp and its maximum four shuffles.  Measured, bf16 with residual and
-// e4m3 output: 65536 x 5120 in 391 us (6.0 TB/s, 0.94 of the measured copy; with a
+// e4m3 output: 65536 x 5120 in 385 us (6.1 TB/s, 0.95 of the measured copy; with a
 // CTA a row and nothing on its way 560 us), one row of 5120 in 2.8 us, of launch
-// and two trips to memory; 777 x 4100 f16 (rows on 8-byte boundaries) 5.9 us.
+// and two trips to memory; 777 x 4100 f16 (rows on 8-byte boundaries) 6.1 us;
+// quantization alone, a CTA a row, of 65536 x 4096 156 us (5.1 TB/s).
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -24,7 +25,6 @@
 #include "sq_vec.cuh"
 
 namespace sq {
-int sms_of(cudaStream_t stream);  // sq_fast.cu
 namespace {
 
 constexpr float kE4m3Max = 448.f;
@@ -72,7 +72,7 @@ __device__ __forceinline__ float cta_sum(float v, float *scratch) {
 // A row is cut in units of 8 LANES channels, eight a lane: neighbours where an
 // access takes WIDTH (8 or 4) of them; LANES apart where rows are aligned for
 // single ones only, so that the lanes of an access are neighbours: 32768 rows of 5119
-// in 314 us, 777 x 4099 f16 in 8 us (eight neighbours a lane there too: 586 and 22 us).
+// in 291 us, 777 x 4099 f16 in 7.3 us (eight neighbours a lane there too: 586 and 22 us).
 template <int WIDTH, int LANES>
 struct Place {
     static constexpr int kStep = WIDTH == 1 ? LANES : 1;
@@ -159,8 +159,7 @@ struct Place {
 constexpr float kShrink = 0x1p-80f;
 
 // 1 / sqrt(mean h^2) of such a row, held by groups of LANES lanes of a warp (scratch null) or by the
-// CTA.  Passed by value and not inlined: the registers of the usual path stay as they are (inlined,
-// 32768 x 5119 took 383 us for 311).
+// CTA.  Passed by value and not inlined: inlined, 32768 x 5119 took 383 us for 291.
 template <int CH>
 struct Values {
     float h[CH][8];
@@ -195,7 +194,7 @@ __device__ __forceinline__ float large_factor_of(const float (&h)[CH][8], int hi
 
 // Short rows: a group of LANES lanes a row, CH units each, the group's next row on
 // its way; the weights stay in registers and nothing is shared between warps.
-// 100000 bf16 rows of 336 to e4m3: 39 us (a grid of all rows, each warp ending after
+// 100000 bf16 rows of 336 to e4m3: 38 us (a grid of all rows, each warp ending after
 // its own, 61 us; two rows a turn, 142 registers, 69 us).
 template <class T, int CH, int LANES, int WIDTH>
 __global__ void __launch_bounds__(256, CH == 1 ? 4 : 3) norm_lanes_kernel(sq_norm_args a) {
@@ -320,7 +319,7 @@ constexpr int kRows = 3;
 
 // The CTA's rows first, first + gridDim.x, ... again, those whose squares overflow (or come near),
 // after all of them: any branch between the sum and the outputs below costs (65536 x 5120 in 417 to
-// 520 us for 387).  Where residual_out is residual's own buffer, it holds the rounded h by now.
+// 520 us for 385).  Where residual_out is residual's own buffer, it holds the rounded h by now.
 template <class T>
 __device__ __noinline__ void redo_large(const sq_norm_args &a, int64_t first) {
     __shared__ float scratch[32];

@@ -17,8 +17,8 @@
 // exponentials and gates of one do not wait on the chain h of the others.
 // Bound by the special function unit (one exponential per token, channel and
 // state at 16 a clock and SM, four more per token and channel) and, next to it, by
-// issue: 142 instructions for 20 special functions of a warp and token.  Measured
-// at 8192 tokens x 4096 channels x 16 states in 32 prompts 206 us, 0.72 of that
+// issue: 145 instructions for 20 special functions of a warp and token.  Measured
+// at 8192 tokens x 4096 channels x 16 states in 32 prompts 200 us, 0.72 of that
 // unit's rate.  Four states a lane with the sums exchanged between lanes took 301
 // us (221 instructions for the same states), softplus and gate behind a run-time
 // branch 230 us: the compiler mixes the tokens of a group only without one.
@@ -27,7 +27,7 @@
 // each chunk's state from zero and its sum of dt' (the decay of a chunk is
 // exp(A sum dt')), a second joins them along each sequence, the third is the scan
 // of every chunk from its state.  Twice the exponentials, on many more lanes: one
-// prompt of 8192 tokens x 2048 channels 84 + 10 + 102 us, against 1430 us whole.
+// prompt of 8192 tokens x 2048 channels 85 + 13 + 104 us, against 1430 us whole.
 #include <type_traits>
 #include "sq_rows.cuh"
 #include "sq_vec.cuh"
@@ -439,13 +439,15 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(sq_scan_args a,
 // A warp alone takes `alone` for a token and a scheduler `turn` for a token of one
 // of its warps, by the states of a lane (16: 178 and 118 measured; 8: 119 and 71);
 // 64 states spread over four lanes cost half as much again.  Four CTAs an SM are
-// resident.  Whole sequences last as long as the longest (the host does not know
-// the lengths: of several, three times the mean is assumed); chunks take 0.75 of
-// the work twice, two launches and the join, whose steps of 16 chunks are one trip
-// to memory.  Measured, whole against chunks: 8 ragged prompts of 16384 tokens x
-// 4096 channels 1103 and 706 us, one of 8192 x 2048 1430 and 197 us, one of 300 x
-// 1024 55 and 18 us, 58 ones of 14223 x 1736 even 197 and
-// 308 us, ragged 380 and 335.
+// resident (fp32 rows with 16 states: three, for their shared memory; not told
+// apart), on the 148 SMs of a whole GPU: a stream of fewer takes the same chunks.
+// Whole sequences last as long as the longest (the host does not know the lengths:
+// of several, three times the mean is assumed); chunks take 1.75 of the passes (the
+// first has no outputs), two launches more and the join, whose steps of 16 chunks
+// are one trip to memory.  Measured, whole against chunks: 8 ragged prompts of 16384
+// tokens x 4096 channels 1103 and 717 us, one of 8192 x 2048 1430 and 202 us, one of
+// 300 x 1024 55 and 18 us, 58 ones of 14223 x 1736 even 197 and 308 us, ragged 380
+// and 335.
 int chunk_length(int tokens, int seqs, int channels, int states, int groups) {
     const int own = states < 16 ? states : 16, lanes = states > 16 ? states / 16 : 1;
     const int each = kScanThreads / (lanes < kScanThreads ? lanes : kScanThreads), per = (channels + groups - 1) / groups;

@@ -6,6 +6,9 @@
 
 namespace sq {
 
+// SMs that kernels launched on `stream` can run on (sq_fast.cu); 0 when the device cannot be asked.
+int sms_of(cudaStream_t stream);
+
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
@@ -33,8 +36,8 @@ __device__ __forceinline__ float reciprocal_approx(float x) {
     return r;
 }
 
-// x sigmoid(x) = x / (1 + e^-x).  Beyond -88 the exponential is infinite and the
-// result -0; -infinity and NaN give NaN as the quotient does.
+// x sigmoid(x) = x / (1 + e^-x).  Below -87.3 the reciprocal is flushed to zero and the
+// result is -0, for less than 10^-36 in size; -infinity and NaN give NaN as the quotient does.
 __device__ __forceinline__ float silu(float x) { return x * reciprocal_approx(1.f + exp2_approx(-kLog2e * x)); }
 
 // Pairs of fp32 values, one instruction for both.
