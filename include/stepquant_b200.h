@@ -123,7 +123,7 @@ typedef struct sq_step_args {
     void *out;
 } sq_step_args;
 
-/* Library version (major * 10000 + minor * 100 + patch). */
+/* Library version (major * 10000 + minor * 100 + patch); from 101 on sq_matmul_args has wait_clocks. */
 int32_t sq_version(void);
 
 /* Human-readable text for an sq_error code. */

@@ -181,8 +181,8 @@ def test_weight_quantization():
                                                (300, 2050, 8192), (512, 6500, 8192), (700, 8200, 4096), (4096, 5120, 1024)])
 def test_waits_that_run_out(rows, width, hidden):
     """Device waits limited to one try or a few clocks give up in the middle of copies and products: every
-    output is what it should be or NaN, NaN exactly where the status is flagged, and the calls
-    after it are whole."""
+    output is what it should be or NaN, NaN only where the status is flagged (and, up to 128 rows,
+    then; a tile's warp without rows of its own may give up alone), and the calls after are whole."""
     import ctypes
     from stepquant_b200 import _native as N
     from stepquant_b200.kernels.matmul import matmul_fp8
@@ -198,7 +198,9 @@ def test_waits_that_run_out(rows, width, hidden):
         N.check(N.lib().sq_matmul_fp8(ctypes.byref(args), N.stream_handle()))
         gone = out.isnan()
         assert torch.equal(out[~gone], want[~gone])
-        assert int(status) == (N.SQ_STATUS_TIMEOUT if bool(gone.any()) else 0)
+        flagged = int(status) == N.SQ_STATUS_TIMEOUT
+        assert flagged or (not bool(gone.any()) and int(status) == 0)
+        assert bool(gone.any()) or not flagged or rows > 128
         seen += bool(gone.any())
         assert torch.equal(matmul_fp8(x, sx, w, sw, status=status.zero_()), want) and int(status) == 0
     assert seen or width * hidden < 1 << 25  # thousands of waits with one try each
