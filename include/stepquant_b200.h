@@ -497,6 +497,140 @@ int32_t sq_selective_scan(const sq_scan_args *args, sq_stream_t stream);
 int32_t sq_selective_scan_step(const sq_scan_args *args, sq_stream_t stream);
 
 /*
+ * Rotary positions: the first `turned` of each head's dim channels, in pairs
+ * (i, i + turned / 2), or (2i, 2i + 1) when interleaved, rotated by the angle
+ * a = position frequencies[i]:  (x1, x2) -> magnitude (x1 cos a - x2 sin a, x1 sin a + x2 cos a).
+ * inverse: rotated back.  The other channels are copied.
+ *   x, out      [tokens, heads, dim] in dtype, strides in elements, last axis contiguous; out may be x
+ *   positions   [tokens], int64 (position_dtype 1) or int32 (0)
+ *   frequencies [turned / 2] fp64, radians a token, magnitudes below pi
+ * Angles are taken modulo a turn in 64-bit fixed point, sine and cosine in fp32.
+ * turned even, 0 <= turned <= dim <= 1024.
+ */
+typedef struct sq_rotary_args {
+    const void *x;
+    void *out;
+    const void *positions;
+    const double *frequencies;
+    int64_t x_stride;
+    int64_t x_head_stride;
+    int64_t out_stride;
+    int64_t out_head_stride;
+    int32_t tokens;
+    int32_t heads;
+    int32_t dim;
+    int32_t turned;
+    int32_t dtype;
+    int32_t position_dtype;
+    int32_t interleaved;
+    int32_t inverse;
+    float magnitude;
+} sq_rotary_args;
+
+int32_t sq_rotary(const sq_rotary_args *args, sq_stream_t stream);
+
+/*
+ * Paged cache of keys and values in 4 bits.  For each token, kv head and group
+ * of 64 channels x: m = min x rounded down to bf16, s = (max x - m) / 15
+ * rounded up to bf16, c = rint((x - m) / s); c stands for m + s c, within s / 2
+ * of x.  A group with a value that is not finite reads back as NaN.
+ *   data [num_pages, heads, page_size / 16, 18 dim] bytes, 16-byte aligned.  A
+ *        tile holds 16 tokens of one head: key codes (8 dim bytes), their (s, m)
+ *        pairs (dim bytes), value codes, their pairs.  32-bit words hold the
+ *        codes of 8 consecutive channels e: bits 2 e for even e, 14 + 2 e for odd.
+ *        Token u's pairs and key codes are in row r = 2 (u % 4) + u / 4 % 2 + u / 8 * 8,
+ *        pairs at [r][group]; key words in blocks of up to 128 channels (n = 1 or 2
+ *        groups), [block][r][2 n t + 2 group + j] for channels 16 t + 8 j of a group;
+ *        value words, number w = dim / 64 i + group for channels 8 i, at [w / 8][u][w % 8].
+ * dim 64, 128 or 256; page_size a multiple of 16.
+ *
+ * Sequence n holds lengths[n] tokens, position p in page page_table[n][p / page_size];
+ * its cu_seqlens[n + 1] - cu_seqlens[n] new tokens (without cu_seqlens: one, and
+ * tokens = num_seqs) are the last of them.  A page <= 0 holds nothing: its tokens
+ * are not written, read as zeros and not attended to.  So are those of a page past
+ * the pool and positions past the table, which are flagged in status
+ * (SQ_STATUS_SLOT_RANGE), and positions below zero, which are not.
+ *
+ * sq_kv_append writes k and v of the new tokens, [tokens, heads, dim] in dtype,
+ * keys rotated as by sq_rotary (turned = 0: not), by positions [tokens] or, when
+ * NULL, by their position in the sequence; the rotation is in 64 bits and its
+ * result not rounded before it is quantized.  sq_kv_read is the other way: it
+ * writes the values that the new tokens' codes stand for to k and v.
+ */
+typedef struct sq_kv_args {
+    void *k;
+    void *v;
+    uint8_t *data;
+    const int32_t *page_table;
+    const int32_t *lengths;
+    const int32_t *cu_seqlens;
+    const void *positions;
+    const double *frequencies;
+    int32_t *status;
+    int64_t k_stride;
+    int64_t k_head_stride;
+    int64_t v_stride;
+    int64_t v_head_stride;
+    int64_t table_stride;
+    int64_t num_pages;
+    int32_t tokens;
+    int32_t num_seqs;
+    int32_t table_width;
+    int32_t heads;
+    int32_t dim;
+    int32_t page_size;
+    int32_t dtype;
+    int32_t turned;
+    int32_t position_dtype;
+    int32_t interleaved;
+    float magnitude;
+} sq_kv_args;
+
+int32_t sq_kv_append(const sq_kv_args *args, sq_stream_t stream);
+int32_t sq_kv_read(const sq_kv_args *args, sq_stream_t stream);
+
+/*
+ * Attention of the new tokens over that cache:
+ *   out[i, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q[i, h] . k_j)
+ * over the positions j of the token's sequence up to its own and, with window > 0,
+ * above its own less window; kv head h / (q_heads / heads).  A token that sees
+ * nothing, and tokens of no sequence, get zeros.
+ *   q, out  [tokens, q_heads, dim] in dtype (SQ_BF16 or SQ_F16); q 16-byte aligned,
+ *           strides multiples of 8; out contiguous, 16-byte aligned
+ *   workspace  sq_kv_attention_workspace_bytes(...) bytes, 16-byte aligned
+ * Prompts take keys as f16 over 256: magnitudes up to 2^23.
+ * status: also SQ_STATUS_TIMEOUT if a bounded device wait gave up; outputs concerned are NaN.
+ */
+typedef struct sq_kv_attention_args {
+    const void *q;
+    const uint8_t *data;
+    void *out;
+    const int32_t *page_table;
+    const int32_t *lengths;
+    const int32_t *cu_seqlens;
+    int32_t *status;
+    void *workspace;
+    int64_t workspace_bytes;
+    int64_t q_stride;
+    int64_t q_head_stride;
+    int64_t table_stride;
+    int64_t num_pages;
+    int32_t tokens;
+    int32_t num_seqs;
+    int32_t table_width;
+    int32_t q_heads;
+    int32_t heads;
+    int32_t dim;
+    int32_t page_size;
+    int32_t dtype;
+    int32_t window;
+    float scale;
+} sq_kv_attention_args;
+
+int64_t sq_kv_attention_workspace_bytes(int32_t tokens, int32_t num_seqs, int32_t q_heads, int32_t heads, int32_t dim);
+int32_t sq_kv_attention(const sq_kv_attention_args *args, sq_stream_t stream);
+
+/*
  * Self-test of the division used by the register-resident decode kernels: for
  * i < n, out[i] = a[i] / b[i] computed with a correctly rounded reciprocal of
  * the fp16 value b[i] (given as its bits) and one Markstein correction.  It

@@ -74,6 +74,30 @@ class SqScanArgs(ctypes.Structure):
                 ("softplus", _i32)]
 
 
+class SqRotaryArgs(ctypes.Structure):
+    _fields_ = [("x", _p), ("out", _p), ("positions", _p), ("frequencies", _p), ("x_stride", _i64), ("x_head_stride", _i64),
+                ("out_stride", _i64), ("out_head_stride", _i64), ("tokens", _i32), ("heads", _i32), ("dim", _i32),
+                ("turned", _i32), ("dtype", _i32), ("position_dtype", _i32), ("interleaved", _i32), ("inverse", _i32),
+                ("magnitude", ctypes.c_float)]
+
+
+class SqKvArgs(ctypes.Structure):
+    _fields_ = [("k", _p), ("v", _p), ("data", _p), ("page_table", _p), ("lengths", _p), ("cu_seqlens", _p),
+                ("positions", _p), ("frequencies", _p), ("status", _p), ("k_stride", _i64), ("k_head_stride", _i64),
+                ("v_stride", _i64), ("v_head_stride", _i64), ("table_stride", _i64), ("num_pages", _i64), ("tokens", _i32),
+                ("num_seqs", _i32), ("table_width", _i32), ("heads", _i32), ("dim", _i32), ("page_size", _i32),
+                ("dtype", _i32), ("turned", _i32), ("position_dtype", _i32), ("interleaved", _i32),
+                ("magnitude", ctypes.c_float)]
+
+
+class SqKvAttentionArgs(ctypes.Structure):
+    _fields_ = [("q", _p), ("data", _p), ("out", _p), ("page_table", _p), ("lengths", _p), ("cu_seqlens", _p),
+                ("status", _p), ("workspace", _p), ("workspace_bytes", _i64), ("q_stride", _i64), ("q_head_stride", _i64),
+                ("table_stride", _i64), ("num_pages", _i64), ("tokens", _i32), ("num_seqs", _i32), ("table_width", _i32),
+                ("q_heads", _i32), ("heads", _i32), ("dim", _i32), ("page_size", _i32), ("dtype", _i32), ("window", _i32),
+                ("scale", ctypes.c_float)]
+
+
 _SIGNATURES = {
     "sq_version": (_i32, []),
     "sq_error_string": (ctypes.c_char_p, [_i32]),
@@ -103,6 +127,11 @@ _SIGNATURES = {
     "sq_selective_scan": (_i32, [_p, _p]),
     "sq_selective_scan_step": (_i32, [_p, _p]),
     "sq_selective_scan_workspace_bytes": (_i64, [_i32] * 5),
+    "sq_rotary": (_i32, [_p, _p]),
+    "sq_kv_append": (_i32, [_p, _p]),
+    "sq_kv_read": (_i32, [_p, _p]),
+    "sq_kv_attention": (_i32, [_p, _p]),
+    "sq_kv_attention_workspace_bytes": (_i64, [_i32] * 5),
 }
 
 EXPORTED = tuple(_SIGNATURES)
@@ -169,7 +198,8 @@ def require_cuda(*tensors):
 
 
 # ---------------------------------------------------------------------------
-# the layer operators' calls (kernels/norm.py, matmul.py, conv.py, scan.py)
+# the layer operators' calls (kernels/norm.py, matmul.py, conv.py, scan.py,
+# rotary.py, kv_cache.py)
 # ---------------------------------------------------------------------------
 _FORMATS = {_p: "P", _i64: "q", _i32: "i", ctypes.c_float: "f"}
 

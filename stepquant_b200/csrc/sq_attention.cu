@@ -1,0 +1,660 @@
+// Attention over the paged 4-bit cache (sq_kv.cu):
+//
+//   out_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i . k_j - max)
+//
+// with k_j = m + s c for each group of 64 channels.  Scale and minimum of a key leave
+// the product, q . k = sum over groups of s (q . c) + m sum(q), and those of a value go
+// to its weight, p v = (p s) c + p m, so the tensor cores work on the codes, which 16
+// bits hold exactly.
+#include "sq_kv.cuh"
+#include "sq_rows.cuh"
+#include "sq_tc.cuh"
+#include "sq_vec.cuh"
+
+namespace sq {
+namespace {
+
+constexpr int kWarps = 8, kAttnThreads = 32 * kWarps;
+constexpr int kMostCtas = 320;
+constexpr int kLeastTiles = 2 * kWarps;  // of a CTA
+
+// ---------------------------------------------------------------------------
+// fragments
+// ---------------------------------------------------------------------------
+// Values are taken as (m + 8 s) + s (c - 8): of all splits of a value into a part that the weights'
+// rounding does not touch and one that it does, the one with the smallest second part.
+constexpr float kMiddle = 8.f;
+
+template <class T>
+struct Codes;
+template <>
+struct Codes<__nv_bfloat16> {
+    static constexpr float kHeld = 128.f;  // pair() is c + this: a bf16 with c in its last bits
+    __device__ static __forceinline__ uint32_t pair(uint32_t w) { return (w & 0x000F000Fu) | 0x43004300u; }
+    __device__ static __forceinline__ uint32_t pack(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+    __device__ static __forceinline__ float2 unpack(uint32_t x) {
+        return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u));
+    }
+    __device__ static __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                               uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+    static constexpr uint32_t kOnes = 0x3F803F80u;
+    static constexpr float kLag = 8.f;
+};
+template <>
+struct Codes<__half> {
+    static constexpr float kHeld = -kMiddle;  // f16 with c in their last bits are 1024 + c, too far from c to leave it in
+    __device__ static __forceinline__ uint32_t pair(uint32_t w) {
+        const uint32_t x = (w & 0x000F000Fu) | 0x64006400u, base = 0x64086408u;
+        const __half2 r = __hsub2(reinterpret_cast<const __half2 &>(x), reinterpret_cast<const __half2 &>(base));
+        return reinterpret_cast<const uint32_t &>(r);
+    }
+    __device__ static __forceinline__ uint32_t pack(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+    __device__ static __forceinline__ float2 unpack(uint32_t x) { return __half22float2(reinterpret_cast<const __half2 &>(x)); }
+    __device__ static __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                               uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+    static constexpr uint32_t kOnes = 0x3C003C00u;
+    static constexpr float kLag = 2.f;  // weights p s reach 4 * 8738 (a group's largest scale in f16), below 65504
+};
+
+// Transpose of an 8 x 8 matrix of 16-bit values, two of row lane / 4 in each lane.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+
+__device__ __forceinline__ float pair_scale(uint32_t p) { return __uint_as_float(p << 16); }
+__device__ __forceinline__ float pair_min(uint32_t p) { return __uint_as_float(p & 0xFFFF0000u); }
+
+// ---------------------------------------------------------------------------
+// work: tiles of 16 tokens in the order (sequence, kv head, block of rows, tile), cut into equal
+// spans of consecutive ones, a span to a CTA
+// ---------------------------------------------------------------------------
+struct Sequence {
+    int first, count;   // new tokens
+    int length;         // tokens that the page table reaches
+    int64_t before;     // position of the first new token
+    int tile, tiles;    // tiles that any of them sees: one at least
+    int blocks;         // of rows (token, query head of the kv head)
+    int64_t cost;
+};
+
+template <int ROWS>
+__device__ __forceinline__ Sequence sequence(const sq_kv_attention_args &a, int n, bool report) {
+    Sequence s;
+    const int2 r = a.cu_seqlens ? sequence_range(a.cu_seqlens, n, a.tokens) : make_int2(n, n + 1);
+    s.first = r.x;
+    s.count = r.y - r.x;
+    const int length = a.lengths[n];
+    const int64_t most = int64_t(a.table_width) * a.page_size;
+    if (report && s.count > 0 && length > most) flag(a.status, SQ_STATUS_SLOT_RANGE);
+    s.length = int(max(int64_t(0), min(int64_t(length), most)));
+    s.before = int64_t(length) - s.count;
+    const int64_t start = a.window > 0 ? max(int64_t(0), s.before - a.window + 1) : 0;
+    s.tile = int(min(start, int64_t(s.length)) / kTile);
+    s.tiles = max(1, (s.length + kTile - 1) / kTile - s.tile);
+    s.blocks = int((int64_t(s.count) * (a.q_heads / a.heads) + ROWS - 1) / ROWS);
+    s.cost = int64_t(s.blocks) * a.heads * s.tiles;
+    return s;
+}
+
+struct Span {
+    int64_t begin, end, per;  // in tiles
+    int sequence;             // that begin lies in
+    int64_t offset;           // of begin in it
+};
+
+// This CTA's span (begin = end: none).  Every thread of the CTA calls it.
+template <int ROWS>
+__device__ __forceinline__ Span span_of(const sq_kv_attention_args &a, bool report) {
+    __shared__ int64_t warp_sums[kWarps];
+    __shared__ int64_t found_offset;
+    __shared__ int found;
+    const int each = (a.num_seqs + kAttnThreads - 1) / kAttnThreads;
+    const int from = min(int(threadIdx.x) * each, a.num_seqs), to = min(from + each, a.num_seqs);
+    int64_t mine = 0;
+    for (int n = from; n < to; ++n) mine += sequence<ROWS>(a, n, report).cost;
+    int64_t sum = mine;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int i = 1; i < 32; i *= 2) {
+        const int64_t other = __shfl_up_sync(~0u, sum, i);
+        if (lane >= i) sum += other;
+    }
+    if (lane == 31) warp_sums[warp] = sum;
+    if (threadIdx.x == 0) found = 0, found_offset = 0;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) sum += warp_sums[w];
+        total += warp_sums[w];
+    }
+    Span s;
+    s.per = max(int64_t(kLeastTiles), (total + gridDim.x - 1) / gridDim.x);
+    s.begin = min(total, s.per * blockIdx.x);
+    s.end = min(total, s.begin + s.per);
+    int64_t at = sum - mine;
+    if (s.begin < s.end && at <= s.begin && s.begin < sum) {
+        for (int n = from; n < to; ++n) {
+            const int64_t cost = sequence<ROWS>(a, n, false).cost;
+            if (s.begin < at + cost) {
+                found = n;
+                found_offset = s.begin - at;
+                break;
+            }
+            at += cost;
+        }
+    }
+    __syncthreads();
+    s.sequence = found;
+    s.offset = found_offset;
+    return s;
+}
+
+template <class T>
+__device__ __forceinline__ T *output_row(const sq_kv_attention_args &a, const Sequence &s, int head, int64_t row) {
+    const int group = a.q_heads / a.heads;
+    return static_cast<T *>(a.out) + ((s.first + row / group) * a.q_heads + head * group + row % group) * a.dim;
+}
+
+// ---------------------------------------------------------------------------
+// few rows: the cache's bytes bound it
+// ---------------------------------------------------------------------------
+template <int D, int NT>
+struct RowsShape {
+    using Tile = KvTile<D>;
+    static constexpr int kRows = 8 * NT;
+    static constexpr int kStages = D == 64 ? 6 : D == 128 ? 5 : 3;
+    static constexpr int kRing = kStages * Tile::kBytes;          // of a warp
+    static constexpr int kMergeRow = D + 4;                       // floats
+    static constexpr int kPart = kRows * D + 2 * kRows;           // floats of a part: sums, maxima, weights' sums
+    static constexpr int kShared = kWarps * kRing;
+    static_assert(kRows * kMergeRow * 4 <= kRing && kRing % 16 == 0 && Tile::kBytes % 16 == 0, "a warp's sums lie in its ring");
+};
+
+template <class T, int D, int NT>
+__global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) rows_kernel(sq_kv_attention_args a) {
+    using Shape = RowsShape<D, NT>;
+    using Tile = KvTile<D>;
+    using C = Codes<T>;
+    constexpr int kGroups = Tile::kGroups, kRows = Shape::kRows, kStages = Shape::kStages;
+    extern __shared__ __align__(128) uint8_t rings[];
+    __shared__ uint64_t bars[kWarps][kStages];
+    __shared__ float row_max[kWarps][kRows], row_sum[kWarps][kRows];
+    __shared__ int abort_flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    uint8_t *ring = rings + warp * Shape::kRing;
+    if (threadIdx.x == 0) abort_flag = 0;
+    if (lane == 0) {
+        for (int i = 0; i < kStages; ++i) tc::bar_init(&bars[warp][i], 1);
+        tc::bar_init_fence();
+    }
+    if (a.cu_seqlens)
+        clear_outside(a.out, int64_t(a.q_heads) * D * sizeof(T), a.cu_seqlens, a.num_seqs, a.tokens, blockIdx.x, gridDim.x);
+    const Span span = span_of<kRows>(a, blockIdx.x == 0);
+    const int group = a.q_heads / a.heads, page_tiles = a.page_size / kTile;
+    const float to_log2 = a.scale * kLog2e;
+    const int64_t head_bytes = int64_t(page_tiles) * Tile::kBytes;
+    uint32_t used = 0;  // of this warp's stages, ever
+    int n = span.sequence;
+    int64_t offset = span.offset;
+    Sequence seq = sequence<kRows>(a, min(n, a.num_seqs - 1), false);
+    for (int64_t at = span.begin; at < span.end;) {
+        while (offset >= seq.cost) {  // on to the next sequence with new tokens: there is one, as at < span.end
+            seq = sequence<kRows>(a, ++n, false);
+            offset = 0;
+        }
+        const int64_t item = offset / seq.tiles;
+        const int head = int(item / seq.blocks), block = int(item % seq.blocks);
+        const int begin = int(offset % seq.tiles), count = int(min(span.end - at, int64_t(seq.tiles - begin)));
+        const bool whole = count == seq.tiles;
+        const int64_t slot = 2 * blockIdx.x + (at == span.begin ? 0 : 1);
+        at += count;
+        offset += count;
+
+        // This warp's tiles of the segment: begin + warp, begin + warp + 8, ...
+        const int mine = (count - warp + kWarps - 1) / kWarps;
+        const int first_tile = seq.tile + begin + warp;
+        const int32_t *table = a.page_table + n * a.table_stride;
+        int pages = 0;
+        uint32_t held = 0;  // by tile, modulo 32: whether there was one to load
+        auto request = [&](int i) {  // tile i of this warp
+            if ((i & 31) == 0) {
+                const int index = (first_tile + (i + lane) * kWarps) / page_tiles;
+                pages = i + lane < mine && index < a.table_width ? table[index] : 0;
+                if (pages >= a.num_pages) {
+                    flag(a.status, SQ_STATUS_SLOT_RANGE);
+                    pages = 0;
+                }
+            }
+            const int page = __shfl_sync(~0u, pages, i & 31);
+            const uint32_t bit = 1u << (i & 31);
+            held = page > 0 ? held | bit : held & ~bit;
+            if (lane == 0) {
+                const int stage = (used + i) % kStages;
+                if (page > 0) {
+                    const int in_page = (first_tile + i * kWarps) % page_tiles;
+                    tc::bar_expect(&bars[warp][stage], Tile::kBytes);
+                    tc::bulk_load(ring + stage * Tile::kBytes,
+                                  a.data + (int64_t(page) * a.heads + head) * head_bytes + int64_t(in_page) * Tile::kBytes,
+                                  Tile::kBytes, &bars[warp][stage]);
+                } else {
+                    tc::bar_arrive(&bars[warp][stage]);
+                }
+            }
+        };
+        for (int i = 0; i < min(mine, kStages); ++i) request(i);
+
+        // Query rows as the product's second operand: row g's channels 16 t + 0..15 of each group.
+        uint32_t q[NT][kGroups][8];
+        float q_sum[NT][kGroups][2];  // of rows 2 t and 2 t + 1: the groups' sums
+        int64_t limit[NT][2];
+        const int64_t row0 = int64_t(block) * kRows, rows = int64_t(seq.count) * group;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int64_t row = row0 + j * 8 + g;
+            const bool live = row < rows;
+            const T *from = static_cast<const T *>(a.q) + (seq.first + (live ? row / group : 0)) * a.q_stride +
+                            (head * group + (live ? row % group : 0)) * a.q_head_stride + 16 * t;
+#pragma unroll
+            for (int b = 0; b < kGroups; ++b) {
+                const uint4 x = reinterpret_cast<const uint4 *>(from + b * kGroup)[0], y = reinterpret_cast<const uint4 *>(from + b * kGroup)[1];
+                const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    q[j][b][i] = live ? w[i] : 0;
+                    const float2 v = C::unpack(q[j][b][i]);
+                    sum += v.x + v.y;
+                }
+                sum += __shfl_xor_sync(~0u, sum, 1);
+                sum += __shfl_xor_sync(~0u, sum, 2);  // of row g; rows 2 t, 2 t + 1 are in lanes 8 t, 8 t + 4
+                q_sum[j][b][0] = __shfl_sync(~0u, sum, 8 * t);
+                q_sum[j][b][1] = __shfl_sync(~0u, sum, 8 * t + 4);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int64_t r = row0 + j * 8 + 2 * t + e;
+                limit[j][e] = r < rows ? min(seq.before + r / group, int64_t(seq.length) - 1) : -1;
+            }
+        }
+        // Tiles that every row sees whole: up to `sees_all`, from `window_all` on.
+        const int64_t last_row = min(row0 + kRows, rows) - 1;
+        const int64_t sees_all = min(seq.before + row0 / group + 1, int64_t(seq.length)) / kTile;
+        const int64_t window_all = a.window > 0 ? (max(int64_t(0), seq.before + last_row / group - a.window + 1) + kTile - 1) / kTile : 0;
+
+        float acc[NT][kGroups][4][4], ones[NT][kGroups][4], least[NT][kGroups][2];
+        float top[NT][2], sum[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int b = 0; b < kGroups; ++b) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    ones[j][b][i] = 0.f;
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) acc[j][b][m][i] = 0.f;
+                }
+                least[j][b][0] = least[j][b][1] = 0.f;
+            }
+            top[j][0] = top[j][1] = -INFINITY;
+            sum[j][0] = sum[j][1] = 0.f;
+        }
+        bool gave_up = false;
+        for (int i = 0; i < mine; ++i) {
+            const uint32_t use = used + i;
+            const int stage = use % kStages;
+            if (!tc::bar_wait(&bars[warp][stage], (use / kStages) & 1, &abort_flag, tc::kWaitClocks)) gave_up = true;
+            if (held >> (i & 31) & 1) {
+                const uint8_t *tile = ring + stage * Tile::kBytes;
+                // Scores of tokens (rows g, g + 8) x query rows (2 t, 2 t + 1).
+                float z[NT][4];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) z[j][0] = z[j][1] = z[j][2] = z[j][3] = 0.f;
+#pragma unroll
+                for (int b = 0; b < kGroups; ++b) {
+                    const int at_word = (b / Tile::kBlockGroups) * kTile * Tile::kBlockRow + (b % Tile::kBlockGroups) * 8 + t * 8 * Tile::kBlockGroups;
+                    const uint2 lo = *reinterpret_cast<const uint2 *>(tile + at_word + g * Tile::kBlockRow);
+                    const uint2 hi = *reinterpret_cast<const uint2 *>(tile + at_word + (g + 8) * Tile::kBlockRow);
+                    float d[NT][4];
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) d[j][0] = d[j][1] = d[j][2] = d[j][3] = 0.f;
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        const uint32_t x = w ? lo.y : lo.x, y = w ? hi.y : hi.x;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t a0 = C::pair(x >> (8 * h)), a1 = C::pair(y >> (8 * h));
+                            const uint32_t a2 = C::pair(x >> (8 * h + 4)), a3 = C::pair(y >> (8 * h + 4));
+#pragma unroll
+                            for (int j = 0; j < NT; ++j) C::mma(d[j], a0, a1, a2, a3, q[j][b][4 * w + 2 * h], q[j][b][4 * w + 2 * h + 1]);
+                        }
+                    }
+                    const uint32_t p0 = *reinterpret_cast<const uint32_t *>(tile + Tile::kKeyPairs + (g * kGroups + b) * 4);
+                    const uint32_t p1 = *reinterpret_cast<const uint32_t *>(tile + Tile::kKeyPairs + ((g + 8) * kGroups + b) * 4);
+                    const float s0 = pair_scale(p0), s1 = pair_scale(p1);
+                    const float m0 = pair_min(p0) - C::kHeld * s0, m1 = pair_min(p1) - C::kHeld * s1;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        z[j][0] += s0 * d[j][0] + m0 * q_sum[j][b][0];
+                        z[j][1] += s0 * d[j][1] + m0 * q_sum[j][b][1];
+                        z[j][2] += s1 * d[j][2] + m1 * q_sum[j][b][0];
+                        z[j][3] += s1 * d[j][3] + m1 * q_sum[j][b][1];
+                    }
+                }
+                const int index = first_tile + i * kWarps;
+                const bool partial = index >= sees_all || index < window_all;
+                uint32_t hidden = 0;  // bits of z
+                if (partial) {
+                    // Row r of a tile is token r / 2 + 4 (r % 2) of its half.
+                    const int64_t token = int64_t(index) * kTile + (g >> 1) + 4 * (g & 1);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int i4 = 0; i4 < 4; ++i4) {
+                            const int64_t p = token + (i4 & 2) * 4, last = limit[j][i4 & 1];
+                            if (p > last || (a.window > 0 && p <= last - a.window)) hidden |= 1u << (4 * j + i4);
+                        }
+                }
+                float most[NT][2];
+                bool grows = false;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; ++i4) z[j][i4] = hidden >> (4 * j + i4) & 1 ? -INFINITY : z[j][i4] * to_log2;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        most[j][e] = fmaxf(z[j][e], z[j][2 + e]);
+                        grows = grows || most[j][e] > top[j][e] + C::kLag;
+                    }
+                }
+                // The maxima that weights are taken against may lag behind by 2^kLag: they move seldom.
+                if (__any_sync(~0u, grows)) {
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float x = most[j][e];
+                            x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
+                            x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
+                            x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
+                            x = fmaxf(x, top[j][e]);
+                            const float factor = x == -INFINITY ? 1.f : exp2_approx(top[j][e] - x);
+                            top[j][e] = x;
+                            sum[j][e] *= factor;
+#pragma unroll
+                            for (int b = 0; b < kGroups; ++b) {
+                                least[j][b][e] *= factor;
+                                ones[j][b][e] *= factor;
+                                ones[j][b][2 + e] *= factor;
+#pragma unroll
+                                for (int m = 0; m < 4; ++m) acc[j][b][m][e] *= factor, acc[j][b][m][2 + e] *= factor;
+                            }
+                        }
+                }
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; ++i4) {
+                        const float against = top[j][i4 & 1];
+                        z[j][i4] = exp2_approx(z[j][i4] - (against == -INFINITY ? 0.f : against));
+                        sum[j][i4 & 1] += z[j][i4];
+                    }
+                // Values: rows are channels (x: even ones, y: odd ones), columns query rows.
+#pragma unroll
+                for (int b = 0; b < kGroups; ++b) {
+                    const uint32_t p0 = *reinterpret_cast<const uint32_t *>(tile + Tile::kValuePairs + (g * kGroups + b) * 4);
+                    const uint32_t p1 = *reinterpret_cast<const uint32_t *>(tile + Tile::kValuePairs + ((g + 8) * kGroups + b) * 4);
+                    const float s0 = pair_scale(p0), s1 = pair_scale(p1), m0 = pair_min(p0) + kMiddle * s0, m1 = pair_min(p1) + kMiddle * s1;
+                    uint32_t w0[NT], w1[NT];
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        float u[4] = {z[j][0] * s0, z[j][1] * s0, z[j][2] * s1, z[j][3] * s1};
+                        float v[4] = {z[j][0] * m0, z[j][1] * m0, z[j][2] * m1, z[j][3] * m1};
+                        if (hidden) {  // a hidden token's scale may be anything
+#pragma unroll
+                            for (int i4 = 0; i4 < 4; ++i4)
+                                if (hidden >> (4 * j + i4) & 1) u[i4] = v[i4] = 0.f;
+                        }
+                        least[j][b][0] += v[0] + v[2];
+                        least[j][b][1] += v[1] + v[3];
+                        w0[j] = transpose8(C::pack(u[0], u[1]));
+                        w1[j] = transpose8(C::pack(u[2], u[3]));
+                        if (C::kHeld != -kMiddle) C::mma(ones[j][b], C::kOnes, C::kOnes, C::kOnes, C::kOnes, w0[j], w1[j]);
+                    }
+                    const int number = kGroups * g + b;
+                    const uint8_t *from = tile + Tile::kValues + (number >> 3) * kTile * 32 + (number & 7) * 4 + t * 32;
+                    uint32_t word[4];
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; ++i4) word[i4] = *reinterpret_cast<const uint32_t *>(from + i4 * 4 * 32);
+                    const uint32_t x0 = __byte_perm(word[0], word[1], 0x5410), y0 = __byte_perm(word[0], word[1], 0x7632);
+                    const uint32_t x1 = __byte_perm(word[2], word[3], 0x5410), y1 = __byte_perm(word[2], word[3], 0x7632);
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) {
+                        const uint32_t a0 = C::pair(x0 >> (4 * m)), a1 = C::pair(y0 >> (4 * m));
+                        const uint32_t a2 = C::pair(x1 >> (4 * m)), a3 = C::pair(y1 >> (4 * m));
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) C::mma(acc[j][b][m], a0, a1, a2, a3, w0[j], w1[j]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (i + kStages < mine) request(i + kStages);
+        }
+        used += mine;
+        if (gave_up) {  // the copies still on their way end before the ring is used again
+            flag(a.status, SQ_STATUS_TIMEOUT);
+            int alone = 0;
+            for (int i = max(0, mine - kStages); i < mine; ++i)
+                tc::bar_wait(&bars[warp][(used - mine + i) % kStages], ((used - mine + i) / kStages) & 1, &alone, tc::kWaitClocks);
+        }
+
+        // The warps' sums, to shared memory (each into its own, idle, ring), then to the output or a part.
+        float *mine_out = reinterpret_cast<float *>(ring);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = j * 8 + 2 * t + e;
+                float total = sum[j][e];
+#pragma unroll
+                for (int i = 4; i < 32; i *= 2) total += __shfl_xor_sync(~0u, total, i);
+                if (g == 0) row_max[warp][row] = gave_up ? NAN : top[j][e], row_sum[warp][row] = total;
+#pragma unroll
+                for (int b = 0; b < kGroups; ++b) {
+                    float low_part = least[j][b][e];
+#pragma unroll
+                    for (int i = 4; i < 32; i *= 2) low_part += __shfl_xor_sync(~0u, low_part, i);
+                    low_part -= (C::kHeld + kMiddle) * ones[j][b][e];
+                    float *to = mine_out + row * Shape::kMergeRow + b * kGroup + 8 * g;
+#pragma unroll
+                    for (int m = 0; m < 4; m += 2)
+                        *reinterpret_cast<float4 *>(to + 2 * m) =
+                            make_float4(acc[j][b][m][e] + low_part, acc[j][b][m][2 + e] + low_part, acc[j][b][m + 1][e] + low_part,
+                                        acc[j][b][m + 1][2 + e] + low_part);
+                }
+            }
+        __syncthreads();
+        const int warps = min(count, kWarps);  // that had tiles
+        float *part = reinterpret_cast<float *>(a.workspace) + slot * Shape::kPart;
+        for (int i = threadIdx.x; i < kRows * D / 4; i += kAttnThreads) {
+            const int row = i / (D / 4), c = i % (D / 4) * 4;
+            float most = -INFINITY;
+            bool bad = false;
+            for (int w = 0; w < warps; ++w) {
+                most = fmaxf(most, row_max[w][row]);
+                bad = bad || row_max[w][row] != row_max[w][row];
+            }
+            if (bad) most = NAN;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            float weight = 0.f;
+            for (int w = 0; w < warps; ++w) {
+                const float factor = row_max[w][row] == -INFINITY ? 0.f : exp2_approx(row_max[w][row] - most);
+                if (factor == 0.f) continue;
+                const float4 y = *reinterpret_cast<const float4 *>(reinterpret_cast<float *>(rings + w * Shape::kRing) + row * Shape::kMergeRow + c);
+                x.x += factor * y.x, x.y += factor * y.y, x.z += factor * y.z, x.w += factor * y.w;
+                weight += factor * row_sum[w][row];
+            }
+            if (whole) {
+                if (row0 + row < rows) {
+                    const float per = weight == 0.f ? 0.f : 1.f / weight;
+                    T *out = output_row<T>(a, seq, head, row0 + row) + c;
+                    *reinterpret_cast<uint2 *>(out) = make_uint2(C::pack(x.x * per, x.y * per), C::pack(x.z * per, x.w * per));
+                }
+            } else {
+                *reinterpret_cast<float4 *>(part + row * D + c) = x;
+                if (c == 0) part[kRows * D + row] = most, part[kRows * D + kRows + row] = weight;
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // before copies into the rings again
+        __syncthreads();
+    }
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+}
+
+// Joins the parts of items that several CTAs had: the CTA in whose span one ends.
+template <class T, int D, int NT>
+__global__ void __launch_bounds__(kAttnThreads) join_kernel(sq_kv_attention_args a) {
+    using Shape = RowsShape<D, NT>;
+    using C = Codes<T>;
+    constexpr int kRows = Shape::kRows;
+    extern __shared__ float factors[];  // [parts][rows]
+    __shared__ float weights[kRows];
+    const Span span = span_of<kRows>(a, false);
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    if (span.begin >= span.end) return;
+    const Sequence seq = sequence<kRows>(a, span.sequence, false);
+    const int done = int(span.offset % seq.tiles);  // tiles of the item before this span
+    if (done == 0 || seq.tiles - done > span.end - span.begin) return;
+    const int64_t item = span.offset / seq.tiles, start = span.begin - done, cta0 = start / span.per;
+    const int head = int(item / seq.blocks), block = int(item % seq.blocks), parts = int(blockIdx.x - cta0) + 1;
+    const float *workspace = static_cast<const float *>(a.workspace);
+    auto part = [&](int i) {
+        const int64_t slot = 2 * (cta0 + i) + (i == 0 && start != cta0 * span.per ? 1 : 0);
+        return workspace + slot * Shape::kPart;
+    };
+    for (int i = threadIdx.x; i < parts * kRows; i += kAttnThreads) factors[i] = part(i / kRows)[kRows * D + i % kRows];
+    __syncthreads();
+    if (threadIdx.x < kRows) {
+        const int row = threadIdx.x;
+        float most = -INFINITY;
+        bool bad = false;
+        for (int i = 0; i < parts; ++i) {
+            most = fmaxf(most, factors[i * kRows + row]);
+            bad = bad || factors[i * kRows + row] != factors[i * kRows + row];
+        }
+        float weight = 0.f;
+        for (int i = 0; i < parts; ++i) {
+            const float f = bad ? NAN : factors[i * kRows + row] == -INFINITY ? 0.f : exp2_approx(factors[i * kRows + row] - most);
+            factors[i * kRows + row] = f;
+            weight += f == 0.f ? 0.f : f * part(i)[kRows * D + kRows + row];
+        }
+        weights[row] = weight;
+    }
+    __syncthreads();
+    const int64_t row0 = int64_t(block) * kRows, rows = int64_t(seq.count) * (a.q_heads / a.heads);
+    for (int i = threadIdx.x; i < kRows * D / 4; i += kAttnThreads) {
+        const int row = i / (D / 4), c = i % (D / 4) * 4;
+        if (row0 + row >= rows) continue;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int p = 0; p < parts; ++p) {
+            const float f = factors[p * kRows + row];
+            const float4 y = *reinterpret_cast<const float4 *>(part(p) + row * D + c);
+            if (f != 0.f) x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
+        }
+        const float per = weights[row] == 0.f ? 0.f : 1.f / weights[row];
+        T *out = output_row<T>(a, seq, head, row0 + row) + c;
+        *reinterpret_cast<uint2 *>(out) = make_uint2(C::pack(x.x * per, x.y * per), C::pack(x.z * per, x.w * per));
+    }
+}
+
+template <class T, int D, int NT>
+cudaError_t launch_rows(const sq_kv_attention_args &a, cudaStream_t s) {
+    using Shape = RowsShape<D, NT>;
+    const int sms = sms_of(s);
+    if (sms < 1) return cudaErrorInvalidDevice;
+    const int resident = NT == 1 && D <= 128 ? 2 : 1;
+    const unsigned grid = unsigned(sms * resident < kMostCtas ? sms * resident : kMostCtas);
+    cudaError_t e = cudaFuncSetAttribute(rows_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kShared);
+    if (e != cudaSuccess) return e;
+    rows_kernel<T, D, NT><<<grid, kAttnThreads, Shape::kShared, s>>>(a);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kAttnThreads);
+    cfg.dynamicSmemBytes = size_t(grid) * Shape::kRows * sizeof(float);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, join_kernel<T, D, NT>, a);
+}
+
+// Blocks of 16 rows where sequences have more than 8 (heads of 256 channels: their sums leave no room).
+bool wide_rows(int tokens, int seqs, int q_heads, int heads, int dim) {
+    return dim < 256 && int64_t(tokens) * (q_heads / heads) > int64_t(seqs) * 8;
+}
+
+template <class T>
+cudaError_t launch_attention(const sq_kv_attention_args &a, cudaStream_t s) {
+    const bool wide = wide_rows(a.tokens, a.num_seqs, a.q_heads, a.heads, a.dim);
+    switch (a.dim) {
+        case 64: return wide ? launch_rows<T, 64, 2>(a, s) : launch_rows<T, 64, 1>(a, s);
+        case 128: return wide ? launch_rows<T, 128, 2>(a, s) : launch_rows<T, 128, 1>(a, s);
+        default: return launch_rows<T, 256, 1>(a, s);
+    }
+}
+
+}  // namespace
+}  // namespace sq
+
+extern "C" int64_t sq_kv_attention_workspace_bytes(int32_t tokens, int32_t num_seqs, int32_t q_heads, int32_t heads, int32_t dim) {
+    if (tokens < 0 || num_seqs < 0 || heads < 1 || q_heads < 1 || (dim != 64 && dim != 128 && dim != 256)) return -1;
+    if (tokens == 0 || num_seqs == 0) return 0;
+    const int64_t rows = sq::wide_rows(tokens, num_seqs, q_heads, heads, dim) ? 16 : 8;
+    return 2 * sq::kMostCtas * (rows * dim + 2 * rows) * int64_t(sizeof(float));
+}
+
+extern "C" int32_t sq_kv_attention(const sq_kv_attention_args *args, sq_stream_t stream) {
+    using namespace sq;
+    if (!args) return SQ_ERR_ARGUMENT;
+    const sq_kv_attention_args &a = *args;
+    if (a.tokens < 0 || a.num_seqs < 0 || a.table_width < 0 || a.num_pages < 0 || a.heads < 1 || a.q_heads < 1 || a.window < 0)
+        return SQ_ERR_ARGUMENT;
+    if (a.dtype < SQ_F32 || a.dtype > SQ_F16 || !(a.scale > 0.f) || !(a.scale < INFINITY)) return SQ_ERR_ARGUMENT;
+    if (a.dtype == SQ_F32 || (a.dim != 64 && a.dim != 128 && a.dim != 256)) return SQ_ERR_UNSUPPORTED;
+    if (a.page_size < kTile || a.page_size % kTile || a.table_stride < 0 || a.q_heads % a.heads) return SQ_ERR_SHAPE;
+    if (a.q_stride < 0 || a.q_head_stride < 0 || a.q_stride % 8 || a.q_head_stride % 8) return SQ_ERR_SHAPE;
+    if (!aligned16(a.q) || !aligned16(a.out) || !aligned16(a.data) || !aligned16(a.workspace)) return SQ_ERR_SHAPE;
+    if (a.heads > 4096 || a.q_heads > 65536 || a.page_size > 65536 || a.tokens > kMostTokens || a.num_seqs > (1 << 30))
+        return SQ_ERR_UNSUPPORTED;
+    if (!a.cu_seqlens && a.tokens != a.num_seqs) return SQ_ERR_ARGUMENT;
+    if (a.tokens == 0 || a.num_seqs == 0) return SQ_OK;
+    if (!a.q || !a.out || !a.lengths || (a.table_width && !a.page_table) || (a.num_pages && !a.data)) return SQ_ERR_ARGUMENT;
+    if (!a.workspace || a.workspace_bytes < sq_kv_attention_workspace_bytes(a.tokens, a.num_seqs, a.q_heads, a.heads, a.dim))
+        return SQ_ERR_CAPACITY;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const cudaError_t e = a.dtype == SQ_BF16 ? launch_attention<__nv_bfloat16>(a, s) : launch_attention<__half>(a, s);
+    return e == cudaSuccess ? SQ_OK : SQ_ERR_CUDA;
+}

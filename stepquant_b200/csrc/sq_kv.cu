@@ -1,0 +1,265 @@
+// Appending keys and values to the paged 4-bit cache, keys rotated on the way, and
+// reading them back.
+//
+// Eight neighbouring lanes hold a group of 64 channels of one token and head, eight
+// channels each: the group's extremes are three shuffles away, and a lane's codes are
+// one 32-bit word of the tile.  A code is that of the definition in exact arithmetic
+// (the extremes, the quotient and the rotation taken in 64 bits), so a token's bytes do
+// not depend on how it was appended.
+#include "sq_kv.cuh"
+#include "sq_rows.cuh"
+#include "sq_vec.cuh"
+
+namespace sq {
+namespace {
+
+constexpr int kKvThreads = 256;
+constexpr int kMostPerCta = 8;
+
+struct Place {
+    int64_t tile;  // byte offset of head 0's tile, -1: nowhere
+    int64_t position;
+    int token;
+};
+
+// Where new token i goes.
+__device__ __forceinline__ Place place_of(const sq_kv_args &a, int i, int tile_bytes) {
+    Place p{-1, 0, 0};
+    int n = i;
+    if (a.cu_seqlens) {
+        if (i < sequence_range(a.cu_seqlens, 0, a.tokens).x || i >= sequence_range(a.cu_seqlens, a.num_seqs - 1, a.tokens).y)
+            return p;
+        int lo = 0, hi = a.num_seqs - 1;  // the last sequence that begins at or before i: the ones between are empty
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (a.cu_seqlens[mid] <= i) lo = mid;
+            else hi = mid - 1;
+        }
+        n = lo;
+        const int2 r = sequence_range(a.cu_seqlens, n, a.tokens);
+        if (i >= r.y) return p;
+        p.position = int64_t(a.lengths[n]) - r.y + i;
+    } else {
+        p.position = int64_t(a.lengths[n]) - 1;
+    }
+    p.tile = tile_at(a.page_table + n * a.table_stride, a.table_width, a.num_pages, p.position, a.page_size, a.heads, 0, tile_bytes,
+                     a.status);
+    p.token = int(p.position & (kTile - 1));
+    return p;
+}
+
+// bf16 next to x towards -infinity, as its bits.
+__device__ __forceinline__ uint32_t bf16_down(double x) {
+    const uint32_t bits = __float_as_uint(__double2float_rd(x));
+    return (bits & 0x80000000u ? bits + 0xFFFFu : bits) >> 16;
+}
+__device__ __forceinline__ uint32_t bf16_up(double x) { return bf16_down(-x) ^ 0x8000u; }
+__device__ __forceinline__ float bf16_value(uint32_t bits) { return __uint_as_float(bits << 16); }
+
+__device__ __forceinline__ double least8(double x, uint32_t lanes) {
+#pragma unroll
+    for (int i = 1; i < 8; i *= 2) x = fmin(x, __shfl_xor_sync(lanes, x, i));
+    return x;
+}
+
+// Word and (s, m) of the group of which each of eight lanes holds x[0..7].
+__device__ __forceinline__ void quantize(const double (&x)[8], uint32_t lanes, uint32_t &word, uint32_t &pair) {
+    double low = x[0], high = -x[0];
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        low = fmin(low, x[i]);
+        high = fmin(high, -x[i]);
+        finite = finite && fabs(x[i]) <= 3.3895313892515355e38;  // the largest bf16; false for NaN
+    }
+    low = least8(low, lanes);
+    high = -least8(high, lanes);
+#pragma unroll
+    for (int i = 1; i < 8; i *= 2) finite = __shfl_xor_sync(lanes, int(finite), i) && finite;
+    if (!finite) {
+        word = 0;
+        pair = 0x7FC07FC0u;
+        return;
+    }
+    const uint32_t m = bf16_down(low);
+    const double base = bf16_value(m);
+    const uint32_t s = bf16_up((high - base) / 15);
+    const double step = s & 0x7FFF ? double(bf16_value(s)) : 1;
+    word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) word |= uint32_t(__double2int_rn((x[i] - base) / step)) << ((i >> 1) * 4 + (i & 1) * 16);
+    pair = (s & 0x7FFF) | (m << 16);
+}
+
+template <class T>
+__device__ __forceinline__ void load8(const T *p, bool wide, T (&x)[8]) {
+    if (wide) {
+#pragma unroll
+        for (int i = 0; i < int(sizeof(T)) / 2; ++i) reinterpret_cast<uint4 *>(x)[i] = reinterpret_cast<const uint4 *>(p)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = p[i];
+    }
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(kKvThreads) kv_append_kernel(sq_kv_args a, int per_cta, bool k_wide, bool v_wide) {
+    using Tile = KvTile<D>;
+    constexpr int kLanes = D / 8;  // of one head's keys or values
+    extern __shared__ double2 table[];  // [per_cta][turned / 2] (cos, sin), times the magnitude
+    __shared__ Place places[kMostPerCta];
+    const int64_t first = int64_t(blockIdx.x) * per_cta;
+    const int count = int(min(int64_t(per_cta), a.tokens - first)), half = a.turned / 2;
+    if (int(threadIdx.x) < count) places[threadIdx.x] = place_of(a, int(first) + threadIdx.x, Tile::kBytes);
+    __syncthreads();
+    for (int i = threadIdx.x; i < count * half; i += kKvThreads) {
+        const int t = i / half, f = i - t * half;
+        if (places[t].tile < 0) continue;
+        const int64_t position = a.positions ? position_at(a.positions, a.position_dtype, first + t) : places[t].position;
+        double sin, cos;
+        sincospi(double(phase_of(position, a.frequencies[f])) * 0x1p-63, &sin, &cos);
+        table[i] = make_double2(a.magnitude * cos, a.magnitude * sin);
+    }
+    __syncthreads();
+    const int lanes = a.heads * 2 * kLanes;  // of a token: a multiple of 16
+    const int64_t head_bytes = int64_t(a.page_size / kTile) * Tile::kBytes;
+    for (int i = threadIdx.x; i < count * lanes; i += kKvThreads) {
+        const uint32_t group_lanes = 0xFFu << (threadIdx.x & 24);
+        const int t = i / lanes, rest = i - t * lanes;
+        const int head = rest / (2 * kLanes), values = rest / kLanes & 1, lane = rest % kLanes;
+        const Place &p = places[t];
+        if (p.tile < 0) continue;
+        T raw[8];
+        double x[8];
+        const int c = lane * 8;
+        if (values) {
+            load8(static_cast<const T *>(a.v) + (first + t) * a.v_stride + head * a.v_head_stride + c, v_wide, raw);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = to_float(raw[e]);
+        } else {
+            const T *k = static_cast<const T *>(a.k) + (first + t) * a.k_stride + head * a.k_head_stride;
+            load8(k + c, k_wide, raw);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = to_float(raw[e]);
+            const double2 *cs = table + t * half;
+            if (a.interleaved) {
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    if (c + e >= a.turned) break;
+                    const double2 z = cs[(c + e) / 2];
+                    const double u = x[e], w = x[e + 1];
+                    x[e] = u * z.x - w * z.y;
+                    x[e + 1] = u * z.y + w * z.x;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (c + e >= a.turned) break;
+                    const bool upper = c + e >= half;
+                    const double other = to_float(k[upper ? c + e - half : c + e + half]);
+                    const double2 z = cs[upper ? c + e - half : c + e];
+                    x[e] = upper ? other * z.y + x[e] * z.x : x[e] * z.x - other * z.y;
+                }
+            }
+        }
+        uint32_t word, pair;
+        quantize(x, group_lanes, word, pair);
+        const int group = lane >> 3, w = lane & 7;
+        uint8_t *tile = a.data + p.tile + head * head_bytes;
+        *reinterpret_cast<uint32_t *>(tile + (values ? Tile::value_word(p.token, group, w) : Tile::key_word(p.token, group, w))) = word;
+        if (w == 0) *reinterpret_cast<uint32_t *>(tile + Tile::pair(values, p.token, group)) = pair;
+    }
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(kKvThreads) kv_read_kernel(sq_kv_args a, int per_cta) {
+    using Tile = KvTile<D>;
+    constexpr int kLanes = D / 8;
+    __shared__ Place places[kMostPerCta];
+    const int64_t first = int64_t(blockIdx.x) * per_cta;
+    const int count = int(min(int64_t(per_cta), a.tokens - first));
+    if (int(threadIdx.x) < count) places[threadIdx.x] = place_of(a, int(first) + threadIdx.x, Tile::kBytes);
+    __syncthreads();
+    const int lanes = a.heads * 2 * kLanes;
+    const int64_t head_bytes = int64_t(a.page_size / kTile) * Tile::kBytes;
+    for (int i = threadIdx.x; i < count * lanes; i += kKvThreads) {
+        const int t = i / lanes, rest = i - t * lanes;
+        const int head = rest / (2 * kLanes), values = rest / kLanes & 1, lane = rest % kLanes;
+        const Place &p = places[t];
+        alignas(16) T x[8];
+        if (p.tile < 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = from_float<T>(0.f);
+        } else {
+            const int group = lane >> 3, w = lane & 7;
+            const uint8_t *tile = a.data + p.tile + head * head_bytes;
+            const uint32_t word =
+                *reinterpret_cast<const uint32_t *>(tile + (values ? Tile::value_word(p.token, group, w) : Tile::key_word(p.token, group, w)));
+            const uint32_t pair = *reinterpret_cast<const uint32_t *>(tile + Tile::pair(values, p.token, group));
+            const float s = bf16_value(pair & 0xFFFF), m = bf16_value(pair >> 16);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = from_float<T>(fmaf(s, float(word >> ((e >> 1) * 4 + (e & 1) * 16) & 15), m));
+        }
+        T *out = values ? static_cast<T *>(a.v) + (first + t) * a.v_stride + head * a.v_head_stride
+                        : static_cast<T *>(a.k) + (first + t) * a.k_stride + head * a.k_head_stride;
+#pragma unroll
+        for (int e = 0; e < int(sizeof(T)) / 2; ++e) reinterpret_cast<uint4 *>(out + lane * 8)[e] = reinterpret_cast<uint4 *>(x)[e];
+    }
+}
+
+template <class T, int D>
+cudaError_t launch_kv(const sq_kv_args &a, bool append, cudaStream_t s) {
+    int per_cta = kMostPerCta;
+    while (per_cta > 1 && (int64_t(a.tokens) + per_cta - 1) / per_cta < 148 * 4) per_cta /= 2;
+    const unsigned grid = unsigned((int64_t(a.tokens) + per_cta - 1) / per_cta);
+    auto wide = [&](const void *p, int64_t token, int64_t head) {
+        constexpr int n = 16 / sizeof(T);
+        return aligned16(p) && token % n == 0 && head % n == 0;
+    };
+    const bool k_wide = wide(a.k, a.k_stride, a.k_head_stride), v_wide = wide(a.v, a.v_stride, a.v_head_stride);
+    if (append) {
+        kv_append_kernel<T, D><<<grid, kKvThreads, size_t(per_cta) * (a.turned / 2) * sizeof(double2), s>>>(a, per_cta, k_wide, v_wide);
+    } else {
+        if (!k_wide || !v_wide) return cudaErrorInvalidValue;
+        kv_read_kernel<T, D><<<grid, kKvThreads, 0, s>>>(a, per_cta);
+    }
+    return cudaGetLastError();
+}
+
+template <class T>
+cudaError_t launch_kv(const sq_kv_args &a, bool append, cudaStream_t s) {
+    switch (a.dim) {
+        case 64: return launch_kv<T, 64>(a, append, s);
+        case 128: return launch_kv<T, 128>(a, append, s);
+        default: return launch_kv<T, 256>(a, append, s);
+    }
+}
+
+int32_t kv_entry(const sq_kv_args *args, bool append, sq_stream_t stream) {
+    if (!args) return SQ_ERR_ARGUMENT;
+    const sq_kv_args &a = *args;
+    if (a.tokens < 0 || a.num_seqs < 0 || a.table_width < 0 || a.num_pages < 0 || a.heads < 1 || a.turned < 0) return SQ_ERR_ARGUMENT;
+    if (a.dtype < SQ_F32 || a.dtype > SQ_F16) return SQ_ERR_ARGUMENT;
+    if (a.dim != 64 && a.dim != 128 && a.dim != 256) return SQ_ERR_UNSUPPORTED;
+    if (a.page_size < kTile || a.page_size % kTile || a.turned % 2 || a.turned > a.dim || a.table_stride < 0) return SQ_ERR_SHAPE;
+    if (a.k_stride < 0 || a.k_head_stride < 0 || a.v_stride < 0 || a.v_head_stride < 0 || !aligned16(a.data)) return SQ_ERR_SHAPE;
+    if (a.heads > 4096 || a.page_size > 65536 || a.tokens > kMostTokens || a.num_seqs > (1 << 30)) return SQ_ERR_UNSUPPORTED;
+    if (!a.cu_seqlens && a.tokens != a.num_seqs) return SQ_ERR_ARGUMENT;
+    if (a.tokens == 0) return SQ_OK;
+    if (!a.k || !a.v || (a.num_seqs && (!a.lengths || (a.table_width && !a.page_table) || (a.num_pages && !a.data)))) return SQ_ERR_ARGUMENT;
+    if (append && a.turned && !a.frequencies) return SQ_ERR_ARGUMENT;
+    if (!append && (!aligned16(a.k) || !aligned16(a.v) || (a.k_stride | a.k_head_stride | a.v_stride | a.v_head_stride) % 8)) return SQ_ERR_SHAPE;
+    if (append && a.num_seqs == 0) return SQ_OK;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const cudaError_t e = a.dtype == SQ_F32    ? launch_kv<float>(a, append, s)
+                          : a.dtype == SQ_BF16 ? launch_kv<__nv_bfloat16>(a, append, s)
+                                               : launch_kv<__half>(a, append, s);
+    return e == cudaSuccess ? SQ_OK : SQ_ERR_CUDA;
+}
+
+}  // namespace
+}  // namespace sq
+
+extern "C" int32_t sq_kv_append(const sq_kv_args *args, sq_stream_t stream) { return sq::kv_entry(args, true, stream); }
+
+extern "C" int32_t sq_kv_read(const sq_kv_args *args, sq_stream_t stream) { return sq::kv_entry(args, false, stream); }

@@ -59,6 +59,12 @@ __device__ __forceinline__ void tma_load(void *dst, const CUtensorMap *map, int 
                  ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
 }
 
+// `bytes` (a multiple of 16) from src to dst, both 16-byte aligned, completing on `bar`.
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
 // K-major operand tile of 128-byte rows under the 128-byte swizzle, 8-row groups of 1024 bytes.
 __device__ __forceinline__ uint64_t operand(uint32_t addr) {
     return uint64_t((addr >> 4) & 0x3FFF) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);

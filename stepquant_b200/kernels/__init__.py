@@ -12,4 +12,9 @@ The operators around the recurrent state of a layer:
 ``matmul``     product of e4m3 matrices with block scales.
 ``conv``       short causal convolution, for prompts and single tokens.
 ``scan``       selective state space scan, its single-token form and state pool.
+
+and those of the attention layers that stand between recurrent ones:
+
+``rotary``     rotary positions.
+``kv_cache``   paged cache of keys and values in 4 bits, and attention over it.
 """
