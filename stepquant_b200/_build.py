@@ -17,7 +17,8 @@ LIBRARY = os.path.join(LIBDIR, "libstepquant_b200.so")
 HEADER = os.path.join(ROOT, "include", "stepquant_b200.h")
 SOURCES = ["sq_abi.cu", "sq_tile.cu", "sq_fast.cu", "sq_pack.cu", "sq_fp32.cu", "sq_noalloc.cu", "sq_prefill.cu",
            "sq_fast_kda.cu", "sq_streams.cu", "sq_fast_two.cu", "sq_prefill_kda.cu", "sq_norm.cu", "sq_conv.cu",
-           "sq_scan.cu", "sq_matmul.cu", "sq_rotary.cu", "sq_kv.cu", "sq_attention.cu"]
+           "sq_scan.cu", "sq_matmul.cu", "sq_rotary.cu", "sq_kv.cu", "sq_attention.cu",
+           "sq_attention_prompt.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -29,7 +30,7 @@ NVCC_FLAGS = [
 # reference fit_state; intended FMAs are written as fmaf()).  The chunked
 # prefill passes and the layer operators are toleranced and are built with contraction.
 CONTRACT = {"sq_prefill.cu", "sq_prefill_kda.cu", "sq_norm.cu", "sq_conv.cu", "sq_scan.cu", "sq_matmul.cu", "sq_rotary.cu",
-            "sq_kv.cu", "sq_attention.cu"}
+            "sq_kv.cu", "sq_attention.cu", "sq_attention_prompt.cu"}
 
 
 def _nvcc():

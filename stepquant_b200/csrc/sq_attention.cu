@@ -12,11 +12,15 @@
 #include "sq_vec.cuh"
 
 namespace sq {
+
+cudaError_t launch_prompt_attention(const sq_kv_attention_args &a, int few_rows, cudaStream_t s);  // sq_attention_prompt.cu
+
 namespace {
 
 constexpr int kWarps = 8, kAttnThreads = 32 * kWarps;
 constexpr int kMostCtas = 320;
 constexpr int kLeastTiles = 2 * kWarps;  // of a CTA
+constexpr int kFewRows = 32;
 
 // ---------------------------------------------------------------------------
 // fragments
@@ -96,7 +100,7 @@ struct Sequence {
 };
 
 template <int ROWS>
-__device__ __forceinline__ Sequence sequence(const sq_kv_attention_args &a, int n, bool report) {
+__device__ __forceinline__ Sequence sequence(const sq_kv_attention_args &a, int most_rows, int n, bool report) {
     Sequence s;
     const int2 r = a.cu_seqlens ? sequence_range(a.cu_seqlens, n, a.tokens) : make_int2(n, n + 1);
     s.first = r.x;
@@ -109,7 +113,8 @@ __device__ __forceinline__ Sequence sequence(const sq_kv_attention_args &a, int 
     const int64_t start = a.window > 0 ? max(int64_t(0), s.before - a.window + 1) : 0;
     s.tile = int(min(start, int64_t(s.length)) / kTile);
     s.tiles = max(1, (s.length + kTile - 1) / kTile - s.tile);
-    s.blocks = int((int64_t(s.count) * (a.q_heads / a.heads) + ROWS - 1) / ROWS);
+    const int64_t rows = int64_t(s.count) * (a.q_heads / a.heads);
+    s.blocks = rows > most_rows ? 0 : int((rows + ROWS - 1) / ROWS);
     s.cost = int64_t(s.blocks) * a.heads * s.tiles;
     return s;
 }
@@ -122,14 +127,14 @@ struct Span {
 
 // This CTA's span (begin = end: none).  Every thread of the CTA calls it.
 template <int ROWS>
-__device__ __forceinline__ Span span_of(const sq_kv_attention_args &a, bool report) {
+__device__ __forceinline__ Span span_of(const sq_kv_attention_args &a, int most_rows, bool report) {
     __shared__ int64_t warp_sums[kWarps];
     __shared__ int64_t found_offset;
     __shared__ int found;
     const int each = (a.num_seqs + kAttnThreads - 1) / kAttnThreads;
     const int from = min(int(threadIdx.x) * each, a.num_seqs), to = min(from + each, a.num_seqs);
     int64_t mine = 0;
-    for (int n = from; n < to; ++n) mine += sequence<ROWS>(a, n, report).cost;
+    for (int n = from; n < to; ++n) mine += sequence<ROWS>(a, most_rows, n, report).cost;
     int64_t sum = mine;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -153,7 +158,7 @@ __device__ __forceinline__ Span span_of(const sq_kv_attention_args &a, bool repo
     int64_t at = sum - mine;
     if (s.begin < s.end && at <= s.begin && s.begin < sum) {
         for (int n = from; n < to; ++n) {
-            const int64_t cost = sequence<ROWS>(a, n, false).cost;
+            const int64_t cost = sequence<ROWS>(a, most_rows, n, false).cost;
             if (s.begin < at + cost) {
                 found = n;
                 found_offset = s.begin - at;
@@ -190,7 +195,7 @@ struct RowsShape {
 };
 
 template <class T, int D, int NT>
-__global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) rows_kernel(sq_kv_attention_args a) {
+__global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) rows_kernel(sq_kv_attention_args a, int most_rows) {
     using Shape = RowsShape<D, NT>;
     using Tile = KvTile<D>;
     using C = Codes<T>;
@@ -208,17 +213,17 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
     }
     if (a.cu_seqlens)
         clear_outside(a.out, int64_t(a.q_heads) * D * sizeof(T), a.cu_seqlens, a.num_seqs, a.tokens, blockIdx.x, gridDim.x);
-    const Span span = span_of<kRows>(a, blockIdx.x == 0);
+    const Span span = span_of<kRows>(a, most_rows, blockIdx.x == 0);
     const int group = a.q_heads / a.heads, page_tiles = a.page_size / kTile;
     const float to_log2 = a.scale * kLog2e;
     const int64_t head_bytes = int64_t(page_tiles) * Tile::kBytes;
     uint32_t used = 0;  // of this warp's stages, ever
     int n = span.sequence;
     int64_t offset = span.offset;
-    Sequence seq = sequence<kRows>(a, min(n, a.num_seqs - 1), false);
+    Sequence seq = sequence<kRows>(a, most_rows, min(n, a.num_seqs - 1), false);
     for (int64_t at = span.begin; at < span.end;) {
         while (offset >= seq.cost) {  // on to the next sequence with new tokens: there is one, as at < span.end
-            seq = sequence<kRows>(a, ++n, false);
+            seq = sequence<kRows>(a, most_rows, ++n, false);
             offset = 0;
         }
         const int64_t item = offset / seq.tiles;
@@ -459,6 +464,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
             if (i + kStages < mine) request(i + kStages);
         }
         used += mine;
+        gave_up = __any_sync(~0u, gave_up);
         if (gave_up) {  // the copies still on their way end before the ring is used again
             flag(a.status, SQ_STATUS_TIMEOUT);
             int alone = 0;
@@ -531,16 +537,16 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
 
 // Joins the parts of items that several CTAs had: the CTA in whose span one ends.
 template <class T, int D, int NT>
-__global__ void __launch_bounds__(kAttnThreads) join_kernel(sq_kv_attention_args a) {
+__global__ void __launch_bounds__(kAttnThreads) join_kernel(sq_kv_attention_args a, int most_rows) {
     using Shape = RowsShape<D, NT>;
     using C = Codes<T>;
     constexpr int kRows = Shape::kRows;
     extern __shared__ float factors[];  // [parts][rows]
     __shared__ float weights[kRows];
-    const Span span = span_of<kRows>(a, false);
+    const Span span = span_of<kRows>(a, most_rows, false);
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     if (span.begin >= span.end) return;
-    const Sequence seq = sequence<kRows>(a, span.sequence, false);
+    const Sequence seq = sequence<kRows>(a, most_rows, span.sequence, false);
     const int done = int(span.offset % seq.tiles);  // tiles of the item before this span
     if (done == 0 || seq.tiles - done > span.end - span.begin) return;
     const int64_t item = span.offset / seq.tiles, start = span.begin - done, cta0 = start / span.per;
@@ -587,7 +593,7 @@ __global__ void __launch_bounds__(kAttnThreads) join_kernel(sq_kv_attention_args
 }
 
 template <class T, int D, int NT>
-cudaError_t launch_rows(const sq_kv_attention_args &a, cudaStream_t s) {
+cudaError_t launch_rows(const sq_kv_attention_args &a, int most_rows, cudaStream_t s) {
     using Shape = RowsShape<D, NT>;
     const int sms = sms_of(s);
     if (sms < 1) return cudaErrorInvalidDevice;
@@ -595,7 +601,7 @@ cudaError_t launch_rows(const sq_kv_attention_args &a, cudaStream_t s) {
     const unsigned grid = unsigned(sms * resident < kMostCtas ? sms * resident : kMostCtas);
     cudaError_t e = cudaFuncSetAttribute(rows_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kShared);
     if (e != cudaSuccess) return e;
-    rows_kernel<T, D, NT><<<grid, kAttnThreads, Shape::kShared, s>>>(a);
+    rows_kernel<T, D, NT><<<grid, kAttnThreads, Shape::kShared, s>>>(a, most_rows);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
@@ -608,7 +614,7 @@ cudaError_t launch_rows(const sq_kv_attention_args &a, cudaStream_t s) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, join_kernel<T, D, NT>, a);
+    return cudaLaunchKernelEx(&cfg, join_kernel<T, D, NT>, a, most_rows);
 }
 
 // Blocks of 16 rows where sequences have more than 8 (heads of 256 channels: their sums leave no room).
@@ -617,13 +623,23 @@ bool wide_rows(int tokens, int seqs, int q_heads, int heads, int dim) {
 }
 
 template <class T>
-cudaError_t launch_attention(const sq_kv_attention_args &a, cudaStream_t s) {
+cudaError_t launch_rows(const sq_kv_attention_args &a, int most_rows, cudaStream_t s) {
     const bool wide = wide_rows(a.tokens, a.num_seqs, a.q_heads, a.heads, a.dim);
     switch (a.dim) {
-        case 64: return wide ? launch_rows<T, 64, 2>(a, s) : launch_rows<T, 64, 1>(a, s);
-        case 128: return wide ? launch_rows<T, 128, 2>(a, s) : launch_rows<T, 128, 1>(a, s);
-        default: return launch_rows<T, 256, 1>(a, s);
+        case 64: return wide ? launch_rows<T, 64, 2>(a, most_rows, s) : launch_rows<T, 64, 1>(a, most_rows, s);
+        case 128: return wide ? launch_rows<T, 128, 2>(a, most_rows, s) : launch_rows<T, 128, 1>(a, most_rows, s);
+        default: return launch_rows<T, 256, 1>(a, most_rows, s);
     }
+}
+
+// Sequences of up to kFewRows rows (new tokens times query heads of a kv head) go through rows_kernel, those
+// of more through the prompts' kernel, each decided on the device: a batch may have both.
+cudaError_t launch_attention(const sq_kv_attention_args &a, cudaStream_t s) {
+    const int group = a.q_heads / a.heads;
+    const bool prompts = a.cu_seqlens && group <= 128 && int64_t(a.tokens) * group > kFewRows;
+    const int most_rows = prompts ? kFewRows : 0x7fffffff;
+    const cudaError_t e = a.dtype == SQ_BF16 ? launch_rows<__nv_bfloat16>(a, most_rows, s) : launch_rows<__half>(a, most_rows, s);
+    return e == cudaSuccess && prompts ? launch_prompt_attention(a, kFewRows, s) : e;
 }
 
 }  // namespace
@@ -655,6 +671,5 @@ extern "C" int32_t sq_kv_attention(const sq_kv_attention_args *args, sq_stream_t
     if (!a.workspace || a.workspace_bytes < sq_kv_attention_workspace_bytes(a.tokens, a.num_seqs, a.q_heads, a.heads, a.dim))
         return SQ_ERR_CAPACITY;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    const cudaError_t e = a.dtype == SQ_BF16 ? launch_attention<__nv_bfloat16>(a, s) : launch_attention<__half>(a, s);
-    return e == cudaSuccess ? SQ_OK : SQ_ERR_CUDA;
+    return launch_attention(a, s) == cudaSuccess ? SQ_OK : SQ_ERR_CUDA;
 }

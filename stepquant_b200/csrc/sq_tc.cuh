@@ -1,4 +1,5 @@
-// tcgen05, TMA and mbarrier wrappers of the block-scaled product (sq_matmul.cu).
+// tcgen05, TMA and mbarrier wrappers of the block-scaled product (sq_matmul.cu) and of prompts' attention
+// (sq_attention_prompt.cu).
 #pragma once
 
 #include <cuda.h>
@@ -76,6 +77,29 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uin
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)) : "memory");
 }
+// 16-bit operands -> fp32, M = 128: both f16 or both bf16; B K-major, or MN-major (its rows are K).
+__device__ __forceinline__ constexpr uint32_t half_product(int n, bool bf16, bool b_mn) {
+    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(b_mn) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+}
+// Operand tile of 128-byte rows (64 values) under the 128-byte swizzle whose rows are K: `lead` bytes to
+// the next 64 values.
+__device__ __forceinline__ uint64_t operand_mn(uint32_t addr, uint32_t lead) {
+    return uint64_t((addr >> 4) & 0x3FFF) | (uint64_t(lead >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// K-major operand tile of 16 values of K without a swizzle: two pieces of 16 bytes a row, `lead` bytes
+// apart, each 8 rows of them contiguous.
+__device__ __forceinline__ uint64_t operand_narrow(uint32_t addr, uint32_t lead) {
+    return uint64_t((addr >> 4) & 0x3FFF) | (uint64_t(lead >> 4) << 16) | (uint64_t(128 >> 4) << 32) | (1ull << 46);
+}
+__device__ __forceinline__ void mma_half(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)) : "memory");
+}
+// A in tensor memory: lanes are its rows, a column holds two values of K.
+__device__ __forceinline__ void mma_half_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)) : "memory");
+}
 __device__ __forceinline__ void mma_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -100,6 +124,27 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[16]) {
                    "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(addr));
 }
+#define SQ_R8(i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define SQ_W8(i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+                 : SQ_R8(0), SQ_R8(8), SQ_R8(16), SQ_R8(24) : "r"(addr));
+}
+// Stores are in tensor memory after tmem_stored().
+__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n"
+                 ::"r"(addr), SQ_W8(0), SQ_W8(8), SQ_W8(16), SQ_W8(24) : "memory");
+}
+__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n"
+                 ::"r"(addr), SQ_W8(0), SQ_W8(8) : "memory");
+}
+#undef SQ_R8
+#undef SQ_W8
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+
 // The registers pass through the wait, so that no use of theirs moves before it.
 template <int N>
 __device__ __forceinline__ void tmem_wait(uint32_t (&r)[N]) {
