@@ -212,7 +212,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(sq_kv_attenti
     auto wait_alone = [&](uint64_t *bar, uint32_t parity) { return tc::bar_wait(bar, parity, &abort_flag, tc::kWaitClocks); };
     auto wait = [&](uint64_t *bar, uint32_t parity) { return bool(__all_sync(~0u, wait_alone(bar, parity))); };  // of a whole warp
 
-    float top = -INFINITY, sum = 0.f;  // of a row
+    float top = -INFINITY;  // of a row
+    float2 sum = make_float2(0.f, 0.f);  // of its weights, in two parts
     if (warp < Shape::kSoftmaxWarps) {
         const int tile = warp >> 2, row = threadIdx.x & 127, index = tile * 128 + row;
         if (tile < live) {
@@ -286,21 +287,32 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(sq_kv_attenti
                     for (int i = 0; i < kKeys / kTile; ++i)
                         if (prompt_tile<D>(a, item, int(begin) + i * kTile) < 0) hole |= 1u << i;
                 const bool whole = __all_sync(~0u, high >= kKeys - 1 && low < 0 && hole == 0);
-                auto seen = [&](int c) { return c <= high && c > low && !(hole >> (c / kTile) & 1); };
-                uint32_t s[32];
+                // Scores c .. c + 31, those that are not seen -infinity.
+                auto hide = [&](uint32_t (&s)[32], int c) {
+                    const int h = min(high - c, 31), l = min(low - c, 31);
+                    uint32_t bits = h < 0 ? 0u : (2u << h) - 1u;
+                    if (l >= 0) bits &= ~((2u << l) - 1u);
+                    if (hole >> (c / kTile) & 1) bits &= 0xFFFF0000u;
+                    if (hole >> (c / kTile + 1) & 1) bits &= 0x0000FFFFu;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) s[i] = bits >> i & 1 ? s[i] : 0xFF800000u;
+                };
+                uint32_t s[2][32];
                 float most = -INFINITY;
+                auto maximum = [&](uint32_t (&s)[32], int c) {
+                    if (!whole) hide(s, c);
 #pragma unroll
-                for (int c = 0; c < kKeys; c += 32) {
-                    tc::tmem_load(scores + c, s);
-                    tc::tmem_wait(s);
-                    if (whole) {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) most = fmaxf(most, fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 1])));
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (seen(c + i)) most = fmaxf(most, __uint_as_float(s[i]));
-                    }
+                    for (int i = 0; i < 32; i += 2) most = fmaxf(most, fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 1])));
+                };
+                tc::tmem_load(scores, s[0]);
+#pragma unroll 1
+                for (int c = 0; c < kKeys; c += 64) {  // 32 columns are on their way while 32 are worked on
+                    tc::tmem_wait(s[0]);
+                    tc::tmem_load(scores + c + 32, s[1]);
+                    maximum(s[0], c);
+                    tc::tmem_wait(s[1]);
+                    tc::tmem_load(scores + (c + 64) % kKeys, s[0]);
+                    maximum(s[1], c + 32);
                 }
                 most *= to_log2;
                 const bool grows = most > top + kPromptLag;
@@ -309,41 +321,46 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(sq_kv_attenti
                 if (__any_sync(~0u, grows)) {
                     const float change = grows ? exp2_approx(top - most) : 1.f;
                     top = grows ? most : top;
-                    sum *= change;
+                    sum.x *= change;
+                    sum.y *= change;
                     if (j > 0) {
                         ok = wait(&bars.sums[tile], (j - 1) & 1);
                         if (!ok) break;
                         waited = true;
                         tc::fence_after();
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < D; c += 32) {
-                            tc::tmem_load(sums + c, s);
-                            tc::tmem_wait(s);
+                            tc::tmem_load(sums + c, s[1]);
+                            tc::tmem_wait(s[1]);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * change);
-                            tc::tmem_store(sums + c, s);
+                            for (int i = 0; i < 32; ++i) s[1][i] = __float_as_uint(__uint_as_float(s[1][i]) * change);
+                            tc::tmem_store(sums + c, s[1]);
                         }
+                        tc::tmem_load(scores, s[0]);  // again: the wait above was for it too
                     }
                 }
-                const float against = top == -INFINITY ? 0.f : top;
-#pragma unroll
-                for (int c = 0; c < kKeys; c += 32) {
-                    tc::tmem_load(scores + c, s);
-                    tc::tmem_wait(s);
+                const float against = top == -INFINITY ? 0.f : -top;
+                auto weigh = [&](uint32_t (&s)[32], int c) {
+                    if (!whole) hide(s, c);
                     uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
                         const float2 z = fma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(to_log2, to_log2),
-                                              make_float2(-against, -against));
-                        float x = exp2_approx(z.x), y = exp2_approx(z.y);
-                        if (!whole) {
-                            x = seen(c + i) ? x : 0.f;
-                            y = seen(c + i + 1) ? y : 0.f;
-                        }
-                        sum += x + y;
-                        p[i / 2] = pack2<__half>(x, y);
+                                              make_float2(against, against));
+                        const float2 w = make_float2(exp2_approx(z.x), exp2_approx(z.y));
+                        sum = add2(sum, w);
+                        p[i / 2] = pack2<__half>(w.x, w.y);
                     }
                     tc::tmem_store(scores + c / 2, p);
+                };
+#pragma unroll 1
+                for (int c = 0; c < kKeys; c += 64) {
+                    tc::tmem_wait(s[0]);
+                    tc::tmem_load(scores + c + 32, s[1]);
+                    weigh(s[0], c);
+                    tc::tmem_wait(s[1]);
+                    if (c + 64 < kKeys) tc::tmem_load(scores + c + 64, s[0]);
+                    weigh(s[1], c + 32);
                 }
                 tc::tmem_stored();
                 if (!waited) {
@@ -370,7 +387,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(sq_kv_attenti
                         }
                     }
                 }
-                const float per = sum == 0.f ? 0.f : 1.f / (sum * value_factor);
+                const float weight = sum.x + sum.y, per = weight == 0.f ? 0.f : 1.f / (weight * value_factor);
                 T *out = static_cast<T *>(a.out) + (int64_t(item.first + token) * a.q_heads + item.head * group + (mine ? index % group : 0)) * D;
 #pragma unroll
                 for (int c = 0; c < D; c += 32) {
@@ -401,22 +418,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(sq_kv_attenti
         // Codes into 16-bit operands: a piece of 16 bytes holds four words of one token.
         const int thread = threadIdx.x - 32 * Shape::kSoftmaxWarps;
         constexpr int kPieces = Shape::kPieces, kPerTile = D / 2;  // pieces of a tile's keys or values
-        int64_t at[kPieces];
         uint4 words[2][kPieces];
         uint32_t pairs[2][kPieces][4];
-        // Piece i of this thread: tile, token of it, and which of the token's pieces.
-        auto locate = [&](int j) {
-            bool hole = false;
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                const int key = item.start + j * kKeys + (i * Shape::kUnpackThreads + thread) / kPerTile * kTile;
-                at[i] = prompt_tile<D>(a, item, key);
-                hole = hole || (at[i] < 0 && key < item.length);
-            }
-            if (hole) holes[j & 3] = j + 1;
+        // Lane i has the place of tile i of a block, which is looked up a block ahead.
+        auto places = [&](int j) {
+            const int key = item.start + j * kKeys + lane * kTile;
+            const int64_t at = lane < kKeys / kTile && j < item.blocks ? prompt_tile<D>(a, item, key) : 0;
+            if (at < 0 && key < item.length) holes[j & 3] = j + 1;
+            return at;
         };
         // Key pieces by (token, block of channels, quarter), value pieces by (token, block of 32 bytes, half).
-        auto load = [&](int j, bool value) {
+        auto load = [&](int j, int64_t place, bool value) {
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
                 const int piece = (i * Shape::kUnpackThreads + thread) % kPerTile;
@@ -426,8 +438,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(sq_kv_attenti
                 w = make_uint4(0, 0, 0, 0);
 #pragma unroll
                 for (int b = 0; b < 4; ++b) pairs[value][i][b] = 0;
-                if (at[i] < 0) continue;
-                const uint8_t *tile = a.data + at[i];
+                const int64_t at = __shfl_sync(~0u, place, (i * Shape::kUnpackThreads + thread) / kPerTile);
+                if (at < 0) continue;
+                const uint8_t *tile = a.data + at;
                 const int row = Tile::row(token);
                 if (value) {
                     w = *reinterpret_cast<const uint4 *>(tile + Tile::kValues + (part >> 1) * kTile * 32 + token * 32 + (part & 1) * 16);
@@ -495,20 +508,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(sq_kv_attenti
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
         };
-        if (item.blocks > 0) {
-            locate(0);
-            load(0, false);
-        }
+        int64_t place = places(0), next_place;
+        if (item.blocks > 0) load(0, place, false);
+#pragma unroll 1
         for (int j = 0; j < item.blocks; ++j) {
             const int stage = j & 1;
-            load(j, true);
+            load(j, place, true);
+            next_place = places(j + 1);
             if (j > 1 && !wait(&bars.keys_free[stage], ((j >> 1) - 1) & 1)) break;
             write(keys + stage * Shape::kKeyBytes, more_keys + stage * Shape::kMoreKey, false);
             if (lane == 0) tc::bar_arrive(&bars.keys[stage]);
-            if (j + 1 < item.blocks) {
-                locate(j + 1);
-                load(j + 1, false);
-            }
+            place = next_place;
+            if (j + 1 < item.blocks) load(j + 1, place, false);
             if (j > 1 && !wait(&bars.values_free[stage], ((j >> 1) - 1) & 1)) break;
             write(values + stage * Shape::kKeyBytes, nullptr, true);
             if (lane == 0) tc::bar_arrive(&bars.values[stage]);

@@ -46,6 +46,11 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
     return reinterpret_cast<float2 &>(r);
 }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return reinterpret_cast<float2 &>(r);
+}
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     uint64_t r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;"
