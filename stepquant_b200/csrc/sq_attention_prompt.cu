@@ -2,11 +2,14 @@
 //
 // A CTA takes 256 query rows of one kv head, (token, query head) pairs, in two tiles of
 // 128 (heads of 256 channels: one tile, as its sums fill the tensor memory), and walks
-// the keys in blocks of 128 (64).  Per block:
-//   four warps (eight) write out the codes as 16-bit keys and values in shared memory,
-//   one thread issues S = Q K^T and O += P V, S, P and O in tensor memory,
+// the keys in blocks of 64.  Per block:
+//   eight warps (four for heads of 64) write out the codes as 16-bit keys and values in
+//   shared memory, two to four blocks ahead,
+//   one warp issues S = Q K^T and O += P V, S, P and O in tensor memory,
 //   four warps a tile, a thread to a row, turn S into P, which overwrites it.
-// While a tile's S becomes P, the other tile's products run (one tile: the next block's S).
+// S and P have two buffers a tile: the next block's S is ready when this block's P is.
+// (Blocks of 128 keys with one buffer left S waiting for O += P V: 1418 us for 4096 tokens
+// over 16384 of 32 heads.)
 // Scores take keys as they are held: s (c - 8) has 3 + 8 significant bits and so is an f16,
 // and the rest of a group, m + 8 s, meets the sum of the query's channels in one more step
 // of K (the sum's f16 and its remainder, each by m and by 8 s).  Queries are f16 with each
@@ -24,7 +27,6 @@
 namespace sq {
 namespace {
 
-constexpr int kPromptThreads = 13 * 32;
 constexpr float kKeyDivisor = 16.f;
 constexpr float kPromptLag = 8.f;
 
@@ -32,44 +34,58 @@ template <int D>
 struct PromptShape {
     using Tile = KvTile<D>;
     static constexpr int kTiles = D == 256 ? 1 : 2;             // of 128 rows
-    static constexpr int kKeys = D == 256 ? 64 : 128;           // of a block
-    static constexpr int kSoftmaxWarps = 4 * kTiles, kUnpackThreads = 32 * (12 - kSoftmaxWarps);
+    static constexpr int kKeys = 64;                            // of a block
+    static constexpr int kStages = D == 256 ? 2 : 4;
+    static constexpr int kSoftmaxWarps = 4 * kTiles, kUnpackWarps = D == 64 ? 4 : 8, kProductWarp = kSoftmaxWarps + kUnpackWarps;
+    static constexpr int kUnpackThreads = 32 * kUnpackWarps, kThreads = 32 * (kProductWarp + 1);
     static constexpr int kQueryBytes = 128 * D * 2, kKeyBytes = kKeys * D * 2;
     static constexpr int kMoreQuery = 128 * 32, kMoreKey = kKeys * 32;  // the last step of K: 16 values a row
-    static constexpr int kShared = kTiles * (kQueryBytes + kMoreQuery) + 4 * kKeyBytes + 2 * kMoreKey + 1024;
-    static constexpr int kColumnsO = 2 * kKeys;                 // S, P: [0, 2 kKeys)
+    static constexpr int kShared = kTiles * (kQueryBytes + kMoreQuery) + kStages * (2 * kKeyBytes + kMoreKey) + 1024;
+    static constexpr int kColumnsO = kTiles * 2 * kKeys;        // S, P: [0, kColumnsO), two buffers a tile
     static constexpr int kPieces = kKeys * D / 32 / kUnpackThreads;  // 16-byte pieces of a block's keys for a thread
-    static_assert(kColumnsO + kTiles * D <= 512 && kPieces * kUnpackThreads * 32 == kKeys * D, "");
+    static_assert(kColumnsO + kTiles * D <= 512 && kPieces * kUnpackThreads * 32 == kKeys * D && kShared <= 227 * 1024, "");
+    static_assert((kStages & (kStages - 1)) == 0 && kStages <= 4, "");
 };
 
 struct PromptBars {
-    uint64_t query, keys[2], keys_free[2], values[2], values_free[2], scores[2], weights[2], sums[2], end;
+    uint64_t query, keys[4], keys_free[4], values[4], values_free[4];  // by stage
+    uint64_t scores[4], weights[4], sums[4];                           // by tile and block modulo 2
+    uint64_t end;
 };
 
-// Codes of 8 channels as f16 pairs (c - 8) s, or as pairs c s + m.
-__device__ __forceinline__ uint4 unpack_middle(uint32_t w, __half2 s) {
+// Codes of 8 channels as f16 pairs (c - 8) s, exactly: in the top of the mantissa a code makes 16 + c, and
+// 24 s has 10 significant bits.
+__device__ __forceinline__ uint4 unpack_middle(uint32_t w, __half2 s, __half2 less_24s) {
     uint32_t r[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t x = ((w >> (4 * i)) & 0x000F000Fu) | 0x64006400u, base = 0x64086408u;  // 1024 + c less 1032
-        const __half2 v = __hmul2(__hsub2(reinterpret_cast<const __half2 &>(x), reinterpret_cast<const __half2 &>(base)), s);
+        const uint32_t x = ((i < 2 ? w << (6 - 4 * i) : w >> (4 * i - 6)) & 0x03C003C0u) | 0x4C004C00u;
+        const __half2 v = __hfma2(reinterpret_cast<const __half2 &>(x), s, less_24s);
         r[i] = reinterpret_cast<const uint32_t &>(v);
     }
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
-__device__ __forceinline__ uint4 unpack_f16(uint32_t w, __half2 s, __half2 m) {
+// Codes of 8 channels as f16 pairs c s + m: 1024 + c and, from the next four bits, 1024 + 16 c, less 1024.
+__device__ __forceinline__ uint4 unpack_value(uint32_t w, __half2 s, __half2 s16, __half2 m) {
     uint32_t r[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t x = ((w >> (4 * i)) & 0x000F000Fu) | 0x64006400u, base = 0x64006400u;
+        const uint32_t x = ((i < 2 ? w : w >> 8) & (i & 1 ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u, base = 0x64006400u;
         const __half2 c = __hsub2(reinterpret_cast<const __half2 &>(x), reinterpret_cast<const __half2 &>(base));
-        const __half2 v = __hfma2(c, s, m);
+        const __half2 v = __hfma2(c, i & 1 ? s16 : s, m);
         r[i] = reinterpret_cast<const uint32_t &>(v);
     }
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
+
 __device__ __forceinline__ float low_bf16(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float high_bf16(uint32_t p) { return __uint_as_float(p & 0xFFFF0000u); }
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 
 template <class T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
@@ -116,19 +132,19 @@ __device__ __forceinline__ int64_t prompt_tile(const sq_kv_attention_args &a, co
 }
 
 template <class T, int D>
-__global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(sq_kv_attention_args a, int tokens_per_item, unsigned strips, int few_rows) {
+__global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_kv_attention_args a, int tokens_per_item, unsigned strips, int few_rows) {
     using Shape = PromptShape<D>;
     using Tile = KvTile<D>;
-    constexpr int kTiles = Shape::kTiles, kKeys = Shape::kKeys, kGroups = Tile::kGroups;
+    constexpr int kTiles = Shape::kTiles, kKeys = Shape::kKeys, kStages = Shape::kStages, kGroups = Tile::kGroups;
     extern __shared__ uint8_t raw[];
     __shared__ PromptBars bars;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, bad_values;
     __shared__ unsigned most_value;
-    __shared__ volatile int holes[4];  // block + 1 of the last one with tiles to leave out, by block modulo 4
+    __shared__ volatile int holes[8];  // block + 1 of the last one with tiles to leave out, by block modulo 8
     uint8_t *const queries = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *const keys = queries + kTiles * Shape::kQueryBytes, *const values = keys + 2 * Shape::kKeyBytes;
-    uint8_t *const more_queries = values + 2 * Shape::kKeyBytes, *const more_keys = more_queries + kTiles * Shape::kMoreQuery;
+    uint8_t *const keys = queries + kTiles * Shape::kQueryBytes, *const values = keys + kStages * Shape::kKeyBytes;
+    uint8_t *const more_queries = values + kStages * Shape::kKeyBytes, *const more_keys = more_queries + kTiles * Shape::kMoreQuery;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = a.q_heads / a.heads;
 
@@ -144,7 +160,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(sq_kv_attenti
         const int64_t token = (int64_t(strip) - (int64_t(r.x) / tokens_per_item + n)) * tokens_per_item;
         if (token < 0 || token >= item.count || int64_t(item.count) * group <= few_rows) return;
         item.token = int(token);
-        const int tokens = min(tokens_per_item, item.count - item.token);
+        // (min() of two ints here came out as tokens_per_item with 17 warps: nvcc 12.9.)
+        const int64_t left = item.count - token;
+        const int tokens = left < tokens_per_item ? int(left) : tokens_per_item;
         item.rows = tokens * group;
         const int64_t length = a.lengths[n], most = int64_t(a.table_width) * a.page_size;
         if (length > most && threadIdx.x == 0) flag(a.status, SQ_STATUS_SLOT_RANGE);
@@ -157,13 +175,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(sq_kv_attenti
     }
     const int live = item.rows > 128 ? kTiles : 1;  // tiles of rows
 
-    if (warp == 12) {
+    if (warp == Shape::kProductWarp) {
         tc::tmem_alloc(&tmem_slot, 512);
         if (lane == 0) {
             tc::bar_init(&bars.query, 4 * live);
-            for (int i = 0; i < 2; ++i) {
-                tc::bar_init(&bars.keys[i], Shape::kUnpackThreads / 32);
-                tc::bar_init(&bars.values[i], Shape::kUnpackThreads / 32);
+            for (int i = 0; i < 4; ++i) {
+                tc::bar_init(&bars.keys[i], Shape::kUnpackWarps);
+                tc::bar_init(&bars.values[i], Shape::kUnpackWarps);
                 tc::bar_init(&bars.keys_free[i], 1);
                 tc::bar_init(&bars.values_free[i], 1);
                 tc::bar_init(&bars.scores[i], 1);
@@ -175,7 +193,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(sq_kv_attenti
             abort_flag = 0;
             bad_values = 0;
             most_value = 0;
-            for (int i = 0; i < 4; ++i) holes[i] = 0;
+            for (int i = 0; i < 8; ++i) holes[i] = 0;
         }
         __syncwarp();
         tc::fence_before();
@@ -190,7 +208,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(sq_kv_attenti
         const int64_t end = min(int64_t(item.start) + int64_t(item.blocks) * kKeys, int64_t(item.length));
         float most = 0.f;
 #pragma unroll 4
-        for (int64_t i = threadIdx.x; i < (end - item.start + kTile - 1) / kTile * kEach; i += kPromptThreads) {
+        for (int64_t i = threadIdx.x; i < (end - item.start + kTile - 1) / kTile * kEach; i += Shape::kThreads) {
             const int key = item.start + int(i / kEach) * kTile, first = int(i % kEach) * 4;
             const int64_t at = prompt_tile<D>(a, item, key);
             if (at < 0) continue;
@@ -209,8 +227,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(sq_kv_attenti
     }
     const int value_shift = most_value == 0 ? 0 : max(-100, min(100, 14 - (int(most_value >> 23) - 127)));
     const float value_factor = __uint_as_float(uint32_t(127 + value_shift) << 23);
-    auto wait_alone = [&](uint64_t *bar, uint32_t parity) { return tc::bar_wait(bar, parity, &abort_flag, tc::kWaitClocks); };
-    auto wait = [&](uint64_t *bar, uint32_t parity) { return bool(__all_sync(~0u, wait_alone(bar, parity))); };  // of a whole warp
+    // Of a whole warp: all lanes go on, or none does.
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+        return bool(__all_sync(~0u, tc::bar_wait(bar, parity, &abort_flag, tc::kWaitClocks)));
+    };
 
     float top = -INFINITY;  // of a row
     float2 sum = make_float2(0.f, 0.f);  // of its weights, in two parts
@@ -273,17 +293,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(sq_kv_attenti
             const uint32_t sums = tmem + lanes + Shape::kColumnsO + tile * D;
             bool ok = true;
             for (int j = 0; j < item.blocks && ok; ++j) {
-                const int buffer = kTiles == 2 ? tile : j & 1;
+                const int buffer = 2 * tile + (j & 1);
                 const uint32_t scores = tmem + lanes + buffer * kKeys;
-                ok = wait(&bars.scores[buffer], (kTiles == 2 ? j : j >> 1) & 1);
+                ok = wait(&bars.scores[buffer], (j >> 1) & 1);
                 if (!ok) break;
                 tc::fence_after();
+                uint32_t s[2][32];
+                tc::tmem_load(scores, s[0]);
+                tc::tmem_load(scores + 32, s[1]);
                 const int64_t begin = item.start + int64_t(j) * kKeys;
                 // Columns low < c <= high are seen.
                 const int high = int(max(int64_t(-1), min(last - begin, int64_t(kKeys))));
                 const int low = a.window > 0 ? int(max(int64_t(-1), min(last - a.window - begin, int64_t(kKeys)))) : -1;
                 uint32_t hole = 0;
-                if (holes[j & 3] == j + 1)
+                if (holes[j & 7] == j + 1)
                     for (int i = 0; i < kKeys / kTile; ++i)
                         if (prompt_tile<D>(a, item, int(begin) + i * kTile) < 0) hole |= 1u << i;
                 const bool whole = __all_sync(~0u, high >= kKeys - 1 && low < 0 && hole == 0);
@@ -297,81 +320,61 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(sq_kv_attenti
 #pragma unroll
                     for (int i = 0; i < 32; ++i) s[i] = bits >> i & 1 ? s[i] : 0xFF800000u;
                 };
-                uint32_t s[2][32];
-                float most = -INFINITY;
-                auto maximum = [&](uint32_t (&s)[32], int c) {
-                    if (!whole) hide(s, c);
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) most = fmaxf(most, fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 1])));
-                };
-                tc::tmem_load(scores, s[0]);
-#pragma unroll 1
-                for (int c = 0; c < kKeys; c += 64) {  // 32 columns are on their way while 32 are worked on
-                    tc::tmem_wait(s[0]);
-                    tc::tmem_load(scores + c + 32, s[1]);
-                    maximum(s[0], c);
-                    tc::tmem_wait(s[1]);
-                    tc::tmem_load(scores + (c + 64) % kKeys, s[0]);
-                    maximum(s[1], c + 32);
+                tc::tmem_wait(s[0]);
+                tc::tmem_wait(s[1]);
+                if (!whole) {
+                    hide(s[0], 0);
+                    hide(s[1], 32);
                 }
-                most *= to_log2;
+                float2 most2 = make_float2(-INFINITY, -INFINITY);
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    most2.x = max3(most2.x, __uint_as_float(s[0][i]), __uint_as_float(s[0][i + 1]));
+                    most2.y = max3(most2.y, __uint_as_float(s[1][i]), __uint_as_float(s[1][i + 1]));
+                }
+                const float most = fmaxf(most2.x, most2.y) * to_log2;
                 const bool grows = most > top + kPromptLag;
-                // One tile's next S may be ready before this block's O is: each phase is waited for in its turn.
-                bool waited = j == 0 || kTiles == 2;
                 if (__any_sync(~0u, grows)) {
                     const float change = grows ? exp2_approx(top - most) : 1.f;
                     top = grows ? most : top;
                     sum.x *= change;
                     sum.y *= change;
                     if (j > 0) {
-                        ok = wait(&bars.sums[tile], (j - 1) & 1);
+                        // This block's S was ready after the O of two blocks before: that barrier's last phase is over.
+                        ok = wait(&bars.sums[2 * tile + ((j - 1) & 1)], ((j - 1) >> 1) & 1);
                         if (!ok) break;
-                        waited = true;
                         tc::fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < D; c += 32) {
-                            tc::tmem_load(sums + c, s[1]);
-                            tc::tmem_wait(s[1]);
+                        for (int c = 0; c < D; c += 16) {
+                            uint32_t o[16];
+                            tc::tmem_load(sums + c, o);
+                            tc::tmem_wait(o);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) s[1][i] = __float_as_uint(__uint_as_float(s[1][i]) * change);
-                            tc::tmem_store(sums + c, s[1]);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * change);
+                            tc::tmem_store(sums + c, o);
                         }
-                        tc::tmem_load(scores, s[0]);  // again: the wait above was for it too
                     }
                 }
                 const float against = top == -INFINITY ? 0.f : -top;
-                auto weigh = [&](uint32_t (&s)[32], int c) {
-                    if (!whole) hide(s, c);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
                     uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
-                        const float2 z = fma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(to_log2, to_log2),
+                        const float2 z = fma2(make_float2(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), make_float2(to_log2, to_log2),
                                               make_float2(against, against));
                         const float2 w = make_float2(exp2_approx(z.x), exp2_approx(z.y));
                         sum = add2(sum, w);
                         p[i / 2] = pack2<__half>(w.x, w.y);
                     }
-                    tc::tmem_store(scores + c / 2, p);
-                };
-#pragma unroll 1
-                for (int c = 0; c < kKeys; c += 64) {
-                    tc::tmem_wait(s[0]);
-                    tc::tmem_load(scores + c + 32, s[1]);
-                    weigh(s[0], c);
-                    tc::tmem_wait(s[1]);
-                    if (c + 64 < kKeys) tc::tmem_load(scores + c + 64, s[0]);
-                    weigh(s[1], c + 32);
+                    tc::tmem_store(scores + c * 16, p);
                 }
                 tc::tmem_stored();
-                if (!waited) {
-                    ok = wait(&bars.sums[tile], (j - 1) & 1);
-                    if (!ok) break;
-                }
                 tc::fence_before();
                 __syncwarp();
                 if (lane == 0) tc::bar_arrive(&bars.weights[buffer]);
             }
-            if (ok && item.blocks > 0) ok = wait(&bars.sums[tile], (item.blocks - 1) & 1);
+            if (ok && item.blocks > 0) ok = wait(&bars.sums[2 * tile + ((item.blocks - 1) & 1)], ((item.blocks - 1) >> 1) & 1);
             tc::fence_after();
             if (__any_sync(~0u, mine)) {
                 uint32_t poison = 0;  // groups whose visible values are not all finite
@@ -414,166 +417,220 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(sq_kv_attenti
             }
             if (!ok && lane == 0) flag(a.status, SQ_STATUS_TIMEOUT);
         }
-    } else if (warp < 12) {
+    } else if (warp < Shape::kProductWarp) {
         // Codes into 16-bit operands: a piece of 16 bytes holds four words of one token.
+        // Piece i of this thread: tile tile0 + i kSpan of a block, the same token and part of it for all i.
+        // Key pieces go by (token, block of channels, quarter), value pieces by (token, block of 32 bytes, half).
+        constexpr int kPieces = Shape::kPieces, kPerTile = D / 2, kSpan = Shape::kUnpackThreads / kPerTile;
         const int thread = threadIdx.x - 32 * Shape::kSoftmaxWarps;
-        constexpr int kPieces = Shape::kPieces, kPerTile = D / 2;  // pieces of a tile's keys or values
-        uint4 words[2][kPieces];
-        uint32_t pairs[2][kPieces][4];
+        const int tile0 = thread / kPerTile, part = thread % (D / 32), token = thread % kPerTile / (D / 32), row = Tile::row(token);
+        constexpr int kParts = Tile::kBlockRow / 16, kKeyGroups = Tile::kBlockGroups;  // pieces of a block's row; groups of a key piece
+        constexpr int kValueGroups = kGroups;
+        const int key_at = (part / kParts) * kTile * Tile::kBlockRow + row * Tile::kBlockRow + (part % kParts) * 16;
+        const int key_pair_at = Tile::kKeyPairs + (row * kGroups + (D == 256 ? part / 4 * 2 : 0)) * 4;
+        const int value_at = Tile::kValues + (part >> 1) * kTile * 32 + token * 32 + (part & 1) * 16;
+        const int value_pair_at = Tile::kValuePairs + row * kGroups * 4;
+        // Where a piece's four words, 8 channels each, go in an operand of rows of 64 channels.
+        uint32_t key_to[4], value_to[4];
+        const uint32_t row0 = uint32_t(tile0 * kTile + token);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int kg = D == 64 ? 0 : part / 4 * 2 + (e >> 1), ko = D == 64 ? 4 * part + e : 2 * (part & 3) + (e & 1);
+            const int number = part * 4 + e, vg = number % kGroups, vo = number / kGroups;
+            key_to[e] = tc::smem_u32(keys) + kg * kKeys * 128 + row0 * 128 + ((ko ^ (token & 7)) << 4);
+            value_to[e] = tc::smem_u32(values) + vg * kKeys * 128 + row0 * 128 + ((vo ^ (token & 7)) << 4);
+        }
+        const uint32_t more_to = tc::smem_u32(more_keys) + row0 * 16 + part / 4 * kKeys * 16;
+        auto put = [](uint32_t to, uint4 x) {
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(to), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+        };
+        uint4 key_words[kPieces], value_words[kPieces];
+        uint32_t key_pairs[kPieces][kKeyGroups], value_pairs[kPieces][kValueGroups];
         // Lane i has the place of tile i of a block, which is looked up a block ahead.
         auto places = [&](int j) {
             const int key = item.start + j * kKeys + lane * kTile;
             const int64_t at = lane < kKeys / kTile && j < item.blocks ? prompt_tile<D>(a, item, key) : 0;
-            if (at < 0 && key < item.length) holes[j & 3] = j + 1;
+            if (at < 0 && key < item.length) holes[j & 7] = j + 1;
             return at;
         };
-        // Key pieces by (token, block of channels, quarter), value pieces by (token, block of 32 bytes, half).
-        auto load = [&](int j, int64_t place, bool value) {
+        auto load_keys = [&](int j, int64_t place) {
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
-                const int piece = (i * Shape::kUnpackThreads + thread) % kPerTile;
-                const int part = piece % (D / 32), token = piece / (D / 32);
-                const int key = item.start + j * kKeys + (i * Shape::kUnpackThreads + thread) / kPerTile * kTile + token;
-                uint4 &w = words[value][i];
-                w = make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int b = 0; b < 4; ++b) pairs[value][i][b] = 0;
-                const int64_t at = __shfl_sync(~0u, place, (i * Shape::kUnpackThreads + thread) / kPerTile);
-                if (at < 0) continue;
+                const int64_t at = __shfl_sync(~0u, place, tile0 + i * kSpan);
                 const uint8_t *tile = a.data + at;
-                const int row = Tile::row(token);
-                if (value) {
-                    w = *reinterpret_cast<const uint4 *>(tile + Tile::kValues + (part >> 1) * kTile * 32 + token * 32 + (part & 1) * 16);
-                } else {
-                    constexpr int kParts = Tile::kBlockRow / 16;  // pieces of a block's row
-                    w = *reinterpret_cast<const uint4 *>(tile + (part / kParts) * kTile * Tile::kBlockRow + row * Tile::kBlockRow + (part % kParts) * 16);
-                }
-                if (key < item.length) {
-                    const uint32_t *from = reinterpret_cast<const uint32_t *>(tile + (value ? Tile::kValuePairs : Tile::kKeyPairs)) + row * kGroups;
-                    if (D == 64) {
-                        pairs[value][i][0] = from[0];
-                    } else if (D == 128 || !value) {
-                        const uint2 p = *reinterpret_cast<const uint2 *>(from + (value ? 0 : part / 4 * 2));
-                        pairs[value][i][0] = p.x, pairs[value][i][1] = p.y;
-                    } else {
-                        const uint4 p = *reinterpret_cast<const uint4 *>(from);
-                        pairs[value][i][0] = p.x, pairs[value][i][1] = p.y, pairs[value][i][2] = p.z, pairs[value][i][3] = p.w;
+                key_words[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int b = 0; b < kKeyGroups; ++b) key_pairs[i][b] = 0;
+                if (at >= 0) {
+                    key_words[i] = *reinterpret_cast<const uint4 *>(tile + key_at);
+                    if (item.start + j * kKeys + (tile0 + i * kSpan) * kTile + token < item.length) {
+                        if (D == 64) {
+                            key_pairs[i][0] = *reinterpret_cast<const uint32_t *>(tile + key_pair_at);
+                        } else {
+                            const uint2 p = *reinterpret_cast<const uint2 *>(tile + key_pair_at);
+                            key_pairs[i][0] = p.x, key_pairs[i][kKeyGroups - 1] = p.y;
+                        }
                     }
                 }
             }
         };
-        auto write = [&](uint8_t *to, uint8_t *more, bool value) {
+        auto load_values = [&](int j, int64_t place) {
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
-                const int piece = (i * Shape::kUnpackThreads + thread) % kPerTile;
-                const int part = piece % (D / 32), token = piece / (D / 32);
-                const int row = (i * Shape::kUnpackThreads + thread) / kPerTile * kTile + token;  // key of the block
-                const uint32_t w[4] = {words[value][i].x, words[value][i].y, words[value][i].z, words[value][i].w};
-                if (!value && part % 4 == 0) {  // groups part / 4 * 2 and, if there is one, the next: m, m, 8 s, 8 s
-                    uint32_t r[4] = {};
+                const int64_t at = __shfl_sync(~0u, place, tile0 + i * kSpan);
+                const uint8_t *tile = a.data + at;
+                value_words[i] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-                    for (int b = 0; b < (kGroups < 2 ? 1 : 2); ++b) {
-                        const float s = low_bf16(pairs[value][i][b]) * (8 / kKeyDivisor), m = high_bf16(pairs[value][i][b]) / kKeyDivisor;
-                        r[2 * b] = pack2<__half>(m, m);
-                        r[2 * b + 1] = pack2<__half>(s, s);
+                for (int b = 0; b < kValueGroups; ++b) value_pairs[i][b] = 0;
+                if (at >= 0) {
+                    value_words[i] = *reinterpret_cast<const uint4 *>(tile + value_at);
+                    if (item.start + j * kKeys + (tile0 + i * kSpan) * kTile + token < item.length) {
+#pragma unroll
+                        for (int b = 0; b < kValueGroups; ++b)
+                            value_pairs[i][b] = reinterpret_cast<const uint32_t *>(tile + value_pair_at)[b];
                     }
-                    uint8_t *const from = more + row * 16;
-                    *reinterpret_cast<uint4 *>(from + part / 4 * kKeys * 16) = make_uint4(r[0], r[1], r[2], r[3]);
-                    if (D < 256) *reinterpret_cast<uint4 *>(from + kKeys * 16) = make_uint4(0, 0, 0, 0);
+                }
+            }
+        };
+        auto write_keys = [&](int stage) {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const uint32_t at = stage * Shape::kKeyBytes + i * kSpan * kTile * 128;
+                const uint32_t w[4] = {key_words[i].x, key_words[i].y, key_words[i].z, key_words[i].w};
+                __half2 s[kKeyGroups], less[kKeyGroups];
+#pragma unroll
+                for (int b = 0; b < kKeyGroups; ++b) {
+                    const float scale = low_bf16(key_pairs[i][b]) / kKeyDivisor;
+                    s[b] = __float2half2_rn(scale);
+                    less[b] = __float2half2_rn(-24.f * scale);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    // Channels 8 oct + 0..7 of group g; its pair is the piece's pair number p.
-                    int g, oct, p;
-                    if (value) {
-                        const int number = part * 4 + e;
-                        g = number % kGroups, oct = number / kGroups;
-                        p = e % kGroups;
-                    } else if (D == 64) {
-                        g = 0, oct = 4 * part + e, p = 0;
-                    } else {
-                        p = e >> 1, g = part / 4 * 2 + p, oct = 2 * (part & 3) + (e & 1);
+                    const int b = D == 64 ? 0 : e >> 1;
+                    put(key_to[e] + at, unpack_middle(w[e], s[b % kKeyGroups], less[b % kKeyGroups]));
+                }
+                if (part % 4 == 0) {  // groups part / 4 * 2 and, if there is one, the next: m, m, 8 s, 8 s
+                    const uint32_t more = more_to + stage * Shape::kMoreKey + i * kSpan * kTile * 16;
+                    uint32_t r[4] = {};
+#pragma unroll
+                    for (int b = 0; b < kKeyGroups; ++b) {
+                        const float m = high_bf16(key_pairs[i][b]) / kKeyDivisor, s8 = low_bf16(key_pairs[i][b]) * (8 / kKeyDivisor);
+                        r[2 * b] = pack2<__half>(m, m);
+                        r[2 * b + 1] = pack2<__half>(s8, s8);
                     }
-                    uint32_t pair = pairs[value][i][p];
-                    uint4 x;
-                    if (value) {
-                        if (high_bf16(pair) != high_bf16(pair)) pair = 0, bad_values = 1;
-                        x = unpack_f16(w[e], __float2half2_rn(low_bf16(pair) * value_factor), __float2half2_rn(high_bf16(pair) * value_factor));
-                    } else {
-                        x = unpack_middle(w[e], __float2half2_rn(low_bf16(pair) / kKeyDivisor));
-                    }
-                    *reinterpret_cast<uint4 *>(to + g * kKeys * 128 + row * 128 + ((oct ^ (row & 7)) << 4)) = x;
+                    put(more, make_uint4(r[0], r[1], r[2], r[3]));
+                    if (D < 256) put(more + kKeys * 16, make_uint4(0, 0, 0, 0));
                 }
             }
+        };
+        auto write_values = [&](int stage) {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const uint32_t at = stage * Shape::kKeyBytes + i * kSpan * kTile * 128;
+                const uint32_t w[4] = {value_words[i].x, value_words[i].y, value_words[i].z, value_words[i].w};
+                __half2 s[kValueGroups], s16[kValueGroups], m[kValueGroups];
+#pragma unroll
+                for (int b = 0; b < kValueGroups; ++b) {
+                    uint32_t pair = value_pairs[i][b];
+                    if ((pair & 0x7FFFFFFFu) > 0x7F800000u) pair = 0, bad_values = 1;  // m is NaN
+                    s[b] = __float2half2_rn(low_bf16(pair) * value_factor);
+                    s16[b] = __float2half2_rn(low_bf16(pair) * (value_factor / 16));
+                    m[b] = __float2half2_rn(high_bf16(pair) * value_factor);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) put(value_to[e] + at, unpack_value(w[e], s[e % kValueGroups], s16[e % kValueGroups], m[e % kValueGroups]));
+            }
+        };
+        auto written = [&](uint64_t *bar) {
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
+            if (lane == 0) tc::bar_arrive(bar);
         };
         int64_t place = places(0), next_place;
-        if (item.blocks > 0) load(0, place, false);
+        if (item.blocks > 0) load_keys(0, place);
 #pragma unroll 1
         for (int j = 0; j < item.blocks; ++j) {
-            const int stage = j & 1;
-            load(j, place, true);
+            const int stage = j % kStages;
+            load_values(j, place);
             next_place = places(j + 1);
-            if (j > 1 && !wait(&bars.keys_free[stage], ((j >> 1) - 1) & 1)) break;
-            write(keys + stage * Shape::kKeyBytes, more_keys + stage * Shape::kMoreKey, false);
-            if (lane == 0) tc::bar_arrive(&bars.keys[stage]);
+            if (j >= kStages && !wait(&bars.keys_free[stage], (j / kStages - 1) & 1)) break;
+            write_keys(stage);
+            written(&bars.keys[stage]);
             place = next_place;
-            if (j + 1 < item.blocks) load(j + 1, place, false);
-            if (j > 1 && !wait(&bars.values_free[stage], ((j >> 1) - 1) & 1)) break;
-            write(values + stage * Shape::kKeyBytes, nullptr, true);
-            if (lane == 0) tc::bar_arrive(&bars.values[stage]);
+            if (j + 1 < item.blocks) load_keys(j + 1, place);
+            if (j >= kStages && !wait(&bars.values_free[stage], (j / kStages - 1) & 1)) break;
+            write_values(stage);
+            written(&bars.values[stage]);
         }
-    } else if (lane == 0) {
+    } else {
         constexpr uint32_t kScores = tc::half_product(kKeys, false, false), kSums = tc::half_product(D, false, true);
-        auto scores = [&](int tile, int buffer, int stage) {
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-                tc::mma_half(tmem + buffer * kKeys, tc::operand(tc::smem_u32(queries + tile * Shape::kQueryBytes + (k >> 2) * 16384) + (k & 3) * 32),
-                             tc::operand(tc::smem_u32(keys + stage * Shape::kKeyBytes + (k >> 2) * kKeys * 128) + (k & 3) * 32), kScores, k > 0);
-            tc::mma_half(tmem + buffer * kKeys, tc::operand_narrow(tc::smem_u32(more_queries + tile * Shape::kMoreQuery), 128 * 16),
-                         tc::operand_narrow(tc::smem_u32(more_keys + stage * Shape::kMoreKey), kKeys * 16), kScores, true);
-            tc::mma_commit(&bars.scores[buffer]);
-        };
-        bool ok = item.blocks == 0 || wait_alone(&bars.query, 0);
-        // The keys of block j, and its products with the queries of each tile.
-        auto begin = [&](int j, int tile) {
-            const int stage = j & 1;
-            if (tile == 0) ok = ok && wait_alone(&bars.keys[stage], (j >> 1) & 1);
+        // Descriptors of the first operands; others are further by bytes / 16.
+        const uint64_t query = tc::operand(tc::smem_u32(queries)), key = tc::operand(tc::smem_u32(keys));
+        const uint64_t value = tc::operand_mn(tc::smem_u32(values), kKeys * 128);
+        const uint64_t more_query = tc::operand_narrow(tc::smem_u32(more_queries), 128 * 16);
+        const uint64_t more_key = tc::operand_narrow(tc::smem_u32(more_keys), kKeys * 16);
+        // The same for all lanes, and known to be: operands stay in uniform registers.
+        const uint32_t base = __shfl_sync(~0u, tmem, 0);
+        const int blocks = __shfl_sync(~0u, item.blocks, 0), tiles = __shfl_sync(~0u, live, 0);
+        bool ok = blocks == 0 || wait(&bars.query, 0);
+        // S of block j for each tile.
+        auto begin = [&](int j) {
+            const int stage = j % kStages;
+            ok = ok && wait(&bars.keys[stage], (j / kStages) & 1);
             if (!ok) return;
             tc::fence_after();
-            scores(tile, kTiles == 2 ? tile : stage, stage);
-            if (tile == live - 1) tc::mma_commit(&bars.keys_free[stage]);
+            const uint64_t k = key + stage * (Shape::kKeyBytes / 16), more = more_key + stage * (Shape::kMoreKey / 16);
+#pragma unroll
+            for (int tile = 0; tile < kTiles; ++tile) {
+                const int buffer = 2 * tile + (j & 1);
+                const uint32_t d = base + buffer * kKeys;
+                const uint64_t q = query + tile * (Shape::kQueryBytes / 16);
+                if (tile < tiles && tc::elected()) {
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i)
+                        tc::mma_half(d, q + ((i >> 2) * 16384 + (i & 3) * 32) / 16, k + ((i >> 2) * kKeys * 128 + (i & 3) * 32) / 16, kScores, i > 0);
+                    tc::mma_half(d, more_query + tile * (Shape::kMoreQuery / 16), more, kScores, true);
+                    tc::mma_commit(&bars.scores[buffer]);
+                    if (tile == tiles - 1) tc::mma_commit(&bars.keys_free[stage]);
+                }
+                __syncwarp();
+            }
         };
-        for (int tile = 0; tile < live && item.blocks > 0; ++tile) begin(0, tile);
-        for (int j = 0; j < item.blocks && ok; ++j) {
-            const int stage = j & 1;
-            if (kTiles == 1 && j + 1 < item.blocks) begin(j + 1, 0);
-            for (int tile = 0; tile < live && ok; ++tile) {
-                const int buffer = kTiles == 2 ? tile : stage;
-                if (tile == 0) ok = wait_alone(&bars.values[stage], (j >> 1) & 1);
-                ok = ok && wait_alone(&bars.weights[buffer], (kTiles == 2 ? j : j >> 1) & 1);
+        if (blocks > 0) begin(0);
+#pragma unroll 1
+        for (int j = 0; j < blocks && ok; ++j) {
+            const int stage = j % kStages;
+            if (j + 1 < blocks) begin(j + 1);
+            ok = ok && wait(&bars.values[stage], (j / kStages) & 1);
+            const uint64_t v = value + stage * (Shape::kKeyBytes / 16);
+#pragma unroll
+            for (int tile = 0; tile < kTiles; ++tile) {
+                if (tile >= tiles || !ok) break;
+                const int buffer = 2 * tile + (j & 1);
+                ok = wait(&bars.weights[buffer], (j >> 1) & 1);
                 if (!ok) break;
                 tc::fence_after();
+                if (tc::elected()) {
 #pragma unroll
-                for (int k = 0; k < kKeys / 16; ++k)
-                    tc::mma_half_tmem(tmem + Shape::kColumnsO + tile * D, tmem + buffer * kKeys + k * 8,
-                                      tc::operand_mn(tc::smem_u32(values + stage * Shape::kKeyBytes + k * 2048), kKeys * 128), kSums, j > 0 || k > 0);
-                tc::mma_commit(&bars.sums[tile]);
-                if (tile == live - 1) tc::mma_commit(&bars.values_free[stage]);
-                if (kTiles == 2 && j + 1 < item.blocks) begin(j + 1, tile);
+                    for (int k = 0; k < kKeys / 16; ++k)
+                        tc::mma_half_tmem(base + Shape::kColumnsO + tile * D, base + buffer * kKeys + k * 8, v + k * 2048 / 16, kSums, j > 0 || k > 0);
+                    tc::mma_commit(&bars.sums[buffer]);
+                    if (tile == tiles - 1) tc::mma_commit(&bars.values_free[stage]);
+                }
+                __syncwarp();
             }
         }
         if (!ok) {  // the products that were issued end before the tensor memory is freed
             int alone = 0;
-            tc::mma_commit(&bars.end);
+            if (tc::elected()) tc::mma_commit(&bars.end);
+            __syncwarp();
             tc::bar_wait(&bars.end, 0, &alone, tc::kWaitClocks);
         }
     }
     __syncwarp();
     tc::fence_before();
     __syncthreads();
-    if (warp == 12) tc::tmem_free(tmem, 512);
+    if (warp == Shape::kProductWarp) tc::tmem_free(tmem, 512);
 }
 
 template <class T, int D>
@@ -585,7 +642,7 @@ cudaError_t launch_prompt(const sq_kv_attention_args &a, int few_rows, cudaStrea
     if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
     const cudaError_t e = cudaFuncSetAttribute(prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kShared);
     if (e != cudaSuccess) return e;
-    prompt_kernel<T, D><<<unsigned(grid), kPromptThreads, Shape::kShared, s>>>(a, per, strips, few_rows);
+    prompt_kernel<T, D><<<unsigned(grid), Shape::kThreads, Shape::kShared, s>>>(a, per, strips, few_rows);
     return cudaGetLastError();
 }
 
