@@ -289,6 +289,11 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
             if (lane == 0) tc::bar_arrive(&bars.query);
             const float to_log2 = a.scale * kLog2e * kKeyDivisor / factor;
             const int64_t last = mine ? min(item.before + token, int64_t(item.length) - 1) : -1;
+            // Columns low < c <= high of the keys from item.start on are seen; the warp sees blocks whole_from to
+            // whole_to - 1 whole.
+            const int high = int(max(int64_t(-1), last - item.start));
+            const int low = a.window > 0 ? int(max(int64_t(-1), last - a.window - item.start)) : -1;
+            const int whole_from = __reduce_max_sync(~0u, (low + kKeys) / kKeys), whole_to = __reduce_min_sync(~0u, (high + 1) / kKeys);
             const uint32_t lanes = uint32_t(warp & 3) << 21;
             const uint32_t sums = tmem + lanes + Shape::kColumnsO + tile * D;
             bool ok = true;
@@ -301,18 +306,14 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
                 uint32_t s[2][32];
                 tc::tmem_load(scores, s[0]);
                 tc::tmem_load(scores + 32, s[1]);
-                const int64_t begin = item.start + int64_t(j) * kKeys;
-                // Columns low < c <= high are seen.
-                const int high = int(max(int64_t(-1), min(last - begin, int64_t(kKeys))));
-                const int low = a.window > 0 ? int(max(int64_t(-1), min(last - a.window - begin, int64_t(kKeys)))) : -1;
+                const bool holed = holes[j & 7] == j + 1, whole = j >= whole_from && j < whole_to && !holed;
                 uint32_t hole = 0;
-                if (holes[j & 7] == j + 1)
+                if (holed)
                     for (int i = 0; i < kKeys / kTile; ++i)
-                        if (prompt_tile<D>(a, item, int(begin) + i * kTile) < 0) hole |= 1u << i;
-                const bool whole = __all_sync(~0u, high >= kKeys - 1 && low < 0 && hole == 0);
+                        if (prompt_tile<D>(a, item, item.start + j * kKeys + i * kTile) < 0) hole |= 1u << i;
                 // Scores c .. c + 31, those that are not seen -infinity.
                 auto hide = [&](uint32_t (&s)[32], int c) {
-                    const int h = min(high - c, 31), l = min(low - c, 31);
+                    const int h = min(high - j * kKeys - c, 31), l = min(low - j * kKeys - c, 31);
                     uint32_t bits = h < 0 ? 0u : (2u << h) - 1u;
                     if (l >= 0) bits &= ~((2u << l) - 1u);
                     if (hole >> (c / kTile) & 1) bits &= 0xFFFF0000u;
@@ -573,18 +574,23 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
         const uint32_t base = __shfl_sync(~0u, tmem, 0);
         const int blocks = __shfl_sync(~0u, item.blocks, 0), tiles = __shfl_sync(~0u, live, 0);
         bool ok = blocks == 0 || wait(&bars.query, 0);
+        // Not formed ahead of the loop, each operand of a block in registers of its own.
+        auto here = [](uint64_t x) {
+            asm volatile("" : "+l"(x));
+            return x;
+        };
         // S of block j for each tile.
         auto begin = [&](int j) {
             const int stage = j % kStages;
             ok = ok && wait(&bars.keys[stage], (j / kStages) & 1);
             if (!ok) return;
             tc::fence_after();
-            const uint64_t k = key + stage * (Shape::kKeyBytes / 16), more = more_key + stage * (Shape::kMoreKey / 16);
+            const uint64_t k = here(key) + stage * (Shape::kKeyBytes / 16), more = here(more_key) + stage * (Shape::kMoreKey / 16);
 #pragma unroll
             for (int tile = 0; tile < kTiles; ++tile) {
                 const int buffer = 2 * tile + (j & 1);
                 const uint32_t d = base + buffer * kKeys;
-                const uint64_t q = query + tile * (Shape::kQueryBytes / 16);
+                const uint64_t q = here(query) + tile * (Shape::kQueryBytes / 16);
                 if (tile < tiles && tc::elected()) {
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i)
@@ -602,7 +608,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
             const int stage = j % kStages;
             if (j + 1 < blocks) begin(j + 1);
             ok = ok && wait(&bars.values[stage], (j / kStages) & 1);
-            const uint64_t v = value + stage * (Shape::kKeyBytes / 16);
+            const uint64_t v = here(value) + stage * (Shape::kKeyBytes / 16);
 #pragma unroll
             for (int tile = 0; tile < kTiles; ++tile) {
                 if (tile >= tiles || !ok) break;
