@@ -2,14 +2,13 @@
 //
 // A CTA takes 256 query rows of one kv head, (token, query head) pairs, in two tiles of
 // 128 (heads of 256 channels: one tile, as its sums fill the tensor memory), and walks
-// the keys in blocks of 64.  Per block:
+// the keys in blocks of 128 (64).  Per block:
 //   eight warps (four for heads of 64) write out the codes as 16-bit keys and values in
 //   shared memory, two to four blocks ahead,
 //   one warp issues S = Q K^T and O += P V, S, P and O in tensor memory,
 //   four warps a tile, a thread to a row, turn S into P, which overwrites it.
-// S and P have two buffers a tile: the next block's S is ready when this block's P is.
-// (Blocks of 128 keys with one buffer left S waiting for O += P V: 1418 us for 4096 tokens
-// over 16384 of 32 heads.)
+// While a tile's S becomes P, the other tile's products run (one tile: S and P have two
+// buffers).  Products of 128 x 64 take as long as those of 128 x 128, 64 clocks.
 // Scores take keys as they are held: s (c - 8) has 3 + 8 significant bits and so is an f16,
 // and the rest of a group, m + 8 s, meets the sum of the query's channels in one more step
 // of K (the sum's f16 and its remainder, each by m and by 8 s).  Queries are f16 with each
@@ -34,14 +33,22 @@ template <int D>
 struct PromptShape {
     using Tile = KvTile<D>;
     static constexpr int kTiles = D == 256 ? 1 : 2;             // of 128 rows
-    static constexpr int kKeys = 64;                            // of a block
-    static constexpr int kStages = D == 256 ? 2 : 4;
+    static constexpr int kKeys = D == 256 ? 64 : 128;           // of a block
+    static constexpr int kBuffers = D == 256 ? 2 : 1;           // of S and P for a tile
+    static constexpr int kStages = D == 64 ? 4 : 2;
     static constexpr int kSoftmaxWarps = 4 * kTiles, kUnpackWarps = D == 64 ? 4 : 8, kProductWarp = kSoftmaxWarps + kUnpackWarps;
-    static constexpr int kUnpackThreads = 32 * kUnpackWarps, kThreads = 32 * (kProductWarp + 1);
+    static constexpr int kUnpackThreads = 32 * kUnpackWarps, kThreads = 32 * (kProductWarp + 4);
+    // With 128 keys a softmax thread holds 128 scores: the registers that 16 or 20 warps are launched with
+    // are shared out anew, and what the three roles take is no more than that.
+    static constexpr bool kShare = kKeys == 128;
+    static constexpr int kLaunchRegisters = D == 128 ? 96 : 128;
+    static constexpr int kSoftmaxRegisters = D == 128 ? 168 : 168, kUnpackRegisters = D == 128 ? 56 : 96, kProductRegisters = D == 128 ? 32 : 48;
+    static_assert(!kShare || 32 * (kSoftmaxWarps * kSoftmaxRegisters + kUnpackWarps * kUnpackRegisters + 4 * kProductRegisters) <=
+                                 kThreads * kLaunchRegisters, "");
     static constexpr int kQueryBytes = 128 * D * 2, kKeyBytes = kKeys * D * 2;
     static constexpr int kMoreQuery = 128 * 32, kMoreKey = kKeys * 32;  // the last step of K: 16 values a row
     static constexpr int kShared = kTiles * (kQueryBytes + kMoreQuery) + kStages * (2 * kKeyBytes + kMoreKey) + 1024;
-    static constexpr int kColumnsO = kTiles * 2 * kKeys;        // S, P: [0, kColumnsO), two buffers a tile
+    static constexpr int kColumnsO = kTiles * kBuffers * kKeys; // S, P: [0, kColumnsO)
     static constexpr int kPieces = kKeys * D / 32 / kUnpackThreads;  // 16-byte pieces of a block's keys for a thread
     static_assert(kColumnsO + kTiles * D <= 512 && kPieces * kUnpackThreads * 32 == kKeys * D && kShared <= 227 * 1024, "");
     static_assert((kStages & (kStages - 1)) == 0 && kStages <= 4, "");
@@ -49,7 +56,8 @@ struct PromptShape {
 
 struct PromptBars {
     uint64_t query, keys[4], keys_free[4], values[4], values_free[4];  // by stage
-    uint64_t scores[4], weights[4], sums[4];                           // by tile and block modulo 2
+    uint64_t scores[2], weights[2];                                    // by tile, or by block modulo 2
+    uint64_t sums[4];                                                  // by tile and block modulo 2
     uint64_t end;
 };
 
@@ -135,7 +143,7 @@ template <class T, int D>
 __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_kv_attention_args a, int tokens_per_item, unsigned strips, int few_rows) {
     using Shape = PromptShape<D>;
     using Tile = KvTile<D>;
-    constexpr int kTiles = Shape::kTiles, kKeys = Shape::kKeys, kStages = Shape::kStages, kGroups = Tile::kGroups;
+    constexpr int kTiles = Shape::kTiles, kKeys = Shape::kKeys, kBuffers = Shape::kBuffers, kStages = Shape::kStages, kGroups = Tile::kGroups;
     extern __shared__ uint8_t raw[];
     __shared__ PromptBars bars;
     __shared__ uint32_t tmem_slot;
@@ -184,9 +192,11 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
                 tc::bar_init(&bars.values[i], Shape::kUnpackWarps);
                 tc::bar_init(&bars.keys_free[i], 1);
                 tc::bar_init(&bars.values_free[i], 1);
+                tc::bar_init(&bars.sums[i], 1);
+            }
+            for (int i = 0; i < 2; ++i) {
                 tc::bar_init(&bars.scores[i], 1);
                 tc::bar_init(&bars.weights[i], 4);
-                tc::bar_init(&bars.sums[i], 1);
             }
             tc::bar_init(&bars.end, 1);
             tc::bar_init_fence();
@@ -235,6 +245,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
     float top = -INFINITY;  // of a row
     float2 sum = make_float2(0.f, 0.f);  // of its weights, in two parts
     if (warp < Shape::kSoftmaxWarps) {
+        if constexpr (Shape::kShare) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(Shape::kSoftmaxRegisters));
         const int tile = warp >> 2, row = threadIdx.x & 127, index = tile * 128 + row;
         if (tile < live) {
             const bool mine = index < item.rows;
@@ -298,14 +309,14 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
             const uint32_t sums = tmem + lanes + Shape::kColumnsO + tile * D;
             bool ok = true;
             for (int j = 0; j < item.blocks && ok; ++j) {
-                const int buffer = 2 * tile + (j & 1);
+                const int buffer = kBuffers == 2 ? j & 1 : tile;
                 const uint32_t scores = tmem + lanes + buffer * kKeys;
-                ok = wait(&bars.scores[buffer], (j >> 1) & 1);
+                ok = wait(&bars.scores[buffer], (kBuffers == 2 ? j >> 1 : j) & 1);
                 if (!ok) break;
                 tc::fence_after();
-                uint32_t s[2][32];
-                tc::tmem_load(scores, s[0]);
-                tc::tmem_load(scores + 32, s[1]);
+                uint32_t s[kKeys / 32][32];
+#pragma unroll
+                for (int c = 0; c < kKeys / 32; ++c) tc::tmem_load(scores + 32 * c, s[c]);
                 const bool holed = holes[j & 7] == j + 1, whole = j >= whole_from && j < whole_to && !holed;
                 uint32_t hole = 0;
                 if (holed)
@@ -321,19 +332,19 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
 #pragma unroll
                     for (int i = 0; i < 32; ++i) s[i] = bits >> i & 1 ? s[i] : 0xFF800000u;
                 };
-                tc::tmem_wait(s[0]);
-                tc::tmem_wait(s[1]);
-                if (!whole) {
-                    hide(s[0], 0);
-                    hide(s[1], 32);
-                }
-                float2 most2 = make_float2(-INFINITY, -INFINITY);
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    most2.x = max3(most2.x, __uint_as_float(s[0][i]), __uint_as_float(s[0][i + 1]));
-                    most2.y = max3(most2.y, __uint_as_float(s[1][i]), __uint_as_float(s[1][i + 1]));
+                for (int c = 0; c < kKeys / 32; ++c) tc::tmem_wait(s[c]);
+                if (!whole) {
+#pragma unroll
+                    for (int c = 0; c < kKeys / 32; ++c) hide(s[c], 32 * c);
                 }
-                const float most = fmaxf(most2.x, most2.y) * to_log2;
+                float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < kKeys / 32; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2)
+                        part[c % 4] = max3(part[c % 4], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
+                const float most = fmaxf(max3(part[0], part[1], part[2]), part[3]) * to_log2;
                 const bool grows = most > top + kPromptLag;
                 if (__any_sync(~0u, grows)) {
                     const float change = grows ? exp2_approx(top - most) : 1.f;
@@ -358,7 +369,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
                 }
                 const float against = top == -INFINITY ? 0.f : -top;
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
+                for (int c = 0; c < kKeys / 32; ++c) {
                     uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
@@ -419,6 +430,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
             if (!ok && lane == 0) flag(a.status, SQ_STATUS_TIMEOUT);
         }
     } else if (warp < Shape::kProductWarp) {
+        if constexpr (Shape::kShare) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(Shape::kUnpackRegisters));
         // Codes into 16-bit operands: a piece of 16 bytes holds four words of one token.
         // Piece i of this thread: tile tile0 + i kSpan of a block, the same token and part of it for all i.
         // Key pieces go by (token, block of channels, quarter), value pieces by (token, block of 32 bytes, half).
@@ -564,6 +576,8 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
             written(&bars.values[stage]);
         }
     } else {
+        if constexpr (Shape::kShare) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(Shape::kProductRegisters));
+        if (warp == Shape::kProductWarp) {
         constexpr uint32_t kScores = tc::half_product(kKeys, false, false), kSums = tc::half_product(D, false, true);
         // Descriptors of the first operands; others are further by bytes / 16.
         const uint64_t query = tc::operand(tc::smem_u32(queries)), key = tc::operand(tc::smem_u32(keys));
@@ -579,51 +593,48 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
             asm volatile("" : "+l"(x));
             return x;
         };
-        // S of block j for each tile.
-        auto begin = [&](int j) {
-            const int stage = j % kStages;
-            ok = ok && wait(&bars.keys[stage], (j / kStages) & 1);
+        // S of block j for a tile.
+        auto begin = [&](int j, int tile) {
+            const int stage = j % kStages, buffer = kBuffers == 2 ? j & 1 : tile;
+            if (tile == 0) ok = ok && wait(&bars.keys[stage], (j / kStages) & 1);
             if (!ok) return;
             tc::fence_after();
-            const uint64_t k = here(key) + stage * (Shape::kKeyBytes / 16), more = here(more_key) + stage * (Shape::kMoreKey / 16);
-#pragma unroll
-            for (int tile = 0; tile < kTiles; ++tile) {
-                const int buffer = 2 * tile + (j & 1);
+            const uint64_t q = here(query) + tile * (Shape::kQueryBytes / 16), k = here(key) + stage * (Shape::kKeyBytes / 16);
+            const uint64_t more = here(more_key) + stage * (Shape::kMoreKey / 16);
+            if (tc::elected()) {
                 const uint32_t d = base + buffer * kKeys;
-                const uint64_t q = here(query) + tile * (Shape::kQueryBytes / 16);
-                if (tile < tiles && tc::elected()) {
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i)
-                        tc::mma_half(d, q + ((i >> 2) * 16384 + (i & 3) * 32) / 16, k + ((i >> 2) * kKeys * 128 + (i & 3) * 32) / 16, kScores, i > 0);
-                    tc::mma_half(d, more_query + tile * (Shape::kMoreQuery / 16), more, kScores, true);
-                    tc::mma_commit(&bars.scores[buffer]);
-                    if (tile == tiles - 1) tc::mma_commit(&bars.keys_free[stage]);
-                }
-                __syncwarp();
+                for (int i = 0; i < D / 16; ++i)
+                    tc::mma_half(d, q + ((i >> 2) * 16384 + (i & 3) * 32) / 16, k + ((i >> 2) * kKeys * 128 + (i & 3) * 32) / 16, kScores, i > 0);
+                tc::mma_half(d, here(more_query) + tile * (Shape::kMoreQuery / 16), more, kScores, true);
+                tc::mma_commit(&bars.scores[buffer]);
+                if (tile == tiles - 1) tc::mma_commit(&bars.keys_free[stage]);
             }
+            __syncwarp();
         };
-        if (blocks > 0) begin(0);
+        for (int tile = 0; tile < tiles && blocks > 0; ++tile) begin(0, tile);
 #pragma unroll 1
         for (int j = 0; j < blocks && ok; ++j) {
             const int stage = j % kStages;
-            if (j + 1 < blocks) begin(j + 1);
+            if (kBuffers == 2 && j + 1 < blocks) begin(j + 1, 0);
             ok = ok && wait(&bars.values[stage], (j / kStages) & 1);
-            const uint64_t v = here(value) + stage * (Shape::kKeyBytes / 16);
 #pragma unroll
             for (int tile = 0; tile < kTiles; ++tile) {
                 if (tile >= tiles || !ok) break;
-                const int buffer = 2 * tile + (j & 1);
-                ok = wait(&bars.weights[buffer], (j >> 1) & 1);
+                const int buffer = kBuffers == 2 ? j & 1 : tile;
+                ok = wait(&bars.weights[buffer], (kBuffers == 2 ? j >> 1 : j) & 1);
                 if (!ok) break;
                 tc::fence_after();
+                const uint64_t v = here(value) + stage * (Shape::kKeyBytes / 16);
                 if (tc::elected()) {
 #pragma unroll
                     for (int k = 0; k < kKeys / 16; ++k)
                         tc::mma_half_tmem(base + Shape::kColumnsO + tile * D, base + buffer * kKeys + k * 8, v + k * 2048 / 16, kSums, j > 0 || k > 0);
-                    tc::mma_commit(&bars.sums[buffer]);
+                    tc::mma_commit(&bars.sums[2 * tile + (j & 1)]);
                     if (tile == tiles - 1) tc::mma_commit(&bars.values_free[stage]);
                 }
                 __syncwarp();
+                if (kBuffers == 1 && j + 1 < blocks) begin(j + 1, tile);
             }
         }
         if (!ok) {  // the products that were issued end before the tensor memory is freed
@@ -631,6 +642,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
             if (tc::elected()) tc::mma_commit(&bars.end);
             __syncwarp();
             tc::bar_wait(&bars.end, 0, &alone, tc::kWaitClocks);
+        }
         }
     }
     __syncwarp();
