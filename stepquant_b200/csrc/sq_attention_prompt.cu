@@ -42,7 +42,7 @@ struct PromptShape {
     // are shared out anew, and what the three roles take is no more than that.
     static constexpr bool kShare = kKeys == 128;
     static constexpr int kLaunchRegisters = D == 128 ? 96 : 128;
-    static constexpr int kSoftmaxRegisters = D == 128 ? 168 : 168, kUnpackRegisters = D == 128 ? 56 : 96, kProductRegisters = D == 128 ? 32 : 48;
+    static constexpr int kSoftmaxRegisters = D == 128 ? 160 : 168, kUnpackRegisters = D == 128 ? 56 : 96, kProductRegisters = D == 128 ? 48 : 48;
     static_assert(!kShare || 32 * (kSoftmaxWarps * kSoftmaxRegisters + kUnpackWarps * kUnpackRegisters + 4 * kProductRegisters) <=
                                  kThreads * kLaunchRegisters, "");
     static constexpr int kQueryBytes = 128 * D * 2, kKeyBytes = kKeys * D * 2;
@@ -443,16 +443,16 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
         const int key_pair_at = Tile::kKeyPairs + (row * kGroups + (D == 256 ? part / 4 * 2 : 0)) * 4;
         const int value_at = Tile::kValues + (part >> 1) * kTile * 32 + token * 32 + (part & 1) * 16;
         const int value_pair_at = Tile::kValuePairs + row * kGroups * 4;
-        // Where a piece's four words, 8 channels each, go in an operand of rows of 64 channels.
-        uint32_t key_to[4], value_to[4];
-        const uint32_t row0 = uint32_t(tile0 * kTile + token);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int kg = D == 64 ? 0 : part / 4 * 2 + (e >> 1), ko = D == 64 ? 4 * part + e : 2 * (part & 3) + (e & 1);
-            const int number = part * 4 + e, vg = number % kGroups, vo = number / kGroups;
-            key_to[e] = tc::smem_u32(keys) + kg * kKeys * 128 + row0 * 128 + ((ko ^ (token & 7)) << 4);
-            value_to[e] = tc::smem_u32(values) + vg * kKeys * 128 + row0 * 128 + ((vo ^ (token & 7)) << 4);
-        }
+        // Where a piece's word e, 8 channels, goes in an operand of rows of 64 channels: the first one's place,
+        // other 16 bytes of the row (the swizzle is an exclusive or) or another group.
+        const uint32_t row0 = uint32_t(tile0 * kTile + token), swizzle = token & 7;
+        const uint32_t key_to = tc::smem_u32(keys) + (D == 256 ? part / 4 * 2 : 0) * kKeys * 128 + row0 * 128 +
+                                (((D == 64 ? 4 * part : 2 * (part & 3)) ^ swizzle) << 4);
+        const uint32_t value_to = tc::smem_u32(values) + row0 * 128 + (((D == 256 ? part : D == 128 ? 2 * part : 4 * part) ^ swizzle) << 4);
+        auto key_word = [&](uint32_t at, int e) { return D == 64 ? at ^ (e << 4) : (at ^ ((e & 1) << 4)) + (e >> 1) * kKeys * 128; };
+        auto value_word = [&](uint32_t at, int e) {
+            return D == 64 ? at ^ (e << 4) : D == 128 ? (at ^ ((e >> 1) << 4)) + (e & 1) * kKeys * 128 : at + e * kKeys * 128;
+        };
         const uint32_t more_to = tc::smem_u32(more_keys) + row0 * 16 + part / 4 * kKeys * 16;
         auto put = [](uint32_t to, uint4 x) {
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(to), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
         auto write_keys = [&](int stage) {
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
-                const uint32_t at = stage * Shape::kKeyBytes + i * kSpan * kTile * 128;
+                const uint32_t at = key_to + stage * Shape::kKeyBytes + i * kSpan * kTile * 128;
                 const uint32_t w[4] = {key_words[i].x, key_words[i].y, key_words[i].z, key_words[i].w};
                 __half2 s[kKeyGroups], less[kKeyGroups];
 #pragma unroll
@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int b = D == 64 ? 0 : e >> 1;
-                    put(key_to[e] + at, unpack_middle(w[e], s[b % kKeyGroups], less[b % kKeyGroups]));
+                    put(key_word(at, e), unpack_middle(w[e], s[b % kKeyGroups], less[b % kKeyGroups]));
                 }
                 if (part % 4 == 0) {  // groups part / 4 * 2 and, if there is one, the next: m, m, 8 s, 8 s
                     const uint32_t more = more_to + stage * Shape::kMoreKey + i * kSpan * kTile * 16;
@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
         auto write_values = [&](int stage) {
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
-                const uint32_t at = stage * Shape::kKeyBytes + i * kSpan * kTile * 128;
+                const uint32_t at = value_to + stage * Shape::kKeyBytes + i * kSpan * kTile * 128;
                 const uint32_t w[4] = {value_words[i].x, value_words[i].y, value_words[i].z, value_words[i].w};
                 __half2 s[kValueGroups], s16[kValueGroups], m[kValueGroups];
 #pragma unroll
@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
                     m[b] = __float2half2_rn(high_bf16(pair) * value_factor);
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) put(value_to[e] + at, unpack_value(w[e], s[e % kValueGroups], s16[e % kValueGroups], m[e % kValueGroups]));
+                for (int e = 0; e < 4; ++e) put(value_word(at, e), unpack_value(w[e], s[e % kValueGroups], s16[e % kValueGroups], m[e % kValueGroups]));
             }
         };
         auto written = [&](uint64_t *bar) {
