@@ -186,13 +186,67 @@ template <int D, int NT>
 struct RowsShape {
     using Tile = KvTile<D>;
     static constexpr int kRows = 8 * NT;
-    static constexpr int kStages = D == 64 ? 6 : D == 128 ? 5 : 3;
+    static constexpr int kStages = D == 64 ? 6 : D == 128 ? 4 : 3;
     static constexpr int kRing = kStages * Tile::kBytes;          // of a warp
     static constexpr int kMergeRow = D + 4;                       // floats
+    static constexpr int kMerge = kRows * kMergeRow * 4;          // of a warp
     static constexpr int kPart = kRows * D + 2 * kRows;           // floats of a part: sums, maxima, weights' sums
-    static constexpr int kShared = kWarps * kRing;
-    static_assert(kRows * kMergeRow * 4 <= kRing && kRing % 16 == 0 && Tile::kBytes % 16 == 0, "a warp's sums lie in its ring");
+    static constexpr int kShared = kWarps * (kRing + kMerge);
+    static_assert(kRing % 16 == 0 && kMerge % 16 == 0 && Tile::kBytes % 16 == 0, "copies and sums are aligned");
 };
+
+// The tiles of one item that lie in a CTA's span.
+struct Segment {
+    int sequence, head, block;
+    int first, tokens, length;  // the sequence's new tokens, tokens that it holds
+    int64_t before;             // position of its first new token
+    int tile, count;            // first tile, tiles; none: the span is over
+    bool whole;                 // the item's tiles
+};
+
+// Where in its span a CTA is.
+struct Cursor {
+    Sequence s;
+    int64_t at;
+    int n, head, block, begin;  // begin: tiles of the item before
+};
+
+template <int ROWS>
+__device__ __forceinline__ void next_segment(const sq_kv_attention_args &a, int most_rows, int64_t end, Cursor &c, Segment &g) {
+    g.count = 0;
+    if (c.at >= end) return;
+    if (c.begin >= c.s.tiles) {
+        c.begin = 0;
+        if (++c.block >= c.s.blocks) {
+            c.block = 0;
+            ++c.head;
+        }
+    }
+    while (c.head >= a.heads || c.s.cost == 0) {  // on to the next sequence with new tokens: there is one, as at < end
+        c.s = sequence<ROWS>(a, most_rows, ++c.n, false);
+        c.head = c.block = c.begin = 0;
+    }
+    g.sequence = c.n, g.head = c.head, g.block = c.block;
+    g.first = c.s.first, g.tokens = c.s.count, g.length = c.s.length, g.before = c.s.before;
+    g.tile = c.s.tile + c.begin;
+    g.count = int(min(end - c.at, int64_t(c.s.tiles - c.begin)));
+    g.whole = g.count == c.s.tiles;
+    c.at += g.count;
+    c.begin += g.count;
+}
+
+template <int N>
+struct Words;
+template <>
+struct Words<1> { using type = uint32_t; };
+template <>
+struct Words<2> { using type = uint2; };
+template <>
+struct Words<4> { using type = uint4; };
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t *from, uint32_t (&w)[N]) {
+    *reinterpret_cast<typename Words<N>::type *>(w) = *reinterpret_cast<const typename Words<N>::type *>(from);
+}
 
 template <class T, int D, int NT>
 __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) rows_kernel(sq_kv_attention_args a, int most_rows) {
@@ -203,9 +257,12 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
     extern __shared__ __align__(128) uint8_t rings[];
     __shared__ uint64_t bars[kWarps][kStages];
     __shared__ float row_max[kWarps][kRows], row_sum[kWarps][kRows];
+    __shared__ Segment segments[4];  // this one, the next (whose first tiles are requested meanwhile) and the one after
+    __shared__ Cursor cursor;
     __shared__ int abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    uint8_t *ring = rings + warp * Shape::kRing;
+    uint8_t *const ring = rings + warp * Shape::kRing;
+    float *const merge = reinterpret_cast<float *>(rings + kWarps * Shape::kRing);
     if (threadIdx.x == 0) abort_flag = 0;
     if (lane == 0) {
         for (int i = 0; i < kStages; ++i) tc::bar_init(&bars[warp][i], 1);
@@ -217,67 +274,99 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
     const int group = a.q_heads / a.heads, page_tiles = a.page_size / kTile;
     const float to_log2 = a.scale * kLog2e;
     const int64_t head_bytes = int64_t(page_tiles) * Tile::kBytes;
-    uint32_t used = 0;  // of this warp's stages, ever
-    int n = span.sequence;
-    int64_t offset = span.offset;
-    Sequence seq = sequence<kRows>(a, most_rows, min(n, a.num_seqs - 1), false);
-    for (int64_t at = span.begin; at < span.end;) {
-        while (offset >= seq.cost) {  // on to the next sequence with new tokens: there is one, as at < span.end
-            seq = sequence<kRows>(a, most_rows, ++n, false);
-            offset = 0;
+    // Queries on their way to L2: two lines of 128 bytes a lane at most.
+    auto fetch_rows = [&](const Segment &s) {
+        constexpr int kLines = (D * 2 + 127) / 128;
+        for (int i = lane; i < kRows * kLines && s.count; i += 32) {
+            const int64_t row = int64_t(s.block) * kRows + i / kLines;
+            if (row < int64_t(s.tokens) * group) {
+                const T *from = static_cast<const T *>(a.q) + (s.first + row / group) * a.q_stride +
+                                (s.head * group + row % group) * a.q_head_stride + i % kLines * 64;
+                asm volatile("prefetch.global.L2 [%0];\n" ::"l"(from));
+            }
         }
-        const int64_t item = offset / seq.tiles;
-        const int head = int(item / seq.blocks), block = int(item % seq.blocks);
-        const int begin = int(offset % seq.tiles), count = int(min(span.end - at, int64_t(seq.tiles - begin)));
-        const bool whole = count == seq.tiles;
-        const int64_t slot = 2 * blockIdx.x + (at == span.begin ? 0 : 1);
-        at += count;
-        offset += count;
+    };
+    if (warp == 0) {
+        if (lane == 0) {
+            Cursor c;
+            c.at = span.begin;
+            c.n = span.sequence;
+            c.s = sequence<kRows>(a, most_rows, min(c.n, a.num_seqs - 1), false);
+            const int64_t item = c.s.cost ? span.offset / c.s.tiles : 0;
+            c.begin = c.s.cost ? int(span.offset % c.s.tiles) : 0;
+            c.head = c.s.cost ? int(item / c.s.blocks) : 0;
+            c.block = c.s.cost ? int(item % c.s.blocks) : 0;
+            next_segment<kRows>(a, most_rows, span.end, c, segments[0]);
+            next_segment<kRows>(a, most_rows, span.end, c, segments[1]);
+            cursor = c;
+        }
+        __syncwarp();
+        fetch_rows(segments[0]);
+        fetch_rows(segments[1]);
+    }
+    __syncthreads();
 
-        // This warp's tiles of the segment: begin + warp, begin + warp + 8, ...
-        const int mine = (count - warp + kWarps - 1) / kWarps;
-        const int first_tile = seq.tile + begin + warp;
-        const int32_t *table = a.page_table + n * a.table_stride;
-        int pages = 0;
-        uint32_t held = 0;  // by tile, modulo 32: whether there was one to load
-        auto request = [&](int i) {  // tile i of this warp
-            if ((i & 31) == 0) {
-                const int index = (first_tile + (i + lane) * kWarps) / page_tiles;
-                pages = i + lane < mine && index < a.table_width ? table[index] : 0;
-                if (pages >= a.num_pages) {
-                    flag(a.status, SQ_STATUS_SLOT_RANGE);
-                    pages = 0;
-                }
+    // This warp's tiles of a segment are number warp, warp + 8, ...; its ring holds those of this segment and then
+    // of the next.
+    auto tiles_of = [&](const Segment &s) { return (s.count - warp + kWarps - 1) / kWarps; };
+    int requests = 0, request_stage = 0;
+    int64_t places = -1;  // lane i: byte offset of tile i, modulo 32, of the segment that is requested; -1: none
+    uint32_t held = 0;    // by stage: whether there was a tile to load
+    auto request = [&](const Segment &s, int i) {
+        if ((i & 31) == 0) {
+            places = -1;
+            const int tile = s.tile + warp + (i + lane) * kWarps, index = tile / page_tiles;
+            if (warp + (i + lane) * kWarps < s.count && index < a.table_width) {
+                const int page = a.page_table[s.sequence * a.table_stride + index];
+                if (page >= a.num_pages) flag(a.status, SQ_STATUS_SLOT_RANGE);
+                else if (page > 0) places = (int64_t(page) * a.heads + s.head) * head_bytes + int64_t(tile - index * page_tiles) * Tile::kBytes;
             }
-            const int page = __shfl_sync(~0u, pages, i & 31);
-            const uint32_t bit = 1u << (i & 31);
-            held = page > 0 ? held | bit : held & ~bit;
+        }
+        const int64_t place = __shfl_sync(~0u, places, i & 31);
+        held = place >= 0 ? held | 1u << request_stage : held & ~(1u << request_stage);
+        if (lane == 0) {
+            uint64_t *bar = &bars[warp][request_stage];
+            if (place >= 0) {
+                tc::bar_expect(bar, Tile::kBytes);
+                tc::bulk_load(ring + request_stage * Tile::kBytes, a.data + place, Tile::kBytes, bar);
+            } else {
+                tc::bar_arrive(bar);
+            }
+        }
+        ++requests;
+        request_stage = request_stage + 1 == kStages ? 0 : request_stage + 1;
+    };
+    int ahead = 0;  // tiles of the next segment that were requested
+    int stage = 0;
+    uint32_t phase = 0;
+    bool gave_up = false;
+    for (int number = 0; segments[number & 3].count; ++number) {
+        const Segment s = segments[number & 3];
+        const Segment &next = segments[(number + 1) & 3];
+        const int mine = tiles_of(s);
+        for (int i = ahead; i < min(mine, kStages); ++i) request(s, i);
+        ahead = min(mine, max(ahead, kStages));
+        if (warp == (number & (kWarps - 1))) {
             if (lane == 0) {
-                const int stage = (used + i) % kStages;
-                if (page > 0) {
-                    const int in_page = (first_tile + i * kWarps) % page_tiles;
-                    tc::bar_expect(&bars[warp][stage], Tile::kBytes);
-                    tc::bulk_load(ring + stage * Tile::kBytes,
-                                  a.data + (int64_t(page) * a.heads + head) * head_bytes + int64_t(in_page) * Tile::kBytes,
-                                  Tile::kBytes, &bars[warp][stage]);
-                } else {
-                    tc::bar_arrive(&bars[warp][stage]);
-                }
+                Cursor c = cursor;
+                next_segment<kRows>(a, most_rows, span.end, c, segments[(number + 2) & 3]);
+                cursor = c;
             }
-        };
-        for (int i = 0; i < min(mine, kStages); ++i) request(i);
+            __syncwarp();
+            fetch_rows(segments[(number + 2) & 3]);
+        }
 
         // Query rows as the product's second operand: row g's channels 16 t + 0..15 of each group.
         uint32_t q[NT][kGroups][8];
         float q_sum[NT][kGroups][2];  // of rows 2 t and 2 t + 1: the groups' sums
-        int64_t limit[NT][2];
-        const int64_t row0 = int64_t(block) * kRows, rows = int64_t(seq.count) * group;
+        int limit[NT][2];
+        const int64_t row0 = int64_t(s.block) * kRows, rows = int64_t(s.tokens) * group;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int64_t row = row0 + j * 8 + g;
             const bool live = row < rows;
-            const T *from = static_cast<const T *>(a.q) + (seq.first + (live ? row / group : 0)) * a.q_stride +
-                            (head * group + (live ? row % group : 0)) * a.q_head_stride + 16 * t;
+            const int token = live ? int(row / group) : 0, head = live ? int(row - int64_t(token) * group) : 0;
+            const T *from = static_cast<const T *>(a.q) + (int64_t(s.first) + token) * a.q_stride + (s.head * group + head) * a.q_head_stride + 16 * t;
 #pragma unroll
             for (int b = 0; b < kGroups; ++b) {
                 const uint4 x = reinterpret_cast<const uint4 *>(from + b * kGroup)[0], y = reinterpret_cast<const uint4 *>(from + b * kGroup)[1];
@@ -297,13 +386,13 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int64_t r = row0 + j * 8 + 2 * t + e;
-                limit[j][e] = r < rows ? min(seq.before + r / group, int64_t(seq.length) - 1) : -1;
+                limit[j][e] = r < rows ? int(max(int64_t(-1), min(s.before + r / group, int64_t(s.length) - 1))) : -1;
             }
         }
         // Tiles that every row sees whole: up to `sees_all`, from `window_all` on.
         const int64_t last_row = min(row0 + kRows, rows) - 1;
-        const int64_t sees_all = min(seq.before + row0 / group + 1, int64_t(seq.length)) / kTile;
-        const int64_t window_all = a.window > 0 ? (max(int64_t(0), seq.before + last_row / group - a.window + 1) + kTile - 1) / kTile : 0;
+        const int sees_all = int(max(int64_t(0), min(s.before + row0 / group + 1, int64_t(s.length))) / kTile);
+        const int window_all = a.window > 0 ? int(min(max(int64_t(0), s.before + last_row / group - a.window + 1) + kTile - 1, int64_t(0x7fffffff)) / kTile) : 0;
 
         float acc[NT][kGroups][4][4], ones[NT][kGroups][4], least[NT][kGroups][2];
         float top[NT][2], sum[NT][2];
@@ -322,59 +411,64 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
             top[j][0] = top[j][1] = -INFINITY;
             sum[j][0] = sum[j][1] = 0.f;
         }
-        bool gave_up = false;
+        int next_ahead = 0;
+        const int next_mine = tiles_of(next);
+#pragma unroll 1
         for (int i = 0; i < mine; ++i) {
-            const uint32_t use = used + i;
-            const int stage = use % kStages;
-            if (!tc::bar_wait(&bars[warp][stage], (use / kStages) & 1, &abort_flag, tc::kWaitClocks)) gave_up = true;
-            if (held >> (i & 31) & 1) {
+            if (!tc::bar_wait(&bars[warp][stage], phase, &abort_flag, tc::kWaitClocks)) gave_up = true;
+            if (held >> stage & 1) {
                 const uint8_t *tile = ring + stage * Tile::kBytes;
                 // Scores of tokens (rows g, g + 8) x query rows (2 t, 2 t + 1).
                 float z[NT][4];
 #pragma unroll
                 for (int j = 0; j < NT; ++j) z[j][0] = z[j][1] = z[j][2] = z[j][3] = 0.f;
+                uint32_t key_pairs[2][kGroups];
+                load_words(tile + Tile::kKeyPairs + g * kGroups * 4, key_pairs[0]);
+                load_words(tile + Tile::kKeyPairs + (g + 8) * kGroups * 4, key_pairs[1]);
 #pragma unroll
-                for (int b = 0; b < kGroups; ++b) {
-                    const int at_word = (b / Tile::kBlockGroups) * kTile * Tile::kBlockRow + (b % Tile::kBlockGroups) * 8 + t * 8 * Tile::kBlockGroups;
-                    const uint2 lo = *reinterpret_cast<const uint2 *>(tile + at_word + g * Tile::kBlockRow);
-                    const uint2 hi = *reinterpret_cast<const uint2 *>(tile + at_word + (g + 8) * Tile::kBlockRow);
-                    float d[NT][4];
+                for (int block = 0; block < kGroups / Tile::kBlockGroups; ++block) {
+                    uint32_t lo[2 * Tile::kBlockGroups], hi[2 * Tile::kBlockGroups];
+                    const uint8_t *from = tile + block * kTile * Tile::kBlockRow + t * 8 * Tile::kBlockGroups;
+                    load_words(from + g * Tile::kBlockRow, lo);
+                    load_words(from + (g + 8) * Tile::kBlockRow, hi);
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) d[j][0] = d[j][1] = d[j][2] = d[j][3] = 0.f;
+                    for (int half = 0; half < Tile::kBlockGroups; ++half) {
+                        const int b = block * Tile::kBlockGroups + half;
+                        float d[NT][4];
 #pragma unroll
-                    for (int w = 0; w < 2; ++w) {
-                        const uint32_t x = w ? lo.y : lo.x, y = w ? hi.y : hi.x;
+                        for (int j = 0; j < NT; ++j) d[j][0] = d[j][1] = d[j][2] = d[j][3] = 0.f;
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const uint32_t a0 = C::pair(x >> (8 * h)), a1 = C::pair(y >> (8 * h));
-                            const uint32_t a2 = C::pair(x >> (8 * h + 4)), a3 = C::pair(y >> (8 * h + 4));
+                        for (int w = 0; w < 2; ++w) {
+                            const uint32_t x = lo[2 * half + w], y = hi[2 * half + w];
 #pragma unroll
-                            for (int j = 0; j < NT; ++j) C::mma(d[j], a0, a1, a2, a3, q[j][b][4 * w + 2 * h], q[j][b][4 * w + 2 * h + 1]);
+                            for (int h = 0; h < 2; ++h) {
+                                const uint32_t a0 = C::pair(x >> (8 * h)), a1 = C::pair(y >> (8 * h));
+                                const uint32_t a2 = C::pair(x >> (8 * h + 4)), a3 = C::pair(y >> (8 * h + 4));
+#pragma unroll
+                                for (int j = 0; j < NT; ++j) C::mma(d[j], a0, a1, a2, a3, q[j][b][4 * w + 2 * h], q[j][b][4 * w + 2 * h + 1]);
+                            }
+                        }
+                        const float s0 = pair_scale(key_pairs[0][b]), s1 = pair_scale(key_pairs[1][b]);
+                        const float m0 = pair_min(key_pairs[0][b]) - C::kHeld * s0, m1 = pair_min(key_pairs[1][b]) - C::kHeld * s1;
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+                            z[j][0] += s0 * d[j][0] + m0 * q_sum[j][b][0];
+                            z[j][1] += s0 * d[j][1] + m0 * q_sum[j][b][1];
+                            z[j][2] += s1 * d[j][2] + m1 * q_sum[j][b][0];
+                            z[j][3] += s1 * d[j][3] + m1 * q_sum[j][b][1];
                         }
                     }
-                    const uint32_t p0 = *reinterpret_cast<const uint32_t *>(tile + Tile::kKeyPairs + (g * kGroups + b) * 4);
-                    const uint32_t p1 = *reinterpret_cast<const uint32_t *>(tile + Tile::kKeyPairs + ((g + 8) * kGroups + b) * 4);
-                    const float s0 = pair_scale(p0), s1 = pair_scale(p1);
-                    const float m0 = pair_min(p0) - C::kHeld * s0, m1 = pair_min(p1) - C::kHeld * s1;
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        z[j][0] += s0 * d[j][0] + m0 * q_sum[j][b][0];
-                        z[j][1] += s0 * d[j][1] + m0 * q_sum[j][b][1];
-                        z[j][2] += s1 * d[j][2] + m1 * q_sum[j][b][0];
-                        z[j][3] += s1 * d[j][3] + m1 * q_sum[j][b][1];
-                    }
                 }
-                const int index = first_tile + i * kWarps;
-                const bool partial = index >= sees_all || index < window_all;
+                const int index = s.tile + warp + i * kWarps;
                 uint32_t hidden = 0;  // bits of z
-                if (partial) {
+                if (index >= sees_all || index < window_all) {
                     // Row r of a tile is token r / 2 + 4 (r % 2) of its half.
-                    const int64_t token = int64_t(index) * kTile + (g >> 1) + 4 * (g & 1);
+                    const int token = index * kTile + (g >> 1) + 4 * (g & 1);
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
                         for (int i4 = 0; i4 < 4; ++i4) {
-                            const int64_t p = token + (i4 & 2) * 4, last = limit[j][i4 & 1];
+                            const int p = token + (i4 & 2) * 4, last = limit[j][i4 & 1];
                             if (p > last || (a.window > 0 && p <= last - a.window)) hidden |= 1u << (4 * j + i4);
                         }
                 }
@@ -383,7 +477,12 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
 #pragma unroll
-                    for (int i4 = 0; i4 < 4; ++i4) z[j][i4] = hidden >> (4 * j + i4) & 1 ? -INFINITY : z[j][i4] * to_log2;
+                    for (int i4 = 0; i4 < 4; ++i4) z[j][i4] *= to_log2;
+                    if (hidden) {
+#pragma unroll
+                        for (int i4 = 0; i4 < 4; ++i4)
+                            if (hidden >> (4 * j + i4) & 1) z[j][i4] = -INFINITY;
+                    }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         most[j][e] = fmaxf(z[j][e], z[j][2 + e]);
@@ -423,34 +522,37 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                         sum[j][i4 & 1] += z[j][i4];
                     }
                 // Values: rows are channels (x: even ones, y: odd ones), columns query rows.
+                uint32_t value_pairs[2][kGroups], word[4][kGroups];
+                load_words(tile + Tile::kValuePairs + g * kGroups * 4, value_pairs[0]);
+                load_words(tile + Tile::kValuePairs + (g + 8) * kGroups * 4, value_pairs[1]);
+                const uint8_t *from = tile + Tile::kValues + (kGroups * g >> 3) * kTile * 32 + (kGroups * g & 7) * 4 + t * 32;
+#pragma unroll
+                for (int i4 = 0; i4 < 4; ++i4) load_words(from + i4 * 4 * 32, word[i4]);
 #pragma unroll
                 for (int b = 0; b < kGroups; ++b) {
-                    const uint32_t p0 = *reinterpret_cast<const uint32_t *>(tile + Tile::kValuePairs + (g * kGroups + b) * 4);
-                    const uint32_t p1 = *reinterpret_cast<const uint32_t *>(tile + Tile::kValuePairs + ((g + 8) * kGroups + b) * 4);
-                    const float s0 = pair_scale(p0), s1 = pair_scale(p1), m0 = pair_min(p0) + kMiddle * s0, m1 = pair_min(p1) + kMiddle * s1;
+                    const float s0 = pair_scale(value_pairs[0][b]), s1 = pair_scale(value_pairs[1][b]);
+                    const float m0 = pair_min(value_pairs[0][b]) + kMiddle * s0, m1 = pair_min(value_pairs[1][b]) + kMiddle * s1;
                     uint32_t w0[NT], w1[NT];
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
                         float u[4] = {z[j][0] * s0, z[j][1] * s0, z[j][2] * s1, z[j][3] * s1};
-                        float v[4] = {z[j][0] * m0, z[j][1] * m0, z[j][2] * m1, z[j][3] * m1};
-                        if (hidden) {  // a hidden token's scale may be anything
+                        if (hidden) {  // a hidden token's scale and minimum may be anything
+                            float v[4] = {z[j][0] * m0, z[j][1] * m0, z[j][2] * m1, z[j][3] * m1};
 #pragma unroll
                             for (int i4 = 0; i4 < 4; ++i4)
                                 if (hidden >> (4 * j + i4) & 1) u[i4] = v[i4] = 0.f;
+                            least[j][b][0] += v[0] + v[2];
+                            least[j][b][1] += v[1] + v[3];
+                        } else {
+                            least[j][b][0] += z[j][0] * m0 + z[j][2] * m1;
+                            least[j][b][1] += z[j][1] * m0 + z[j][3] * m1;
                         }
-                        least[j][b][0] += v[0] + v[2];
-                        least[j][b][1] += v[1] + v[3];
                         w0[j] = transpose8(C::pack(u[0], u[1]));
                         w1[j] = transpose8(C::pack(u[2], u[3]));
                         if (C::kHeld != -kMiddle) C::mma(ones[j][b], C::kOnes, C::kOnes, C::kOnes, C::kOnes, w0[j], w1[j]);
                     }
-                    const int number = kGroups * g + b;
-                    const uint8_t *from = tile + Tile::kValues + (number >> 3) * kTile * 32 + (number & 7) * 4 + t * 32;
-                    uint32_t word[4];
-#pragma unroll
-                    for (int i4 = 0; i4 < 4; ++i4) word[i4] = *reinterpret_cast<const uint32_t *>(from + i4 * 4 * 32);
-                    const uint32_t x0 = __byte_perm(word[0], word[1], 0x5410), y0 = __byte_perm(word[0], word[1], 0x7632);
-                    const uint32_t x1 = __byte_perm(word[2], word[3], 0x5410), y1 = __byte_perm(word[2], word[3], 0x7632);
+                    const uint32_t x0 = __byte_perm(word[0][b], word[1][b], 0x5410), y0 = __byte_perm(word[0][b], word[1][b], 0x7632);
+                    const uint32_t x1 = __byte_perm(word[2][b], word[3][b], 0x5410), y1 = __byte_perm(word[2][b], word[3][b], 0x7632);
 #pragma unroll
                     for (int m = 0; m < 4; ++m) {
                         const uint32_t a0 = C::pair(x0 >> (4 * m)), a1 = C::pair(y0 >> (4 * m));
@@ -461,19 +563,15 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                 }
             }
             __syncwarp();
-            if (i + kStages < mine) request(i + kStages);
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+            phase ^= stage == 0;
+            if (ahead < mine) request(s, ahead++);
+            else if (next_ahead < next_mine) request(next, next_ahead++);
         }
-        used += mine;
+        ahead = next_ahead;
         gave_up = __any_sync(~0u, gave_up);
-        if (gave_up) {  // the copies still on their way end before the ring is used again
-            flag(a.status, SQ_STATUS_TIMEOUT);
-            int alone = 0;
-            for (int i = max(0, mine - kStages); i < mine; ++i)
-                tc::bar_wait(&bars[warp][(used - mine + i) % kStages], ((used - mine + i) / kStages) & 1, &alone, tc::kWaitClocks);
-        }
 
-        // The warps' sums, to shared memory (each into its own, idle, ring), then to the output or a part.
-        float *mine_out = reinterpret_cast<float *>(ring);
+        // The warps' sums, to shared memory, then to the output or a part.
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -489,7 +587,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
 #pragma unroll
                     for (int i = 4; i < 32; i *= 2) low_part += __shfl_xor_sync(~0u, low_part, i);
                     low_part -= (C::kHeld + kMiddle) * ones[j][b][e];
-                    float *to = mine_out + row * Shape::kMergeRow + b * kGroup + 8 * g;
+                    float *to = merge + (warp * kRows + row) * Shape::kMergeRow + b * kGroup + 8 * g;
 #pragma unroll
                     for (int m = 0; m < 4; m += 2)
                         *reinterpret_cast<float4 *>(to + 2 * m) =
@@ -498,7 +596,8 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                 }
             }
         __syncthreads();
-        const int warps = min(count, kWarps);  // that had tiles
+        const int warps = min(s.count, kWarps);  // that had tiles
+        const int64_t slot = 2 * blockIdx.x + (number == 0 ? 0 : 1);
         float *part = reinterpret_cast<float *>(a.workspace) + slot * Shape::kPart;
         for (int i = threadIdx.x; i < kRows * D / 4; i += kAttnThreads) {
             const int row = i / (D / 4), c = i % (D / 4) * 4;
@@ -514,14 +613,15 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
             for (int w = 0; w < warps; ++w) {
                 const float factor = row_max[w][row] == -INFINITY ? 0.f : exp2_approx(row_max[w][row] - most);
                 if (factor == 0.f) continue;
-                const float4 y = *reinterpret_cast<const float4 *>(reinterpret_cast<float *>(rings + w * Shape::kRing) + row * Shape::kMergeRow + c);
+                const float4 y = *reinterpret_cast<const float4 *>(merge + (w * kRows + row) * Shape::kMergeRow + c);
                 x.x += factor * y.x, x.y += factor * y.y, x.z += factor * y.z, x.w += factor * y.w;
                 weight += factor * row_sum[w][row];
             }
-            if (whole) {
+            if (s.whole) {
                 if (row0 + row < rows) {
                     const float per = weight == 0.f ? 0.f : 1.f / weight;
-                    T *out = output_row<T>(a, seq, head, row0 + row) + c;
+                    const int token = int((row0 + row) / group), head = s.head * group + int((row0 + row) - int64_t(token) * group);
+                    T *out = static_cast<T *>(a.out) + ((int64_t(s.first) + token) * a.q_heads + head) * D + c;
                     *reinterpret_cast<uint2 *>(out) = make_uint2(C::pack(x.x * per, x.y * per), C::pack(x.z * per, x.w * per));
                 }
             } else {
@@ -529,8 +629,13 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                 if (c == 0) part[kRows * D + row] = most, part[kRows * D + kRows + row] = weight;
             }
         }
-        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // before copies into the rings again
         __syncthreads();
+    }
+    if (gave_up) {  // the copies still on their way end before the CTA does
+        if (lane == 0) flag(a.status, SQ_STATUS_TIMEOUT);
+        int alone = 0;
+        for (int r = max(0, requests - kStages); r < requests; ++r)
+            tc::bar_wait(&bars[warp][r % kStages], (r / kStages) & 1, &alone, tc::kWaitClocks);
     }
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 }
