@@ -19,7 +19,9 @@ namespace {
 
 constexpr int kWarps = 8, kAttnThreads = 32 * kWarps;
 constexpr int kMostCtas = 320;
-constexpr int kLeastTiles = 2 * kWarps;  // of a CTA
+constexpr int kUnit = 32;             // tokens that a warp takes at a time: two tiles of the cache
+constexpr int kLeastUnits = kWarps;   // of a CTA
+constexpr float kNone = -3.402823466e38f;  // a maximum over nothing
 constexpr int kFewRows = 32;
 
 // ---------------------------------------------------------------------------
@@ -87,14 +89,14 @@ __device__ __forceinline__ float pair_scale(uint32_t p) { return __uint_as_float
 __device__ __forceinline__ float pair_min(uint32_t p) { return __uint_as_float(p & 0xFFFF0000u); }
 
 // ---------------------------------------------------------------------------
-// work: tiles of 16 tokens in the order (sequence, kv head, block of rows, tile), cut into equal
+// work: units of 32 tokens in the order (sequence, kv head, block of rows, unit), cut into equal
 // spans of consecutive ones, a span to a CTA
 // ---------------------------------------------------------------------------
 struct Sequence {
     int first, count;   // new tokens
     int length;         // tokens that the page table reaches
     int64_t before;     // position of the first new token
-    int tile, tiles;    // tiles that any of them sees: one at least
+    int unit, units;    // units that any of them sees: one at least
     int blocks;         // of rows (token, query head of the kv head)
     int64_t cost;
 };
@@ -111,16 +113,16 @@ __device__ __forceinline__ Sequence sequence(const sq_kv_attention_args &a, int 
     s.length = int(max(int64_t(0), min(int64_t(length), most)));
     s.before = int64_t(length) - s.count;
     const int64_t start = a.window > 0 ? max(int64_t(0), s.before - a.window + 1) : 0;
-    s.tile = int(min(start, int64_t(s.length)) / kTile);
-    s.tiles = max(1, (s.length + kTile - 1) / kTile - s.tile);
+    s.unit = int(min(start, int64_t(s.length)) / kUnit);
+    s.units = max(1, int((int64_t(s.length) + kUnit - 1) / kUnit) - s.unit);
     const int64_t rows = int64_t(s.count) * (a.q_heads / a.heads);
     s.blocks = rows > most_rows ? 0 : int((rows + ROWS - 1) / ROWS);
-    s.cost = int64_t(s.blocks) * a.heads * s.tiles;
+    s.cost = int64_t(s.blocks) * a.heads * s.units;
     return s;
 }
 
 struct Span {
-    int64_t begin, end, per;  // in tiles
+    int64_t begin, end, per;  // in units
     int sequence;             // that begin lies in
     int64_t offset;           // of begin in it
 };
@@ -152,7 +154,7 @@ __device__ __forceinline__ Span span_of(const sq_kv_attention_args &a, int most_
         total += warp_sums[w];
     }
     Span s;
-    s.per = max(int64_t(kLeastTiles), (total + gridDim.x - 1) / gridDim.x);
+    s.per = max(int64_t(kLeastUnits), (total + gridDim.x - 1) / gridDim.x);
     s.begin = min(total, s.per * blockIdx.x);
     s.end = min(total, s.begin + s.per);
     int64_t at = sum - mine;
@@ -186,8 +188,8 @@ template <int D, int NT>
 struct RowsShape {
     using Tile = KvTile<D>;
     static constexpr int kRows = 8 * NT;
-    static constexpr int kStages = D == 64 ? 6 : D == 128 ? 4 : 3;
-    static constexpr int kRing = kStages * Tile::kBytes;          // of a warp
+    static constexpr int kStages = D == 64 ? 3 : 2;  // units
+    static constexpr int kStage = 2 * Tile::kBytes, kRing = kStages * kStage;  // of a warp
     static constexpr int kMergeRow = D + 4;                       // floats
     static constexpr int kMerge = kRows * kMergeRow * 4;          // of a warp
     static constexpr int kPart = kRows * D + 2 * kRows;           // floats of a part: sums, maxima, weights' sums
@@ -195,27 +197,27 @@ struct RowsShape {
     static_assert(kRing % 16 == 0 && kMerge % 16 == 0 && Tile::kBytes % 16 == 0, "copies and sums are aligned");
 };
 
-// The tiles of one item that lie in a CTA's span.
+// The units of one item that lie in a CTA's span.
 struct Segment {
     int sequence, head, block;
     int first, tokens, length;  // the sequence's new tokens, tokens that it holds
     int64_t before;             // position of its first new token
-    int tile, count;            // first tile, tiles; none: the span is over
-    bool whole;                 // the item's tiles
+    int unit, count;            // first unit, units; none: the span is over
+    bool whole;                 // the item's units
 };
 
 // Where in its span a CTA is.
 struct Cursor {
     Sequence s;
     int64_t at;
-    int n, head, block, begin;  // begin: tiles of the item before
+    int n, head, block, begin;  // begin: units of the item before
 };
 
 template <int ROWS>
 __device__ __forceinline__ void next_segment(const sq_kv_attention_args &a, int most_rows, int64_t end, Cursor &c, Segment &g) {
     g.count = 0;
     if (c.at >= end) return;
-    if (c.begin >= c.s.tiles) {
+    if (c.begin >= c.s.units) {
         c.begin = 0;
         if (++c.block >= c.s.blocks) {
             c.block = 0;
@@ -228,9 +230,9 @@ __device__ __forceinline__ void next_segment(const sq_kv_attention_args &a, int 
     }
     g.sequence = c.n, g.head = c.head, g.block = c.block;
     g.first = c.s.first, g.tokens = c.s.count, g.length = c.s.length, g.before = c.s.before;
-    g.tile = c.s.tile + c.begin;
-    g.count = int(min(end - c.at, int64_t(c.s.tiles - c.begin)));
-    g.whole = g.count == c.s.tiles;
+    g.unit = c.s.unit + c.begin;
+    g.count = int(min(end - c.at, int64_t(c.s.units - c.begin)));
+    g.whole = g.count == c.s.units;
     c.at += g.count;
     c.begin += g.count;
 }
@@ -257,7 +259,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
     extern __shared__ __align__(128) uint8_t rings[];
     __shared__ uint64_t bars[kWarps][kStages];
     __shared__ float row_max[kWarps][kRows], row_sum[kWarps][kRows];
-    __shared__ Segment segments[4];  // this one, the next (whose first tiles are requested meanwhile) and the one after
+    __shared__ Segment segments[4];  // this one, the next (whose first units are requested meanwhile) and the one after
     __shared__ Cursor cursor;
     __shared__ int abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -272,7 +274,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
         clear_outside(a.out, int64_t(a.q_heads) * D * sizeof(T), a.cu_seqlens, a.num_seqs, a.tokens, blockIdx.x, gridDim.x);
     const Span span = span_of<kRows>(a, most_rows, blockIdx.x == 0);
     const int group = a.q_heads / a.heads, page_tiles = a.page_size / kTile;
-    const float to_log2 = a.scale * kLog2e;
+    const float to_log2 = a.scale * kLog2e, lag = C::kLag / to_log2;
     const int64_t head_bytes = int64_t(page_tiles) * Tile::kBytes;
     // Queries on their way to L2: two lines of 128 bytes a lane at most.
     auto fetch_rows = [&](const Segment &s) {
@@ -292,8 +294,8 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
             c.at = span.begin;
             c.n = span.sequence;
             c.s = sequence<kRows>(a, most_rows, min(c.n, a.num_seqs - 1), false);
-            const int64_t item = c.s.cost ? span.offset / c.s.tiles : 0;
-            c.begin = c.s.cost ? int(span.offset % c.s.tiles) : 0;
+            const int64_t item = c.s.cost ? span.offset / c.s.units : 0;
+            c.begin = c.s.cost ? int(span.offset % c.s.units) : 0;
             c.head = c.s.cost ? int(item / c.s.blocks) : 0;
             c.block = c.s.cost ? int(item % c.s.blocks) : 0;
             next_segment<kRows>(a, most_rows, span.end, c, segments[0]);
@@ -306,44 +308,41 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
     }
     __syncthreads();
 
-    // This warp's tiles of a segment are number warp, warp + 8, ...; its ring holds those of this segment and then
+    // This warp's units of a segment are number warp, warp + 8, ...; its ring holds those of this segment and then
     // of the next.
-    auto tiles_of = [&](const Segment &s) { return (s.count - warp + kWarps - 1) / kWarps; };
+    auto units_of = [&](const Segment &s) { return (s.count - warp + kWarps - 1) / kWarps; };
     int requests = 0, request_stage = 0;
-    int64_t places = -1;  // lane i: byte offset of tile i, modulo 32, of the segment that is requested; -1: none
-    uint32_t held = 0;    // by stage: whether there was a tile to load
+    int64_t places = -1;  // lane 2 i + h: byte offset of tile h of unit i, modulo 16, of the segment that is requested; -1: none
+    uint32_t missing = 0; // by stage, two bits: whether there was no tile to load
     auto request = [&](const Segment &s, int i) {
-        if ((i & 31) == 0) {
+        if ((i & 15) == 0) {
             places = -1;
-            const int tile = s.tile + warp + (i + lane) * kWarps, index = tile / page_tiles;
-            if (warp + (i + lane) * kWarps < s.count && index < a.table_width) {
+            const int unit = warp + (i + lane / 2) * kWarps, tile = (s.unit + unit) * 2 + (lane & 1), index = tile / page_tiles;
+            if (unit < s.count && index < a.table_width) {
                 const int page = a.page_table[s.sequence * a.table_stride + index];
                 if (page >= a.num_pages) flag(a.status, SQ_STATUS_SLOT_RANGE);
                 else if (page > 0) places = (int64_t(page) * a.heads + s.head) * head_bytes + int64_t(tile - index * page_tiles) * Tile::kBytes;
             }
         }
-        const int64_t place = __shfl_sync(~0u, places, i & 31);
-        held = place >= 0 ? held | 1u << request_stage : held & ~(1u << request_stage);
-        if (lane == 0) {
-            uint64_t *bar = &bars[warp][request_stage];
-            if (place >= 0) {
-                tc::bar_expect(bar, Tile::kBytes);
-                tc::bulk_load(ring + request_stage * Tile::kBytes, a.data + place, Tile::kBytes, bar);
-            } else {
-                tc::bar_arrive(bar);
-            }
-        }
+        // Lanes 0 and 1 fetch a tile each.
+        const int64_t place = __shfl_sync(~0u, places, 2 * (i & 15) + (lane & 1));
+        const uint32_t none = __ballot_sync(~0u, place < 0) & 3;
+        missing = (missing & ~(3u << 2 * request_stage)) | none << 2 * request_stage;
+        uint64_t *const bar = &bars[warp][request_stage];
+        if (lane == 0) tc::bar_expect(bar, (none == 0 ? 2 : none == 3 ? 0 : 1) * Tile::kBytes);
+        if (lane < 2 && place >= 0)
+            tc::bulk_load(ring + request_stage * Shape::kStage + lane * Tile::kBytes, a.data + place, Tile::kBytes, bar);
         ++requests;
         request_stage = request_stage + 1 == kStages ? 0 : request_stage + 1;
     };
-    int ahead = 0;  // tiles of the next segment that were requested
+    int ahead = 0;  // units of the next segment that were requested
     int stage = 0;
     uint32_t phase = 0;
     bool gave_up = false;
     for (int number = 0; segments[number & 3].count; ++number) {
         const Segment s = segments[number & 3];
         const Segment &next = segments[(number + 1) & 3];
-        const int mine = tiles_of(s);
+        const int mine = units_of(s);
         for (int i = ahead; i < min(mine, kStages); ++i) request(s, i);
         ahead = min(mine, max(ahead, kStages));
         if (warp == (number & (kWarps - 1))) {
@@ -389,13 +388,13 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                 limit[j][e] = r < rows ? int(max(int64_t(-1), min(s.before + r / group, int64_t(s.length) - 1))) : -1;
             }
         }
-        // Tiles that every row sees whole: up to `sees_all`, from `window_all` on.
+        // Units that every row sees whole: up to `sees_all`, from `window_all` on.
         const int64_t last_row = min(row0 + kRows, rows) - 1;
-        const int sees_all = int(max(int64_t(0), min(s.before + row0 / group + 1, int64_t(s.length))) / kTile);
-        const int window_all = a.window > 0 ? int(min(max(int64_t(0), s.before + last_row / group - a.window + 1) + kTile - 1, int64_t(0x7fffffff)) / kTile) : 0;
+        const int sees_all = int(max(int64_t(0), min(s.before + row0 / group + 1, int64_t(s.length))) / kUnit);
+        const int window_all = a.window > 0 ? int(min(max(int64_t(0), s.before + last_row / group - a.window + 1) + kUnit - 1, int64_t(0x7fffffff)) / kUnit) : 0;
 
         float acc[NT][kGroups][4][4], ones[NT][kGroups][4], least[NT][kGroups][2];
-        float top[NT][2], sum[NT][2];
+        float top[NT][2], against[NT][2], sum[NT][2];  // maxima of scores before `to_log2`
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -408,20 +407,23 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                 }
                 least[j][b][0] = least[j][b][1] = 0.f;
             }
-            top[j][0] = top[j][1] = -INFINITY;
+            top[j][0] = top[j][1] = kNone;
             sum[j][0] = sum[j][1] = 0.f;
+            against[j][0] = against[j][1] = 0.f;
         }
         int next_ahead = 0;
-        const int next_mine = tiles_of(next);
+        const int next_mine = units_of(next);
 #pragma unroll 1
         for (int i = 0; i < mine; ++i) {
             if (!tc::bar_wait(&bars[warp][stage], phase, &abort_flag, tc::kWaitClocks)) gave_up = true;
-            if (held >> stage & 1) {
-                const uint8_t *tile = ring + stage * Tile::kBytes;
-                // Scores of tokens (rows g, g + 8) x query rows (2 t, 2 t + 1).
-                float z[NT][4];
+            const uint8_t *const unit = ring + stage * Shape::kStage;
+            // Scores of tokens (rows g, g + 8 of each tile) x query rows (2 t, 2 t + 1).
+            float z[2][NT][4];
 #pragma unroll
-                for (int j = 0; j < NT; ++j) z[j][0] = z[j][1] = z[j][2] = z[j][3] = 0.f;
+            for (int h = 0; h < 2; ++h) {
+                const uint8_t *const tile = unit + h * Tile::kBytes;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) z[h][j][0] = z[h][j][1] = z[h][j][2] = z[h][j][3] = 0.f;
                 uint32_t key_pairs[2][kGroups];
                 load_words(tile + Tile::kKeyPairs + g * kGroups * 4, key_pairs[0]);
                 load_words(tile + Tile::kKeyPairs + (g + 8) * kGroups * 4, key_pairs[1]);
@@ -441,87 +443,91 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                         for (int w = 0; w < 2; ++w) {
                             const uint32_t x = lo[2 * half + w], y = hi[2 * half + w];
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const uint32_t a0 = C::pair(x >> (8 * h)), a1 = C::pair(y >> (8 * h));
-                                const uint32_t a2 = C::pair(x >> (8 * h + 4)), a3 = C::pair(y >> (8 * h + 4));
+                            for (int k = 0; k < 2; ++k) {
+                                const uint32_t a0 = C::pair(x >> (8 * k)), a1 = C::pair(y >> (8 * k));
+                                const uint32_t a2 = C::pair(x >> (8 * k + 4)), a3 = C::pair(y >> (8 * k + 4));
 #pragma unroll
-                                for (int j = 0; j < NT; ++j) C::mma(d[j], a0, a1, a2, a3, q[j][b][4 * w + 2 * h], q[j][b][4 * w + 2 * h + 1]);
+                                for (int j = 0; j < NT; ++j) C::mma(d[j], a0, a1, a2, a3, q[j][b][4 * w + 2 * k], q[j][b][4 * w + 2 * k + 1]);
                             }
                         }
                         const float s0 = pair_scale(key_pairs[0][b]), s1 = pair_scale(key_pairs[1][b]);
                         const float m0 = pair_min(key_pairs[0][b]) - C::kHeld * s0, m1 = pair_min(key_pairs[1][b]) - C::kHeld * s1;
 #pragma unroll
                         for (int j = 0; j < NT; ++j) {
-                            z[j][0] += s0 * d[j][0] + m0 * q_sum[j][b][0];
-                            z[j][1] += s0 * d[j][1] + m0 * q_sum[j][b][1];
-                            z[j][2] += s1 * d[j][2] + m1 * q_sum[j][b][0];
-                            z[j][3] += s1 * d[j][3] + m1 * q_sum[j][b][1];
+                            z[h][j][0] += s0 * d[j][0] + m0 * q_sum[j][b][0];
+                            z[h][j][1] += s0 * d[j][1] + m0 * q_sum[j][b][1];
+                            z[h][j][2] += s1 * d[j][2] + m1 * q_sum[j][b][0];
+                            z[h][j][3] += s1 * d[j][3] + m1 * q_sum[j][b][1];
                         }
                     }
                 }
-                const int index = s.tile + warp + i * kWarps;
-                uint32_t hidden = 0;  // bits of z
-                if (index >= sees_all || index < window_all) {
-                    // Row r of a tile is token r / 2 + 4 (r % 2) of its half.
-                    const int token = index * kTile + (g >> 1) + 4 * (g & 1);
+            }
+            const int index = s.unit + warp + i * kWarps;
+            const uint32_t none = missing >> 2 * stage & 3;
+            uint32_t hidden = 0;  // bits of z
+            if (index >= sees_all || index < window_all || none) {
+                // Row r of a tile is token r / 2 + 4 (r % 2) of its half.
+                const int token = index * kUnit + (g >> 1) + 4 * (g & 1);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
                         for (int i4 = 0; i4 < 4; ++i4) {
-                            const int p = token + (i4 & 2) * 4, last = limit[j][i4 & 1];
-                            if (p > last || (a.window > 0 && p <= last - a.window)) hidden |= 1u << (4 * j + i4);
-                        }
-                }
-                float most[NT][2];
-                bool grows = false;
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-#pragma unroll
-                    for (int i4 = 0; i4 < 4; ++i4) z[j][i4] *= to_log2;
-                    if (hidden) {
-#pragma unroll
-                        for (int i4 = 0; i4 < 4; ++i4)
-                            if (hidden >> (4 * j + i4) & 1) z[j][i4] = -INFINITY;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        most[j][e] = fmaxf(z[j][e], z[j][2 + e]);
-                        grows = grows || most[j][e] > top[j][e] + C::kLag;
-                    }
-                }
-                // The maxima that weights are taken against may lag behind by 2^kLag: they move seldom.
-                if (__any_sync(~0u, grows)) {
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float x = most[j][e];
-                            x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
-                            x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
-                            x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
-                            x = fmaxf(x, top[j][e]);
-                            const float factor = x == -INFINITY ? 1.f : exp2_approx(top[j][e] - x);
-                            top[j][e] = x;
-                            sum[j][e] *= factor;
-#pragma unroll
-                            for (int b = 0; b < kGroups; ++b) {
-                                least[j][b][e] *= factor;
-                                ones[j][b][e] *= factor;
-                                ones[j][b][2 + e] *= factor;
-#pragma unroll
-                                for (int m = 0; m < 4; ++m) acc[j][b][m][e] *= factor, acc[j][b][m][2 + e] *= factor;
+                            const int p = token + h * kTile + (i4 & 2) * 4, last = limit[j][i4 & 1];
+                            if (p > last || (a.window > 0 && p <= last - a.window) || (none >> h & 1)) {
+                                hidden |= 1u << (4 * (h * NT + j) + i4);
+                                z[h][j][i4] = -INFINITY;
                             }
                         }
+            }
+            float most[NT][2];
+            bool grows = false;
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    most[j][e] = fmaxf(fmaxf(z[0][j][e], z[0][j][2 + e]), fmaxf(z[1][j][e], z[1][j][2 + e]));
+                    grows = grows || most[j][e] > top[j][e] + lag;
                 }
+            // The maxima that weights are taken against may lag behind by 2^kLag: they move seldom.
+            if (__any_sync(~0u, grows)) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float x = most[j][e];
+                        x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
+                        x = fmaxf(x, top[j][e]);
+                        const float factor = exp2_approx((top[j][e] - x) * to_log2);
+                        top[j][e] = x;
+                        against[j][e] = -x * to_log2;
+                        sum[j][e] *= factor;
+#pragma unroll
+                        for (int b = 0; b < kGroups; ++b) {
+                            least[j][b][e] *= factor;
+                            ones[j][b][e] *= factor;
+                            ones[j][b][2 + e] *= factor;
+#pragma unroll
+                            for (int m = 0; m < 4; ++m) acc[j][b][m][e] *= factor, acc[j][b][m][2 + e] *= factor;
+                        }
+                    }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
                     for (int i4 = 0; i4 < 4; ++i4) {
-                        const float against = top[j][i4 & 1];
-                        z[j][i4] = exp2_approx(z[j][i4] - (against == -INFINITY ? 0.f : against));
-                        sum[j][i4 & 1] += z[j][i4];
+                        z[h][j][i4] = exp2_approx(fmaf(z[h][j][i4], to_log2, against[j][i4 & 1]));
+                        sum[j][i4 & 1] += z[h][j][i4];
                     }
-                // Values: rows are channels (x: even ones, y: odd ones), columns query rows.
+            // Values: rows are channels (x: even ones, y: odd ones), columns query rows.
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint8_t *const tile = unit + h * Tile::kBytes;
                 uint32_t value_pairs[2][kGroups], word[4][kGroups];
                 load_words(tile + Tile::kValuePairs + g * kGroups * 4, value_pairs[0]);
                 load_words(tile + Tile::kValuePairs + (g + 8) * kGroups * 4, value_pairs[1]);
@@ -535,18 +541,15 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                     uint32_t w0[NT], w1[NT];
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
-                        float u[4] = {z[j][0] * s0, z[j][1] * s0, z[j][2] * s1, z[j][3] * s1};
+                        float u[4] = {z[h][j][0] * s0, z[h][j][1] * s0, z[h][j][2] * s1, z[h][j][3] * s1};
+                        float v[4] = {z[h][j][0] * m0, z[h][j][1] * m0, z[h][j][2] * m1, z[h][j][3] * m1};
                         if (hidden) {  // a hidden token's scale and minimum may be anything
-                            float v[4] = {z[j][0] * m0, z[j][1] * m0, z[j][2] * m1, z[j][3] * m1};
 #pragma unroll
                             for (int i4 = 0; i4 < 4; ++i4)
-                                if (hidden >> (4 * j + i4) & 1) u[i4] = v[i4] = 0.f;
-                            least[j][b][0] += v[0] + v[2];
-                            least[j][b][1] += v[1] + v[3];
-                        } else {
-                            least[j][b][0] += z[j][0] * m0 + z[j][2] * m1;
-                            least[j][b][1] += z[j][1] * m0 + z[j][3] * m1;
+                                if (hidden >> (4 * (h * NT + j) + i4) & 1) u[i4] = v[i4] = 0.f;
                         }
+                        least[j][b][0] += v[0] + v[2];
+                        least[j][b][1] += v[1] + v[3];
                         w0[j] = transpose8(C::pack(u[0], u[1]));
                         w1[j] = transpose8(C::pack(u[2], u[3]));
                         if (C::kHeld != -kMiddle) C::mma(ones[j][b], C::kOnes, C::kOnes, C::kOnes, C::kOnes, w0[j], w1[j]);
@@ -580,7 +583,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                 float total = sum[j][e];
 #pragma unroll
                 for (int i = 4; i < 32; i *= 2) total += __shfl_xor_sync(~0u, total, i);
-                if (g == 0) row_max[warp][row] = gave_up ? NAN : top[j][e], row_sum[warp][row] = total;
+                if (g == 0) row_max[warp][row] = gave_up ? NAN : top[j][e] == kNone ? kNone : -against[j][e], row_sum[warp][row] = total;
 #pragma unroll
                 for (int b = 0; b < kGroups; ++b) {
                     float low_part = least[j][b][e];
@@ -596,12 +599,12 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                 }
             }
         __syncthreads();
-        const int warps = min(s.count, kWarps);  // that had tiles
+        const int warps = min(s.count, kWarps);  // that had units
         const int64_t slot = 2 * blockIdx.x + (number == 0 ? 0 : 1);
         float *part = reinterpret_cast<float *>(a.workspace) + slot * Shape::kPart;
         for (int i = threadIdx.x; i < kRows * D / 4; i += kAttnThreads) {
             const int row = i / (D / 4), c = i % (D / 4) * 4;
-            float most = -INFINITY;
+            float most = kNone;
             bool bad = false;
             for (int w = 0; w < warps; ++w) {
                 most = fmaxf(most, row_max[w][row]);
@@ -611,8 +614,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
             float weight = 0.f;
             for (int w = 0; w < warps; ++w) {
-                const float factor = row_max[w][row] == -INFINITY ? 0.f : exp2_approx(row_max[w][row] - most);
-                if (factor == 0.f) continue;
+                const float factor = exp2_approx(row_max[w][row] - most);
                 const float4 y = *reinterpret_cast<const float4 *>(merge + (w * kRows + row) * Shape::kMergeRow + c);
                 x.x += factor * y.x, x.y += factor * y.y, x.z += factor * y.z, x.w += factor * y.w;
                 weight += factor * row_sum[w][row];
@@ -652,9 +654,9 @@ __global__ void __launch_bounds__(kAttnThreads) join_kernel(sq_kv_attention_args
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     if (span.begin >= span.end) return;
     const Sequence seq = sequence<kRows>(a, most_rows, span.sequence, false);
-    const int done = int(span.offset % seq.tiles);  // tiles of the item before this span
-    if (done == 0 || seq.tiles - done > span.end - span.begin) return;
-    const int64_t item = span.offset / seq.tiles, start = span.begin - done, cta0 = start / span.per;
+    const int done = int(span.offset % seq.units);  // units of the item before this span
+    if (done == 0 || seq.units - done > span.end - span.begin) return;
+    const int64_t item = span.offset / seq.units, start = span.begin - done, cta0 = start / span.per;
     const int head = int(item / seq.blocks), block = int(item % seq.blocks), parts = int(blockIdx.x - cta0) + 1;
     const float *workspace = static_cast<const float *>(a.workspace);
     auto part = [&](int i) {
@@ -665,7 +667,7 @@ __global__ void __launch_bounds__(kAttnThreads) join_kernel(sq_kv_attention_args
     __syncthreads();
     if (threadIdx.x < kRows) {
         const int row = threadIdx.x;
-        float most = -INFINITY;
+        float most = kNone;
         bool bad = false;
         for (int i = 0; i < parts; ++i) {
             most = fmaxf(most, factors[i * kRows + row]);
@@ -673,9 +675,9 @@ __global__ void __launch_bounds__(kAttnThreads) join_kernel(sq_kv_attention_args
         }
         float weight = 0.f;
         for (int i = 0; i < parts; ++i) {
-            const float f = bad ? NAN : factors[i * kRows + row] == -INFINITY ? 0.f : exp2_approx(factors[i * kRows + row] - most);
+            const float f = bad ? NAN : exp2_approx(factors[i * kRows + row] - most);
             factors[i * kRows + row] = f;
-            weight += f == 0.f ? 0.f : f * part(i)[kRows * D + kRows + row];
+            weight += f * part(i)[kRows * D + kRows + row];
         }
         weights[row] = weight;
     }
@@ -689,7 +691,7 @@ __global__ void __launch_bounds__(kAttnThreads) join_kernel(sq_kv_attention_args
         for (int p = 0; p < parts; ++p) {
             const float f = factors[p * kRows + row];
             const float4 y = *reinterpret_cast<const float4 *>(part(p) + row * D + c);
-            if (f != 0.f) x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
+            x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
         }
         const float per = weights[row] == 0.f ? 0.f : 1.f / weights[row];
         T *out = output_row<T>(a, seq, head, row0 + row) + c;
