@@ -36,7 +36,7 @@ struct Codes;
 template <>
 struct Codes<__nv_bfloat16> {
     static constexpr float kHeld = 128.f;  // pair() is c + this: a bf16 with c in its last bits
-    __device__ static __forceinline__ uint32_t pair(uint32_t w) { return (w & 0x000F000Fu) | 0x43004300u; }
+    __device__ static __forceinline__ uint32_t pair(uint32_t w) { return and_or(w, 0x000F000Fu, 0x43004300u); }
     __device__ static __forceinline__ uint32_t pack(float lo, float hi) {
         uint32_t r;
         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -58,7 +58,7 @@ template <>
 struct Codes<__half> {
     static constexpr float kHeld = -kMiddle;  // f16 with c in their last bits are 1024 + c, too far from c to leave it in
     __device__ static __forceinline__ uint32_t pair(uint32_t w) {
-        const uint32_t x = (w & 0x000F000Fu) | 0x64006400u, base = 0x64086408u;
+        const uint32_t x = and_or(w, 0x000F000Fu, 0x64006400u), base = 0x64086408u;
         const __half2 r = __hsub2(reinterpret_cast<const __half2 &>(x), reinterpret_cast<const __half2 &>(base));
         return reinterpret_cast<const uint32_t &>(r);
     }

@@ -67,7 +67,7 @@ __device__ __forceinline__ uint4 unpack_middle(uint32_t w, __half2 s, __half2 le
     uint32_t r[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t x = ((i < 2 ? w << (6 - 4 * i) : w >> (4 * i - 6)) & 0x03C003C0u) | 0x4C004C00u;
+        const uint32_t x = and_or(i < 2 ? w << (6 - 4 * i) : w >> (4 * i - 6), 0x03C003C0u, 0x4C004C00u);
         const __half2 v = __hfma2(reinterpret_cast<const __half2 &>(x), s, less_24s);
         r[i] = reinterpret_cast<const uint32_t &>(v);
     }
@@ -78,7 +78,7 @@ __device__ __forceinline__ uint4 unpack_value(uint32_t w, __half2 s, __half2 s16
     uint32_t r[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t x = ((i < 2 ? w : w >> 8) & (i & 1 ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u, base = 0x64006400u;
+        const uint32_t x = and_or(i < 2 ? w : w >> 8, i & 1 ? 0x00F000F0u : 0x000F000Fu, 0x64006400u), base = 0x64006400u;
         const __half2 c = __hsub2(reinterpret_cast<const __half2 &>(x), reinterpret_cast<const __half2 &>(base));
         const __half2 v = __hfma2(c, i & 1 ? s16 : s, m);
         r[i] = reinterpret_cast<const uint32_t &>(v);
