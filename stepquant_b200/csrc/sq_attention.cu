@@ -21,6 +21,7 @@ constexpr int kWarps = 8, kAttnThreads = 32 * kWarps;
 constexpr int kMostCtas = 320;
 constexpr int kUnit = 32;             // tokens that a warp takes at a time: two tiles of the cache
 constexpr int kLeastUnits = kWarps;   // of a CTA
+constexpr int kItemUnits = 16;        // what the start and the end of an item cost a CTA
 constexpr float kNone = -3.402823466e38f;  // a maximum over nothing
 constexpr int kFewRows = 32;
 
@@ -89,8 +90,8 @@ __device__ __forceinline__ float pair_scale(uint32_t p) { return __uint_as_float
 __device__ __forceinline__ float pair_min(uint32_t p) { return __uint_as_float(p & 0xFFFF0000u); }
 
 // ---------------------------------------------------------------------------
-// work: units of 32 tokens in the order (sequence, kv head, block of rows, unit), cut into equal
-// spans of consecutive ones, a span to a CTA
+// work: units of 32 tokens in the order (sequence, kv head, block of rows, unit), each item's after
+// kItemUnits for its start and end, cut into equal spans of consecutive ones, a span to a CTA
 // ---------------------------------------------------------------------------
 struct Sequence {
     int first, count;   // new tokens
@@ -117,7 +118,7 @@ __device__ __forceinline__ Sequence sequence(const sq_kv_attention_args &a, int 
     s.units = max(1, int((int64_t(s.length) + kUnit - 1) / kUnit) - s.unit);
     const int64_t rows = int64_t(s.count) * (a.q_heads / a.heads);
     s.blocks = rows > most_rows ? 0 : int((rows + ROWS - 1) / ROWS);
-    s.cost = int64_t(s.blocks) * a.heads * s.units;
+    s.cost = int64_t(s.blocks) * a.heads * (kItemUnits + s.units);
     return s;
 }
 
@@ -176,9 +177,9 @@ __device__ __forceinline__ Span span_of(const sq_kv_attention_args &a, int most_
 }
 
 template <class T>
-__device__ __forceinline__ T *output_row(const sq_kv_attention_args &a, const Sequence &s, int head, int64_t row) {
+__device__ __forceinline__ T *output_row(const sq_kv_attention_args &a, const Sequence &s, int head, int row) {
     const int group = a.q_heads / a.heads;
-    return static_cast<T *>(a.out) + ((s.first + row / group) * a.q_heads + head * group + row % group) * a.dim;
+    return static_cast<T *>(a.out) + ((int64_t(s.first) + row / group) * a.q_heads + head * group + row % group) * a.dim;
 }
 
 // ---------------------------------------------------------------------------
@@ -210,31 +211,34 @@ struct Segment {
 struct Cursor {
     Sequence s;
     int64_t at;
-    int n, head, block, begin;  // begin: units of the item before
+    int n, head, block, begin;  // begin: what lies before in the item
 };
 
 template <int ROWS>
 __device__ __forceinline__ void next_segment(const sq_kv_attention_args &a, int most_rows, int64_t end, Cursor &c, Segment &g) {
     g.count = 0;
-    if (c.at >= end) return;
-    if (c.begin >= c.s.units) {
-        c.begin = 0;
-        if (++c.block >= c.s.blocks) {
-            c.block = 0;
-            ++c.head;
+    while (c.at < end && g.count == 0) {
+        if (c.begin >= kItemUnits + c.s.units) {
+            c.begin = 0;
+            if (++c.block >= c.s.blocks) {
+                c.block = 0;
+                ++c.head;
+            }
         }
-    }
-    while (c.head >= a.heads || c.s.cost == 0) {  // on to the next sequence with new tokens: there is one, as at < end
-        c.s = sequence<ROWS>(a, most_rows, ++c.n, false);
-        c.head = c.block = c.begin = 0;
+        while (c.head >= a.heads || c.s.cost == 0) {  // on to the next sequence with new tokens: there is one, as at < end
+            c.s = sequence<ROWS>(a, most_rows, ++c.n, false);
+            c.head = c.block = c.begin = 0;
+        }
+        const int step = int(min(end - c.at, int64_t(kItemUnits + c.s.units - c.begin)));
+        const int first = max(0, c.begin - kItemUnits);
+        c.at += step;
+        c.begin += step;
+        g.count = max(0, c.begin - kItemUnits) - first;  // none: the span ends with the item's start
+        g.unit = c.s.unit + first;
     }
     g.sequence = c.n, g.head = c.head, g.block = c.block;
     g.first = c.s.first, g.tokens = c.s.count, g.length = c.s.length, g.before = c.s.before;
-    g.unit = c.s.unit + c.begin;
-    g.count = int(min(end - c.at, int64_t(c.s.units - c.begin)));
     g.whole = g.count == c.s.units;
-    c.at += g.count;
-    c.begin += g.count;
 }
 
 template <int N>
@@ -280,10 +284,11 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
     auto fetch_rows = [&](const Segment &s) {
         constexpr int kLines = (D * 2 + 127) / 128;
         for (int i = lane; i < kRows * kLines && s.count; i += 32) {
-            const int64_t row = int64_t(s.block) * kRows + i / kLines;
-            if (row < int64_t(s.tokens) * group) {
-                const T *from = static_cast<const T *>(a.q) + (s.first + row / group) * a.q_stride +
-                                (s.head * group + row % group) * a.q_head_stride + i % kLines * 64;
+            const int row = s.block * kRows + i / kLines;
+            if (row < s.tokens * group) {
+                const int token = row / group;
+                const T *from = static_cast<const T *>(a.q) + (int64_t(s.first) + token) * a.q_stride +
+                                int64_t(s.head * group + row - token * group) * a.q_head_stride + i % kLines * 64;
                 asm volatile("prefetch.global.L2 [%0];\n" ::"l"(from));
             }
         }
@@ -294,8 +299,8 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
             c.at = span.begin;
             c.n = span.sequence;
             c.s = sequence<kRows>(a, most_rows, min(c.n, a.num_seqs - 1), false);
-            const int64_t item = c.s.cost ? span.offset / c.s.units : 0;
-            c.begin = c.s.cost ? int(span.offset % c.s.units) : 0;
+            const int64_t item = c.s.cost ? span.offset / (kItemUnits + c.s.units) : 0;
+            c.begin = c.s.cost ? int(span.offset % (kItemUnits + c.s.units)) : 0;
             c.head = c.s.cost ? int(item / c.s.blocks) : 0;
             c.block = c.s.cost ? int(item % c.s.blocks) : 0;
             next_segment<kRows>(a, most_rows, span.end, c, segments[0]);
@@ -359,13 +364,13 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
         uint32_t q[NT][kGroups][8];
         float q_sum[NT][kGroups][2];  // of rows 2 t and 2 t + 1: the groups' sums
         int limit[NT][2];
-        const int64_t row0 = int64_t(s.block) * kRows, rows = int64_t(s.tokens) * group;
+        const int row0 = s.block * kRows, rows = s.tokens * group;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int64_t row = row0 + j * 8 + g;
+            const int row = row0 + j * 8 + g;
             const bool live = row < rows;
-            const int token = live ? int(row / group) : 0, head = live ? int(row - int64_t(token) * group) : 0;
-            const T *from = static_cast<const T *>(a.q) + (int64_t(s.first) + token) * a.q_stride + (s.head * group + head) * a.q_head_stride + 16 * t;
+            const int token = live ? row / group : 0, head = live ? row - token * group : 0;
+            const T *from = static_cast<const T *>(a.q) + (int64_t(s.first) + token) * a.q_stride + int64_t(s.head * group + head) * a.q_head_stride + 16 * t;
 #pragma unroll
             for (int b = 0; b < kGroups; ++b) {
                 const uint4 x = reinterpret_cast<const uint4 *>(from + b * kGroup)[0], y = reinterpret_cast<const uint4 *>(from + b * kGroup)[1];
@@ -384,12 +389,12 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int64_t r = row0 + j * 8 + 2 * t + e;
+                const int r = row0 + j * 8 + 2 * t + e;
                 limit[j][e] = r < rows ? int(max(int64_t(-1), min(s.before + r / group, int64_t(s.length) - 1))) : -1;
             }
         }
         // Units that every row sees whole: up to `sees_all`, from `window_all` on.
-        const int64_t last_row = min(row0 + kRows, rows) - 1;
+        const int last_row = min(row0 + kRows, rows) - 1;
         const int sees_all = int(max(int64_t(0), min(s.before + row0 / group + 1, int64_t(s.length))) / kUnit);
         const int window_all = a.window > 0 ? int(min(max(int64_t(0), s.before + last_row / group - a.window + 1) + kUnit - 1, int64_t(0x7fffffff)) / kUnit) : 0;
 
@@ -622,7 +627,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
             if (s.whole) {
                 if (row0 + row < rows) {
                     const float per = weight == 0.f ? 0.f : 1.f / weight;
-                    const int token = int((row0 + row) / group), head = s.head * group + int((row0 + row) - int64_t(token) * group);
+                    const int token = (row0 + row) / group, head = s.head * group + row0 + row - token * group;
                     T *out = static_cast<T *>(a.out) + ((int64_t(s.first) + token) * a.q_heads + head) * D + c;
                     *reinterpret_cast<uint2 *>(out) = make_uint2(C::pack(x.x * per, x.y * per), C::pack(x.z * per, x.w * per));
                 }
@@ -654,13 +659,14 @@ __global__ void __launch_bounds__(kAttnThreads) join_kernel(sq_kv_attention_args
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     if (span.begin >= span.end) return;
     const Sequence seq = sequence<kRows>(a, most_rows, span.sequence, false);
-    const int done = int(span.offset % seq.units);  // units of the item before this span
-    if (done == 0 || seq.units - done > span.end - span.begin) return;
-    const int64_t item = span.offset / seq.units, start = span.begin - done, cta0 = start / span.per;
+    const int per_item = kItemUnits + seq.units, done = int(span.offset % per_item);  // of the item, before this span
+    if (done <= kItemUnits || per_item - done > span.end - span.begin) return;
+    // The first part is that of the CTA with the item's first unit: its only segment where its span begins in the item.
+    const int64_t item = span.offset / per_item, start = span.begin - done, cta0 = (start + kItemUnits) / span.per;
     const int head = int(item / seq.blocks), block = int(item % seq.blocks), parts = int(blockIdx.x - cta0) + 1;
     const float *workspace = static_cast<const float *>(a.workspace);
     auto part = [&](int i) {
-        const int64_t slot = 2 * (cta0 + i) + (i == 0 && start != cta0 * span.per ? 1 : 0);
+        const int64_t slot = 2 * (cta0 + i) + (i == 0 && cta0 * span.per < start ? 1 : 0);
         return workspace + slot * Shape::kPart;
     };
     for (int i = threadIdx.x; i < parts * kRows; i += kAttnThreads) factors[i] = part(i / kRows)[kRows * D + i % kRows];
@@ -682,7 +688,7 @@ __global__ void __launch_bounds__(kAttnThreads) join_kernel(sq_kv_attention_args
         weights[row] = weight;
     }
     __syncthreads();
-    const int64_t row0 = int64_t(block) * kRows, rows = int64_t(seq.count) * (a.q_heads / a.heads);
+    const int row0 = block * kRows, rows = seq.count * (a.q_heads / a.heads);
     for (int i = threadIdx.x; i < kRows * D / 4; i += kAttnThreads) {
         const int row = i / (D / 4), c = i % (D / 4) * 4;
         if (row0 + row >= rows) continue;
@@ -772,6 +778,7 @@ extern "C" int32_t sq_kv_attention(const sq_kv_attention_args *args, sq_stream_t
     if (!aligned16(a.q) || !aligned16(a.out) || !aligned16(a.data) || !aligned16(a.workspace)) return SQ_ERR_SHAPE;
     if (a.heads > 4096 || a.q_heads > 65536 || a.page_size > 65536 || a.tokens > kMostTokens || a.num_seqs > (1 << 30))
         return SQ_ERR_UNSUPPORTED;
+    if (int64_t(a.tokens) * (a.q_heads / a.heads) > kMostTokens) return SQ_ERR_UNSUPPORTED;  // rows of a kv head
     if (!a.cu_seqlens && a.tokens != a.num_seqs) return SQ_ERR_ARGUMENT;
     if (a.tokens == 0 || a.num_seqs == 0) return SQ_OK;
     if (!a.q || !a.out || !a.lengths || (a.table_width && !a.page_table) || (a.num_pages && !a.data)) return SQ_ERR_ARGUMENT;
