@@ -122,6 +122,11 @@ __device__ __forceinline__ Sequence sequence(const sq_kv_attention_args &a, int 
     return s;
 }
 
+// a / b of numbers that seldom need 64 bits.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    return uint64_t(a | b) >> 32 ? a / b : int64_t(uint32_t(a) / uint32_t(b));
+}
+
 struct Span {
     int64_t begin, end, per;  // in units
     int sequence;             // that begin lies in
@@ -155,7 +160,7 @@ __device__ __forceinline__ Span span_of(const sq_kv_attention_args &a, int most_
         total += warp_sums[w];
     }
     Span s;
-    s.per = max(int64_t(kLeastUnits), (total + gridDim.x - 1) / gridDim.x);
+    s.per = max(int64_t(kLeastUnits), quotient(total + gridDim.x - 1, gridDim.x));
     s.begin = min(total, s.per * blockIdx.x);
     s.end = min(total, s.begin + s.per);
     int64_t at = sum - mine;
@@ -299,10 +304,10 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
             c.at = span.begin;
             c.n = span.sequence;
             c.s = sequence<kRows>(a, most_rows, min(c.n, a.num_seqs - 1), false);
-            const int64_t item = c.s.cost ? span.offset / (kItemUnits + c.s.units) : 0;
-            c.begin = c.s.cost ? int(span.offset % (kItemUnits + c.s.units)) : 0;
-            c.head = c.s.cost ? int(item / c.s.blocks) : 0;
-            c.block = c.s.cost ? int(item % c.s.blocks) : 0;
+            const int item = c.s.cost ? int(quotient(span.offset, kItemUnits + c.s.units)) : 0;
+            c.begin = c.s.cost ? int(span.offset - int64_t(item) * (kItemUnits + c.s.units)) : 0;
+            c.head = c.s.cost ? item / c.s.blocks : 0;
+            c.block = c.s.cost ? item % c.s.blocks : 0;
             next_segment<kRows>(a, most_rows, span.end, c, segments[0]);
             next_segment<kRows>(a, most_rows, span.end, c, segments[1]);
             cursor = c;
@@ -647,62 +652,77 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 }
 
-// Joins the parts of items that several CTAs had: the CTA in whose span one ends.
+// Joins the parts of items that several CTAs had: CTAs (c, y), c that in whose span an item ends, take a
+// quarter of its sums each.
+constexpr int kJoins = 4;
+
 template <class T, int D, int NT>
 __global__ void __launch_bounds__(kAttnThreads) join_kernel(sq_kv_attention_args a, int most_rows) {
     using Shape = RowsShape<D, NT>;
     using C = Codes<T>;
-    constexpr int kRows = Shape::kRows;
+    constexpr int kRows = Shape::kRows, kMine = kRows * D / 4 / kJoins, kSplit = kAttnThreads / kMine;  // accesses of four; threads to each
     extern __shared__ float factors[];  // [parts][rows]
     __shared__ float weights[kRows];
+    __shared__ float4 sums[kAttnThreads];
     const Span span = span_of<kRows>(a, most_rows, false);
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     if (span.begin >= span.end) return;
     const Sequence seq = sequence<kRows>(a, most_rows, span.sequence, false);
-    const int per_item = kItemUnits + seq.units, done = int(span.offset % per_item);  // of the item, before this span
+    const int per_item = kItemUnits + seq.units, done = int(span.offset - quotient(span.offset, per_item) * per_item);  // of the item, before this span
     if (done <= kItemUnits || per_item - done > span.end - span.begin) return;
     // The first part is that of the CTA with the item's first unit: its only segment where its span begins in the item.
-    const int64_t item = span.offset / per_item, start = span.begin - done, cta0 = (start + kItemUnits) / span.per;
-    const int head = int(item / seq.blocks), block = int(item % seq.blocks), parts = int(blockIdx.x - cta0) + 1;
+    const int item = int(quotient(span.offset, per_item));
+    const int64_t start = span.begin - done, cta0 = quotient(start + kItemUnits, span.per);
+    const int head = item / seq.blocks, block = item % seq.blocks, parts = int(blockIdx.x - cta0) + 1;
     const float *workspace = static_cast<const float *>(a.workspace);
     auto part = [&](int i) {
         const int64_t slot = 2 * (cta0 + i) + (i == 0 && cta0 * span.per < start ? 1 : 0);
         return workspace + slot * Shape::kPart;
     };
-    for (int i = threadIdx.x; i < parts * kRows; i += kAttnThreads) factors[i] = part(i / kRows)[kRows * D + i % kRows];
-    __syncthreads();
-    if (threadIdx.x < kRows) {
-        const int row = threadIdx.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int row = warp; row < kRows; row += kWarps) {
         float most = kNone;
         bool bad = false;
-        for (int i = 0; i < parts; ++i) {
-            most = fmaxf(most, factors[i * kRows + row]);
-            bad = bad || factors[i * kRows + row] != factors[i * kRows + row];
+        for (int i = lane; i < parts; i += 32) {
+            const float x = part(i)[kRows * D + row];
+            factors[i * kRows + row] = x;
+            most = fmaxf(most, x);
+            bad = bad || x != x;
         }
+#pragma unroll
+        for (int i = 1; i < 32; i *= 2) most = fmaxf(most, __shfl_xor_sync(~0u, most, i));
+        if (__any_sync(~0u, bad)) most = NAN;
         float weight = 0.f;
-        for (int i = 0; i < parts; ++i) {
-            const float f = bad ? NAN : exp2_approx(factors[i * kRows + row] - most);
+        for (int i = lane; i < parts; i += 32) {
+            const float f = exp2_approx(factors[i * kRows + row] - most);
             factors[i * kRows + row] = f;
             weight += f * part(i)[kRows * D + kRows + row];
         }
-        weights[row] = weight;
+#pragma unroll
+        for (int i = 1; i < 32; i *= 2) weight += __shfl_xor_sync(~0u, weight, i);
+        if (lane == 0) weights[row] = weight;
     }
     __syncthreads();
-    const int row0 = block * kRows, rows = seq.count * (a.q_heads / a.heads);
-    for (int i = threadIdx.x; i < kRows * D / 4; i += kAttnThreads) {
-        const int row = i / (D / 4), c = i % (D / 4) * 4;
-        if (row0 + row >= rows) continue;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int i = blockIdx.y * kMine + threadIdx.x % kMine, row = i / (D / 4), c = i % (D / 4) * 4;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int p = 0; p < parts; ++p) {
-            const float f = factors[p * kRows + row];
-            const float4 y = *reinterpret_cast<const float4 *>(part(p) + row * D + c);
-            x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
-        }
-        const float per = weights[row] == 0.f ? 0.f : 1.f / weights[row];
-        T *out = output_row<T>(a, seq, head, row0 + row) + c;
-        *reinterpret_cast<uint2 *>(out) = make_uint2(C::pack(x.x * per, x.y * per), C::pack(x.z * per, x.w * per));
+    for (int p = threadIdx.x / kMine; p < parts; p += kSplit) {
+        const float f = factors[p * kRows + row];
+        const float4 y = *reinterpret_cast<const float4 *>(part(p) + row * D + c);
+        x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
     }
+    sums[threadIdx.x] = x;
+    __syncthreads();
+    const int row0 = block * kRows, rows = seq.count * (a.q_heads / a.heads);
+    if (threadIdx.x >= kMine || row0 + row >= rows) return;
+#pragma unroll
+    for (int k = 1; k < kSplit; ++k) {
+        const float4 y = sums[threadIdx.x + k * kMine];
+        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+    }
+    const float per = weights[row] == 0.f ? 0.f : 1.f / weights[row];
+    T *out = output_row<T>(a, seq, head, row0 + row) + c;
+    *reinterpret_cast<uint2 *>(out) = make_uint2(C::pack(x.x * per, x.y * per), C::pack(x.z * per, x.w * per));
 }
 
 template <class T, int D, int NT>
@@ -718,7 +738,7 @@ cudaError_t launch_rows(const sq_kv_attention_args &a, int most_rows, cudaStream
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = dim3(grid, kJoins);
     cfg.blockDim = dim3(kAttnThreads);
     cfg.dynamicSmemBytes = size_t(grid) * Shape::kRows * sizeof(float);
     cfg.stream = s;

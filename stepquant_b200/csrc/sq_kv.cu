@@ -3,9 +3,10 @@
 //
 // Eight neighbouring lanes hold a group of 64 channels of one token and head, eight
 // channels each: the group's extremes are three shuffles away, and a lane's codes are
-// one 32-bit word of the tile.  A code is that of the definition in exact arithmetic
-// (the extremes, the quotient and the rotation taken in 64 bits), so a token's bytes do
-// not depend on how it was appended.
+// one 32-bit word of the tile.  A code is that of the definition in exact arithmetic:
+// fp32 finds it, with a bound on what its roundings may have changed, and groups where
+// that reaches a border (a few in ten thousand, and those at slow pairs near position 0)
+// are done again in 64 bits.  All in 64 bits, 8192 tokens of 8 heads took 88 us.
 #include "sq_kv.cuh"
 #include "sq_rows.cuh"
 #include "sq_vec.cuh"
@@ -91,14 +92,79 @@ __device__ __forceinline__ void quantize(const double (&x)[8], uint32_t lanes, u
     pair = (s & 0x7FFF) | (m << 16);
 }
 
+// The same in fp32 of x[0..7], each within `off` of the value that is meant (0: exact).  False in all eight
+// lanes where a result may be another in exact arithmetic.
+__device__ __forceinline__ bool quantize_fast(const float (&x)[8], float off, uint32_t lanes, uint32_t &word, uint32_t &pair) {
+    float low = x[0], high = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        low = fminf(low, x[i]);
+        high = fmaxf(high, x[i]);
+    }
+#pragma unroll
+    for (int i = 1; i < 8; i *= 2) {
+        low = fminf(low, __shfl_xor_sync(lanes, low, i));
+        high = fmaxf(high, __shfl_xor_sync(lanes, high, i));
+        off = fmaxf(off, __shfl_xor_sync(lanes, off, i));
+    }
+    auto down = [](float y) {
+        const uint32_t bits = __float_as_uint(y);
+        return (bits & 0x80000000u ? bits + 0xFFFFu : bits) & 0xFFFF0000u;
+    };
+    // The minimum: on one side of a border with all that it may be.
+    const uint32_t m_bits = down(low);
+    bool sure = off == 0.f || (down(low - 2.f * off) == m_bits && down(low + 2.f * off) == m_bits);
+    const float m = __uint_as_float(m_bits);
+    // The scale: s the least bf16 with 15 s >= d.  15 s has 12 bits.
+    const float d = high - m;
+    sure = sure && (off != 0.f || (d + m == high && high - d == m)) && d < 1e38f && d > 1e-30f && fmaxf(high, -low) < 3e38f;
+    uint32_t s_bits = (__float_as_uint(d / 15.f) + 0xFFFFu) & 0xFFFF0000u;
+    if (15.f * __uint_as_float(s_bits - 0x10000u) >= d) s_bits -= 0x10000u;
+    if (15.f * __uint_as_float(s_bits) < d) s_bits += 0x10000u;
+    const float s = __uint_as_float(s_bits), slack = off == 0.f ? 0.f : 4.f * off + d * 0x1p-22f;
+    sure = sure && 15.f * s - d >= slack && d - 15.f * __uint_as_float(s_bits - 0x10000u) > slack;
+    const float per = reciprocal_approx(s);
+    word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float e = x[i] - m;
+        float r = rintf(e * per);
+        const float rest = fmaf(-r, s, e), beyond = 2.f * fabsf(rest) - s;  // above 0: the next; 0: a tie, to the even one
+        if (beyond > 0.f || (beyond == 0.f && int(r) & 1)) r += copysignf(1.f, rest);
+        sure = sure && (off == 0.f ? e + m == x[i] && x[i] - e == m : fabsf(beyond) > slack);
+        word |= uint32_t(int(r)) << ((i >> 1) * 4 + (i & 1) * 16);
+    }
+    pair = (s_bits >> 16) | m_bits;
+    return (__ballot_sync(lanes, sure) & lanes) == lanes;
+}
+
 template <class T>
 __device__ __forceinline__ void load8(const T *p, bool wide, T (&x)[8]) {
     if (wide) {
 #pragma unroll
-        for (int i = 0; i < int(sizeof(T)) / 2; ++i) reinterpret_cast<uint4 *>(x)[i] = reinterpret_cast<const uint4 *>(p)[i];
+        for (int i = 0; i < int(sizeof(T)) / 2; ++i) reinterpret_cast<uint4 *>(x)[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = p[i];
+    }
+}
+
+// Channels c..c + 7 of a key in 64 bits, rotated.
+template <class T>
+__device__ __noinline__ void turn_exactly(const sq_kv_args &a, const T *k, int c, int64_t position, double (&x)[8]) {
+    const int half = a.turned / 2;
+    for (int e = 0; e < 8; ++e) {
+        const int at = c + e;
+        x[e] = to_float(k[at]);
+        if (at >= a.turned) continue;
+        const int f = a.interleaved ? at / 2 : at < half ? at : at - half;
+        const bool second = a.interleaved ? at & 1 : at >= half;
+        const double other = to_float(k[a.interleaved ? at ^ 1 : second ? at - half : at + half]);
+        double sin, cos;
+        sincospi(double(phase_of(position, a.frequencies[f])) * 0x1p-63, &sin, &cos);
+        cos *= a.magnitude;
+        sin *= a.magnitude;
+        x[e] = second ? other * sin + x[e] * cos : x[e] * cos - other * sin;
     }
 }
 
@@ -106,64 +172,95 @@ template <class T, int D>
 __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(sq_kv_args a, int per_cta, bool k_wide, bool v_wide) {
     using Tile = KvTile<D>;
     constexpr int kLanes = D / 8;  // of one head's keys or values
-    extern __shared__ double2 table[];  // [per_cta][turned / 2] (cos, sin), times the magnitude
+    extern __shared__ __align__(16) float2 table[];  // [per_cta][turned / 2] (cos, sin), times the magnitude
     __shared__ Place places[kMostPerCta];
     const int64_t first = int64_t(blockIdx.x) * per_cta;
     const int count = int(min(int64_t(per_cta), a.tokens - first)), half = a.turned / 2;
-    if (int(threadIdx.x) < count) places[threadIdx.x] = place_of(a, int(first) + threadIdx.x, Tile::kBytes);
+    if (int(threadIdx.x) < count) {
+        Place p = place_of(a, int(first) + threadIdx.x, Tile::kBytes);
+        if (a.positions) p.position = position_at(a.positions, a.position_dtype, first + threadIdx.x);
+        places[threadIdx.x] = p;
+    }
     __syncthreads();
     for (int i = threadIdx.x; i < count * half; i += kKvThreads) {
         const int t = i / half, f = i - t * half;
-        if (places[t].tile < 0) continue;
-        const int64_t position = a.positions ? position_at(a.positions, a.position_dtype, first + t) : places[t].position;
-        double sin, cos;
-        sincospi(double(phase_of(position, a.frequencies[f])) * 0x1p-63, &sin, &cos);
-        table[i] = make_double2(a.magnitude * cos, a.magnitude * sin);
+        float sin, cos;
+        sincospif(float(int32_t(phase_of(places[t].position, a.frequencies[f]) >> 32)) * 0x1p-31f, &sin, &cos);
+        table[i] = make_float2(a.magnitude * cos, a.magnitude * sin);
     }
     __syncthreads();
     const int lanes = a.heads * 2 * kLanes;  // of a token: a multiple of 16
     const int64_t head_bytes = int64_t(a.page_size / kTile) * Tile::kBytes;
-    for (int i = threadIdx.x; i < count * lanes; i += kKvThreads) {
-        const uint32_t group_lanes = 0xFFu << (threadIdx.x & 24);
-        const int t = i / lanes, rest = i - t * lanes;
+    const uint32_t group_lanes = 0xFFu << (threadIdx.x & 24);
+    const bool pairs_wide = k_wide && half % 8 == 0;
+    // What a rotated channel is off by at most: sine and cosine by 2^-22 (their argument's rounding to fp32, the
+    // function's two units, the magnitude's product), the products and their sum by 2^-24 each.
+    const float turn_off = 0x1p-21f * fabsf(a.magnitude);
+    int t = int(threadIdx.x) / lanes, rest = int(threadIdx.x) - t * lanes;
+    const int t_step = kKvThreads / lanes, rest_step = kKvThreads - t_step * lanes;
+    for (; t < count; t += t_step, rest += rest_step, t += rest >= lanes, rest -= rest >= lanes ? lanes : 0) {
         const int head = rest / (2 * kLanes), values = rest / kLanes & 1, lane = rest % kLanes;
         const Place &p = places[t];
         if (p.tile < 0) continue;
-        T raw[8];
-        double x[8];
         const int c = lane * 8;
-        if (values) {
-            load8(static_cast<const T *>(a.v) + (first + t) * a.v_stride + head * a.v_head_stride + c, v_wide, raw);
+        const T *from = values ? static_cast<const T *>(a.v) + (first + t) * a.v_stride + head * a.v_head_stride
+                               : static_cast<const T *>(a.k) + (first + t) * a.k_stride + head * a.k_head_stride;
+        alignas(16) T raw[8];
+        float x[8], off = 0.f;
+        load8(from + c, values ? v_wide : k_wide, raw);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = to_float(raw[e]);
-        } else {
-            const T *k = static_cast<const T *>(a.k) + (first + t) * a.k_stride + head * a.k_head_stride;
-            load8(k + c, k_wide, raw);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = to_float(raw[e]);
-            const double2 *cs = table + t * half;
+        for (int e = 0; e < 8; ++e) x[e] = to_float(raw[e]);
+        if (!values && c < a.turned) {
+            const float2 *cs = table + t * half;
             if (a.interleaved) {
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
-                    if (c + e >= a.turned) break;
-                    const double2 z = cs[(c + e) / 2];
-                    const double u = x[e], w = x[e + 1];
-                    x[e] = u * z.x - w * z.y;
-                    x[e + 1] = u * z.y + w * z.x;
+                    if (c + e < a.turned) {
+                        const float2 z = cs[(c + e) / 2];
+                        const float u = x[e], w = x[e + 1];
+                        off = fmaxf(off, fabsf(u) + fabsf(w));
+                        x[e] = u * z.x - w * z.y;
+                        x[e + 1] = u * z.y + w * z.x;
+                    }
+                }
+            } else if (pairs_wide) {
+                const bool upper = c >= half;
+                const int f = upper ? c - half : c;
+                alignas(16) T other[8];
+                load8(from + (upper ? f : c + half), true, other);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float2 z = cs[f + e];
+                    const float w = to_float(other[e]);
+                    off = fmaxf(off, fabsf(x[e]) + fabsf(w));
+                    x[e] = x[e] * z.x + (upper ? w : -w) * z.y;
                 }
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    if (c + e >= a.turned) break;
-                    const bool upper = c + e >= half;
-                    const double other = to_float(k[upper ? c + e - half : c + e + half]);
-                    const double2 z = cs[upper ? c + e - half : c + e];
-                    x[e] = upper ? other * z.y + x[e] * z.x : x[e] * z.x - other * z.y;
+                    if (c + e < a.turned) {
+                        const bool upper = c + e >= half;
+                        const int f = upper ? c + e - half : c + e;
+                        const float w = to_float(from[upper ? f : c + e + half]);
+                        const float2 z = cs[f];
+                        off = fmaxf(off, fabsf(x[e]) + fabsf(w));
+                        x[e] = x[e] * z.x + (upper ? w : -w) * z.y;
+                    }
                 }
             }
+            off *= turn_off;
         }
         uint32_t word, pair;
-        quantize(x, group_lanes, word, pair);
+        if (!quantize_fast(x, off, group_lanes, word, pair)) {
+            double exact[8];
+            if (values || c >= a.turned) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) exact[e] = to_float(raw[e]);
+            } else {
+                turn_exactly(a, from, c, p.position, exact);
+            }
+            quantize(exact, group_lanes, word, pair);
+        }
         const int group = lane >> 3, w = lane & 7;
         uint8_t *tile = a.data + p.tile + head * head_bytes;
         *reinterpret_cast<uint32_t *>(tile + (values ? Tile::value_word(p.token, group, w) : Tile::key_word(p.token, group, w))) = word;
@@ -182,24 +279,23 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(sq_kv_args a, int p
     __syncthreads();
     const int lanes = a.heads * 2 * kLanes;
     const int64_t head_bytes = int64_t(a.page_size / kTile) * Tile::kBytes;
-    for (int i = threadIdx.x; i < count * lanes; i += kKvThreads) {
-        const int t = i / lanes, rest = i - t * lanes;
+    int t = int(threadIdx.x) / lanes, rest = int(threadIdx.x) - t * lanes;
+    const int t_step = kKvThreads / lanes, rest_step = kKvThreads - t_step * lanes;
+#pragma unroll 4
+    for (; t < count; t += t_step, rest += rest_step, t += rest >= lanes, rest -= rest >= lanes ? lanes : 0) {
         const int head = rest / (2 * kLanes), values = rest / kLanes & 1, lane = rest % kLanes;
         const Place &p = places[t];
-        alignas(16) T x[8];
-        if (p.tile < 0) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = from_float<T>(0.f);
-        } else {
-            const int group = lane >> 3, w = lane & 7;
+        const int group = lane >> 3, w = lane & 7;
+        uint32_t word = 0, pair = 0;
+        if (p.tile >= 0) {
             const uint8_t *tile = a.data + p.tile + head * head_bytes;
-            const uint32_t word =
-                *reinterpret_cast<const uint32_t *>(tile + (values ? Tile::value_word(p.token, group, w) : Tile::key_word(p.token, group, w)));
-            const uint32_t pair = *reinterpret_cast<const uint32_t *>(tile + Tile::pair(values, p.token, group));
-            const float s = bf16_value(pair & 0xFFFF), m = bf16_value(pair >> 16);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = from_float<T>(fmaf(s, float(word >> ((e >> 1) * 4 + (e & 1) * 16) & 15), m));
+            word = __ldg(reinterpret_cast<const uint32_t *>(tile + (values ? Tile::value_word(p.token, group, w) : Tile::key_word(p.token, group, w))));
+            pair = __ldg(reinterpret_cast<const uint32_t *>(tile + Tile::pair(values, p.token, group)));
         }
+        const float s = bf16_value(pair & 0xFFFF), m = bf16_value(pair >> 16);
+        alignas(16) T x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = from_float<T>(fmaf(s, float(word >> ((e >> 1) * 4 + (e & 1) * 16) & 15), m));
         T *out = values ? static_cast<T *>(a.v) + (first + t) * a.v_stride + head * a.v_head_stride
                         : static_cast<T *>(a.k) + (first + t) * a.k_stride + head * a.k_head_stride;
 #pragma unroll
@@ -218,7 +314,7 @@ cudaError_t launch_kv(const sq_kv_args &a, bool append, cudaStream_t s) {
     };
     const bool k_wide = wide(a.k, a.k_stride, a.k_head_stride), v_wide = wide(a.v, a.v_stride, a.v_head_stride);
     if (append) {
-        kv_append_kernel<T, D><<<grid, kKvThreads, size_t(per_cta) * (a.turned / 2) * sizeof(double2), s>>>(a, per_cta, k_wide, v_wide);
+        kv_append_kernel<T, D><<<grid, kKvThreads, size_t(per_cta) * (a.turned / 2) * sizeof(float2), s>>>(a, per_cta, k_wide, v_wide);
     } else {
         if (!k_wide || !v_wide) return cudaErrorInvalidValue;
         kv_read_kernel<T, D><<<grid, kKvThreads, 0, s>>>(a, per_cta);
