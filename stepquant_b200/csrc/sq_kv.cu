@@ -121,19 +121,34 @@ __device__ __forceinline__ bool quantize_fast(const float (&x)[8], float off, ui
     uint32_t s_bits = (__float_as_uint(d / 15.f) + 0xFFFFu) & 0xFFFF0000u;
     if (15.f * __uint_as_float(s_bits - 0x10000u) >= d) s_bits -= 0x10000u;
     if (15.f * __uint_as_float(s_bits) < d) s_bits += 0x10000u;
-    const float s = __uint_as_float(s_bits), slack = off == 0.f ? 0.f : 4.f * off + d * 0x1p-22f;
-    sure = sure && 15.f * s - d >= slack && d - 15.f * __uint_as_float(s_bits - 0x10000u) > slack;
-    const float per = reciprocal_approx(s);
+    const float s = __uint_as_float(s_bits), slack = 4.f * off + d * 0x1p-20f, least = off == 0.f ? 0.f : slack;
+    sure = sure && 15.f * s - d >= least && d - 15.f * __uint_as_float(s_bits - 0x10000u) > least;
+    // Whole numbers near 1.5 * 2^23 have theirs in the last bits; a code whose rest is not within the slack of half a
+    // step is the right one.
+    constexpr float kWhole = 12582912.f;
+    const float per = reciprocal_approx(s), clear = 0.5f * (s - slack);
+    bool all = true;
     word = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float e = x[i] - m;
-        float r = rintf(e * per);
-        const float rest = fmaf(-r, s, e), beyond = 2.f * fabsf(rest) - s;  // above 0: the next; 0: a tie, to the even one
-        if (beyond > 0.f || (beyond == 0.f && int(r) & 1)) r += copysignf(1.f, rest);
-        sure = sure && (off == 0.f ? e + m == x[i] && x[i] - e == m : fabsf(beyond) > slack);
-        word |= uint32_t(int(r)) << ((i >> 1) * 4 + (i & 1) * 16);
+        const float e = x[i] - m, near = fmaf(e, per, kWhole), rest = fmaf(kWhole - near, s, e);
+        all &= fabsf(rest) < clear;
+        word += (__float_as_uint(near) - 0x4B400000u) << ((i >> 1) * 4 + (i & 1) * 16);
     }
+    if (!all && off == 0.f) {  // exact values: ties, to the even code, and their neighbours
+        all = true;
+        word = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float e = x[i] - m, near = fmaf(e, per, kWhole), rest = fmaf(kWhole - near, s, e);
+            const float beyond = 2.f * fabsf(rest) - s;  // above 0: the next; 0: a tie
+            const uint32_t code = __float_as_uint(near) - 0x4B400000u;
+            const bool next = bool(beyond > 0.f) | (bool(beyond == 0.f) & bool(code & 1));
+            word += (code + (next ? (rest > 0.f ? 1u : ~0u) : 0u)) << ((i >> 1) * 4 + (i & 1) * 16);
+            all &= bool(fabsf(rest) < clear) | (bool(e + m == x[i]) & bool(x[i] - e == m));
+        }
+    }
+    sure = sure && all;
     pair = (s_bits >> 16) | m_bits;
     return (__ballot_sync(lanes, sure) & lanes) == lanes;
 }
@@ -189,7 +204,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(sq_kv_args a, int
         table[i] = make_float2(a.magnitude * cos, a.magnitude * sin);
     }
     __syncthreads();
-    const int lanes = a.heads * 2 * kLanes;  // of a token: a multiple of 16
+    const int lanes = a.heads * 2 * kLanes;  // of a token, keys first: a multiple of 16
     const int64_t head_bytes = int64_t(a.page_size / kTile) * Tile::kBytes;
     const uint32_t group_lanes = 0xFFu << (threadIdx.x & 24);
     const bool pairs_wide = k_wide && half % 8 == 0;
@@ -199,7 +214,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(sq_kv_args a, int
     int t = int(threadIdx.x) / lanes, rest = int(threadIdx.x) - t * lanes;
     const int t_step = kKvThreads / lanes, rest_step = kKvThreads - t_step * lanes;
     for (; t < count; t += t_step, rest += rest_step, t += rest >= lanes, rest -= rest >= lanes ? lanes : 0) {
-        const int head = rest / (2 * kLanes), values = rest / kLanes & 1, lane = rest % kLanes;
+        const int values = 2 * rest >= lanes, head = (values ? rest - lanes / 2 : rest) / kLanes, lane = rest % kLanes;
         const Place &p = places[t];
         if (p.tile < 0) continue;
         const int c = lane * 8;
@@ -283,7 +298,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(sq_kv_args a, int p
     const int t_step = kKvThreads / lanes, rest_step = kKvThreads - t_step * lanes;
 #pragma unroll 4
     for (; t < count; t += t_step, rest += rest_step, t += rest >= lanes, rest -= rest >= lanes ? lanes : 0) {
-        const int head = rest / (2 * kLanes), values = rest / kLanes & 1, lane = rest % kLanes;
+        const int values = 2 * rest >= lanes, head = (values ? rest - lanes / 2 : rest) / kLanes, lane = rest % kLanes;
         const Place &p = places[t];
         const int group = lane >> 3, w = lane & 7;
         uint32_t word = 0, pair = 0;
