@@ -26,6 +26,7 @@ struct Place {
 // Where new token i goes.
 __device__ __forceinline__ Place place_of(const sq_kv_args &a, int i, int tile_bytes) {
     Place p{-1, 0, 0};
+    if (a.num_seqs == 0) return p;
     int n = i;
     if (a.cu_seqlens) {
         if (i < sequence_range(a.cu_seqlens, 0, a.tokens).x || i >= sequence_range(a.cu_seqlens, a.num_seqs - 1, a.tokens).y)
@@ -113,7 +114,7 @@ __device__ __forceinline__ bool quantize_fast(const float (&x)[8], float off, ui
     };
     // The minimum: on one side of a border with all that it may be.
     const uint32_t m_bits = down(low);
-    bool sure = off == 0.f || (down(low - 2.f * off) == m_bits && down(low + 2.f * off) == m_bits);
+    bool sure = off == 0.f || (down(low - 1.25f * off) == m_bits && down(low + 1.25f * off) == m_bits);
     const float m = __uint_as_float(m_bits);
     // The scale: s the least bf16 with 15 s >= d.  15 s has 12 bits.
     const float d = high - m;
@@ -121,7 +122,7 @@ __device__ __forceinline__ bool quantize_fast(const float (&x)[8], float off, ui
     uint32_t s_bits = (__float_as_uint(d / 15.f) + 0xFFFFu) & 0xFFFF0000u;
     if (15.f * __uint_as_float(s_bits - 0x10000u) >= d) s_bits -= 0x10000u;
     if (15.f * __uint_as_float(s_bits) < d) s_bits += 0x10000u;
-    const float s = __uint_as_float(s_bits), slack = 4.f * off + d * 0x1p-20f, least = off == 0.f ? 0.f : slack;
+    const float s = __uint_as_float(s_bits), slack = 2.f * off + d * 0x1p-20f, least = off == 0.f ? 0.f : slack;
     sure = sure && 15.f * s - d >= least && d - 15.f * __uint_as_float(s_bits - 0x10000u) > least;
     // Whole numbers near 1.5 * 2^23 have theirs in the last bits; a code whose rest is not within the slack of half a
     // step is the right one.
@@ -184,7 +185,7 @@ __device__ __noinline__ void turn_exactly(const sq_kv_args &a, const T *k, int c
 }
 
 template <class T, int D>
-__global__ void __launch_bounds__(kKvThreads) kv_append_kernel(sq_kv_args a, int per_cta, bool k_wide, bool v_wide) {
+__global__ void __launch_bounds__(kKvThreads, 4) kv_append_kernel(sq_kv_args a, int per_cta, bool k_wide, bool v_wide) {
     using Tile = KvTile<D>;
     constexpr int kLanes = D / 8;  // of one head's keys or values
     extern __shared__ __align__(16) float2 table[];  // [per_cta][turned / 2] (cos, sin), times the magnitude
@@ -208,21 +209,27 @@ __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(sq_kv_args a, int
     const int64_t head_bytes = int64_t(a.page_size / kTile) * Tile::kBytes;
     const uint32_t group_lanes = 0xFFu << (threadIdx.x & 24);
     const bool pairs_wide = k_wide && half % 8 == 0;
-    // What a rotated channel is off by at most: sine and cosine by 2^-22 (their argument's rounding to fp32, the
-    // function's two units, the magnitude's product), the products and their sum by 2^-24 each.
-    const float turn_off = 0x1p-21f * fabsf(a.magnitude);
-    int t = int(threadIdx.x) / lanes, rest = int(threadIdx.x) - t * lanes;
-    const int t_step = kKvThreads / lanes, rest_step = kKvThreads - t_step * lanes;
-    for (; t < count; t += t_step, rest += rest_step, t += rest >= lanes, rest -= rest >= lanes ? lanes : 0) {
+    // What a rotated channel is off by at most, in units of 2^-24 (|x1| + |x2|): sine and cosine by pi / 2 (their
+    // argument in half turns is rounded to fp32), 1 (the functions) and 1/2 (the magnitude's product), then the
+    // products and their sum by 1/2 each; 4.1 in all.
+    const float turn_off = 0x1.1p-22f * fabsf(a.magnitude);
+    // Threads are [token][lane] where a token's lanes are fewer than them.
+    const int t_step = max(1, kKvThreads / lanes), t0 = int(threadIdx.x) / lanes < t_step ? int(threadIdx.x) / lanes : 0;
+    if (lanes < kKvThreads && int(threadIdx.x) >= t_step * lanes) return;
+    for (int rest = int(threadIdx.x) - t0 * lanes; rest < lanes; rest += kKvThreads) {
         const int values = 2 * rest >= lanes, head = (values ? rest - lanes / 2 : rest) / kLanes, lane = rest % kLanes;
+        const int c = lane * 8, group = lane >> 3, w = lane & 7;
+        const int64_t stride = values ? a.v_stride : a.k_stride;
+        const T *from = values ? static_cast<const T *>(a.v) + head * a.v_head_stride : static_cast<const T *>(a.k) + head * a.k_head_stride;
+        from += (first + t0) * stride;
+        uint8_t *const to = a.data + head * head_bytes;
+        const bool wide = values ? v_wide : k_wide;
+        for (int t = t0; t < count; t += t_step, from += t_step * stride) {
         const Place &p = places[t];
         if (p.tile < 0) continue;
-        const int c = lane * 8;
-        const T *from = values ? static_cast<const T *>(a.v) + (first + t) * a.v_stride + head * a.v_head_stride
-                               : static_cast<const T *>(a.k) + (first + t) * a.k_stride + head * a.k_head_stride;
         alignas(16) T raw[8];
         float x[8], off = 0.f;
-        load8(from + c, values ? v_wide : k_wide, raw);
+        load8(from + c, wide, raw);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = to_float(raw[e]);
         if (!values && c < a.turned) {
@@ -276,10 +283,10 @@ __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(sq_kv_args a, int
             }
             quantize(exact, group_lanes, word, pair);
         }
-        const int group = lane >> 3, w = lane & 7;
-        uint8_t *tile = a.data + p.tile + head * head_bytes;
+        uint8_t *tile = to + p.tile;
         *reinterpret_cast<uint32_t *>(tile + (values ? Tile::value_word(p.token, group, w) : Tile::key_word(p.token, group, w))) = word;
         if (w == 0) *reinterpret_cast<uint32_t *>(tile + Tile::pair(values, p.token, group)) = pair;
+        }
     }
 }
 

@@ -39,7 +39,7 @@ struct Piece {
 // Units of a head: pieces of VEC channels; `turned_units` of them are rotated, each with its partner piece
 // VEC channels of the other half, or (interleaved) pairs of its own.
 template <class T, int VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(sq_rotary_args a, int per_cta, int turned_units, int units, bool copy) {
+__global__ void __launch_bounds__(kRotaryThreads, 4) rotary_kernel(sq_rotary_args a, int per_cta, int turned_units, int units, bool copy) {
     extern __shared__ float2 table[];  // [per_cta][turned / 2] (cos, sin), times the magnitude
     const int half = a.turned / 2;
     const int64_t first = int64_t(blockIdx.x) * per_cta;
@@ -62,49 +62,77 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(sq_rotary_args a
         const int head = slot / live, unit = slot - head * live;
         const T *x = static_cast<const T *>(a.x) + head * a.x_head_stride;
         T *out = static_cast<T *>(a.out) + head * a.out_head_stride;
+        // Two tokens are read before either is written (out may be x, so the compiler would not).
+        constexpr int K = 2;
+        const int64_t x_step = lanes * a.x_stride, out_step = lanes * a.out_stride;
+        x += (first + lane) * a.x_stride;
+        out += (first + lane) * a.out_stride;
         if (unit >= turned_units) {
             const int c = a.turned + (unit - turned_units) * VEC;
-#pragma unroll 4
-            for (int t = lane; t < count; t += lanes) {
-                Piece<T, VEC> p;
-                p.load(x + (first + t) * a.x_stride + c);
-                p.store(out + (first + t) * a.out_stride + c);
+            x += c;
+            out += c;
+            for (int t = lane; t < count; t += K * lanes, x += K * x_step, out += K * out_step) {
+                Piece<T, VEC> p[K];
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (t + k * lanes < count) p[k].load(x + k * x_step);
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (t + k * lanes < count) p[k].store(out + k * out_step);
             }
         } else if (INTERLEAVED) {
             constexpr int W = VEC < 2 ? 2 : VEC, S = VEC < 2 ? 1 : VEC;  // channels of a unit, and of an access
-            const int c = unit * W;
-#pragma unroll 4
-            for (int t = lane; t < count; t += lanes) {
-                Piece<T, S> p[W / S];
+            x += unit * W;
+            out += unit * W;
+            for (int t = lane; t < count; t += K * lanes, x += K * x_step, out += K * out_step) {
+                Piece<T, S> p[K][W / S];
 #pragma unroll
-                for (int i = 0; i < W / S; ++i) p[i].load(x + (first + t) * a.x_stride + c + i * S);
+                for (int k = 0; k < K; ++k)
 #pragma unroll
-                for (int i = 0; i < W; i += 2) {
-                    const float2 cs = table[t * half + (c + i) / 2];
-                    T &e = p[i / S].x[i % S], &o = p[(i + 1) / S].x[(i + 1) % S];
-                    const float u = to_float(e), v = to_float(o);
-                    e = from_float<T>(u * cs.x - v * cs.y);
-                    o = from_float<T>(u * cs.y + v * cs.x);
+                    for (int i = 0; i < W / S; ++i)
+                        if (t + k * lanes < count) p[k][i].load(x + k * x_step + i * S);
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    if (t + k * lanes >= count) break;
+                    const float2 *cs = table + (t + k * lanes) * half + unit * (W / 2);
+#pragma unroll
+                    for (int i = 0; i < W; i += 2) {
+                        const float2 z = cs[i / 2];
+                        T &e = p[k][i / S].x[i % S], &o = p[k][(i + 1) / S].x[(i + 1) % S];
+                        const float u = to_float(e), v = to_float(o);
+                        e = from_float<T>(u * z.x - v * z.y);
+                        o = from_float<T>(u * z.y + v * z.x);
+                    }
+#pragma unroll
+                    for (int i = 0; i < W / S; ++i) p[k][i].store(out + k * out_step + i * S);
                 }
-#pragma unroll
-                for (int i = 0; i < W / S; ++i) p[i].store(out + (first + t) * a.out_stride + c + i * S);
             }
         } else {
             const int c = unit * VEC;
-#pragma unroll 4
-            for (int t = lane; t < count; t += lanes) {
-                Piece<T, VEC> p, q;
-                p.load(x + (first + t) * a.x_stride + c);
-                q.load(x + (first + t) * a.x_stride + half + c);
+            x += c;
+            out += c;
+            for (int t = lane; t < count; t += K * lanes, x += K * x_step, out += K * out_step) {
+                Piece<T, VEC> p[K], q[K];
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const float2 cs = table[t * half + c + i];
-                    const float u = to_float(p.x[i]), v = to_float(q.x[i]);
-                    p.x[i] = from_float<T>(u * cs.x - v * cs.y);
-                    q.x[i] = from_float<T>(u * cs.y + v * cs.x);
+                for (int k = 0; k < K; ++k)
+                    if (t + k * lanes < count) {
+                        p[k].load(x + k * x_step);
+                        q[k].load(x + k * x_step + half);
+                    }
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    if (t + k * lanes >= count) break;
+                    const float2 *cs = table + (t + k * lanes) * half + c;
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        const float2 z = cs[i];
+                        const float u = to_float(p[k].x[i]), v = to_float(q[k].x[i]);
+                        p[k].x[i] = from_float<T>(u * z.x - v * z.y);
+                        q[k].x[i] = from_float<T>(u * z.y + v * z.x);
+                    }
+                    p[k].store(out + k * out_step);
+                    q[k].store(out + k * out_step + half);
                 }
-                p.store(out + (first + t) * a.out_stride + c);
-                q.store(out + (first + t) * a.out_stride + half + c);
             }
         }
     }
