@@ -1,10 +1,12 @@
-"""A two-layer recurrent stack on the package's operators: prompts, then tokens.
+"""A stack of recurrent layers on the package's operators: prompts, then tokens.
 
     residual norm -> e4m3 activations -> e4m3 projection -> short convolution
                   -> state pass -> e4m3 projection added to the residual
 
 once with a gated delta rule layer, whose states live packed in a
-``PackedStatePool``, and once with a selective layer (``SelectiveStatePool``).
+``PackedStatePool``, and once with a selective layer (``SelectiveStatePool``);
+with ``attention`` a softmax attention layer stands between them, its keys and
+values in 4 bits (``QuantizedKVPool``), queries and keys rotated.
 Random weights; ``python examples/recurrent_layers.py`` runs a batch of ragged
 prompts, decodes from the kept states and compares the decoded tokens' outputs
 with one pass over the whole sequences.
@@ -18,9 +20,11 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 from stepquant_b200 import QuantizationPlan  # noqa: E402
 from stepquant_b200.kernels.conv import causal_conv1d_extend, causal_conv1d_step  # noqa: E402
+from stepquant_b200.kernels.kv_cache import QuantizedKVPool  # noqa: E402
 from stepquant_b200.kernels.matmul import matmul_fp8, quantize_weight_fp8  # noqa: E402
 from stepquant_b200.kernels.norm import quantize_fp8, rms_norm_fp8  # noqa: E402
 from stepquant_b200.kernels.pool import PackedStatePool  # noqa: E402
+from stepquant_b200.kernels.rotary import rotary, rotary_frequencies  # noqa: E402
 from stepquant_b200.kernels.scan import SelectiveStatePool  # noqa: E402
 
 
@@ -98,7 +102,38 @@ class DeltaLayer:
         return self.w_out(quantize_fp8(out.reshape(x.shape[0], -1)), residual=x)
 
 
-def run(lengths=(37, 5, 64, 18), decode=6, hidden=512, seed=0):
+class AttentionLayer:
+    """Softmax attention over a 4-bit cache; slot n owns `pages` pages of it."""
+
+    def __init__(self, gen, slots, hidden, heads, kv_heads, dim=128, pages=2, page_size=64):
+        self.heads, self.kv_heads, self.dim = heads, kv_heads, dim
+        self.norm = torch.ones(hidden, device="cuda", dtype=torch.bfloat16)
+        self.w_in = Projection(gen, (heads + 2 * kv_heads) * dim, hidden)
+        self.w_out = Projection(gen, hidden, heads * dim)
+        self.frequencies = rotary_frequencies(dim)
+        self.pool = QuantizedKVPool(1 + (slots - 1) * pages, kv_heads, dim, page_size)
+        self.table = torch.arange(1 - pages, 1 + (slots - 1) * pages, device="cuda", dtype=torch.int32).view(slots, pages)
+        self.lengths = torch.zeros(slots, device="cuda", dtype=torch.int32)
+
+    def __call__(self, x, slots, cu_seqlens=None):
+        heads = self.w_in(rms_norm_fp8(x, self.norm)).unflatten(1, (-1, self.dim))
+        q, k, v = heads.split([self.heads, self.kv_heads, self.kv_heads], 1)
+        if cu_seqlens is None:
+            self.lengths[slots] += 1
+            positions = self.lengths[slots] - 1
+        else:
+            self.lengths[slots] += cu_seqlens.diff()
+            token = torch.arange(x.shape[0], device="cuda")
+            seq = torch.searchsorted(cu_seqlens[1:].contiguous(), token, right=True)
+            positions = (self.lengths[slots] - cu_seqlens[1:])[seq] + token
+        table, lengths = self.table[slots], self.lengths[slots]
+        q = rotary(q, positions, self.frequencies)
+        self.pool.append(k, v, table, lengths, cu_seqlens=cu_seqlens, frequencies=self.frequencies)
+        out = self.pool.attend(q, table, lengths, cu_seqlens=cu_seqlens)
+        return self.w_out(quantize_fp8(out.flatten(1)), residual=x)
+
+
+def run(lengths=(37, 5, 64, 18), decode=6, hidden=512, seed=0, attention=False):
     """Largest relative difference, per layer stack output, between tokens decoded
     from the prompts' states and the same tokens inside whole-sequence passes."""
     batch = len(lengths)
@@ -106,7 +141,8 @@ def run(lengths=(37, 5, 64, 18), decode=6, hidden=512, seed=0):
 
     def stack():
         gen = torch.Generator("cuda").manual_seed(seed)
-        return [DeltaLayer(gen, batch + 1, hidden, heads=4), SelectiveLayer(gen, batch + 1, hidden, channels=768)]
+        middle = [AttentionLayer(gen, batch + 1, hidden, heads=4, kv_heads=2)] if attention else []
+        return [DeltaLayer(gen, batch + 1, hidden, heads=4), *middle, SelectiveLayer(gen, batch + 1, hidden, channels=768)]
 
     gen = torch.Generator("cuda").manual_seed(seed + 1)
     rows = [torch.randn(n + decode, hidden, generator=gen, device="cuda").bfloat16() for n in lengths]
@@ -133,5 +169,7 @@ def run(lengths=(37, 5, 64, 18), decode=6, hidden=512, seed=0):
 
 
 if __name__ == "__main__":
-    same, off = run()
-    print(f"prompt outputs in two batchings differ by at most {same:.3g}; decoded tokens by {off:.3g} of their norm")
+    for attention in (False, True):
+        same, off = run(attention=attention)
+        print(f"{'with' if attention else 'without'} attention: prompt outputs in two batchings differ by at most {same:.3g}; "
+              f"decoded tokens by {off:.3g} of their norm")

@@ -218,3 +218,15 @@ def test_attention_is_what_the_reference_computes_without_a_cache():
     # A value is within s / 2 of what is held, uniformly: s / sqrt(12) in the mean, s below 6 / 15 of a deviation, so
     # 0.12 of v; keys move a score by 0.12 of a deviation, which moves weights by as much. Twice their sum bounds it.
     assert float((out.double() - want).norm() / want.norm()) < 2 * 0.24
+
+
+def test_the_example_runs_with_an_attention_layer():
+    import importlib.util
+    import os
+
+    from conftest import ROOT
+    spec = importlib.util.spec_from_file_location("recurrent_layers", os.path.join(ROOT, "examples", "recurrent_layers.py"))
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    same, off = module.run(attention=True)
+    assert same == same and off == off
