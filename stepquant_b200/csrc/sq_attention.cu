@@ -732,7 +732,8 @@ cudaError_t launch_rows(const sq_kv_attention_args &a, int most_rows, cudaStream
     if (sms < 1) return cudaErrorInvalidDevice;
     const int resident = NT == 1 && D <= 128 ? 2 : 1;
     const unsigned grid = unsigned(sms * resident < kMostCtas ? sms * resident : kMostCtas);
-    cudaError_t e = cudaFuncSetAttribute(rows_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kShared);
+    static std::atomic<uint64_t> devices{0};
+    cudaError_t e = allow_shared(rows_kernel<T, D, NT>, Shape::kShared, devices);
     if (e != cudaSuccess) return e;
     rows_kernel<T, D, NT><<<grid, kAttnThreads, Shape::kShared, s>>>(a, most_rows);
     e = cudaGetLastError();

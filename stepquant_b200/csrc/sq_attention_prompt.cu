@@ -658,7 +658,8 @@ cudaError_t launch_prompt(const sq_kv_attention_args &a, int few_rows, cudaStrea
     const unsigned strips = unsigned(a.tokens / per + a.num_seqs);
     const int64_t grid = int64_t(strips) * a.heads;
     if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    const cudaError_t e = cudaFuncSetAttribute(prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kShared);
+    static std::atomic<uint64_t> devices{0};
+    const cudaError_t e = allow_shared(prompt_kernel<T, D>, Shape::kShared, devices);
     if (e != cudaSuccess) return e;
     prompt_kernel<T, D><<<unsigned(grid), Shape::kThreads, Shape::kShared, s>>>(a, per, strips, few_rows);
     return cudaGetLastError();

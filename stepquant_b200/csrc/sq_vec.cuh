@@ -2,6 +2,8 @@
 // convolution, scan, block-scaled product).
 #pragma once
 
+#include <atomic>
+
 #include "sq_common.cuh"
 
 namespace sq {
@@ -56,6 +58,19 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;"
         : "=l"(r) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)), "l"(reinterpret_cast<uint64_t &>(c)));
     return reinterpret_cast<float2 &>(r);
+}
+
+// Dynamic shared memory of a kernel, set once for each device (a call to the driver of its own otherwise).
+template <class K>
+inline cudaError_t allow_shared(K kernel, int bytes, std::atomic<uint64_t> &devices) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = uint64_t(1) << (device & 63);
+    if (device < 64 && (devices.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) devices.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

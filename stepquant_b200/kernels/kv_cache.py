@@ -18,6 +18,7 @@ pages): nothing is written there or attended to, and zeros are read.  The same
 goes for positions past the table and pages past the pool, which set a bit in
 ``status``.  Asynchronous on the current stream.
 """
+import functools
 import math
 
 import torch
@@ -32,11 +33,12 @@ _pack = N.packer(N.SqKvArgs)
 _pack_attention = N.packer(N.SqKvAttentionArgs)
 
 
-def _int32(x, shape, device, name):
+_WIDTHS = {18 * d: d for d in HEAD_DIMS}
+
+
+def _int32(x, index, device):
     """int32 tensor with a contiguous last axis on ``device``."""
-    if x.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, x.shape)):
-        raise ValueError(f"{name}: expected [{', '.join('any' if n is None else str(n) for n in shape)}], got {list(x.shape)}")
-    if x.dtype == torch.int32 and x.device == device and (x.stride(-1) == 1 or x.shape[-1] < 2):
+    if x.dtype is torch.int32 and x.get_device() == index and (x.stride(-1) == 1 or x.shape[-1] < 2):
         return x
     return x.to(device=device, dtype=torch.int32).contiguous()
 
@@ -44,41 +46,49 @@ def _int32(x, shape, device, name):
 class _Call:
     """Checked pool and sequences of one call."""
 
-    __slots__ = ("data", "table", "lengths", "cu", "seqs", "dim", "heads", "page_size", "kept")
+    __slots__ = ("data", "table", "lengths", "cu", "seqs", "width", "dim", "heads", "pages", "page_size", "index")
 
     def __init__(self, data, page_table, lengths, cu_seqlens, tokens):
-        if data.dim() != 4 or data.dtype != torch.uint8 or data.shape[3] not in [18 * d for d in HEAD_DIMS] or not data.is_contiguous():
+        shape = data.shape
+        if len(shape) != 4 or data.dtype is not torch.uint8 or shape[3] not in _WIDTHS or not data.is_contiguous():
             raise ValueError("data: expected contiguous uint8 [pages, heads, page size / 16, 18 D] with D in (64, 128, 256), got "
-                             f"{data.dtype} {list(data.shape)}")
-        if data.data_ptr() % 16 or data.shape[1] < 1 or data.shape[2] < 1:
+                             f"{data.dtype} {list(shape)}")
+        self.pages, self.heads, tiles, width = shape
+        if data.data_ptr() % 16 or self.heads < 1 or tiles < 1:
             raise ValueError("data: expected a 16-byte aligned pool of at least one head and one tile a page")
-        self.data, self.heads, self.page_size, self.dim = data, data.shape[1], TILE * data.shape[2], data.shape[3] // 18
+        self.data, self.page_size, self.dim, self.index = data, TILE * tiles, _WIDTHS[width], data.get_device()
         device = data.device
-        self.lengths = _int32(lengths, (None,), device, "lengths")
-        self.seqs = self.lengths.numel()
-        self.table = _int32(page_table, (self.seqs, None), device, "page_table")
+        if lengths.dim() != 1:
+            raise ValueError(f"lengths: expected [sequences], got {list(lengths.shape)}")
+        self.lengths, self.seqs = _int32(lengths, self.index, device), lengths.shape[0]
+        rows = page_table.shape
+        if len(rows) != 2 or rows[0] != self.seqs:
+            raise ValueError(f"page_table: expected [{self.seqs}, pages], got {list(rows)}")
+        self.table, self.width = _int32(page_table, self.index, device), rows[1]
         if cu_seqlens is None:
             if tokens != self.seqs:
                 raise ValueError(f"expected one token of each of {self.seqs} sequences without cu_seqlens, got {tokens}")
             self.cu = None
+        elif cu_seqlens.shape != (self.seqs + 1,):
+            raise ValueError(f"cu_seqlens: expected [{self.seqs + 1}], got {list(cu_seqlens.shape)}")
         else:
-            self.cu = _int32(cu_seqlens, (self.seqs + 1,), device, "cu_seqlens")
+            self.cu = _int32(cu_seqlens, self.index, device)
 
 
-def _rows(x, tokens, heads, dim, dtype, name):
-    if x.shape != (tokens, heads, dim) or x.dtype != dtype:
-        raise ValueError(f"{name}: expected {dtype} [{tokens}, {heads}, {dim}], got {x.dtype} {list(x.shape)}")
+def _rows(x, shape, dtype, name):
+    if x.shape != shape or x.dtype is not dtype:
+        raise ValueError(f"{name}: expected {dtype} {list(shape)}, got {x.dtype} {list(x.shape)}")
     return x if x.stride(2) == 1 else x.contiguous()
 
 
 def _launch(entry, call, k, v, frequencies, positions, interleaved, magnitude, status):
-    p, table = N.address, call.table
+    p, table, (ks, kh, _), (vs, vh, _) = N.address, call.table, k.stride(), v.stride()
     index = N.device_index(call.data, k, v, frequencies, positions, N.status_word(status))
     N.launch(entry, _pack(k.data_ptr(), v.data_ptr(), call.data.data_ptr(), table.data_ptr(), call.lengths.data_ptr(), p(call.cu),
-                          p(positions), p(frequencies), p(status), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                          table.stride(0), call.data.shape[0], k.shape[0], call.seqs, table.shape[1], call.heads, call.dim,
-                          call.page_size, N.dtype_code(k.dtype), 0 if frequencies is None else 2 * frequencies.numel(),
-                          positions is not None and positions.dtype == torch.int64, bool(interleaved), magnitude), index)
+                          p(positions), p(frequencies), p(status), ks, kh, vs, vh, table.stride(0), call.pages, k.shape[0], call.seqs,
+                          call.width, call.heads, call.dim, call.page_size, N.dtype_code(k.dtype),
+                          0 if frequencies is None else 2 * frequencies.numel(),
+                          positions is not None and positions.dtype is torch.int64, bool(interleaved), magnitude), index)
 
 
 def kv_append(data, k, v, page_table, lengths, *, cu_seqlens=None, frequencies=None, interleaved=False, magnitude=1.0,
@@ -97,8 +107,9 @@ def kv_append(data, k, v, page_table, lengths, *, cu_seqlens=None, frequencies=N
         raise ValueError("k: expected [tokens, heads, dim]")
     call = _Call(data, page_table, lengths, cu_seqlens, k.shape[0])
     N.dtype_code(k.dtype)
-    k = _rows(k, k.shape[0], call.heads, call.dim, k.dtype, "k")
-    v = _rows(v, k.shape[0], call.heads, call.dim, k.dtype, "v")
+    shape = (k.shape[0], call.heads, call.dim)
+    k = _rows(k, shape, k.dtype, "k")
+    v = _rows(v, shape, k.dtype, "v")
     frequencies = checked_frequencies(frequencies, call.dim)
     if positions is not None:
         positions = checked_positions(positions, k.shape[0])
@@ -124,6 +135,11 @@ def kv_read(data, page_table, lengths, *, cu_seqlens=None, tokens=None, dtype=to
     return k, v
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(*sizes):
+    return N.lib().sq_kv_attention_workspace_bytes(*sizes)
+
+
 def kv_attention(q, data, page_table, lengths, *, cu_seqlens=None, scale=None, window=None, status=None):
     """Softmax attention of the new tokens over their sequences: [T, Hq, D] like q.
 
@@ -137,7 +153,7 @@ def kv_attention(q, data, page_table, lengths, *, cu_seqlens=None, scale=None, w
         raise ValueError("q: expected [tokens, heads, dim]")
     tokens, q_heads, dim = q.shape
     call = _Call(data, page_table, lengths, cu_seqlens, tokens)
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    if q.dtype is not torch.bfloat16 and q.dtype is not torch.float16:
         raise NotImplementedError(f"attention is built for bfloat16 and float16 queries, got {q.dtype}")
     if dim != call.dim or q_heads < 1 or q_heads % call.heads:
         raise ValueError(f"q: expected [{tokens}, a multiple of {call.heads}, {call.dim}], got {list(q.shape)}")
@@ -155,12 +171,11 @@ def kv_attention(q, data, page_table, lengths, *, cu_seqlens=None, scale=None, w
     out = data.new_empty((tokens, q_heads, dim), dtype=q.dtype)
     if not call.seqs:
         return out.zero_()
-    lib, p = N.lib(), N.address
-    size = lib.sq_kv_attention_workspace_bytes(tokens, call.seqs, q_heads, call.heads, dim)
+    p, size = N.address, _workspace_bytes(tokens, call.seqs, q_heads, call.heads, dim)
     workspace = data.new_empty(size) if size > 0 else None
-    N.launch(lib.sq_kv_attention, _pack_attention(
+    N.launch(N.lib().sq_kv_attention, _pack_attention(
         q.data_ptr(), data.data_ptr(), out.data_ptr(), table.data_ptr(), call.lengths.data_ptr(), p(call.cu), p(status), p(workspace),
-        size, rows, heads, table.stride(0), data.shape[0], tokens, call.seqs, table.shape[1], q_heads, call.heads, dim,
+        size, rows, heads, table.stride(0), call.pages, tokens, call.seqs, call.width, q_heads, call.heads, dim,
         call.page_size, N.dtype_code(q.dtype), 0 if window is None else min(window, 2 ** 31 - 1), scale), index)
     return out
 

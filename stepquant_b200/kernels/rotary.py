@@ -62,7 +62,7 @@ def checked_frequencies(frequencies, dim):
         return None
     if frequencies.dim() != 1 or 2 * frequencies.numel() > dim:
         raise ValueError(f"frequencies: expected [turned / 2] for at most {dim} channels, got {list(frequencies.shape)}")
-    return frequencies if frequencies.dtype == torch.float64 and frequencies.is_contiguous() else frequencies.double().contiguous()
+    return frequencies if frequencies.dtype is torch.float64 and frequencies.is_contiguous() else frequencies.double().contiguous()
 
 
 def checked_positions(positions, tokens):
