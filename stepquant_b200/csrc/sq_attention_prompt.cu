@@ -89,12 +89,6 @@ __device__ __forceinline__ uint4 unpack_value(uint32_t w, __half2 s, __half2 s16
 __device__ __forceinline__ float low_bf16(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float high_bf16(uint32_t p) { return __uint_as_float(p & 0xFFFF0000u); }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-
 template <class T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>

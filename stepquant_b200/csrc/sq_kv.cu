@@ -96,12 +96,9 @@ __device__ __forceinline__ void quantize(const double (&x)[8], uint32_t lanes, u
 // The same in fp32 of x[0..7], each within `off` of the value that is meant (0: exact).  False in all eight
 // lanes where a result may be another in exact arithmetic.
 __device__ __forceinline__ bool quantize_fast(const float (&x)[8], float off, uint32_t lanes, uint32_t &word, uint32_t &pair) {
-    float low = x[0], high = x[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) {
-        low = fminf(low, x[i]);
-        high = fmaxf(high, x[i]);
-    }
+    float low = fminf(min3(x[0], x[1], x[2]), min3(x[3], x[4], x[5])), high = fmaxf(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]));
+    low = min3(low, x[6], x[7]);
+    high = max3(high, x[6], x[7]);
 #pragma unroll
     for (int i = 1; i < 8; i *= 2) {
         low = fminf(low, __shfl_xor_sync(lanes, low, i));
@@ -119,7 +116,7 @@ __device__ __forceinline__ bool quantize_fast(const float (&x)[8], float off, ui
     // The scale: s the least bf16 with 15 s >= d.  15 s has 12 bits.
     const float d = high - m;
     sure = sure && (off != 0.f || (d + m == high && high - d == m)) && d < 1e38f && d > 1e-30f && fmaxf(high, -low) < 3e38f;
-    uint32_t s_bits = (__float_as_uint(d / 15.f) + 0xFFFFu) & 0xFFFF0000u;
+    uint32_t s_bits = (__float_as_uint(d * (1.f / 15.f)) + 0xFFFFu) & 0xFFFF0000u;  // or one above or below
     if (15.f * __uint_as_float(s_bits - 0x10000u) >= d) s_bits -= 0x10000u;
     if (15.f * __uint_as_float(s_bits) < d) s_bits += 0x10000u;
     const float s = __uint_as_float(s_bits), slack = 2.f * off + d * 0x1p-20f, least = off == 0.f ? 0.f : slack;
@@ -128,14 +125,17 @@ __device__ __forceinline__ bool quantize_fast(const float (&x)[8], float off, ui
     // step is the right one.
     constexpr float kWhole = 12582912.f;
     const float per = reciprocal_approx(s), clear = 0.5f * (s - slack);
-    bool all = true;
+    float farthest = 0.f;
     word = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 8; i += 2) {
         const float e = x[i] - m, near = fmaf(e, per, kWhole), rest = fmaf(kWhole - near, s, e);
-        all &= fabsf(rest) < clear;
-        word += (__float_as_uint(near) - 0x4B400000u) << ((i >> 1) * 4 + (i & 1) * 16);
+        const float e1 = x[i + 1] - m, near1 = fmaf(e1, per, kWhole), rest1 = fmaf(kWhole - near1, s, e1);
+        farthest = max3_or_nan(farthest, fabsf(rest), fabsf(rest1));  // not a number where a value is not finite
+        // Codes i and i + 1 to bits 2 i and 2 i + 16, by multiplications (the adders are the busier ones).
+        word += (__float_as_uint(near) - 0x4B400000u) * (1u << (2 * i)) + (__float_as_uint(near1) - 0x4B400000u) * (1u << (2 * i + 16));
     }
+    bool all = farthest < clear;
     if (!all && off == 0.f) {  // exact values: ties, to the even code, and their neighbours
         all = true;
         word = 0;
@@ -211,8 +211,8 @@ __global__ void __launch_bounds__(kKvThreads, 4) kv_append_kernel(sq_kv_args a, 
     const bool pairs_wide = k_wide && half % 8 == 0;
     // What a rotated channel is off by at most, in units of 2^-24 (|x1| + |x2|): sine and cosine by pi / 2 (their
     // argument in half turns is rounded to fp32), 1 (the functions) and 1/2 (the magnitude's product), then the
-    // products and their sum by 1/2 each; 4.1 in all.
-    const float turn_off = 0x1.1p-22f * fabsf(a.magnitude);
+    // products and their sum by 1/2 each; 4.1 in all, and |x1| + |x2| is at most twice the larger.
+    const float turn_off = 0x1.1p-21f * fabsf(a.magnitude);
     // Threads are [token][lane] where a token's lanes are fewer than them.
     const int t_step = max(1, kKvThreads / lanes), t0 = int(threadIdx.x) / lanes < t_step ? int(threadIdx.x) / lanes : 0;
     if (lanes < kKvThreads && int(threadIdx.x) >= t_step * lanes) return;
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kKvThreads, 4) kv_append_kernel(sq_kv_args a, 
                     if (c + e < a.turned) {
                         const float2 z = cs[(c + e) / 2];
                         const float u = x[e], w = x[e + 1];
-                        off = fmaxf(off, fabsf(u) + fabsf(w));
+                        off = max3(off, fabsf(u), fabsf(w));
                         x[e] = u * z.x - w * z.y;
                         x[e + 1] = u * z.y + w * z.x;
                     }
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kKvThreads, 4) kv_append_kernel(sq_kv_args a, 
                 for (int e = 0; e < 8; ++e) {
                     const float2 z = cs[f + e];
                     const float w = to_float(other[e]);
-                    off = fmaxf(off, fabsf(x[e]) + fabsf(w));
+                    off = max3(off, fabsf(x[e]), fabsf(w));
                     x[e] = x[e] * z.x + (upper ? w : -w) * z.y;
                 }
             } else {
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kKvThreads, 4) kv_append_kernel(sq_kv_args a, 
                         const int f = upper ? c + e - half : c + e;
                         const float w = to_float(from[upper ? f : c + e + half]);
                         const float2 z = cs[f];
-                        off = fmaxf(off, fabsf(x[e]) + fabsf(w));
+                        off = max3(off, fabsf(x[e]), fabsf(w));
                         x[e] = x[e] * z.x + (upper ? w : -w) * z.y;
                     }
                 }

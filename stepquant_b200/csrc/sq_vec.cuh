@@ -42,6 +42,23 @@ __device__ __forceinline__ float reciprocal_approx(float x) {
 // result is -0, for less than 10^-36 in size; -infinity and NaN give NaN as the quotient does.
 __device__ __forceinline__ float silu(float x) { return x * reciprocal_approx(1.f + exp2_approx(-kLog2e * x)); }
 
+// Largest and smallest of three, NaN aside.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float max3_or_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float r;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // Pairs of fp32 values, one instruction for both.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     uint64_t r;
