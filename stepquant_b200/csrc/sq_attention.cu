@@ -6,6 +6,14 @@
 // the product, q . k = sum over groups of s (q . c) + m sum(q), and those of a value go
 // to its weight, p v = (p s) c + p m, so the tensor cores work on the codes, which 16
 // bits hold exactly.
+//
+// Few rows (rows_kernel): mma.sync with tokens (scores) or channels (values) as the 16
+// rows and eight query rows as columns; a warp's fragments are the tile's words with a
+// shift and a mask.  The products are 17 % of the tensor pipe's time: with eight columns
+// tcgen05 would idle as much and want the codes unpacked into shared memory first.
+// Instructions bound it: 390 a tile of 16 tokens and 2304 bytes (64 masks, 48 shifts, 34
+// products, the rest scales, exponentials and waits), at 2.2 a clock and SM, 256 ragged
+// requests of up to 8192 tokens (1.3 GB) in 357 us, 3.6 TB/s.
 #include "sq_kv.cuh"
 #include "sq_rows.cuh"
 #include "sq_tc.cuh"
@@ -650,6 +658,8 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
             tc::bar_wait(&bars[warp][r % kStages], (r / kStages) & 1, &alone, tc::kWaitClocks);
     }
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    // Beside prompts it started when their last CTAs had: what comes after it in the stream waits for them too.
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
 }
 
 // Joins the parts of items that several CTAs had: CTAs (c, y), c that in whose span an item ends, take a
@@ -726,7 +736,7 @@ __global__ void __launch_bounds__(kAttnThreads) join_kernel(sq_kv_attention_args
 }
 
 template <class T, int D, int NT>
-cudaError_t launch_rows(const sq_kv_attention_args &a, int most_rows, cudaStream_t s) {
+cudaError_t launch_rows(const sq_kv_attention_args &a, int most_rows, bool beside, cudaStream_t s) {
     using Shape = RowsShape<D, NT>;
     const int sms = sms_of(s);
     if (sms < 1) return cudaErrorInvalidDevice;
@@ -735,18 +745,20 @@ cudaError_t launch_rows(const sq_kv_attention_args &a, int most_rows, cudaStream
     static std::atomic<uint64_t> devices{0};
     cudaError_t e = allow_shared(rows_kernel<T, D, NT>, Shape::kShared, devices);
     if (e != cudaSuccess) return e;
-    rows_kernel<T, D, NT><<<grid, kAttnThreads, Shape::kShared, s>>>(a, most_rows);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid, kJoins);
+    cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kAttnThreads);
-    cfg.dynamicSmemBytes = size_t(grid) * Shape::kRows * sizeof(float);
+    cfg.dynamicSmemBytes = Shape::kShared;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
+    cfg.numAttrs = beside ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, rows_kernel<T, D, NT>, a, most_rows);
+    if (e != cudaSuccess) return e;
+    cfg.gridDim = dim3(grid, kJoins);
+    cfg.dynamicSmemBytes = size_t(grid) * Shape::kRows * sizeof(float);
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, join_kernel<T, D, NT>, a, most_rows);
 }
@@ -757,23 +769,28 @@ bool wide_rows(int tokens, int seqs, int q_heads, int heads, int dim) {
 }
 
 template <class T>
-cudaError_t launch_rows(const sq_kv_attention_args &a, int most_rows, cudaStream_t s) {
+cudaError_t launch_rows(const sq_kv_attention_args &a, int most_rows, bool beside, cudaStream_t s) {
     const bool wide = wide_rows(a.tokens, a.num_seqs, a.q_heads, a.heads, a.dim);
     switch (a.dim) {
-        case 64: return wide ? launch_rows<T, 64, 2>(a, most_rows, s) : launch_rows<T, 64, 1>(a, most_rows, s);
-        case 128: return wide ? launch_rows<T, 128, 2>(a, most_rows, s) : launch_rows<T, 128, 1>(a, most_rows, s);
-        default: return launch_rows<T, 256, 1>(a, most_rows, s);
+        case 64: return wide ? launch_rows<T, 64, 2>(a, most_rows, beside, s) : launch_rows<T, 64, 1>(a, most_rows, beside, s);
+        case 128: return wide ? launch_rows<T, 128, 2>(a, most_rows, beside, s) : launch_rows<T, 128, 1>(a, most_rows, beside, s);
+        default: return launch_rows<T, 256, 1>(a, most_rows, beside, s);
     }
 }
 
 // Sequences of up to kFewRows rows (new tokens times query heads of a kv head) go through rows_kernel, those
-// of more through the prompts' kernel, each decided on the device: a batch may have both.
+// of more through the prompts' kernel, each decided on the device: a batch may have both.  The few rows are a
+// programmatic dependent of the prompts, whose outputs they do not touch: they fill the SMs that the prompts'
+// last CTAs leave (8 ragged prompts, two of them short: 318 us one after the other).
 cudaError_t launch_attention(const sq_kv_attention_args &a, cudaStream_t s) {
     const int group = a.q_heads / a.heads;
     const bool prompts = a.cu_seqlens && group <= 128 && int64_t(a.tokens) * group > kFewRows;
     const int most_rows = prompts ? kFewRows : 0x7fffffff;
-    const cudaError_t e = a.dtype == SQ_BF16 ? launch_rows<__nv_bfloat16>(a, most_rows, s) : launch_rows<__half>(a, most_rows, s);
-    return e == cudaSuccess && prompts ? launch_prompt_attention(a, kFewRows, s) : e;
+    if (prompts) {
+        const cudaError_t e = launch_prompt_attention(a, kFewRows, s);
+        if (e != cudaSuccess) return e;
+    }
+    return a.dtype == SQ_BF16 ? launch_rows<__nv_bfloat16>(a, most_rows, prompts, s) : launch_rows<__half>(a, most_rows, prompts, s);
 }
 
 }  // namespace

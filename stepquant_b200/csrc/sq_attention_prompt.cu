@@ -18,6 +18,12 @@
 // values and weights were half as exact: 2.6e-3 of an output's norm, of which 1.7e-3 are
 // its own rounding).
 // Row maxima may lag by 2^8, so sums in tensor memory are seldom rescaled.
+//
+// 4096 tokens over 16384 of 32 / 8 heads of 128: 1120 us, 860 TFLOP/s, 0.52 of the burst
+// rate of a library product.  A tile's chain bounds it (products, a commit, S read, maxima,
+// weights stored, an arrival), of which the other tile's products hide half; blocks of 64
+// keys with S and P in two buffers measured 1371 us, as a product of 128 x 64 takes the 64
+// clocks of one of 128 x 128.
 #include "sq_kv.cuh"
 #include "sq_rows.cuh"
 #include "sq_tc.cuh"
@@ -149,6 +155,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
     uint8_t *const more_queries = values + kStages * Shape::kKeyBytes, *const more_keys = more_queries + kTiles * Shape::kMoreQuery;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = a.q_heads / a.heads;
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");  // the few rows' kernel, once every CTA has begun
 
     // Later strips, which see more keys, first.
     PromptItem item;
