@@ -542,7 +542,7 @@ int32_t sq_rotary(const sq_rotary_args *args, sq_stream_t stream);
  *        pairs at [r][group]; key words in blocks of up to 128 channels (n = 1 or 2
  *        groups), [block][r][2 n t + 2 group + j] for channels 16 t + 8 j of a group;
  *        value words, number w = dim / 64 i + group for channels 8 i, at [w / 8][u][w % 8].
- * dim 64, 128 or 256; page_size a multiple of 16.
+ * dim 64, 128 or 256; page_size a multiple of 16, up to 65536; a table reaches fewer than 2^31 - 2^16 tokens.
  *
  * Sequence n holds lengths[n] tokens, position p in page page_table[n][p / page_size];
  * its cu_seqlens[n + 1] - cu_seqlens[n] new tokens (without cu_seqlens: one, and

@@ -817,6 +817,7 @@ extern "C" int32_t sq_kv_attention(const sq_kv_attention_args *args, sq_stream_t
     if (a.heads > 4096 || a.q_heads > 65536 || a.page_size > 65536 || a.tokens > kMostTokens || a.num_seqs > (1 << 30))
         return SQ_ERR_UNSUPPORTED;
     if (int64_t(a.tokens) * (a.q_heads / a.heads) > kMostTokens) return SQ_ERR_UNSUPPORTED;  // rows of a kv head
+    if (int64_t(a.table_width) * a.page_size > kMostTokens) return SQ_ERR_UNSUPPORTED;  // positions are ints
     if (!a.cu_seqlens && a.tokens != a.num_seqs) return SQ_ERR_ARGUMENT;
     if (a.tokens == 0 || a.num_seqs == 0) return SQ_OK;
     if (!a.q || !a.out || !a.lengths || (a.table_width && !a.page_table) || (a.num_pages && !a.data)) return SQ_ERR_ARGUMENT;

@@ -365,6 +365,7 @@ int32_t kv_entry(const sq_kv_args *args, bool append, sq_stream_t stream) {
     if (a.page_size < kTile || a.page_size % kTile || a.turned % 2 || a.turned > a.dim || a.table_stride < 0) return SQ_ERR_SHAPE;
     if (a.k_stride < 0 || a.k_head_stride < 0 || a.v_stride < 0 || a.v_head_stride < 0 || !aligned16(a.data)) return SQ_ERR_SHAPE;
     if (a.heads > 4096 || a.page_size > 65536 || a.tokens > kMostTokens || a.num_seqs > (1 << 30)) return SQ_ERR_UNSUPPORTED;
+    if (int64_t(a.table_width) * a.page_size > kMostTokens) return SQ_ERR_UNSUPPORTED;  // positions are ints
     if (!a.cu_seqlens && a.tokens != a.num_seqs) return SQ_ERR_ARGUMENT;
     if (a.tokens == 0) return SQ_OK;
     if (!a.k || !a.v || (a.num_seqs && (!a.lengths || (a.table_width && !a.page_table) || (a.num_pages && !a.data)))) return SQ_ERR_ARGUMENT;

@@ -214,3 +214,42 @@ def test_strided_queries():
         wide[:, pad:pad + 8 * dim] = q.flatten(1)
         assert torch.equal(pool.attend(wide[:, pad:pad + 8 * dim].unflatten(1, (8, dim)), table, device_lengths), want)
     assert torch.equal(pool.attend(q.transpose(0, 1).contiguous().transpose(0, 1), table.long(), device_lengths.long()), want)
+
+
+@pytest.mark.parametrize("dim,q_heads,heads", [(64, 128, 1), (128, 8, 2), (256, 128, 1), (128, 66, 1)])
+def test_prompts_longer_than_what_is_held(dim, q_heads, heads):
+    """More new tokens than a sequence holds: those at positions below zero see nothing; many heads a kv head."""
+    page, length, count = 32, 150, 200
+    table, device_lengths, _, pages = _sequences([length], page)
+    pool = _pool(pages, heads, page, dim)
+    q = _rand(count, q_heads, dim, seed=5).bfloat16()
+    for window in (None, 40):
+        got = pool.attend(q, table, device_lengths, cu_seqlens=torch.tensor([0, count], device="cuda"), window=window)
+        assert not bool(got[:count - length].any())
+        _check(got[count - length:], q[count - length:], pool.data, table, [length], [length], page, window=window)
+    pool.check_status()
+
+
+@pytest.mark.parametrize("factor", [2.0 ** -100, 2.0 ** -20, 2.0 ** 13])
+@pytest.mark.parametrize("counts", [None, [130]])
+def test_values_of_any_size(factor, counts):
+    """Values far from one, some of them much larger than the others; tiny and large queries."""
+    lengths, page, dim = [400], 16, 128
+    table, device_lengths, cu, pages = _sequences(lengths, page, counts)
+    pool = _pool(pages, 1, page, dim)
+    k, v = _rand(400, 1, dim, seed=3).bfloat16(), _rand(400, 1, dim, seed=4) * factor
+    v[::50] *= 100
+    pool.append(k, v.bfloat16(), table, device_lengths, cu_seqlens=torch.tensor([0, 400], device="cuda"))
+    tokens = 1 if counts is None else 130
+    q = (_rand(tokens, 4, dim, seed=6) * torch.tensor([1.0, 1e-20, 20.0, 3.0], device="cuda")[:, None]).bfloat16()
+    got = pool.attend(q, table, device_lengths, cu_seqlens=cu)
+    _check(got / factor, q, _scaled(pool.data, factor), table, lengths, counts or [1], page)
+
+
+def _scaled(data, factor):
+    """The pool's bytes with values' scales and minima over `factor`, a power of two: values are near one again."""
+    dim = data.shape[3] // 18
+    out = data.clone()
+    pairs = out[..., 17 * dim:].contiguous().view(torch.bfloat16)
+    out[..., 17 * dim:] = (pairs.double() / factor).bfloat16().view(torch.uint8)
+    return out

@@ -104,7 +104,7 @@ def test_c_entries_refuse_before_launch():
         for change, want in ((dict(k=None), 1), (dict(v=None), 1), (dict(data=None), 1), (dict(page_table=None), 1), (dict(lengths=None), 1),
                              (dict(dim=96), 3), (dict(page_size=24), 2), (dict(page_size=0), 2), (dict(heads=0), 1), (dict(num_seqs=3), 1),
                              (dict(data=fake + 8), 2), (dict(table_stride=-1), 2), (dict(k_stride=-1), 2), (dict(dtype=5), 1),
-                             (dict(num_pages=-1), 1), (dict(tokens=0, num_seqs=0), 0)):
+                             (dict(num_pages=-1), 1), (dict(table_width=1 << 27), 3), (dict(tokens=0, num_seqs=0), 0)):
             assert code(entry, N.SqKvArgs, **{**kv, **change}) == want, change
     assert code(lib.sq_kv_append, N.SqKvArgs, **{**kv, "turned": 64}) == 1  # without frequencies
     assert code(lib.sq_kv_append, N.SqKvArgs, **{**kv, "turned": 66, "frequencies": fake}) == 2
@@ -118,5 +118,5 @@ def test_c_entries_refuse_before_launch():
     for change, want in ((dict(q=None), 1), (dict(out=None), 1), (dict(lengths=None), 1), (dict(dtype=0), 3), (dict(dtype=4), 1), (dict(dim=72), 3),
                          (dict(scale=0.0), 1), (dict(scale=math.nan), 1), (dict(scale=math.inf), 1), (dict(window=-1), 1), (dict(q_heads=0), 1),
                          (dict(heads=3), 2), (dict(q_stride=4), 2), (dict(q=fake + 2), 2), (dict(out=fake + 8), 2), (dict(workspace=None), 5),
-                         (dict(workspace_bytes=size - 1), 5), (dict(num_seqs=1), 1), (dict(page_size=8), 2), (dict(tokens=0, num_seqs=0), 0)):
+                         (dict(workspace_bytes=size - 1), 5), (dict(num_seqs=1), 1), (dict(table_width=1 << 27), 3), (dict(page_size=8), 2), (dict(tokens=0, num_seqs=0), 0)):
         assert code(lib.sq_kv_attention, N.SqKvAttentionArgs, **{**attend, **change}) == want, change
