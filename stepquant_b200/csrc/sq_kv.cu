@@ -7,7 +7,7 @@
 // fp32 finds it, with a bound on what its roundings may have changed, and groups where
 // that reaches a border (a few in ten thousand, and those at slow pairs near position 0)
 // are done again in 64 bits.  Instructions bound append: 32768 tokens of 8 heads of 128 in
-// 170 us, 430 for a warp's 256 values (8192 tokens 57 us; all in 64 bits 88), of which
+// 166 us, 430 for a warp's 256 values (8192 tokens 57 us; all in 64 bits 88), of which
 // loads, stores and places take 140, the rotation 30 and the groups done again, which
 // hold their CTA up, a quarter of the time.  Read: 48 us, 3.6 TB/s.
 #include "sq_kv.cuh"
@@ -18,7 +18,7 @@ namespace sq {
 namespace {
 
 constexpr int kKvThreads = 256;
-constexpr int kMostPerCta = 8;
+constexpr int kMostPerCta = 16;
 
 struct Place {
     int64_t tile;  // byte offset of head 0's tile, -1: nowhere
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(sq_kv_args a, int p
 template <class T, int D>
 cudaError_t launch_kv(const sq_kv_args &a, bool append, cudaStream_t s) {
     int per_cta = kMostPerCta;
-    while (per_cta > 1 && (int64_t(a.tokens) + per_cta - 1) / per_cta < 148 * 4) per_cta /= 2;
+    while (per_cta > 1 && (int64_t(a.tokens) + per_cta - 1) / per_cta < 148 * 2) per_cta /= 2;
     const unsigned grid = unsigned((int64_t(a.tokens) + per_cta - 1) / per_cta);
     auto wide = [&](const void *p, int64_t token, int64_t head) {
         constexpr int n = 16 / sizeof(T);
