@@ -196,7 +196,7 @@ __device__ __forceinline__ T *output_row(const sq_kv_attention_args &a, const Se
 }
 
 // ---------------------------------------------------------------------------
-// few rows: the cache's bytes bound it
+// few rows
 // ---------------------------------------------------------------------------
 template <int D, int NT>
 struct RowsShape {

@@ -5,7 +5,7 @@
 // channels each: the group's extremes are three shuffles away, and a lane's codes are
 // one 32-bit word of the tile.  A code is that of the definition in exact arithmetic:
 // fp32 finds it, with a bound on what its roundings may have changed, and groups where
-// that reaches a border (a few in ten thousand, and those at slow pairs near position 0)
+// that reaches a border (a few in a thousand, more near position 0)
 // are done again in 64 bits.  Instructions bound append: 32768 tokens of 8 heads of 128 in
 // 166 us, 430 for a warp's 256 values (8192 tokens 57 us; all in 64 bits 88), of which
 // loads, stores and places take 140, the rotation 30 and the groups done again, which
