@@ -132,11 +132,6 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[32]) {
                  : SQ_R8(0), SQ_R8(8), SQ_R8(16), SQ_R8(24) : "r"(addr));
 }
 // Stores are in tensor memory after tmem_stored().
-__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[32]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n"
-                 ::"r"(addr), SQ_W8(0), SQ_W8(8), SQ_W8(16), SQ_W8(24) : "memory");
-}
 __device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n"
                  ::"r"(addr), SQ_W8(0), SQ_W8(8) : "memory");
