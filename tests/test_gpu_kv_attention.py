@@ -10,8 +10,9 @@ p s, whose roundings to fp32 stay where a value's two parts happen to vanish, m 
 -8 s and c = 8.  At most 4 roundings of 2^-24 count there, as every further tile
 of tokens brings other codes: 143 * 4 * 2^-24 < 2^-14 of p s, and that is 4 u
 times 2^-8 s, so W takes 2^-8 s more.)  A score is off by
-no more than 2^-12 of scale sum |q| |k| (prompts round keys to f16; codes, exact,
-lose 2^-17), which moves weights by E = 2^-11 of that at most.  In norm roundings
+no more than 2^-12 of scale sum |q| |k| (queries and codes are exact in 16 bits;
+the fp32 sums of their products, 128 times a code's step beside it, lose 2^-17),
+which moves weights by E = 2^-11 of that at most.  In norm roundings
 add up as independent ones do: three of u / sqrt(3) each, u together, taken as 2 u.
 """
 import math
