@@ -62,6 +62,7 @@ struct Codes<__nv_bfloat16> {
     }
     static constexpr uint32_t kOnes = 0x3F803F80u;
     static constexpr float kLag = 8.f;
+    static constexpr bool kNarrow = false;  // p s has fp32's range
 };
 template <>
 struct Codes<__half> {
@@ -84,7 +85,12 @@ struct Codes<__half> {
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
     static constexpr uint32_t kOnes = 0x3C003C00u;
-    static constexpr float kLag = 2.f;  // weights p s reach 4 * 8738 (a group's largest scale in f16), below 65504
+    // p s has f16's range only, so what weights are taken against depends on p s: a row's reference R, p = 2^(score - R),
+    // rises where a p s is above kMostWeight, to bring that one to 2^8 .. 2^9 (what rounding loses of the others is then
+    // 2^-33 of the row's largest), or a p above 2^kMostPower, to bring it to 2^kLag (the scales are tiny then, and
+    // 2^-25 over 2^kLag is far below what an f16 output holds).
+    static constexpr bool kNarrow = true;
+    static constexpr float kLag = 24.f, kMostPower = 32.f, kMostWeight = 61440.f;
 };
 
 // Transpose of an 8 x 8 matrix of 16-bit values, two of row lane / 4 in each lane.
@@ -427,7 +433,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
             }
             top[j][0] = top[j][1] = kNone;
             sum[j][0] = sum[j][1] = 0.f;
-            against[j][0] = against[j][1] = 0.f;
+            against[j][0] = against[j][1] = C::kNarrow ? -kNone : 0.f;
         }
         int next_ahead = 0;
         const int next_mine = units_of(next);
@@ -506,8 +512,20 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     most[j][e] = fmaxf(fmaxf(z[0][j][e], z[0][j][2 + e]), fmaxf(z[1][j][e], z[1][j][2 + e]));
-                    grows = grows || most[j][e] > top[j][e] + lag;
+                    if constexpr (C::kNarrow) grows = grows || fmaf(most[j][e], to_log2, against[j][e]) > C::kMostPower;
+                    else grows = grows || most[j][e] > top[j][e] + lag;
                 }
+            auto rescale = [&](int j, int e, float factor) {
+                sum[j][e] *= factor;
+#pragma unroll
+                for (int b = 0; b < kGroups; ++b) {
+                    least[j][b][e] *= factor;
+                    ones[j][b][e] *= factor;
+                    ones[j][b][2 + e] *= factor;
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) acc[j][b][m][e] *= factor, acc[j][b][m][2 + e] *= factor;
+                }
+            };
             // The maxima that weights are taken against may lag behind by 2^kLag: they move seldom.
             if (__any_sync(~0u, grows)) {
 #pragma unroll
@@ -518,19 +536,18 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                         x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
                         x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
                         x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
-                        x = fmaxf(x, top[j][e]);
-                        const float factor = exp2_approx((top[j][e] - x) * to_log2);
-                        top[j][e] = x;
-                        against[j][e] = -x * to_log2;
-                        sum[j][e] *= factor;
-#pragma unroll
-                        for (int b = 0; b < kGroups; ++b) {
-                            least[j][b][e] *= factor;
-                            ones[j][b][e] *= factor;
-                            ones[j][b][2 + e] *= factor;
-#pragma unroll
-                            for (int m = 0; m < 4; ++m) acc[j][b][m][e] *= factor, acc[j][b][m][2 + e] *= factor;
+                        float factor;
+                        if constexpr (C::kNarrow) {
+                            const float now = fminf(against[j][e], C::kLag - x * to_log2);
+                            factor = exp2_approx(now - against[j][e]);
+                            against[j][e] = now;
+                        } else {
+                            x = fmaxf(x, top[j][e]);
+                            factor = exp2_approx((top[j][e] - x) * to_log2);
+                            top[j][e] = x;
+                            against[j][e] = -x * to_log2;
                         }
+                        rescale(j, e, factor);
                     }
             }
 #pragma unroll
@@ -542,6 +559,44 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                         z[h][j][i4] = exp2_approx(fmaf(z[h][j][i4], to_log2, against[j][i4 & 1]));
                         sum[j][i4 & 1] += z[h][j][i4];
                     }
+            if constexpr (C::kNarrow) {
+                float scale[2][2];  // largest of a token's groups
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t pairs[kGroups];
+                        load_words(unit + h * Tile::kBytes + Tile::kValuePairs + (g + 8 * i) * kGroups * 4, pairs);
+                        scale[h][i] = pair_scale(pairs[0]);
+#pragma unroll
+                        for (int b = 1; b < kGroups; ++b) scale[h][i] = fmaxf(scale[h][i], pair_scale(pairs[b]));
+                    }
+                // NaN aside, which a hidden token's may be too: its weight is 0.
+                auto largest = [&](int j, int e) {
+                    return fmaxf(fmaxf(z[0][j][e] * scale[0][0], z[0][j][2 + e] * scale[0][1]),
+                                 fmaxf(z[1][j][e] * scale[1][0], z[1][j][2 + e] * scale[1][1]));
+                };
+                bool over = false;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) over = over || fmaxf(largest(j, 0), largest(j, 1)) > C::kMostWeight;
+                if (__any_sync(~0u, over)) {
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float x = largest(j, e);
+                            x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
+                            x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
+                            x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
+                            const int less = x > C::kMostWeight ? int(__float_as_uint(x) >> 23) - 127 - 8 : 0;
+                            const float factor = __uint_as_float(uint32_t(127 - less) << 23);
+                            against[j][e] -= float(less);
+                            rescale(j, e, factor);
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) z[h][j][e] *= factor, z[h][j][2 + e] *= factor;
+                        }
+                }
+            }
             // Values: rows are channels (x: even ones, y: odd ones), columns query rows.
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -601,7 +656,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                 float total = sum[j][e];
 #pragma unroll
                 for (int i = 4; i < 32; i *= 2) total += __shfl_xor_sync(~0u, total, i);
-                if (g == 0) row_max[warp][row] = gave_up ? NAN : top[j][e] == kNone ? kNone : -against[j][e], row_sum[warp][row] = total;
+                if (g == 0) row_max[warp][row] = gave_up ? NAN : !C::kNarrow && top[j][e] == kNone ? kNone : -against[j][e], row_sum[warp][row] = total;
 #pragma unroll
                 for (int b = 0; b < kGroups; ++b) {
                     float low_part = least[j][b][e];

@@ -1,0 +1,63 @@
+"""kv_attention where values, weights, keys or lengths leave the ordinary range.
+
+Tolerances are those of test_gpu_kv_attention.py.  f16 outputs are 2^-14 and more in
+size but for single channels, whose rounding by 2^-25 is 2^-11 of 2^-14, a small part of
+4 u W, so no absolute term is needed.  The scores' share of the bound grows with the
+sharpest key, the bound in norm does not.
+"""
+import math
+
+import pytest
+import torch
+
+from kv_reference import attend, cached
+from test_gpu_kv_attention import _check, _pool, _scaled
+from test_gpu_kv_cache import _rand, _sequences
+
+pytestmark = pytest.mark.gpu
+
+BOTH = [torch.bfloat16, torch.float16]
+
+
+def _fill(pool, k, v, table, lengths):
+    ends = torch.tensor([0, k.shape[0]], device="cuda", dtype=torch.int32)
+    pool.append(k, v, table, lengths, cu_seqlens=ends)
+
+
+def _sharp(length, count, dim, values, boost, sink, dtype, q_heads=4, page=64, cache=None):
+    """(pool, q, table, lengths, cu): one key in each of the first eight units of 32 lies `boost` above the others, whose
+    scores have a deviation of one.  Each channel's values have a mean of their own, of size values[0], and the deviation
+    values[1]; those of the sharp keys are 0 with `sink`."""
+    table, lengths, cu, pages = _sequences([length], page, None if count is None else [count])
+    pool = _pool(pages, 1, page, dim)
+    tokens = count or 1
+    k, v = _rand(length, 1, dim, seed=3), values[0] * _rand(1, 1, dim, seed=6) + values[1] * _rand(length, 1, dim, seed=4)
+    q = _rand(tokens, q_heads, dim, seed=5)
+    k[:, :, 0], q[:, :, 0] = 0, 8
+    k[5:256:32, :, 0] = boost / (8 * dim ** -0.5)
+    if sink:
+        v[5:256:32] = 0
+    cache = cache or dtype
+    _fill(pool, k.to(cache), v.to(cache), table, lengths)
+    return pool, q.to(dtype), table, lengths, cu
+
+
+@pytest.mark.parametrize("count", [None, 3])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("values,boost,sink", [
+    ((0.01, 0.003), 10, False), ((5e-4, 1e-4), 0, False), ((5e-4, 1e-4), 10, False), ((5e-4, 1e-4), 12, False),
+    ((0.03, 0.01), 12, True), ((0.1, 0.03), 14, True), ((2.0, 0.6), 18, True)])
+def test_small_weights_of_few_rows(values, boost, sink, dim, count):
+    """Weights times values' scales far below 2^-14, in f16."""
+    pool, q, table, lengths, cu = _sharp(16384, count, dim, values, boost, sink, torch.float16)
+    got = pool.attend(q, table, lengths, cu_seqlens=cu)
+    _check(got, q, pool.data, table, [16384], [count or 1], 64)
+
+
+@pytest.mark.parametrize("count", [None, 3])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_large_scales_of_few_rows(dim, count):
+    """f16 queries over a cache of bf16 values that f16 does not reach, whose average it does."""
+    pool, q, table, lengths, cu = _sharp(16384, count, dim, (1e4, 2e5), 0, False, torch.float16, cache=torch.bfloat16)
+    got = pool.attend(q, table, lengths, cu_seqlens=cu)
+    _check(got, q, pool.data, table, [16384], [count or 1], 64)
