@@ -34,6 +34,9 @@ namespace {
 
 constexpr float kKeyDivisor = 16.f;
 constexpr float kPromptLag = 8.f;
+// Weights are 2^kPromptLift over what the maximum would make them, 2^15 at most: f16 then drops those below 2^-32 of
+// the row's largest and not those below 2^-25, which count where the largest belong to keys without a value.
+constexpr float kPromptLift = 7.f;
 
 template <int D>
 struct PromptShape {
@@ -368,7 +371,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
                         }
                     }
                 }
-                const float against = top == -INFINITY ? 0.f : -top;
+                const float against = top == -INFINITY ? 0.f : kPromptLift - top;
 #pragma unroll
                 for (int c = 0; c < kKeys / 32; ++c) {
                     uint32_t p[16];

@@ -61,3 +61,13 @@ def test_large_scales_of_few_rows(dim, count):
     pool, q, table, lengths, cu = _sharp(16384, count, dim, (1e4, 2e5), 0, False, torch.float16, cache=torch.bfloat16)
     got = pool.attend(q, table, lengths, cu_seqlens=cu)
     _check(got, q, pool.data, table, [16384], [count or 1], 64)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("boost", [12, 14, 18])
+def test_small_weights_of_prompts(boost, dim, dtype):
+    """A few keys without values take nearly all the weight: the output is what the others give."""
+    pool, q, table, lengths, cu = _sharp(16384, 200, dim, (64.0, 20.0), boost, True, dtype)
+    got = pool.attend(q, table, lengths, cu_seqlens=cu)
+    _check(got, q, pool.data, table, [16384], [200], 64)
