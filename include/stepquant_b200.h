@@ -598,7 +598,8 @@ int32_t sq_kv_read(const sq_kv_args *args, sq_stream_t stream);
  *   q, out  [tokens, q_heads, dim] in dtype (SQ_BF16 or SQ_F16); q 16-byte aligned,
  *           strides multiples of 8; out contiguous, 16-byte aligned
  *   workspace  sq_kv_attention_workspace_bytes(...) bytes, 16-byte aligned
- * Sequences of many new tokens take keys in f16 over 16: magnitudes up to 2^19.
+ * Sequences of many new tokens take keys and values in f16, over powers of two by the largest that any
+ * of 128 or 256 rows reaches: what is below 2^-24 of that loses bits.
  * status: also SQ_STATUS_TIMEOUT if a bounded device wait gave up; outputs concerned are NaN.
  */
 typedef struct sq_kv_attention_args {

@@ -12,11 +12,11 @@
 // Scores take keys as they are held: s (c - 8) has 3 + 8 significant bits and so is an f16,
 // and the rest of a group, m + 8 s, meets the sum of the query's channels in one more step
 // of K (the sum's f16 and its remainder, each by m and by 8 s).  Queries are f16 with each
-// row's largest value near 2^8, keys over 16.  Values m + s c and weights are rounded to f16
-// too, whatever the cache's type, values times a power of two that brings the largest of
-// the item's keys near 2^14, which a scan of their scales and minima finds first (bf16
-// values and weights were half as exact: 2.6e-3 of an output's norm, of which 1.7e-3 are
-// its own rounding).
+// row's largest value near 2^8.  Values m + s c and weights are rounded to f16 too, whatever
+// the cache's type (bf16 values and weights were half as exact: 2.6e-3 of an output's norm,
+// of which 1.7e-3 are its own rounding).  Keys and values are times a power of two each that
+// brings the largest of the item's to 2^13 .. 2^15, which a scan of scales and minima finds
+// first: f16 then keeps a key exactly down to 2^-24 of the largest.
 // Row maxima may lag by 2^8, so sums in tensor memory are seldom rescaled.
 //
 // 4096 tokens over 16384 of 32 / 8 heads of 128: 1120 us, 860 TFLOP/s, 0.52 of the burst
@@ -32,7 +32,7 @@
 namespace sq {
 namespace {
 
-constexpr float kKeyDivisor = 16.f;
+constexpr int kKeyPower = 13, kValuePower = 14;  // of the largest |m| + 15 s of an item's keys and values
 constexpr float kPromptLag = 8.f;
 // Weights are 2^kPromptLift over what the maximum would make them, 2^15 at most: f16 then drops those below 2^-32 of
 // the row's largest and not those below 2^-25, which count where the largest belong to keys without a value.
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
     __shared__ PromptBars bars;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, bad_values;
-    __shared__ unsigned most_value;
+    __shared__ unsigned most_key, most_value;
     __shared__ volatile int holes[8];  // block + 1 of the last one with tiles to leave out, by block modulo 8
     uint8_t *const queries = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     uint8_t *const keys = queries + kTiles * Shape::kQueryBytes, *const values = keys + kStages * Shape::kKeyBytes;
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
             tc::bar_init_fence();
             abort_flag = 0;
             bad_values = 0;
-            most_value = 0;
+            most_key = most_value = 0;
             for (int i = 0; i < 8; ++i) holes[i] = 0;
         }
         __syncwarp();
@@ -216,31 +216,40 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
     tc::fence_after();
     const uint32_t tmem = tmem_slot;
 
-    // Largest |m| + 15 s of the item's values.
+    // Largest |m| + 15 s of the item's keys and values.
     {
-        constexpr int kEach = D / 16;  // accesses of four pairs a tile
+        constexpr int kEach = D / 16;  // accesses of four pairs a tile, of keys and of values
         const int64_t end = min(int64_t(item.start) + int64_t(item.blocks) * kKeys, int64_t(item.length));
-        float most = 0.f;
+        float key_most = 0.f, value_most = 0.f;
 #pragma unroll 4
         for (int64_t i = threadIdx.x; i < (end - item.start + kTile - 1) / kTile * kEach; i += Shape::kThreads) {
             const int key = item.start + int(i / kEach) * kTile, first = int(i % kEach) * 4;
             const int64_t at = prompt_tile<D>(a, item, key);
             if (at < 0) continue;
-            const uint4 x = *reinterpret_cast<const uint4 *>(a.data + at + Tile::kValuePairs + first * 4);
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            const uint4 x = *reinterpret_cast<const uint4 *>(a.data + at + Tile::kKeyPairs + first * 4);
+            const uint4 y = *reinterpret_cast<const uint4 *>(a.data + at + Tile::kValuePairs + first * 4);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w}, v[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int row = (first + e) / kGroups, token = (row & 8) | ((row & 1) << 2) | ((row >> 1) & 3);
-                if (key + token < item.length) most = fmaxf(most, fabsf(high_bf16(w[e])) + 15.f * low_bf16(w[e]));
+                if (key + token < item.length) {
+                    key_most = fmaxf(key_most, fabsf(high_bf16(w[e])) + 15.f * low_bf16(w[e]));
+                    value_most = fmaxf(value_most, fabsf(high_bf16(v[e])) + 15.f * low_bf16(v[e]));
+                }
             }
         }
-#pragma unroll
-        for (int i = 1; i < 32; i *= 2) most = fmaxf(most, __shfl_xor_sync(~0u, most, i));
-        if (lane == 0) atomicMax(&most_value, __float_as_uint(fminf(most, 3e38f)));
+        const unsigned k = __reduce_max_sync(~0u, __float_as_uint(fminf(key_most, 3e38f)));
+        const unsigned v = __reduce_max_sync(~0u, __float_as_uint(fminf(value_most, 3e38f)));
+        if (lane == 0) {
+            atomicMax(&most_key, k);
+            atomicMax(&most_value, v);
+        }
         __syncthreads();
     }
-    const int value_shift = most_value == 0 ? 0 : max(-100, min(100, 14 - (int(most_value >> 23) - 127)));
+    const int value_shift = most_value == 0 ? 0 : max(-100, min(100, kValuePower - (int(most_value >> 23) - 127)));
     const float value_factor = __uint_as_float(uint32_t(127 + value_shift) << 23);
+    const int key_shift = most_key == 0 ? 0 : min(126, kKeyPower - (int(most_key >> 23) - 127));  // -115 at least
+    const float key_factor = __uint_as_float(uint32_t(127 + key_shift) << 23);
     // Of a whole warp: all lanes go on, or none does.
     auto wait = [&](uint64_t *bar, uint32_t parity) {
         return bool(__all_sync(~0u, tc::bar_wait(bar, parity, &abort_flag, tc::kWaitClocks)));
@@ -302,7 +311,8 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
             if (lane == 0) tc::bar_arrive(&bars.query);
-            const float to_log2 = a.scale * kLog2e * kKeyDivisor / factor;
+            // At least what scores of up to 2^33 vanish under: zero would make a hidden one's -infinity a NaN.
+            const float to_log2 = fmaxf(ldexpf(a.scale * kLog2e, -shift - key_shift), 0x1p-100f);
             const int64_t last = mine ? min(item.before + token, int64_t(item.length) - 1) : -1;
             // Columns low < c <= high of the keys from item.start on are seen; the warp sees blocks whole_from to
             // whole_to - 1 whole.
@@ -517,7 +527,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
                 __half2 s[kKeyGroups], less[kKeyGroups];
 #pragma unroll
                 for (int b = 0; b < kKeyGroups; ++b) {
-                    const float scale = low_bf16(key_pairs[i][b]) / kKeyDivisor;
+                    const float scale = low_bf16(key_pairs[i][b]) * key_factor;
                     s[b] = __float2half2_rn(scale);
                     less[b] = __float2half2_rn(-24.f * scale);
                 }
@@ -531,7 +541,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
                     uint32_t r[4] = {};
 #pragma unroll
                     for (int b = 0; b < kKeyGroups; ++b) {
-                        const float m = high_bf16(key_pairs[i][b]) / kKeyDivisor, s8 = low_bf16(key_pairs[i][b]) * (8 / kKeyDivisor);
+                        const float m = high_bf16(key_pairs[i][b]) * key_factor, s8 = low_bf16(key_pairs[i][b]) * key_factor * 8.f;
                         r[2 * b] = pack2<__half>(m, m);
                         r[2 * b + 1] = pack2<__half>(s8, s8);
                     }

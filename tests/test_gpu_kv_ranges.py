@@ -71,3 +71,32 @@ def test_small_weights_of_prompts(boost, dim, dtype):
     pool, q, table, lengths, cu = _sharp(16384, 200, dim, (64.0, 20.0), boost, True, dtype)
     got = pool.attend(q, table, lengths, cu_seqlens=cu)
     _check(got, q, pool.data, table, [16384], [200], 64)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("count", [None, 130])
+@pytest.mark.parametrize("power", [-60, -30, -17, 17, 60, 100])
+def test_keys_of_any_size(power, count, dim, dtype):
+    """Keys from tiny to huge, of both signs, against a scale that brings the scores back."""
+    page = 32
+    table, lengths, cu, pages = _sequences([400], page, None if count is None else [count])
+    pool = _pool(pages, 2, page, dim)
+    k, v = _rand(400, 2, dim, seed=3) * 2.0 ** power, _rand(400, 2, dim, seed=4)
+    _fill(pool, k.bfloat16(), v.bfloat16(), table, lengths)
+    q, scale = (2 * _rand(count or 1, 8, dim, seed=5)).to(dtype), dim ** -0.5 * 2.0 ** -power
+    got = pool.attend(q, table, lengths, cu_seqlens=cu, scale=scale)
+    _check(got, q, pool.data, table, [400], [count or 1], page, scale=scale)
+
+
+@pytest.mark.parametrize("count", [None, 130])
+def test_scores_that_vanish(count):
+    """Queries, keys and a scale whose product is nothing in fp32: every key has the same weight."""
+    page, dim = 16, 128
+    table, lengths, cu, pages = _sequences([400], page, None if count is None else [count])
+    pool = _pool(pages, 1, page, dim)
+    k, v = _rand(400, 1, dim, seed=3) * 1e-30, _rand(400, 1, dim, seed=4)
+    _fill(pool, k.bfloat16(), v.bfloat16(), table, lengths)
+    q = (_rand(count or 1, 4, dim, seed=5) * 1e-37).bfloat16()
+    got = pool.attend(q, table, lengths, cu_seqlens=cu, scale=1e-20)
+    _check(got, q, pool.data, table, [400], [count or 1], page, scale=1e-20)
