@@ -599,7 +599,8 @@ int32_t sq_kv_read(const sq_kv_args *args, sq_stream_t stream);
  *           strides multiples of 8; out contiguous, 16-byte aligned
  *   workspace  sq_kv_attention_workspace_bytes(...) bytes, 16-byte aligned
  * Sequences of many new tokens take keys and values in f16, over powers of two by the largest that any
- * of 128 or 256 rows reaches: what is below 2^-24 of that loses bits.
+ * of 128 or 256 rows reaches: what is below 2^-24 of that loses bits.  Sums are fp32: values of up to
+ * 2^80 in magnitude do not overflow them at any length.
  * status: also SQ_STATUS_TIMEOUT if a bounded device wait gave up; outputs concerned are NaN.
  */
 typedef struct sq_kv_attention_args {

@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
         }
         __syncthreads();
     }
-    const int value_shift = most_value == 0 ? 0 : max(-100, min(100, kValuePower - (int(most_value >> 23) - 127)));
+    const int value_shift = most_value == 0 ? 0 : min(126, kValuePower - (int(most_value >> 23) - 127));  // -114 at least
     const float value_factor = __uint_as_float(uint32_t(127 + value_shift) << 23);
     const int key_shift = most_key == 0 ? 0 : min(126, kKeyPower - (int(most_key >> 23) - 127));  // -115 at least
     const float key_factor = __uint_as_float(uint32_t(127 + key_shift) << 23);
@@ -416,7 +416,9 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
                         }
                     }
                 }
-                const float weight = sum.x + sum.y, per = weight == 0.f ? 0.f : 1.f / (weight * value_factor);
+                // The values' factor apart: its product with the weights' sum may leave fp32.
+                const float weight = sum.x + sum.y, per = weight == 0.f ? 0.f : 1.f / weight;
+                const float back = __uint_as_float(uint32_t(127 - value_shift) << 23);
                 T *out = static_cast<T *>(a.out) + (int64_t(item.first + token) * a.q_heads + item.head * group + (mine ? index % group : 0)) * D;
 #pragma unroll
                 for (int c = 0; c < D; c += 32) {
@@ -435,7 +437,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
                             uint32_t r[4];
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
-                                r[e] = pack2<T>(__uint_as_float(s[i + 2 * e]) * by, __uint_as_float(s[i + 2 * e + 1]) * by);
+                                r[e] = pack2<T>(__uint_as_float(s[i + 2 * e]) * by * back, __uint_as_float(s[i + 2 * e + 1]) * by * back);
                             *reinterpret_cast<uint4 *>(out + c + i) = make_uint4(r[0], r[1], r[2], r[3]);
                         }
                     }

@@ -100,3 +100,15 @@ def test_scores_that_vanish(count):
     q = (_rand(count or 1, 4, dim, seed=5) * 1e-37).bfloat16()
     got = pool.attend(q, table, lengths, cu_seqlens=cu, scale=1e-20)
     _check(got, q, pool.data, table, [400], [count or 1], page, scale=1e-20)
+
+
+@pytest.mark.parametrize("power", [-118, 104, 116, 120])
+def test_values_of_prompts_of_any_size(power):
+    page, dim, count = 16, 128, 130
+    table, lengths, cu, pages = _sequences([400], page, [count])
+    pool = _pool(pages, 1, page, dim)
+    k, v = _rand(400, 1, dim, seed=3), _rand(400, 1, dim, seed=4) * 2.0 ** power
+    _fill(pool, k.bfloat16(), v.bfloat16(), table, lengths)
+    q = _rand(count, 4, dim, seed=6).bfloat16()
+    got = pool.attend(q, table, lengths, cu_seqlens=cu)
+    _check(got / 2.0 ** power, q, _scaled(pool.data, 2.0 ** power), table, [400], [count], page)
