@@ -165,8 +165,10 @@ def kv_attention(q, data, page_table, lengths, *, cu_seqlens=None, scale=None, w
         raise ValueError("window must be at least 1")
     index = N.device_index(data, q, N.status_word(status))
     (rows, heads, last), table = q.stride(), call.table
+    # The stride of an axis of one is nobody's (contiguous() leaves it too).
+    rows, heads = rows if tokens > 1 else 0, heads if q_heads > 1 else 0
     if last != 1 or rows % 8 or heads % 8 or q.data_ptr() % 16:
-        q = q.contiguous() if last != 1 or rows % 8 or heads % 8 else q.clone()
+        q = q.clone(memory_format=torch.contiguous_format)
         rows, heads, _ = q.stride()
     out = data.new_empty((tokens, q_heads, dim), dtype=q.dtype)
     if not call.seqs:

@@ -112,3 +112,22 @@ def test_values_of_prompts_of_any_size(power):
     q = _rand(count, 4, dim, seed=6).bfloat16()
     got = pool.attend(q, table, lengths, cu_seqlens=cu)
     _check(got / 2.0 ** power, q, _scaled(pool.data, 2.0 ** power), table, [400], [count], page)
+
+
+@pytest.mark.parametrize("q_heads,heads", [(8, 2), (1, 1)])
+@pytest.mark.parametrize("pad,stride", [(0, 4), (8, 3), (3, 8), (1, 0)])
+@pytest.mark.parametrize("cu", [False, True])
+def test_one_token_of_any_stride(cu, pad, stride, q_heads, heads):
+    """The strides of an axis of one are nobody's; a base off 16 bytes is copied."""
+    page, dim = 32, 128
+    table, lengths, ends, pages = _sequences([77], page, [1] if cu else None)
+    pool = _pool(pages, heads, page, dim)
+    q = _rand(1, q_heads, dim).bfloat16()
+    want = pool.attend(q, table, lengths, cu_seqlens=ends)
+    flat = torch.zeros(pad + q_heads * dim + stride, device="cuda", dtype=torch.bfloat16)
+    flat[pad:pad + q_heads * dim] = q.flatten()
+    wide = flat[None, pad:pad + q_heads * dim].as_strided((1, q_heads, dim), (q_heads * dim + stride, dim, 1))
+    assert torch.equal(pool.attend(wide, table, lengths, cu_seqlens=ends), want)
+    if q_heads == 1:
+        wide = flat.as_strided((1, 1, dim), (dim, dim + stride, 1), pad)
+        assert torch.equal(pool.attend(wide, table, lengths, cu_seqlens=ends), want)
