@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
         // Query rows as the product's second operand: row g's channels 16 t + 0..15 of each group.
         uint32_t q[NT][kGroups][8];
         float q_sum[NT][kGroups][2];  // of rows 2 t and 2 t + 1: the groups' sums
-        int limit[NT][2];
+        int place[NT][2];     // their positions, which may lie past the table
         const int row0 = s.block * kRows, rows = s.tokens * group;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int r = row0 + j * 8 + 2 * t + e;
-                limit[j][e] = r < rows ? int(max(int64_t(-1), min(s.before + r / group, int64_t(s.length) - 1))) : -1;
+                place[j][e] = r < rows ? int(max(int64_t(-1), s.before + r / group)) : -1;
             }
         }
         // Units that every row sees whole: up to `sees_all`, from `window_all` on.
@@ -498,8 +498,8 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
                         for (int i4 = 0; i4 < 4; ++i4) {
-                            const int p = token + h * kTile + (i4 & 2) * 4, last = limit[j][i4 & 1];
-                            if (p > last || (a.window > 0 && p <= last - a.window) || (none >> h & 1)) {
+                            const int p = token + h * kTile + (i4 & 2) * 4, own = place[j][i4 & 1];
+                            if (p > own || p >= s.length || (a.window > 0 && p <= own - a.window) || (none >> h & 1)) {
                                 hidden |= 1u << (4 * (h * NT + j) + i4);
                                 z[h][j][i4] = -INFINITY;
                             }

@@ -317,7 +317,8 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
             // Columns low < c <= high of the keys from item.start on are seen; the warp sees blocks whole_from to
             // whole_to - 1 whole.
             const int high = int(max(int64_t(-1), last - item.start));
-            const int low = a.window > 0 ? int(max(int64_t(-1), last - a.window - item.start)) : -1;
+            // (The window is of the token's own position, which may lie past the table.)
+            const int low = a.window > 0 ? int(max(int64_t(-1), min(item.before + token - a.window - item.start, int64_t(item.length)))) : -1;
             const int whole_from = __reduce_max_sync(~0u, (low + kKeys) / kKeys), whole_to = __reduce_min_sync(~0u, (high + 1) / kKeys);
             const uint32_t lanes = uint32_t(warp & 3) << 21;
             const uint32_t sums = tmem + lanes + Shape::kColumnsO + tile * D;
@@ -406,7 +407,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
                 uint32_t poison = 0;  // groups whose visible values are not all finite
                 if (mine && bad_values) {
                     for (int64_t key = item.start; key <= last; ++key) {
-                        if (a.window > 0 && key <= last - a.window) continue;
+                        if (a.window > 0 && key <= item.before + token - a.window) continue;
                         const int64_t at = prompt_tile<D>(a, item, int(key) & ~(kTile - 1));
                         if (at < 0) continue;
 #pragma unroll

@@ -131,3 +131,26 @@ def test_one_token_of_any_stride(cu, pad, stride, q_heads, heads):
     if q_heads == 1:
         wide = flat.as_strided((1, 1, dim), (dim, dim + stride, 1), pad)
         assert torch.equal(pool.attend(wide, table, lengths, cu_seqlens=ends), want)
+
+
+@pytest.mark.parametrize("dim,q_heads,heads", [(64, 4, 2), (128, 8, 1), (256, 4, 2)])
+@pytest.mark.parametrize("window", [30, 100, 1000])
+@pytest.mark.parametrize("count", [None, 5, 60])
+def test_windows_past_the_table(count, window, dim, q_heads, heads):
+    """Tokens past the page table see what their own window reaches of it."""
+    page, held, length = 16, 400, 421
+    table, _, _, pages = _sequences([held], page)
+    table = table[:, :held // page].contiguous()
+    pool = _pool(pages, heads, page, dim)
+    tokens = count or 1
+    q = (2 * _rand(tokens, q_heads, dim, seed=5)).bfloat16()
+    cu = None if count is None else torch.tensor([0, count], device="cuda", dtype=torch.int32)
+    got = pool.attend(q, table, torch.tensor([length], device="cuda", dtype=torch.int32), cu_seqlens=cu, window=window).double()
+    with pytest.raises(IndexError):
+        pool.check_status()
+    k, v, sizes = cached(pool.data, table[0].tolist(), page, held)
+    want, size = attend(q, k, v, sizes, length - tokens, dim ** -0.5, window)
+    u = torch.finfo(q.dtype).eps / 2
+    error = dim ** -0.5 * (q.double().abs() * k.abs().amax((0, 1))).sum(-1, keepdim=True) * 2.0 ** -11
+    assert bool(((got - want).abs() <= u * want.abs() + (4 * u + 2 * error) * size).all())
+    assert float((got - want).norm()) <= 2 * u * float(want.norm())
