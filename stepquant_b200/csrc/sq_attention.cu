@@ -111,6 +111,7 @@ struct Sequence {
     int first, count;   // new tokens
     int length;         // tokens that the page table reaches
     int64_t before;     // position of the first new token
+    int seen_from;      // first position that any of them sees, `length` if none does
     int unit, units;    // units that any of them sees: one at least
     int blocks;         // of rows (token, query head of the kv head)
     int64_t cost;
@@ -128,7 +129,8 @@ __device__ __forceinline__ Sequence sequence(const sq_kv_attention_args &a, int 
     s.length = int(max(int64_t(0), min(int64_t(length), most)));
     s.before = int64_t(length) - s.count;
     const int64_t start = a.window > 0 ? max(int64_t(0), s.before - a.window + 1) : 0;
-    s.unit = int(min(start, int64_t(s.length)) / kUnit);
+    s.seen_from = int(min(start, int64_t(s.length)));
+    s.unit = s.seen_from / kUnit;
     s.units = max(1, int((int64_t(s.length) + kUnit - 1) / kUnit) - s.unit);
     const int64_t rows = int64_t(s.count) * (a.q_heads / a.heads);
     s.blocks = rows > most_rows ? 0 : int((rows + ROWS - 1) / ROWS);
@@ -222,6 +224,7 @@ struct Segment {
     int sequence, head, block;
     int first, tokens, length;  // the sequence's new tokens, tokens that it holds
     int64_t before;             // position of its first new token
+    int seen_from;              // first position that any of them sees
     int unit, count;            // first unit, units; none: the span is over
     bool whole;                 // the item's units
 };
@@ -256,7 +259,7 @@ __device__ __forceinline__ void next_segment(const sq_kv_attention_args &a, int 
         g.unit = c.s.unit + first;
     }
     g.sequence = c.n, g.head = c.head, g.block = c.block;
-    g.first = c.s.first, g.tokens = c.s.count, g.length = c.s.length, g.before = c.s.before;
+    g.first = c.s.first, g.tokens = c.s.count, g.length = c.s.length, g.before = c.s.before, g.seen_from = c.s.seen_from;
     g.whole = g.count == c.s.units;
 }
 
@@ -342,7 +345,9 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
         if ((i & 15) == 0) {
             places = -1;
             const int unit = warp + (i + lane / 2) * kWarps, tile = (s.unit + unit) * 2 + (lane & 1), index = tile / page_tiles;
-            if (unit < s.count && index < a.table_width) {
+            // A unit's tile past the sequence's end or in front of every row's window is not looked up: the table may hold
+            // anything there.
+            if (unit < s.count && index < a.table_width && tile * kTile < s.length && (tile + 1) * kTile > s.seen_from) {
                 const int page = a.page_table[s.sequence * a.table_stride + index];
                 if (page >= a.num_pages) flag(a.status, SQ_STATUS_SLOT_RANGE);
                 else if (page > 0) places = (int64_t(page) * a.heads + s.head) * head_bytes + int64_t(tile - index * page_tiles) * Tile::kBytes;
@@ -364,10 +369,11 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
     uint32_t phase = 0;
     bool gave_up = false;
     for (int number = 0; segments[number & 3].count; ++number) {
-        const Segment s = segments[number & 3];
+        const Segment &here = segments[number & 3];  // for what is seldom read
+        const Segment s = here;
         const Segment &next = segments[(number + 1) & 3];
         const int mine = units_of(s);
-        for (int i = ahead; i < min(mine, kStages); ++i) request(s, i);
+        for (int i = ahead; i < min(mine, kStages); ++i) request(here, i);
         ahead = min(mine, max(ahead, kStages));
         if (warp == (number & (kWarps - 1))) {
             if (lane == 0) {
@@ -641,7 +647,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
             __syncwarp();
             stage = stage + 1 == kStages ? 0 : stage + 1;
             phase ^= stage == 0;
-            if (ahead < mine) request(s, ahead++);
+            if (ahead < mine) request(here, ahead++);
             else if (next_ahead < next_mine) request(next, next_ahead++);
         }
         ahead = next_ahead;

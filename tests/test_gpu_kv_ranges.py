@@ -154,3 +154,20 @@ def test_windows_past_the_table(count, window, dim, q_heads, heads):
     error = dim ** -0.5 * (q.double().abs() * k.abs().amax((0, 1))).sum(-1, keepdim=True) * 2.0 ** -11
     assert bool(((got - want).abs() <= u * want.abs() + (4 * u + 2 * error) * size).all())
     assert float((got - want).norm()) <= 2 * u * float(want.norm())
+
+
+@pytest.mark.parametrize("page,lengths,window", [(16, [16, 33, 1, 80], None), (48, [48, 40, 144, 100], None), (16, [100, 65, 16, 500], 20)])
+@pytest.mark.parametrize("count", [None, 2])
+def test_entries_that_hold_no_token_of_the_sequence(page, lengths, window, count):
+    """What a table holds past a sequence's last page, or in front of its window, may be anything."""
+    counts = None if count is None else [min(count, n) for n in lengths]
+    table, device_lengths, cu, pages = _sequences(lengths, page, counts)
+    pool = _pool(pages, 2, page, 128)
+    q = _rand(sum(counts or [1] * len(lengths)), 8, 128, seed=5).bfloat16()
+    want = pool.attend(q, table, device_lengths, cu_seqlens=cu, window=window)
+    for n, length in enumerate(lengths):
+        table[n, -(-length // page):] = 2 ** 31 - 1
+        if window is not None:
+            table[n, :max(0, length - (1 if counts is None else counts[n]) - window + 1) // page] = pages + 5
+    assert torch.equal(pool.attend(q, table, device_lengths, cu_seqlens=cu, window=window), want)
+    pool.check_status()
