@@ -123,7 +123,7 @@ typedef struct sq_step_args {
     void *out;
 } sq_step_args;
 
-/* Library version (major * 10000 + minor * 100 + patch); from 101 on sq_matmul_args has wait_clocks. */
+/* Library version (major * 10000 + minor * 100 + patch); from 101 on sq_matmul_args has wait_clocks, from 103 on sq_kv_attention_args. */
 int32_t sq_version(void);
 
 /* Human-readable text for an sq_error code. */
@@ -602,6 +602,7 @@ int32_t sq_kv_read(const sq_kv_args *args, sq_stream_t stream);
  * of 128 or 256 rows reaches: what is below 2^-24 of that loses bits.  Sums are fp32: values of up to
  * 2^80 in magnitude do not overflow them at any length.
  * status: also SQ_STATUS_TIMEOUT if a bounded device wait gave up; outputs concerned are NaN.
+ * wait_clocks: how many clocks a wait may take, 0 for 2^32 (about two seconds), negative for one look.
  */
 typedef struct sq_kv_attention_args {
     const void *q;
@@ -627,6 +628,7 @@ typedef struct sq_kv_attention_args {
     int32_t dtype;
     int32_t window;
     float scale;
+    int64_t wait_clocks;
 } sq_kv_attention_args;
 
 int64_t sq_kv_attention_workspace_bytes(int32_t tokens, int32_t num_seqs, int32_t q_heads, int32_t heads, int32_t dim);

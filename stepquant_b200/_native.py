@@ -95,7 +95,7 @@ class SqKvAttentionArgs(ctypes.Structure):
                 ("status", _p), ("workspace", _p), ("workspace_bytes", _i64), ("q_stride", _i64), ("q_head_stride", _i64),
                 ("table_stride", _i64), ("num_pages", _i64), ("tokens", _i32), ("num_seqs", _i32), ("table_width", _i32),
                 ("q_heads", _i32), ("heads", _i32), ("dim", _i32), ("page_size", _i32), ("dtype", _i32), ("window", _i32),
-                ("scale", ctypes.c_float)]
+                ("scale", ctypes.c_float), ("wait_clocks", _i64)]
 
 
 _SIGNATURES = {

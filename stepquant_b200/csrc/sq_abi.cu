@@ -124,7 +124,7 @@ int32_t run(int mode, sq::TileParams t, int32_t batch, cudaStream_t stream) {
 
 extern "C" {
 
-int32_t sq_version(void) { return 102; }
+int32_t sq_version(void) { return 103; }
 
 const char *sq_error_string(int32_t code) {
     switch (code) {

@@ -338,9 +338,10 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
     // This warp's units of a segment are number warp, warp + 8, ...; its ring holds those of this segment and then
     // of the next.
     auto units_of = [&](const Segment &s) { return (s.count - warp + kWarps - 1) / kWarps; };
-    int requests = 0, request_stage = 0;
+    int request_stage = 0;
     int64_t places = -1;  // lane 2 i + h: byte offset of tile h of unit i, modulo 16, of the segment that is requested; -1: none
-    uint32_t missing = 0; // by stage, two bits: whether there was no tile to load
+    uint32_t missing = 0; // by stage, two bits: whether there was no tile to load; from kArmed on, one: not waited for yet
+    constexpr int kArmed = 16;
     auto request = [&](const Segment &s, int i) {
         if ((i & 15) == 0) {
             places = -1;
@@ -356,24 +357,23 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
         // Lanes 0 and 1 fetch a tile each.
         const int64_t place = __shfl_sync(~0u, places, 2 * (i & 15) + (lane & 1));
         const uint32_t none = __ballot_sync(~0u, place < 0) & 3;
-        missing = (missing & ~(3u << 2 * request_stage)) | none << 2 * request_stage;
+        missing = (missing & ~(3u << 2 * request_stage)) | none << 2 * request_stage | 1u << (kArmed + request_stage);
         uint64_t *const bar = &bars[warp][request_stage];
         if (lane == 0) tc::bar_expect(bar, (none == 0 ? 2 : none == 3 ? 0 : 1) * Tile::kBytes);
         if (lane < 2 && place >= 0)
             tc::bulk_load(ring + request_stage * Shape::kStage + lane * Tile::kBytes, a.data + place, Tile::kBytes, bar);
-        ++requests;
         request_stage = request_stage + 1 == kStages ? 0 : request_stage + 1;
     };
     int ahead = 0;  // units of the next segment that were requested
     int stage = 0;
     uint32_t phase = 0;
-    bool gave_up = false;
+    bool gave_up = false;  // of the whole warp: it waits for no more units and requests none
     for (int number = 0; segments[number & 3].count; ++number) {
         const Segment &here = segments[number & 3];  // for what is seldom read
         const Segment s = here;
         const Segment &next = segments[(number + 1) & 3];
         const int mine = units_of(s);
-        for (int i = ahead; i < min(mine, kStages); ++i) request(here, i);
+        for (int i = ahead; i < min(mine, kStages) && !gave_up; ++i) request(here, i);
         ahead = min(mine, max(ahead, kStages));
         if (warp == (number & (kWarps - 1))) {
             if (lane == 0) {
@@ -444,8 +444,12 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
         int next_ahead = 0;
         const int next_mine = units_of(next);
 #pragma unroll 1
-        for (int i = 0; i < mine; ++i) {
-            if (!tc::bar_wait(&bars[warp][stage], phase, &abort_flag, tc::kWaitClocks)) gave_up = true;
+        for (int i = 0; i < mine && !gave_up; ++i) {
+            if (!__all_sync(~0u, tc::bar_wait_or_look(&bars[warp][stage], phase, &abort_flag, a.wait_clocks))) {
+                gave_up = true;
+                break;
+            }
+            missing &= ~(1u << (kArmed + stage));
             const uint8_t *const unit = ring + stage * Shape::kStage;
             // Scores of tokens (rows g, g + 8 of each tile) x query rows (2 t, 2 t + 1).
             float z[2][NT][4];
@@ -651,7 +655,6 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
             else if (next_ahead < next_mine) request(next, next_ahead++);
         }
         ahead = next_ahead;
-        gave_up = __any_sync(~0u, gave_up);
 
         // The warps' sums, to shared memory, then to the output or a part.
 #pragma unroll
@@ -715,8 +718,8 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
     if (gave_up) {  // the copies still on their way end before the CTA does
         if (lane == 0) flag(a.status, SQ_STATUS_TIMEOUT);
         int alone = 0;
-        for (int r = max(0, requests - kStages); r < requests; ++r)
-            tc::bar_wait(&bars[warp][r % kStages], (r / kStages) & 1, &alone, tc::kWaitClocks);
+        for (int i = 0; i < kStages; ++i)
+            if (missing >> (kArmed + i) & 1) tc::bar_wait(&bars[warp][i], i < stage ? phase ^ 1 : phase, &alone, tc::kWaitClocks);
     }
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     // Beside prompts it started when their last CTAs had: what comes after it in the stream waits for them too.
@@ -867,7 +870,7 @@ extern "C" int64_t sq_kv_attention_workspace_bytes(int32_t tokens, int32_t num_s
 extern "C" int32_t sq_kv_attention(const sq_kv_attention_args *args, sq_stream_t stream) {
     using namespace sq;
     if (!args) return SQ_ERR_ARGUMENT;
-    const sq_kv_attention_args &a = *args;
+    sq_kv_attention_args a = *args;
     if (a.tokens < 0 || a.num_seqs < 0 || a.table_width < 0 || a.num_pages < 0 || a.heads < 1 || a.q_heads < 1 || a.window < 0)
         return SQ_ERR_ARGUMENT;
     if (a.dtype < SQ_F32 || a.dtype > SQ_F16 || !(a.scale > 0.f) || !(a.scale < INFINITY)) return SQ_ERR_ARGUMENT;
@@ -884,6 +887,7 @@ extern "C" int32_t sq_kv_attention(const sq_kv_attention_args *args, sq_stream_t
     if (!a.q || !a.out || !a.lengths || (a.table_width && !a.page_table) || (a.num_pages && !a.data)) return SQ_ERR_ARGUMENT;
     if (!a.workspace || a.workspace_bytes < sq_kv_attention_workspace_bytes(a.tokens, a.num_seqs, a.q_heads, a.heads, a.dim))
         return SQ_ERR_CAPACITY;
+    if (a.wait_clocks == 0) a.wait_clocks = tc::kWaitClocks;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     return launch_attention(a, s) == cudaSuccess ? SQ_OK : SQ_ERR_CUDA;
 }

@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
     const float key_factor = __uint_as_float(uint32_t(127 + key_shift) << 23);
     // Of a whole warp: all lanes go on, or none does.
     auto wait = [&](uint64_t *bar, uint32_t parity) {
-        return bool(__all_sync(~0u, tc::bar_wait(bar, parity, &abort_flag, tc::kWaitClocks)));
+        return bool(__all_sync(~0u, tc::bar_wait_or_look(bar, parity, &abort_flag, a.wait_clocks)));
     };
 
     float top = -INFINITY;  // of a row
@@ -654,18 +654,20 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
                 if (kBuffers == 1 && j + 1 < blocks) begin(j + 1, tile);
             }
         }
-        if (!ok) {  // the products that were issued end before the tensor memory is freed
-            int alone = 0;
-            if (tc::elected()) tc::mma_commit(&bars.end);
-            __syncwarp();
-            tc::bar_wait(&bars.end, 0, &alone, tc::kWaitClocks);
-        }
         }
     }
     __syncwarp();
     tc::fence_before();
     __syncthreads();
-    if (warp == Shape::kProductWarp) tc::tmem_free(tmem, 512);
+    if (warp == Shape::kProductWarp) {
+        if (*static_cast<volatile int *>(&abort_flag)) {  // a role gave up: the products that were issued end first
+            int alone = 0;
+            if (tc::elected()) tc::mma_commit(&bars.end);
+            __syncwarp();
+            tc::bar_wait(&bars.end, 0, &alone, tc::kWaitClocks);
+        }
+        tc::tmem_free(tmem, 512);
+    }
 }
 
 template <class T, int D>

@@ -47,6 +47,17 @@ __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatil
     }
 }
 
+// The same, but a negative limit allows one look, which suspends nothing: a copy just begun is not there yet, so
+// that the way out can be tested.
+__device__ __forceinline__ bool bar_wait_or_look(uint64_t *bar, uint32_t parity, volatile int *abort, int64_t limit) {
+    if (limit >= 0) return bar_wait(bar, parity, abort, limit);
+    uint32_t done;
+    asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    if (!done) *abort = 1;
+    return done;
+}
+
 // One lane of the (converged) warp.
 __device__ __forceinline__ bool elected() {
     uint32_t r;

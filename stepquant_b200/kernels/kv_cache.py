@@ -147,7 +147,8 @@ def kv_attention(q, data, page_table, lengths, *, cu_seqlens=None, scale=None, w
     heads any stride apart; data, page_table, lengths, cu_seqlens as in
     ``kv_append``, which comes first: a token sees its sequence up to itself and,
     with ``window``, the last ``window`` positions of that.  scale: D^-1/2.  A
-    token that sees nothing, and tokens of no sequence, get zeros.
+    token that sees nothing, and tokens of no sequence, get zeros.  Should a bounded
+    device wait give up, outputs left undone are NaN and ``status`` has SQ_STATUS_TIMEOUT.
     """
     if q.dim() != 3:
         raise ValueError("q: expected [tokens, heads, dim]")
@@ -178,7 +179,7 @@ def kv_attention(q, data, page_table, lengths, *, cu_seqlens=None, scale=None, w
     N.launch(N.lib().sq_kv_attention, _pack_attention(
         q.data_ptr(), data.data_ptr(), out.data_ptr(), table.data_ptr(), call.lengths.data_ptr(), p(call.cu), p(status), p(workspace),
         size, rows, heads, table.stride(0), call.pages, tokens, call.seqs, call.width, q_heads, call.heads, dim,
-        call.page_size, N.dtype_code(q.dtype), 0 if window is None else min(window, 2 ** 31 - 1), scale), index)
+        call.page_size, N.dtype_code(q.dtype), 0 if window is None else min(window, 2 ** 31 - 1), scale, 0), index)
     return out
 
 

@@ -171,3 +171,39 @@ def test_entries_that_hold_no_token_of_the_sequence(page, lengths, window, count
             table[n, :max(0, length - (1 if counts is None else counts[n]) - window + 1) // page] = pages + 5
     assert torch.equal(pool.attend(q, table, device_lengths, cu_seqlens=cu, window=window), want)
     pool.check_status()
+
+
+@pytest.mark.parametrize("dim,q_heads,heads", [(64, 8, 2), (128, 16, 4), (256, 8, 2)])
+@pytest.mark.parametrize("lengths,counts", [([4000] * 40 + [17, 0, 300], None), ([3000, 900, 40], [700, 1, 33]), ([6000], [300])],
+                         ids=["tokens", "both", "prompt"])
+def test_waits_that_run_out(lengths, counts, dim, q_heads, heads):
+    """Device waits limited to one look or a few clocks give up in the middle of copies and products: every output
+    is what it should be or NaN, NaN only where the status is flagged, and the calls after are whole."""
+    import ctypes
+    from stepquant_b200 import _native as N
+    page = 64
+    table, device_lengths, cu, pages = _sequences(lengths, page, counts)
+    pool = _pool(pages, heads, page, dim)
+    tokens = sum(counts or [1] * len(lengths))
+    q = _rand(tokens, q_heads, dim, seed=5).bfloat16()
+    want = pool.attend(q, table, device_lengths, cu_seqlens=cu)
+    flush = torch.empty(1 << 26, device="cuda")
+    size = N.lib().sq_kv_attention_workspace_bytes(tokens, len(lengths), q_heads, heads, dim)
+    workspace = torch.empty(size, dtype=torch.uint8, device="cuda")
+    seen = 0
+    for limit in (-1, -1, -1, -1, 1, 1000, 100000):
+        out, status = torch.full_like(want, 7.0), torch.zeros(1, device="cuda", dtype=torch.int32)
+        flush.zero_()  # the pages leave L2: copies take longer
+        args = N.SqKvAttentionArgs(q.data_ptr(), pool.data.data_ptr(), out.data_ptr(), table.data_ptr(), device_lengths.data_ptr(),
+                                   N.address(cu), status.data_ptr(), workspace.data_ptr(), size, q.stride(0), q.stride(1),
+                                   table.stride(0), pages, tokens, len(lengths), table.shape[1], q_heads, heads, dim, page, N.SQ_BF16,
+                                   0, dim ** -0.5, limit)
+        N.check(N.lib().sq_kv_attention(ctypes.byref(args), N.stream_handle()))
+        gone = out.isnan()
+        assert torch.equal(out[~gone], want[~gone])
+        flagged = int(status) == N.SQ_STATUS_TIMEOUT
+        assert flagged or (not bool(gone.any()) and int(status) == 0)
+        seen += bool(gone.any())
+        assert torch.equal(pool.attend(q, table, device_lengths, cu_seqlens=cu), want)
+        pool.check_status()
+    assert seen  # a copy or a product that was just begun is not there at one look
