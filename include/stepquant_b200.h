@@ -503,7 +503,7 @@ int32_t sq_selective_scan_step(const sq_scan_args *args, sq_stream_t stream);
  * inverse: rotated back.  The other channels are copied.
  *   x, out      [tokens, heads, dim] in dtype, strides in elements, last axis contiguous; out may be x
  *   positions   [tokens], int64 (position_dtype 1) or int32 (0)
- *   frequencies [turned / 2] fp64, radians a token, magnitudes below pi
+ *   frequencies [turned / 2] fp64, radians a token
  * Angles are taken modulo a turn in 64-bit fixed point, sine and cosine in fp32.
  * turned even, 0 <= turned <= dim <= 1024.
  */

@@ -179,10 +179,17 @@ __device__ __noinline__ void turn_exactly(const sq_kv_args &a, const T *k, int c
         const int f = a.interleaved ? at / 2 : at < half ? at : at - half;
         const bool second = a.interleaved ? at & 1 : at >= half;
         const double other = to_float(k[a.interleaved ? at ^ 1 : second ? at - half : at + half]);
+        // The nearest quarter of a turn goes first: what is left of an angle near it keeps its bits in 64.
+        const uint64_t phase = uint64_t(phase_of(position, a.frequencies[f])), quarters = (phase + (uint64_t(1) << 61)) >> 62;
         double sin, cos;
-        sincospi(double(phase_of(position, a.frequencies[f])) * 0x1p-63, &sin, &cos);
-        cos *= a.magnitude;
-        sin *= a.magnitude;
+        sincospi(double(int64_t(phase - (quarters << 62))) * 0x1p-63, &sin, &cos);
+        if (quarters & 1) {
+            const double other_one = cos;
+            cos = -sin;
+            sin = other_one;
+        }
+        cos *= quarters & 2 ? -a.magnitude : a.magnitude;
+        sin *= quarters & 2 ? -a.magnitude : a.magnitude;
         x[e] = second ? other * sin + x[e] * cos : x[e] * cos - other * sin;
     }
 }

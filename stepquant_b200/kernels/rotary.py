@@ -77,8 +77,8 @@ def rotary(x, positions, frequencies, *, interleaved=False, magnitude=1.0, inver
 
     x: float32, bfloat16 or float16, tokens and heads any stride apart; positions:
     [T] int32 or int64; frequencies: [R / 2] radians a token, float64 (others are
-    converted on every call), magnitudes below pi.  ``magnitude`` scales the
-    rotated channels; ``inverse`` turns them back (the rotation's gradient).
+    converted on every call).  ``magnitude`` scales the rotated channels;
+    ``inverse`` turns them back (the rotation's gradient).
     ``out``: a tensor like x, x itself among them, or None (a new one).
     """
     if x.dim() != 3 or not 1 <= x.shape[2] <= MOST_DIM:
