@@ -37,9 +37,11 @@ _WIDTHS = {18 * d: d for d in HEAD_DIMS}
 
 
 def _int32(x, index, device):
-    """int32 tensor with a contiguous last axis on ``device``."""
+    """int32 tensor with a contiguous last axis on ``device``; what int32 does not hold becomes its ends, and so stays outside."""
     if x.dtype is torch.int32 and x.get_device() == index and (x.stride(-1) == 1 or x.shape[-1] < 2):
         return x
+    if x.dtype is torch.int64:
+        x = x.clamp(-2 ** 31, 2 ** 31 - 1)
     return x.to(device=device, dtype=torch.int32).contiguous()
 
 
