@@ -172,9 +172,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
         const int64_t token = (int64_t(strip) - (int64_t(r.x) / tokens_per_item + n)) * tokens_per_item;
         if (token < 0 || token >= item.count || int64_t(item.count) * group <= few_rows) return;
         item.token = int(token);
-        // (min() of two ints here came out as tokens_per_item with 17 warps: nvcc 12.9.)
-        const int64_t left = item.count - token;
-        const int tokens = left < tokens_per_item ? int(left) : tokens_per_item;
+        const int tokens = int(min(item.count - token, int64_t(tokens_per_item)));
         item.rows = tokens * group;
         const int64_t length = a.lengths[n], most = int64_t(a.table_width) * a.page_size;
         if (length > most && threadIdx.x == 0) flag(a.status, SQ_STATUS_SLOT_RANGE);
