@@ -676,8 +676,20 @@ cudaError_t launch_prompt(const sq_kv_attention_args &a, int few_rows, cudaStrea
     const int64_t grid = int64_t(strips) * a.heads;
     if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
     static std::atomic<uint64_t> devices{0};
-    const cudaError_t e = allow_shared(prompt_kernel<T, D>, Shape::kShared, devices);
+    cudaError_t e = allow_shared(prompt_kernel<T, D>, Shape::kShared, devices);
     if (e != cudaSuccess) return e;
+    if (Shape::kShare) {
+        // A warp that asks for more registers than the block was launched with and others gave back waits for ever:
+        // what the compiler allotted (in eights) is what the shares were added up against, or nothing is launched.
+        static std::atomic<int> registers{0};
+        if (registers.load(std::memory_order_relaxed) == 0) {
+            cudaFuncAttributes attributes;
+            e = cudaFuncGetAttributes(&attributes, prompt_kernel<T, D>);
+            if (e != cudaSuccess) return e;
+            registers.store((attributes.numRegs + 7) / 8 * 8, std::memory_order_relaxed);
+        }
+        if (registers.load(std::memory_order_relaxed) < Shape::kLaunchRegisters) return cudaErrorInvalidKernelImage;
+    }
     prompt_kernel<T, D><<<unsigned(grid), Shape::kThreads, Shape::kShared, s>>>(a, per, strips, few_rows);
     return cudaGetLastError();
 }
