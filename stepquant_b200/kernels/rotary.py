@@ -79,7 +79,7 @@ def rotary(x, positions, frequencies, *, interleaved=False, magnitude=1.0, inver
     [T] int32 or int64; frequencies: [R / 2] radians a token, float64 (others are
     converted on every call).  ``magnitude`` scales the rotated channels;
     ``inverse`` turns them back (the rotation's gradient).
-    ``out``: a tensor like x, x itself among them, or None (a new one).
+    ``out``: x itself, a tensor like x whose memory is apart from it, or None (a new one).
     """
     if x.dim() != 3 or not 1 <= x.shape[2] <= MOST_DIM:
         raise ValueError(f"x: expected [tokens, heads, dim] with 1 <= dim <= {MOST_DIM}, got {list(x.shape)}")
@@ -95,6 +95,8 @@ def rotary(x, positions, frequencies, *, interleaved=False, magnitude=1.0, inver
         out = x.new_empty(x.shape)
     elif out.shape != x.shape or out.dtype != x.dtype or (dim > 1 and out.stride(2) != 1):
         raise ValueError(f"out: expected {x.dtype} {list(x.shape)} with a contiguous last axis")
+    elif out.data_ptr() == x.data_ptr() and any(n > 1 and a != b for n, a, b in zip(x.shape, x.stride(), out.stride())):
+        raise ValueError(f"out: x's memory in another order, strides {list(out.stride())} for {list(x.stride())}")
     index = N.device_index(source, positions, frequencies, out)
     p, (xs, xh, _), (os, oh, _) = N.address, source.stride(), out.stride()
     N.launch(N.lib().sq_rotary, _pack(p(source), p(out), p(positions), p(frequencies), xs, xh, os, oh, tokens, heads, dim,
