@@ -214,8 +214,8 @@ def packer(arguments):
     def pack(*values):
         try:
             return fmt.pack(*values)
-        except (struct.error, OverflowError):  # the second: a number beyond fp32
-            raise ValueError(f"a size, a stride or a number is out of the C structure's range: {values}") from None
+        except struct.error:
+            raise ValueError(f"a size or a stride is out of the C structure's range: {values}") from None
 
     return pack
 
