@@ -367,7 +367,7 @@ int32_t kv_entry(const sq_kv_args *args, bool append, sq_stream_t stream) {
     if (!args) return SQ_ERR_ARGUMENT;
     const sq_kv_args &a = *args;
     if (a.tokens < 0 || a.num_seqs < 0 || a.table_width < 0 || a.num_pages < 0 || a.heads < 1 || a.turned < 0) return SQ_ERR_ARGUMENT;
-    if (a.dtype < SQ_F32 || a.dtype > SQ_F16) return SQ_ERR_ARGUMENT;
+    if (a.dtype < SQ_F32 || a.dtype > SQ_F16 || !(fabsf(a.magnitude) < INFINITY)) return SQ_ERR_ARGUMENT;
     if (a.dim != 64 && a.dim != 128 && a.dim != 256) return SQ_ERR_UNSUPPORTED;
     if (a.page_size < kTile || a.page_size % kTile || a.turned % 2 || a.turned > a.dim || a.table_stride < 0) return SQ_ERR_SHAPE;
     if (a.k_stride < 0 || a.k_head_stride < 0 || a.v_stride < 0 || a.v_head_stride < 0 || !aligned16(a.data)) return SQ_ERR_SHAPE;

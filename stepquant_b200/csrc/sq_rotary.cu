@@ -178,6 +178,7 @@ extern "C" int32_t sq_rotary(const sq_rotary_args *args, sq_stream_t stream) {
     if (!args) return SQ_ERR_ARGUMENT;
     const sq_rotary_args &a = *args;
     if (a.tokens < 0 || a.heads < 0 || a.dim < 1 || a.turned < 0 || a.dtype < SQ_F32 || a.dtype > SQ_F16) return SQ_ERR_ARGUMENT;
+    if (!(fabsf(a.magnitude) < INFINITY)) return SQ_ERR_ARGUMENT;
     if (a.turned % 2 || a.turned > a.dim || a.x_stride < 0 || a.x_head_stride < 0 || a.out_stride < 0 || a.out_head_stride < 0)
         return SQ_ERR_SHAPE;
     if (a.dim > 1024 || a.heads > (1 << 20) || a.tokens > kMostTokens) return SQ_ERR_UNSUPPORTED;

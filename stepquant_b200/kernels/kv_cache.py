@@ -19,12 +19,11 @@ goes for positions past the table and pages past the pool, which set a bit in
 ``status``.  Asynchronous on the current stream.
 """
 import functools
-import math
 
 import torch
 
 from .. import _native as N
-from .rotary import checked_frequencies, checked_positions
+from .rotary import MOST_FLOAT, check_magnitude, checked_frequencies, checked_positions
 
 HEAD_DIMS = (64, 128, 256)
 TILE = 16
@@ -115,8 +114,7 @@ def kv_append(data, k, v, page_table, lengths, *, cu_seqlens=None, frequencies=N
     frequencies = checked_frequencies(frequencies, call.dim)
     if positions is not None:
         positions = checked_positions(positions, k.shape[0])
-    if not math.isfinite(magnitude):
-        raise ValueError("magnitude must be finite")
+    check_magnitude(magnitude)
     _launch(N.lib().sq_kv_append, call, k, v, frequencies, positions, interleaved, magnitude, status)
 
 
@@ -162,7 +160,7 @@ def kv_attention(q, data, page_table, lengths, *, cu_seqlens=None, scale=None, w
         raise ValueError(f"q: expected [{tokens}, a multiple of {call.heads}, {call.dim}], got {list(q.shape)}")
     if scale is None:
         scale = dim ** -0.5
-    if not 0 < scale < math.inf:
+    if not 0 < scale <= MOST_FLOAT:
         raise ValueError("scale must be above zero and finite")
     if window is not None and window < 1:
         raise ValueError("window must be at least 1")

@@ -16,6 +16,7 @@ import torch
 from .. import _native as N
 
 MOST_DIM = 1024
+MOST_FLOAT = torch.finfo(torch.float32).max
 
 _pack = N.packer(N.SqRotaryArgs)
 
@@ -72,6 +73,11 @@ def checked_positions(positions, tokens):
     return positions if tokens < 2 or positions.stride(0) == 1 else positions.contiguous()
 
 
+def check_magnitude(magnitude):
+    if not abs(magnitude) <= MOST_FLOAT:
+        raise ValueError("magnitude must be finite in float32")
+
+
 def rotary(x, positions, frequencies, *, interleaved=False, magnitude=1.0, inverse=False, out=None):
     """x [T, H, D] with the first 2 len(frequencies) channels of each head rotated.
 
@@ -88,8 +94,7 @@ def rotary(x, positions, frequencies, *, interleaved=False, magnitude=1.0, inver
     frequencies, positions = checked_frequencies(frequencies, dim), checked_positions(positions, tokens)
     if frequencies is None:
         raise ValueError("frequencies is required")
-    if not math.isfinite(magnitude):
-        raise ValueError("magnitude must be finite")
+    check_magnitude(magnitude)
     source = x if dim == 1 or x.stride(2) == 1 else x.contiguous()
     if out is None:
         out = x.new_empty(x.shape)
