@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(PromptShape<D>::kThreads, 1) prompt_kernel(sq_
     } else {
         if constexpr (Shape::kShare) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(Shape::kProductRegisters));
         if (warp == Shape::kProductWarp) {
-        constexpr uint32_t kScores = tc::half_product(kKeys, false, false), kSums = tc::half_product(D, false, true);
+        constexpr uint32_t kScores = tc::half_product(kKeys, false), kSums = tc::half_product(D, true);
         // Descriptors of the first operands; others are further by bytes / 16.
         const uint64_t query = tc::operand(tc::smem_u32(queries)), key = tc::operand(tc::smem_u32(keys));
         const uint64_t value = tc::operand_mn(tc::smem_u32(values), kKeys * 128);

@@ -88,9 +88,9 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uin
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)) : "memory");
 }
-// 16-bit operands -> fp32, M = 128: both f16 or both bf16; B K-major, or MN-major (its rows are K).
-__device__ __forceinline__ constexpr uint32_t half_product(int n, bool bf16, bool b_mn) {
-    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(b_mn) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+// f16 operands -> fp32, M = 128; B K-major, or MN-major (its rows are K).
+__device__ __forceinline__ constexpr uint32_t half_product(int n, bool b_mn) {
+    return (1u << 4) | (uint32_t(b_mn) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
 }
 // Operand tile of 128-byte rows (64 values) under the 128-byte swizzle whose rows are K: `lead` bytes to
 // the next 64 values.
