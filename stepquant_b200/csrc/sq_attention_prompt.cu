@@ -19,7 +19,7 @@
 // first: f16 then keeps a key exactly down to 2^-24 of the largest.
 // Row maxima may lag by 2^8, so sums in tensor memory are seldom rescaled.
 //
-// 4096 tokens over 16384 of 32 / 8 heads of 128: 1120 us, 860 TFLOP/s, 0.52 of the burst
+// 4096 tokens over 16384 of 32 / 8 heads of 128: 1103 us, 870 TFLOP/s, 0.52 of the burst
 // rate of a library product.  A tile's chain bounds it (products, a commit, S read, maxima,
 // weights stored, an arrival), of which the other tile's products hide half; blocks of 64
 // keys with S and P in two buffers measured 1371 us, as a product of 128 x 64 takes the 64

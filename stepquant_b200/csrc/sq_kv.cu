@@ -6,10 +6,13 @@
 // one 32-bit word of the tile.  A code is that of the definition in exact arithmetic:
 // fp32 finds it, with a bound on what its roundings may have changed, and groups where
 // that reaches a border (a few in a thousand, more near position 0)
-// are done again in 64 bits.  Instructions bound append: 32768 tokens of 8 heads of 128 in
-// 166 us, 430 for a warp's 256 values (8192 tokens 57 us; all in 64 bits 88), of which
-// loads, stores and places take 140, the rotation 30 and the groups done again, which
-// hold their CTA up, a quarter of the time.  Read: 48 us, 3.6 TB/s.
+// are done again in 64 bits.  Append of 32768 tokens of 8 heads of 128: 171 us, 417
+// instructions for a warp's 256 values at 2.2 a clock and SM (8192 tokens in one profiled session 57
+// us; all in 64 bits 88), of which loads, stores and places take 140, the rotation 30 and the
+// groups done again, which hold their CTA up, a quarter of the time.  No unit is full
+// (adders 0.45): waits for loads, and stores of four bytes a lane, are what is left.  Read:
+// 48 us, 3.6 TB/s, 135 instructions for a warp's 256 values at 2.0 a clock; its warps wait
+// for words and pairs (four bytes a lane each) that follow a chain of boundaries, length and page.
 #include "sq_kv.cuh"
 #include "sq_rows.cuh"
 #include "sq_vec.cuh"

@@ -100,7 +100,8 @@ def kv_append(data, k, v, page_table, lengths, *, cu_seqlens=None, frequencies=N
     tokens and heads any stride apart; page_table: [S, pages] and lengths: [S],
     the new tokens counted, int32 (others are converted on every call);
     cu_seqlens: [S + 1] boundaries of the sequences' new tokens, None for one
-    each (T = S).  With ``frequencies`` keys are rotated as by ``rotary.rotary``,
+    each (T = S).  No two new tokens share a place: pages that sequences have in
+    common hold earlier tokens.  With ``frequencies`` keys are rotated as by ``rotary.rotary``,
     by ``positions`` [T] or their position in the sequence, and quantized without
     a rounding between.
     """
