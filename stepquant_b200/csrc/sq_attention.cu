@@ -560,7 +560,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                             x = fmaxf(x, top[j][e]);
                             factor = exp2_approx((top[j][e] - x) * to_log2);
                             top[j][e] = x;
-                            against[j][e] = -x * to_log2;
+                            against[j][e] = x == kNone ? 0.f : -x * to_log2;  // (a row that has seen nothing yet)
                         }
                         rescale(j, e, factor);
                     }

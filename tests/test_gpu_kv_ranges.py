@@ -207,3 +207,20 @@ def test_waits_that_run_out(lengths, counts, dim, q_heads, heads):
         assert torch.equal(pool.attend(q, table, device_lengths, cu_seqlens=cu), want)
         pool.check_status()
     assert seen  # a copy or a product that was just begun is not there at one look
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("dim,q_heads", [(64, 2), (128, 4), (256, 7)])
+@pytest.mark.parametrize("lengths,counts", [([31, 40, 230], [9, 12, 8]), ([1, 36], [1, 4]), ([70, 33], [3, 2]), ([300], [130])])
+@pytest.mark.parametrize("scale", [0.5, 1.0, 30.0, 1e6, 1e20])
+def test_large_scales_of_scores(scale, lengths, counts, dim, q_heads, dtype):
+    """A scale above one over small keys, where some tokens see nothing of what others in their block see."""
+    page = 32
+    table, device_lengths, cu, pages = _sequences(lengths, page, counts)
+    pool = _pool(pages, 1, page, dim)
+    k, v = (_rand((pages - 1) * page, 1, dim, seed=s) for s in (3, 4))
+    ends = torch.tensor([0, k.shape[0]], device="cuda", dtype=torch.int32)
+    pool.append((k * dim ** -0.5 / scale).bfloat16(), v.bfloat16(), torch.arange(1, pages, device="cuda")[None], ends[1:], cu_seqlens=ends)
+    q = _rand(sum(counts), q_heads, dim, seed=5).to(dtype)
+    got = pool.attend(q, table, device_lengths, cu_seqlens=cu, scale=scale)
+    _check(got, q, pool.data, table, lengths, counts, page, scale=scale)
