@@ -6,7 +6,7 @@
 // one 32-bit word of the tile.  A code is that of the definition in exact arithmetic:
 // fp32 finds it, with a bound on what its roundings may have changed, and groups where
 // that reaches a border (a few in a thousand, more near position 0)
-// are done again in 64 bits.  Append of 32768 tokens of 8 heads of 128: 171 us, 417
+// are done again in 64 bits.  Append of 32768 tokens of 8 heads of 128: 169 us, 417
 // instructions for a warp's 256 values at 2.2 a clock and SM (8192 tokens in one profiled session 57
 // us; all in 64 bits 88), of which loads, stores and places take 140, the rotation 30 and the
 // groups done again, which hold their CTA up, a quarter of the time.  No unit is full

@@ -9,12 +9,16 @@ namespace sq {
 // The angle position * frequency as a fraction of a turn in units of 2^-64: a product of
 // integers, whose whole turns fall off its top.  The frequency's rounding is 2^-65 turns
 // (or, above 2^-11 turns a token, 2^-53 of itself): below 10^-7 turns at position 2^31.
-// Frequencies of half a turn and more lose their whole turns first, the quotient by a turn in two parts.
-__device__ __forceinline__ int64_t turn_per_token(double frequency) {
-    if (fabs(frequency) < 3.14159265) return __double2ll_rn(frequency * (18446744073709551616.0 / 6.283185307179586476925));
+// Frequencies of half a turn and more lose their whole turns first, the quotient by a turn in two parts (not inlined:
+// few models have any, and beside it append of 256 tokens took 10.5 us for 10.2).
+static __device__ __noinline__ int64_t turn_per_token_fast(double frequency) {
     constexpr double kPerTurn = 0.15915494309189535, kRest = -9.839338337591243e-18;  // 1 / (2 pi)
     const double turns = frequency * kPerTurn, rest = fma(frequency, kRest, fma(frequency, kPerTurn, -turns));
     return int64_t(uint64_t(__double2ll_rn((turns - floor(turns + 0.5)) * 0x1p64)) + uint64_t(__double2ll_rn(rest * 0x1p64)));
+}
+__device__ __forceinline__ int64_t turn_per_token(double frequency) {
+    if (fabs(frequency) >= 3.14159265) return turn_per_token_fast(frequency);
+    return __double2ll_rn(frequency * (18446744073709551616.0 / 6.283185307179586476925));
 }
 __device__ __forceinline__ int64_t phase_of(int64_t position, double frequency) {
     return int64_t(uint64_t(position) * uint64_t(turn_per_token(frequency)));
