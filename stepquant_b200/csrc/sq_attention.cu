@@ -51,6 +51,13 @@ struct Codes<__nv_bfloat16> {
     // p s (below; 369 us for 353) and more, as bf16 values go far beyond f16 either way.
     static constexpr float kHeld = 128.f;  // pair() is c + this: a bf16 with c in its last bits
     __device__ static __forceinline__ uint32_t pair(uint32_t w) { return and_or(w, 0x000F000Fu, 0x43004300u); }
+    // c - 8, for sums over many tokens: the tensor cores cut sums off, and those of 128 + c, 136 times the weights' sum
+    // taken off at the end, were 4 % of the outputs' norm off where a warp had 4096 tokens (256 requests 353 -> 338 us, too).
+    __device__ static __forceinline__ uint32_t centred(uint32_t w) {
+        const uint32_t x = pair(w), base = 0x43084308u;
+        const __nv_bfloat162 r = __hsub2(reinterpret_cast<const __nv_bfloat162 &>(x), reinterpret_cast<const __nv_bfloat162 &>(base));
+        return reinterpret_cast<const uint32_t &>(r);
+    }
     __device__ static __forceinline__ uint32_t pack(float lo, float hi) {
         uint32_t r;
         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -65,7 +72,6 @@ struct Codes<__nv_bfloat16> {
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
-    static constexpr uint32_t kOnes = 0x3F803F80u;
     static constexpr float kLag = 8.f;
     static constexpr bool kNarrow = false;  // p s has fp32's range
 };
@@ -77,6 +83,7 @@ struct Codes<__half> {
         const __half2 r = __hsub2(reinterpret_cast<const __half2 &>(x), reinterpret_cast<const __half2 &>(base));
         return reinterpret_cast<const uint32_t &>(r);
     }
+    __device__ static __forceinline__ uint32_t centred(uint32_t w) { return pair(w); }
     __device__ static __forceinline__ uint32_t pack(float lo, float hi) {
         uint32_t r;
         asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -89,7 +96,6 @@ struct Codes<__half> {
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
-    static constexpr uint32_t kOnes = 0x3C003C00u;
     // p s has f16's range only, so what weights are taken against depends on p s: a row's reference R, p = 2^(score - R),
     // rises where a p s is above kMostWeight, to bring that one to 2^8 .. 2^9 (what rounding loses of the others is then
     // 2^-33 of the row's largest), or a p above 2^kMostPower, to bring it to 2^kLag (the scales are tiny then, and
@@ -428,7 +434,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
         const int sees_all = int(max(int64_t(0), min(s.before + row0 / group + 1, int64_t(s.length))) / kUnit);
         const int window_all = a.window > 0 ? int(min(max(int64_t(0), s.before + last_row / group - a.window + 1) + kUnit - 1, int64_t(0x7fffffff)) / kUnit) : 0;
 
-        float acc[NT][kGroups][4][4], ones[NT][kGroups][4], least[NT][kGroups][2];
+        float acc[NT][kGroups][4][4], least[NT][kGroups][2];
         float top[NT][2], against[NT][2], sum[NT][2];  // maxima of scores before `to_log2`
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -436,7 +442,6 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
             for (int b = 0; b < kGroups; ++b) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    ones[j][b][i] = 0.f;
 #pragma unroll
                     for (int m = 0; m < 4; ++m) acc[j][b][m][i] = 0.f;
                 }
@@ -535,8 +540,6 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
 #pragma unroll
                 for (int b = 0; b < kGroups; ++b) {
                     least[j][b][e] *= factor;
-                    ones[j][b][e] *= factor;
-                    ones[j][b][2 + e] *= factor;
 #pragma unroll
                     for (int m = 0; m < 4; ++m) acc[j][b][m][e] *= factor, acc[j][b][m][2 + e] *= factor;
                 }
@@ -640,14 +643,13 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                         least[j][b][1] += v[1] + v[3];
                         w0[j] = transpose8(C::pack(u[0], u[1]));
                         w1[j] = transpose8(C::pack(u[2], u[3]));
-                        if (C::kHeld != -kMiddle) C::mma(ones[j][b], C::kOnes, C::kOnes, C::kOnes, C::kOnes, w0[j], w1[j]);
                     }
                     const uint32_t x0 = __byte_perm(word[0][b], word[1][b], 0x5410), y0 = __byte_perm(word[0][b], word[1][b], 0x7632);
                     const uint32_t x1 = __byte_perm(word[2][b], word[3][b], 0x5410), y1 = __byte_perm(word[2][b], word[3][b], 0x7632);
 #pragma unroll
                     for (int m = 0; m < 4; ++m) {
-                        const uint32_t a0 = C::pair(x0 >> (4 * m)), a1 = C::pair(y0 >> (4 * m));
-                        const uint32_t a2 = C::pair(x1 >> (4 * m)), a3 = C::pair(y1 >> (4 * m));
+                        const uint32_t a0 = C::centred(x0 >> (4 * m)), a1 = C::centred(y0 >> (4 * m));
+                        const uint32_t a2 = C::centred(x1 >> (4 * m)), a3 = C::centred(y1 >> (4 * m));
 #pragma unroll
                         for (int j = 0; j < NT; ++j) C::mma(acc[j][b][m], a0, a1, a2, a3, w0[j], w1[j]);
                     }
@@ -676,7 +678,6 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                     float low_part = least[j][b][e];
 #pragma unroll
                     for (int i = 4; i < 32; i *= 2) low_part += __shfl_xor_sync(~0u, low_part, i);
-                    low_part -= (C::kHeld + kMiddle) * ones[j][b][e];
                     float *to = merge + (warp * kRows + row) * Shape::kMergeRow + b * kGroup + 8 * g;
 #pragma unroll
                     for (int m = 0; m < 4; m += 2)

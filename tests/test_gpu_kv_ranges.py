@@ -224,3 +224,20 @@ def test_large_scales_of_scores(scale, lengths, counts, dim, q_heads, dtype):
     q = _rand(sum(counts), q_heads, dim, seed=5).to(dtype)
     got = pool.attend(q, table, device_lengths, cu_seqlens=cu, scale=scale)
     _check(got, q, pool.data, table, lengths, counts, page, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("dim,q_heads", [(64, 16), (128, 16), (128, 256), (256, 16)])
+@pytest.mark.parametrize("scale", [0.05, 1.0])
+def test_long_sums(scale, dim, q_heads, dtype):
+    """Thousands of tokens a warp: more requests and heads than CTAs, each of one long document that all share."""
+    length, page, seqs, heads = 32768, 64, 20, 16
+    table, lengths, _, pages = _sequences([length], page)
+    pool = _pool(pages, heads, page, dim)
+    k, v = _rand(length, heads, dim, seed=3), _rand(length, heads, dim, seed=4)
+    _fill(pool, k.to(dtype), v.to(dtype), table, lengths)
+    q = _rand(seqs, q_heads, dim, seed=5).to(dtype)
+    got = pool.attend(q, table.expand(seqs, -1), lengths.expand(seqs), scale=scale * dim ** -0.5)
+    pool.check_status()
+    for n in (0, 7):
+        _check(got[n:n + 1], q[n:n + 1], pool.data, table, [length], [1], page, scale=scale * dim ** -0.5)
