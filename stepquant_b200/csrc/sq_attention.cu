@@ -38,9 +38,7 @@ constexpr int kFewRows = 32;
 // ---------------------------------------------------------------------------
 // fragments
 // ---------------------------------------------------------------------------
-// Values are taken as (m + 8 s) + s (c - 8): of all splits of a value into a part that the weights'
-// rounding does not touch and one that it does, the one with the smallest second part.
-constexpr float kMiddle = 8.f;
+constexpr float kMiddle = 8.f;  // values' codes are multiplied as c - 8
 
 template <class T>
 struct Codes;
@@ -627,22 +625,45 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                 for (int i4 = 0; i4 < 4; ++i4) load_words(from + i4 * 4 * 32, word[i4]);
 #pragma unroll
                 for (int b = 0; b < kGroups; ++b) {
+                    // A weight p s is rounded before it meets a code, so the rest of the value has to go by the rounded weight
+                    // too, or what is lost is not p v's but that of two parts that cancel: with weights nearly alike, whose
+                    // roundings are then alike, that was up to 12 % of the outputs' norm (20000 tokens).  With zero's code k (0
+                    // to 15, the nearest where zero is outside): p v = p s (c - k) + p (m + k s), the second part 0 or, where
+                    // all of a group's values have one sign, the smallest of them.  (256 requests 338 -> 357 us.)
+                    // Here 8 - k and m + k s; any k in that range gives the same sum but for roundings.
+                    auto zero_of = [](float step, float low, float &below, float &rest) {
+                        const float range = 15.f * step, at = __saturatef(-low * reciprocal_approx(range));
+                        below = fmaf(at, -15.f, kMiddle);
+                        rest = fmaf(at, range, low);
+                    };
                     const float s0 = pair_scale(value_pairs[0][b]), s1 = pair_scale(value_pairs[1][b]);
-                    const float m0 = pair_min(value_pairs[0][b]) + kMiddle * s0, m1 = pair_min(value_pairs[1][b]) + kMiddle * s1;
+                    float below0, below1, rest0, rest1;
+                    zero_of(s0, pair_min(value_pairs[0][b]), below0, rest0);
+                    zero_of(s1, pair_min(value_pairs[1][b]), below1, rest1);
                     uint32_t w0[NT], w1[NT];
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
                         float u[4] = {z[h][j][0] * s0, z[h][j][1] * s0, z[h][j][2] * s1, z[h][j][3] * s1};
-                        float v[4] = {z[h][j][0] * m0, z[h][j][1] * m0, z[h][j][2] * m1, z[h][j][3] * m1};
                         if (hidden) {  // a hidden token's scale and minimum may be anything
 #pragma unroll
                             for (int i4 = 0; i4 < 4; ++i4)
-                                if (hidden >> (4 * (h * NT + j) + i4) & 1) u[i4] = v[i4] = 0.f;
+                                if (hidden >> (4 * (h * NT + j) + i4) & 1) u[i4] = 0.f;
                         }
-                        least[j][b][0] += v[0] + v[2];
-                        least[j][b][1] += v[1] + v[3];
-                        w0[j] = transpose8(C::pack(u[0], u[1]));
-                        w1[j] = transpose8(C::pack(u[2], u[3]));
+                        w0[j] = C::pack(u[0], u[1]);
+                        w1[j] = C::pack(u[2], u[3]);
+                        const float2 r0 = C::unpack(w0[j]), r1 = C::unpack(w1[j]);
+                        if (hidden) {
+                            const float v[4] = {fmaf(r0.x, below0, z[h][j][0] * rest0), fmaf(r0.y, below0, z[h][j][1] * rest0),
+                                                fmaf(r1.x, below1, z[h][j][2] * rest1), fmaf(r1.y, below1, z[h][j][3] * rest1)};
+#pragma unroll
+                            for (int i4 = 0; i4 < 4; ++i4)
+                                if (!(hidden >> (4 * (h * NT + j) + i4) & 1)) least[j][b][i4 & 1] += v[i4];
+                        } else {
+                            least[j][b][0] = fmaf(r1.x, below1, fmaf(z[h][j][2], rest1, fmaf(r0.x, below0, fmaf(z[h][j][0], rest0, least[j][b][0]))));
+                            least[j][b][1] = fmaf(r1.y, below1, fmaf(z[h][j][3], rest1, fmaf(r0.y, below0, fmaf(z[h][j][1], rest0, least[j][b][1]))));
+                        }
+                        w0[j] = transpose8(w0[j]);
+                        w1[j] = transpose8(w1[j]);
                     }
                     const uint32_t x0 = __byte_perm(word[0][b], word[1][b], 0x5410), y0 = __byte_perm(word[0][b], word[1][b], 0x7632);
                     const uint32_t x1 = __byte_perm(word[2][b], word[3][b], 0x5410), y1 = __byte_perm(word[2][b], word[3][b], 0x7632);

@@ -241,3 +241,23 @@ def test_long_sums(scale, dim, q_heads, dtype):
     pool.check_status()
     for n in (0, 7):
         _check(got[n:n + 1], q[n:n + 1], pool.data, table, [length], [1], page, scale=scale * dim ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("dim,count", [(64, None), (128, None), (128, 7), (256, None), (128, 40)])
+@pytest.mark.parametrize("skewed", [False, True])
+@pytest.mark.parametrize("spread", [0.0, 1e-4, 3e-4, 1e-3, 3e-3, 0.03])
+def test_nearly_flat_scores(spread, skewed, dim, count, dtype):
+    """Weights alike, whose roundings are then alike too, over values that all but cancel (in one channel of skewed
+    groups they do not: the extremes are far from symmetric).  What is rounded has to be what cancels."""
+    length, page = 20000, 64
+    table, lengths, cu, pages = _sequences([length], page, None if count is None else [count])
+    pool = _pool(pages, 1, page, dim)
+    k, v = _rand(length, 1, dim, seed=3), _rand(length, 1, dim, seed=4)
+    if skewed:
+        v = v.exp() - math.exp(0.5)
+    _fill(pool, k.bfloat16(), v.bfloat16(), table, lengths)
+    q = _rand(count or 1, 4, dim, seed=5).to(dtype)
+    scale = max(spread, 1e-9) * dim ** -0.5
+    got = pool.attend(q, table, lengths, cu_seqlens=cu, scale=scale)
+    _check(got, q, pool.data, table, [length], [count or 1], page, scale=scale)
