@@ -599,8 +599,9 @@ int32_t sq_kv_read(const sq_kv_args *args, sq_stream_t stream);
  *           strides multiples of 8; out contiguous, 16-byte aligned
  *   workspace  sq_kv_attention_workspace_bytes(...) bytes, 16-byte aligned
  * Sequences of many new tokens take keys and values in f16, over powers of two by the largest that any
- * of 128 or 256 rows reaches: what is below 2^-24 of that loses bits.  Sums are fp32: values of up to
- * 2^80 in magnitude do not overflow them at any length.
+ * of 128 or 256 rows reaches: what is below 2^-24 of that loses bits, and weights below 2^-32 of a row's
+ * largest count for nothing.  Sums are fp32: values of up to 2^80 in magnitude do not overflow them at
+ * any length.
  * status: also SQ_STATUS_TIMEOUT if a bounded device wait gave up; outputs concerned are NaN.
  * wait_clocks: how many clocks a wait may take, 0 for 2^32 (about two seconds), negative for one look.
  */

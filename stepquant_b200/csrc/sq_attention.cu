@@ -11,11 +11,14 @@
 // rows and eight query rows as columns; a warp's fragments are the tile's words with a
 // shift and a mask.  The products are a fifth of the tensor pipe's time: with eight columns
 // tcgen05 would idle as much and want the codes unpacked into shared memory first.
-// 256 ragged requests of up to 8192 tokens (1.3 GB) take 353 us, 3.7 TB/s: 400 instructions
-// a tile of 16 tokens and 2304 bytes (64 masks, 48 shifts, 34 products, the rest scales,
-// exponentials and waits) at 2.3 a clock and SM.  No unit is full (adders 0.54, DRAM 0.55 of
-// the copy rate): sixteen warps an SM, at 128 registers each, do not hide what each
-// instruction waits for the one before.
+// 256 ragged requests of up to 8192 tokens (1.3 GB) take 357 us, 3.7 TB/s: 444 instructions
+// a tile of 16 tokens and 2304 bytes (64 masks, 48 shifts, 32 differences, 32 products, the
+// rest scales, exponentials and waits) at 2.5 a clock and SM.  No unit is full (adders 0.56,
+// DRAM 0.55 of the copy rate): sixteen warps an SM, at 128 registers each, do not hide what
+// each instruction waits for the one before.
+//
+// Sums are fp32, but the tensor cores cut theirs off: up to 6e-9 of a sum a token (8e-4 at
+// 131072 tokens of equal weights and values), in both kernels.
 #include "sq_kv.cuh"
 #include "sq_rows.cuh"
 #include "sq_tc.cuh"
@@ -45,8 +48,8 @@ struct Codes;
 template <>
 struct Codes<__nv_bfloat16> {
     // Weights of bf16 queries are bf16 too: half a step of 2^-9, the size of an output's own rounding (256 requests: off
-    // by 2.2e-3 of the outputs' norm in all, of which that is 1.7e-3).  f16 weights would need what f16 queries do about
-    // p s (below; 369 us for 353) and more, as bf16 values go far beyond f16 either way.
+    // by 2.1e-3 of the outputs' norm in all, of which that is 1.7e-3).  f16 weights would need what f16 queries do about
+    // p s (below; 385 us for 357) and more, as bf16 values go far beyond f16 either way.
     static constexpr float kHeld = 128.f;  // pair() is c + this: a bf16 with c in its last bits
     __device__ static __forceinline__ uint32_t pair(uint32_t w) { return and_or(w, 0x000F000Fu, 0x43004300u); }
     // c - 8, for sums over many tokens: the tensor cores cut sums off, and those of 128 + c, 136 times the weights' sum

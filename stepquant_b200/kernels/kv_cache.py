@@ -148,7 +148,9 @@ def kv_attention(q, data, page_table, lengths, *, cu_seqlens=None, scale=None, w
     heads any stride apart; data, page_table, lengths, cu_seqlens as in
     ``kv_append``, which comes first: a token sees its sequence up to itself and,
     with ``window``, the last ``window`` positions of that.  scale: D^-1/2.  A
-    token that sees nothing, and tokens of no sequence, get zeros.  Should a bounded
+    token that sees nothing, and tokens of no sequence, get zeros.  In sequences of
+    more than 32 rows (new tokens times query heads of a kv head) weights below 2^-32
+    of a row's largest count for nothing.  Should a bounded
     device wait give up, outputs left undone are NaN and ``status`` has SQ_STATUS_TIMEOUT.
     """
     if q.dim() != 3:
