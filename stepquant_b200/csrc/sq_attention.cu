@@ -18,7 +18,8 @@
 // each instruction waits for the one before.
 //
 // Sums are fp32, but the tensor cores cut theirs off: up to 6e-9 of a sum a token (8e-4 at
-// 131072 tokens of equal weights and values), in both kernels.
+// 131072 tokens of equal weights and values), in both kernels.  So codes are summed about a
+// middle.
 #include "sq_kv.cuh"
 #include "sq_rows.cuh"
 #include "sq_tc.cuh"
@@ -49,12 +50,12 @@ template <>
 struct Codes<__nv_bfloat16> {
     // Weights of bf16 queries are bf16 too: half a step of 2^-9, the size of an output's own rounding (256 requests: off
     // by 2.1e-3 of the outputs' norm in all, of which that is 1.7e-3).  f16 weights would need what f16 queries do about
-    // p s (below; 385 us for 357) and more, as bf16 values go far beyond f16 either way.
+    // p s (below; 403 us for 357) and more, as bf16 values go far beyond f16 either way.
     static constexpr float kHeld = 128.f;  // pair() is c + this: a bf16 with c in its last bits
     __device__ static __forceinline__ uint32_t pair(uint32_t w) { return and_or(w, 0x000F000Fu, 0x43004300u); }
     // c - 8, for sums over many tokens: the tensor cores cut sums off, and those of 128 + c, 136 times the weights' sum
     // taken off at the end, were 4 % of the outputs' norm off where a warp had 4096 tokens (256 requests 353 -> 338 us, too).
-    __device__ static __forceinline__ uint32_t centred(uint32_t w) {
+    __device__ static __forceinline__ uint32_t centred(uint32_t w, uint32_t) {
         const uint32_t x = pair(w), base = 0x43084308u;
         const __nv_bfloat162 r = __hsub2(reinterpret_cast<const __nv_bfloat162 &>(x), reinterpret_cast<const __nv_bfloat162 &>(base));
         return reinterpret_cast<const uint32_t &>(r);
@@ -84,7 +85,11 @@ struct Codes<__half> {
         const __half2 r = __hsub2(reinterpret_cast<const __half2 &>(x), reinterpret_cast<const __half2 &>(base));
         return reinterpret_cast<const uint32_t &>(r);
     }
-    __device__ static __forceinline__ uint32_t centred(uint32_t w) { return pair(w); }
+    __device__ static __forceinline__ uint32_t centred(uint32_t w, uint32_t base) {
+        const uint32_t x = and_or(w, 0x000F000Fu, 0x64006400u);
+        const __half2 r = __hsub2(reinterpret_cast<const __half2 &>(x), reinterpret_cast<const __half2 &>(base));
+        return reinterpret_cast<const uint32_t &>(r);
+    }
     __device__ static __forceinline__ uint32_t pack(float lo, float hi) {
         uint32_t r;
         asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -435,6 +440,10 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
         const int sees_all = int(max(int64_t(0), min(s.before + row0 / group + 1, int64_t(s.length))) / kUnit);
         const int window_all = a.window > 0 ? int(min(max(int64_t(0), s.before + last_row / group - a.window + 1) + kUnit - 1, int64_t(0x7fffffff)) / kUnit) : 0;
 
+        uint32_t base[kGroups];  // the middle, as codes are before it is taken off
+        float middle[kGroups];
+#pragma unroll
+        for (int b = 0; b < kGroups; ++b) base[b] = 0x64086408u, middle[b] = kMiddle;
         float acc[NT][kGroups][4][4], least[NT][kGroups][2];
         float top[NT][2], against[NT][2], sum[NT][2];  // maxima of scores before `to_log2`
 #pragma unroll
@@ -462,6 +471,32 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
             }
             missing &= ~(1u << (kArmed + stage));
             const uint8_t *const unit = ring + stage * Shape::kStage;
+            const int index = s.unit + warp + i * kWarps;
+            const uint32_t none = missing >> 2 * stage & 3;
+            if (C::kNarrow && i == 0) {
+                // The code that sums over tokens are about: the whole number nearest to zero's in this warp's first tokens.
+                // About 8, with values whose extremes are far from symmetric, sums that the tensor cores cut off were 5e-3 of
+                // the outputs' norm off at 14000 tokens a warp (bf16: 2.9e-3, of which its own roundings are 2.4e-3; there it
+                // costs 357 -> 384 us with 256 requests, here 385 -> 403).
+                float steps[kGroups] = {}, lows[kGroups] = {};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t pairs[kGroups];
+                    load_words(unit + (e >> 1) * Tile::kBytes + Tile::kValuePairs + (g + 8 * (e & 1)) * kGroups * 4, pairs);
+                    const int p = index * kUnit + 8 * e + (g >> 1) + 4 * (g & 1);
+                    if (p >= here.seen_from && p < s.length && !(none >> (e >> 1) & 1)) {
+#pragma unroll
+                        for (int b = 0; b < kGroups; ++b) steps[b] += pair_scale(pairs[b]), lows[b] += pair_min(pairs[b]);
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < kGroups; ++b) {
+                    const float at = 15.f * __saturatef(-lows[b] * reciprocal_approx(15.f * steps[b]));
+                    const uint32_t code = (__reduce_add_sync(~0u, steps[b] > 0.f ? __float2uint_rn(at) : 8u) + 16) / 32;  // the lanes' mean
+                    base[b] = 0x64006400u + code * 0x10001u;
+                    middle[b] = float(code);
+                }
+            }
             // Scores of tokens (rows g, g + 8 of each tile) x query rows (2 t, 2 t + 1).
             float z[2][NT][4];
 #pragma unroll
@@ -507,8 +542,6 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                     }
                 }
             }
-            const int index = s.unit + warp + i * kWarps;
-            const uint32_t none = missing >> 2 * stage & 3;
             uint32_t hidden = 0;  // bits of z
             if (index >= sees_all || index < window_all || none) {
                 // Row r of a tile is token r / 2 + 4 (r % 2) of its half.
@@ -634,9 +667,9 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                     // to 15, the nearest where zero is outside): p v = p s (c - k) + p (m + k s), the second part 0 or, where
                     // all of a group's values have one sign, the smallest of them.  (256 requests 338 -> 357 us.)
                     // Here 8 - k and m + k s; any k in that range gives the same sum but for roundings.
-                    auto zero_of = [](float step, float low, float &below, float &rest) {
+                    auto zero_of = [&](float step, float low, float &below, float &rest) {
                         const float range = 15.f * step, at = __saturatef(-low * reciprocal_approx(range));
-                        below = fmaf(at, -15.f, kMiddle);
+                        below = fmaf(at, -15.f, middle[b]);
                         rest = fmaf(at, range, low);
                     };
                     const float s0 = pair_scale(value_pairs[0][b]), s1 = pair_scale(value_pairs[1][b]);
@@ -672,8 +705,8 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1) row
                     const uint32_t x1 = __byte_perm(word[2][b], word[3][b], 0x5410), y1 = __byte_perm(word[2][b], word[3][b], 0x7632);
 #pragma unroll
                     for (int m = 0; m < 4; ++m) {
-                        const uint32_t a0 = C::centred(x0 >> (4 * m)), a1 = C::centred(y0 >> (4 * m));
-                        const uint32_t a2 = C::centred(x1 >> (4 * m)), a3 = C::centred(y1 >> (4 * m));
+                        const uint32_t a0 = C::centred(x0 >> (4 * m), base[b]), a1 = C::centred(y0 >> (4 * m), base[b]);
+                        const uint32_t a2 = C::centred(x1 >> (4 * m), base[b]), a3 = C::centred(y1 >> (4 * m), base[b]);
 #pragma unroll
                         for (int j = 0; j < NT; ++j) C::mma(acc[j][b][m], a0, a1, a2, a3, w0[j], w1[j]);
                     }

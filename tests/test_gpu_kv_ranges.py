@@ -261,3 +261,18 @@ def test_nearly_flat_scores(spread, skewed, dim, count, dtype):
     scale = max(spread, 1e-9) * dim ** -0.5
     got = pool.attend(q, table, lengths, cu_seqlens=cu, scale=scale)
     _check(got, q, pool.data, table, [length], [count or 1], page, scale=scale)
+
+
+@pytest.mark.parametrize("scale", [0.05, 1.0])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_long_sums_of_skewed_values(dim, scale):
+    """Sums of codes about the middle that cancel against the middle's, over 16000 tokens a warp, in f16."""
+    length, page, seqs, heads = 131072, 64, 20, 16
+    table, lengths, _, pages = _sequences([length], page)
+    pool = _pool(pages, heads, page, dim)
+    k, v = _rand(length, heads, dim, seed=3), _rand(length, heads, dim, seed=4).exp() - math.exp(0.5)
+    _fill(pool, k.half(), v.half(), table, lengths)
+    q = _rand(seqs, heads, dim, seed=5).half()
+    got = pool.attend(q, table.expand(seqs, -1), lengths.expand(seqs), scale=scale * dim ** -0.5)
+    del k, v
+    _check(got[3:4], q[3:4], pool.data, table, [length], [1], page, scale=scale * dim ** -0.5)
