@@ -276,3 +276,36 @@ def test_long_sums_of_skewed_values(dim, scale):
     got = pool.attend(q, table.expand(seqs, -1), lengths.expand(seqs), scale=scale * dim ** -0.5)
     del k, v
     _check(got[3:4], q[3:4], pool.data, table, [length], [1], page, scale=scale * dim ** -0.5)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("counts", [None, [1, 1, 7], [40, 3, 170]])
+@pytest.mark.parametrize("window", [None, 50])
+def test_hidden_bytes_in_f16(window, counts, dim):
+    """Bytes past the lengths, in front of the window, of other pages and of pages <= 0 change no bit of what is seen,
+    whatever they hold."""
+    lengths, page = [61, 3, 200], 16
+    table, device_lengths, cu, pages = _sequences(lengths, page, counts)
+    pool = _pool(pages, 2, page, dim, dtype=torch.float16)
+    q = (2 * _rand(sum(counts or [1] * 3), 8, dim, seed=5)).half()
+    table[2, 10], table[2, 11] = 0, -3
+    want = pool.attend(q, table, device_lengths, cu_seqlens=cu, window=window)
+    assert bool(want.isfinite().all())
+    for fill in (255, 0x7F, 0xBF, 0x3C):
+        new = torch.full_like(pool.data, fill)
+        for n, length in enumerate(lengths):
+            first = 0 if window is None else max(0, length - (1 if counts is None else counts[n]) - window + 1)
+            for p in range(first // page, -(-length // page)):
+                held = int(table[n, p])
+                if held > 0:
+                    new[held] = pool.data[held]
+                    rest = length - p * page
+                    if rest < page:  # the pairs of the tokens past the end (their codes share no word with others)
+                        for u in range(rest, page):
+                            row = 2 * (u % 4) + u // 4 % 2 + u // 8 * 8
+                            for at in (8 * dim, 17 * dim):
+                                new[held, :, :, at + row * dim // 16:at + (row + 1) * dim // 16] = fill
+        old, pool.data = pool.data, new
+        got = pool.attend(q, table, device_lengths, cu_seqlens=cu, window=window)
+        pool.data = old
+        assert torch.equal(got, want), fill
