@@ -80,16 +80,12 @@ struct Codes<__nv_bfloat16> {
 template <>
 struct Codes<__half> {
     static constexpr float kHeld = -kMiddle;  // f16 with c in their last bits are 1024 + c, too far from c to leave it in
-    __device__ static __forceinline__ uint32_t pair(uint32_t w) {
-        const uint32_t x = and_or(w, 0x000F000Fu, 0x64006400u), base = 0x64086408u;
-        const __half2 r = __hsub2(reinterpret_cast<const __half2 &>(x), reinterpret_cast<const __half2 &>(base));
-        return reinterpret_cast<const uint32_t &>(r);
-    }
     __device__ static __forceinline__ uint32_t centred(uint32_t w, uint32_t base) {
         const uint32_t x = and_or(w, 0x000F000Fu, 0x64006400u);
         const __half2 r = __hsub2(reinterpret_cast<const __half2 &>(x), reinterpret_cast<const __half2 &>(base));
         return reinterpret_cast<const uint32_t &>(r);
     }
+    __device__ static __forceinline__ uint32_t pair(uint32_t w) { return centred(w, 0x64086408u); }
     __device__ static __forceinline__ uint32_t pack(float lo, float hi) {
         uint32_t r;
         asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
